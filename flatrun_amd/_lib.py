@@ -28,6 +28,8 @@ Q8_0, Q4_K, Q5_K, Q6_K, Q1_0 = 8, 12, 13, 14, 41
 Q4_0, Q5_0, Q5_1 = 2, 6, 7          # dequant only
 QTYPES = {"Q8_0": Q8_0, "Q4_K": Q4_K, "Q5_K": Q5_K, "Q6_K": Q6_K, "Q1_0": Q1_0,
           "Q4_0": Q4_0, "Q5_0": Q5_0, "Q5_1": Q5_1}
+F32, F16, BF16 = 0, 1, 30           # activations of the attention step
+VTYPES = {"f32": F32, "f16": F16, "bf16": BF16}
 BLOCKS = {Q8_0: (34, 32), Q4_K: (144, 256), Q5_K: (176, 256), Q6_K: (210, 256), Q1_0: (18, 128)}
 
 
@@ -117,6 +119,15 @@ SIGNATURES: dict[str, list] = {
     "frq_dev_silu_mul": [_vp, _i64, _vp, _i64, _i64, _i64, _vp],
     "frq_dev_gemv_swiglu": [_i32, _vp, _sz, _i32, _vp, _sz, _i64, _vp, _i64, _vp, _vp, _i64, _vp],
     "frq_gemv_swiglu_fusable": [_i32, _vp, _i32, _vp, _i64],
+    "frq_dev_qk_norm_rope": [_i32, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+                             _vp, _i64, _vp, _vp, _vp, _c.c_float, _vp],
+    "frq_kv4_bytes": [_i64, _i64, _i64, _i64, _c.POINTER(_sz)],
+    "frq_dev_kv4_write": [_vp, _sz, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp],
+    "frq_dev_kv4_read": [_vp, _sz, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp],
+    "frq_dev_attn_decode": [_i32, _vp, _i64, _vp, _sz, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64,
+                            _i64, _c.c_float, _vp],
+    "frq_dev_attn_prefill": [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp,
+                             _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _c.c_float, _vp],
     "frq_set_device": [_i32],
     "frq_malloc": [_c.POINTER(_vp), _sz],
     "frq_free": [_vp],

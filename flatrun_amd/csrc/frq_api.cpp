@@ -1156,6 +1156,178 @@ int frq_gemv_swiglu_fusable(int qtype_gate, const void* w_gate, int qtype_up, co
                : 0;
 }
 
+// ------------------------------------------------- the attention step
+static bool val_type(int type, int64_t* size) {
+    *size = type == FRQ_F32 ? 4 : 2;
+    return type == FRQ_F32 || type == FRQ_F16 || type == FRQ_BF16;
+}
+// A strided operand: 16-byte aligned rows that hold `need` elements.
+static bool rows_aligned(const void* p, int64_t ld, int64_t size) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+}
+// Every product of sizes below stays far from 2^63.
+static bool in_range(int64_t v, int64_t lo, int64_t hi) { return v >= lo && v <= hi; }
+constexpr int64_t kMaxTokens = (int64_t)1 << 31, kMaxHeads = 1024, kMaxLd = (int64_t)1 << 31;
+
+int frq_dev_qk_norm_rope(int x_type, const void* x, int64_t ld_x, int out_type, void* q, int64_t ld_q, void* k,
+                         int64_t ld_k, void* v, int64_t ld_v, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                         int64_t head_dim, int64_t rot, int interleaved, const float* table, int64_t n_pos,
+                         const int32_t* positions, const float* q_norm, const float* k_norm, float eps, void* stream) {
+    int64_t xs, os;
+    if (!val_type(x_type, &xs) || !val_type(out_type, &os))
+        return fail(FRQ_ERR_INVALID, "qk_norm_rope: types are F32, F16 or BF16, got %d and %d", x_type, out_type);
+    if (!in_range(tokens, 0, kMaxTokens) || !in_range(q_heads, 1, kMaxHeads) || !in_range(kv_heads, 1, kMaxHeads))
+        return fail(FRQ_ERR_SHAPE, "qk_norm_rope: tokens or heads out of range");
+    if (head_dim < 8 || head_dim > 256 || head_dim % 8)
+        return fail(FRQ_ERR_UNSUPPORTED, "qk_norm_rope: head size %lld is not a multiple of 8 up to 256", (long long)head_dim);
+    if (rot < 0 || rot > head_dim || rot % 2)
+        return fail(FRQ_ERR_SHAPE, "qk_norm_rope: the rotated part must be even and within the head");
+    const int64_t heads = q_heads + (v ? 2 : 1) * kv_heads;
+    if (!in_range(ld_x, heads * head_dim, kMaxLd) || !in_range(ld_q, q_heads * head_dim, kMaxLd) ||
+        !in_range(ld_k, kv_heads * head_dim, kMaxLd) || (v && !in_range(ld_v, kv_heads * head_dim, kMaxLd)))
+        return fail(FRQ_ERR_SHAPE, "qk_norm_rope: a row stride is shorter than its heads");
+    if (!(eps >= 0.f)) return fail(FRQ_ERR_INVALID, "qk_norm_rope: eps must not be negative");
+    if (tokens == 0) return FRQ_OK;
+    if (!x || !q || !k || (rot && (!positions || !table || n_pos < 1))) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (!rows_aligned(x, ld_x, xs) || !rows_aligned(q, ld_q, os) || !rows_aligned(k, ld_k, os) ||
+        (v && !rows_aligned(v, ld_v, os)))
+        return fail(FRQ_ERR_ALIGN, "qk_norm_rope: rows must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(table) & 7) || (reinterpret_cast<uintptr_t>(positions) & 3) ||
+        ((reinterpret_cast<uintptr_t>(q_norm) | reinterpret_cast<uintptr_t>(k_norm)) & 15))
+        return fail(FRQ_ERR_ALIGN, "qk_norm_rope: table 8-byte, positions 4-byte, norm weights 16-byte aligned");
+    if (tokens * heads > ((int64_t)1 << 34)) return fail(FRQ_ERR_UNSUPPORTED, "qk_norm_rope: too many heads for a launch");
+    frq::RopeArgs a{x_type, out_type, x,      ld_x, q,           k,     v,     ld_q,      ld_k,   ld_v,   tokens, q_heads,
+                    kv_heads, head_dim, rot, interleaved != 0, table, n_pos, positions, q_norm, k_norm, eps};
+    FRQ_HIP(frq::launch_qk_norm_rope(a, static_cast<hipStream_t>(stream)));
+    return FRQ_OK;
+}
+
+static int kv4_checks(const char* what, const void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens,
+                      int64_t kv_heads, int64_t head_dim) {
+    size_t need = 0;
+    if (int rc = frq_kv4_bytes(pages, page_tokens, kv_heads, head_dim, &need)) return rc;
+    if (cache_bytes < need)
+        return fail(FRQ_ERR_SIZE, "%s: the cache holds %zu bytes, %lld pages need %zu", what, cache_bytes, (long long)pages,
+                    need);
+    if (!cache && need) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (reinterpret_cast<uintptr_t>(cache) & 15) return fail(FRQ_ERR_ALIGN, "%s: the cache must be 16-byte aligned", what);
+    return FRQ_OK;
+}
+
+int frq_kv4_bytes(int64_t pages, int64_t page_tokens, int64_t kv_heads, int64_t head_dim, size_t* bytes) {
+    if (!bytes) return fail(FRQ_ERR_INVALID, "null bytes");
+    *bytes = 0;
+    if (!in_range(pages, 0, kMaxTokens) || !in_range(kv_heads, 1, kMaxHeads))
+        return fail(FRQ_ERR_SHAPE, "kv4: pages or heads out of range");
+    if (page_tokens < 32 || page_tokens > 4096 || page_tokens % 32)
+        return fail(FRQ_ERR_UNSUPPORTED, "kv4: a page holds a multiple of 32 tokens up to 4096, got %lld",
+                    (long long)page_tokens);
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail(FRQ_ERR_UNSUPPORTED, "kv4: head size %lld is not 64, 128 or 256", (long long)head_dim);
+    *bytes = (size_t)pages * (size_t)kv_heads * (size_t)(page_tokens / 32) * (size_t)(head_dim / 32 * 1152);
+    return FRQ_OK;
+}
+
+static int kv4_move(const char* what, bool write, void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens,
+                    int64_t kv_heads, int64_t head_dim, int type, void* k, int64_t ld_k, void* v, int64_t ld_v,
+                    const int64_t* slots, int64_t tokens, void* stream) {
+    int64_t size;
+    if (!val_type(type, &size)) return fail(FRQ_ERR_INVALID, "%s: the type is F32, F16 or BF16, got %d", what, type);
+    if (int rc = kv4_checks(what, cache, cache_bytes, pages, page_tokens, kv_heads, head_dim)) return rc;
+    if (!in_range(tokens, 0, kMaxTokens)) return fail(FRQ_ERR_SHAPE, "%s: tokens out of range", what);
+    if (!in_range(ld_k, kv_heads * head_dim, kMaxLd) || !in_range(ld_v, kv_heads * head_dim, kMaxLd))
+        return fail(FRQ_ERR_SHAPE, "%s: a row stride is shorter than its heads", what);
+    if (tokens == 0) return FRQ_OK;
+    if (!k || !v || !slots) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (!rows_aligned(k, ld_k, size) || !rows_aligned(v, ld_v, size) || (reinterpret_cast<uintptr_t>(slots) & 7))
+        return fail(FRQ_ERR_ALIGN, "%s: k and v rows must be 16-byte aligned, slots 8-byte", what);
+    if (tokens * kv_heads > ((int64_t)1 << 33)) return fail(FRQ_ERR_UNSUPPORTED, "%s: too many heads for a launch", what);
+    frq::KvArgs a{cache, pages, page_tokens, kv_heads, head_dim, type, k, v, ld_k, ld_v, slots, tokens};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    FRQ_HIP(write ? frq::launch_kv_write(a, s) : frq::launch_kv_read(a, s));
+    return FRQ_OK;
+}
+
+int frq_dev_kv4_write(void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens, int64_t kv_heads,
+                      int64_t head_dim, int type, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
+                      const int64_t* slots, int64_t tokens, void* stream) {
+    return kv4_move("kv4_write", true, cache, cache_bytes, pages, page_tokens, kv_heads, head_dim, type,
+                    const_cast<void*>(k), ld_k, const_cast<void*>(v), ld_v, slots, tokens, stream);
+}
+
+int frq_dev_kv4_read(const void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens, int64_t kv_heads,
+                     int64_t head_dim, int type, void* k, int64_t ld_k, void* v, int64_t ld_v, const int64_t* slots,
+                     int64_t tokens, void* stream) {
+    return kv4_move("kv4_read", false, const_cast<void*>(cache), cache_bytes, pages, page_tokens, kv_heads, head_dim,
+                    type, k, ld_k, v, ld_v, slots, tokens, stream);
+}
+
+int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
+                        int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
+                        const int32_t* lens, int64_t max_len, void* out, int64_t ld_out, int64_t batch, int64_t q_heads,
+                        float scale, void* stream) {
+    int64_t size;
+    if (!val_type(type, &size)) return fail(FRQ_ERR_INVALID, "attn_decode: the type is F32, F16 or BF16, got %d", type);
+    if (int rc = kv4_checks("attn_decode", cache, cache_bytes, pages, page_tokens, kv_heads, head_dim)) return rc;
+    if (!in_range(batch, 0, (int64_t)1 << 20) || !in_range(q_heads, 1, kMaxHeads) || q_heads % kv_heads)
+        return fail(FRQ_ERR_SHAPE, "attn_decode: q_heads must be a multiple of kv_heads, the batch up to 2^20");
+    if (!in_range(max_len, 0, kMaxTokens - 64) || !in_range(ld_table, (max_len + page_tokens - 1) / page_tokens, kMaxLd))
+        return fail(FRQ_ERR_SHAPE, "attn_decode: a row of the page table is shorter than max_len");
+    if (!in_range(ld_q, q_heads * head_dim, kMaxLd) || !in_range(ld_out, q_heads * head_dim, kMaxLd))
+        return fail(FRQ_ERR_SHAPE, "attn_decode: a row stride is shorter than its heads");
+    if (!(scale > 0.f && scale < __builtin_inff())) return fail(FRQ_ERR_INVALID, "attn_decode: scale must be positive");
+    if (batch == 0) return FRQ_OK;
+    if (!q || !out || !lens || (!table && max_len)) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (!rows_aligned(q, ld_q, size) || !rows_aligned(out, ld_out, size) ||
+        ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(lens)) & 3))
+        return fail(FRQ_ERR_ALIGN, "attn_decode: q and out rows must be 16-byte aligned, table and lens 4-byte");
+    frq::DecodeArgs a{type,  q,        ld_q, cache,   pages, page_tokens, kv_heads, head_dim, table, ld_table, lens,
+                      max_len, out,    ld_out, batch, q_heads, scale,     0,        0,        nullptr, nullptr};
+    frq::plan_attn_decode(&a);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    float* part;
+    uint32_t* cnt;
+    std::lock_guard<std::mutex> lk(g_sk_mu);
+    if (int rc = sk_scratch_locked(s, frq::attn_decode_scratch(a), 0, &part, &cnt)) return rc;
+    FRQ_HIP(frq::launch_attn_decode(a, part, s));
+    return FRQ_OK;
+}
+
+int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
+                         const void* v, int64_t ld_v, int64_t hs_v, int out_type, void* out, int64_t ld_out,
+                         int64_t hs_out, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tokens_q,
+                         int64_t tokens_k, int64_t max_q, int64_t max_k, int64_t q_heads, int64_t kv_heads,
+                         int64_t head_dim, int causal, float scale, void* stream) {
+    if ((type != FRQ_F16 && type != FRQ_BF16) || (out_type != type && out_type != FRQ_F32))
+        return fail(FRQ_ERR_INVALID, "attn_prefill: inputs are F16 or BF16, the output the same or F32, got %d and %d", type,
+                    out_type);
+    if (!in_range(seqs, 0, (int64_t)1 << 20) || !in_range(tokens_q, 0, kMaxTokens - 256) ||
+        !in_range(tokens_k, 0, kMaxTokens - 256) || !in_range(max_q, 0, tokens_q) || !in_range(max_k, 0, tokens_k))
+        return fail(FRQ_ERR_SHAPE, "attn_prefill: sequences or lengths out of range");
+    if (!in_range(q_heads, 1, kMaxHeads) || !in_range(kv_heads, 1, kMaxHeads) || q_heads % kv_heads)
+        return fail(FRQ_ERR_SHAPE, "attn_prefill: q_heads must be a multiple of kv_heads");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_prefill: head size %lld is not 64, 128 or 256", (long long)head_dim);
+    const int64_t strides[8] = {ld_q, hs_q, ld_k, hs_k, ld_v, hs_v, ld_out, hs_out};
+    for (int64_t s : strides)
+        if (!in_range(s, head_dim, kMaxLd)) return fail(FRQ_ERR_SHAPE, "attn_prefill: a stride is shorter than a head");
+    if (!(scale > 0.f && scale < __builtin_inff())) return fail(FRQ_ERR_INVALID, "attn_prefill: scale must be positive");
+    if (seqs == 0 || max_q == 0) return FRQ_OK;
+    if (!q || !out || !cu_q || !cu_k || (tokens_k && (!k || !v))) return fail(FRQ_ERR_INVALID, "null buffer");
+    const int64_t os = out_type == FRQ_F32 ? 4 : 2;
+    if (!rows_aligned(q, ld_q, 2) || !rows_aligned(k, ld_k, 2) || !rows_aligned(v, ld_v, 2) ||
+        !rows_aligned(out, ld_out, os) || hs_q % 8 || hs_k % 8 || hs_v % 8 || (hs_out * os) % 16 ||
+        ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) & 3))
+        return fail(FRQ_ERR_ALIGN, "attn_prefill: every head's row must be 16-byte aligned, the offsets 4-byte");
+    if ((max_q + 127) / 128 * seqs > ((int64_t)1 << 31) / q_heads - 1)
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_prefill: more blocks than a launch takes");
+    frq::PrefillArgs a{type, out_type, q,    k,    v,        ld_q,     hs_q,  ld_k,    hs_k,     ld_v,     hs_v,   out,
+                       ld_out, hs_out, cu_q, cu_k, seqs, tokens_q, tokens_k, max_q, q_heads, kv_heads, head_dim, causal != 0,
+                       scale, 0};
+    FRQ_HIP(frq::launch_attn_prefill(a, static_cast<hipStream_t>(stream)));
+    return FRQ_OK;
+}
+
 int frq_set_device(int device) { FRQ_HIP(hipSetDevice(device)); return FRQ_OK; }
 int frq_malloc(void** ptr, size_t bytes) {
     if (!ptr) return fail(FRQ_ERR_INVALID, "null ptr");

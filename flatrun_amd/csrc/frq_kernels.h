@@ -264,6 +264,72 @@ hipError_t launch_copy16(const void* src, void* dst, size_t bytes, hipStream_t s
 hipError_t launch_silu_mul(const float* gateup, int64_t ld_in, float* out, int64_t ld_out, int64_t rows,
                            int64_t inter, hipStream_t stream);
 
+// The attention step of a decoder block. Types are GGML ids (F32 0, F16 1,
+// BF16 30), ld_* / hs_* strides of a token and of a head in elements.
+struct RopeArgs {
+    int x_type, out_type;
+    const void* x;
+    int64_t ld_x;
+    void *q, *k, *v;             // v null: the projection's v stays where it is
+    int64_t ld_q, ld_k, ld_v;
+    int64_t tokens, q_heads, kv_heads, head_dim, rot;
+    int interleaved;
+    const float* table;          // [n_pos][rot / 2][cos, sin]
+    int64_t n_pos;
+    const int32_t* positions;
+    const float *q_norm, *k_norm;
+    float eps;
+};
+hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t stream);
+
+struct KvArgs {
+    void* cache;
+    int64_t pages, page_tokens, kv_heads, head_dim;
+    int type;
+    void *k, *v;                 // read by write, written by read
+    int64_t ld_k, ld_v;
+    const int64_t* slots;
+    int64_t tokens;
+};
+hipError_t launch_kv_write(const KvArgs& a, hipStream_t stream);
+hipError_t launch_kv_read(const KvArgs& a, hipStream_t stream);
+
+struct DecodeArgs {
+    int type;
+    const void* q;
+    int64_t ld_q;
+    const void* cache;
+    int64_t pages, page_tokens, kv_heads, head_dim;
+    const int32_t* table;
+    int64_t ld_table;
+    const int32_t* lens;
+    int64_t max_len;
+    void* out;
+    int64_t ld_out;
+    int64_t batch, q_heads;
+    float scale;
+    int splits, chunk_tiles;     // plan_attn_decode
+    float *part_o, *part_ml;     // set by the launcher
+};
+void plan_attn_decode(DecodeArgs* a);
+size_t attn_decode_scratch(const DecodeArgs& a);
+hipError_t launch_attn_decode(DecodeArgs a, float* scratch, hipStream_t stream);
+
+struct PrefillArgs {
+    int type, out_type;
+    const void *q, *k, *v;
+    int64_t ld_q, hs_q, ld_k, hs_k, ld_v, hs_v;
+    void* out;
+    int64_t ld_out, hs_out;
+    const int32_t *cu_q, *cu_k;
+    int64_t seqs, tokens_q, tokens_k, max_q;
+    int64_t q_heads, kv_heads, head_dim;
+    int causal;
+    float scale;
+    int64_t q_blocks;            // set by the launcher
+};
+hipError_t launch_attn_prefill(PrefillArgs a, hipStream_t stream);
+
 // Scratch a caller brings in place of the stream registry's: exchange slots
 // (zero before a launch, left zero by every launch) and split-K partials.
 struct FixedScratch {

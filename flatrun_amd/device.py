@@ -419,3 +419,161 @@ def silu_mul(gateup, out, rows: int, inter: int, ld_in: int = 0, ld_out: int = 0
     li = int(ld_in) or 2 * int(inter)
     lo = int(ld_out) or int(inter)
     check(lib().frq_dev_silu_mul(_addr(gateup), li, _addr(out), lo, int(rows), int(inter), _stream(stream)))
+
+
+# ------------------------------------------------- a block's attention step
+
+def vtype_id(t) -> int:
+    """Type id of activations: "f32", "f16" or "bf16" (or the id itself)."""
+    if isinstance(t, str):
+        if t.lower() not in _lib.VTYPES:
+            raise ValueError(f"activations are f32, f16 or bf16, not {t!r}")
+        return _lib.VTYPES[t.lower()]
+    return int(t)
+
+
+def _vsize(t) -> int:
+    return 4 if vtype_id(t) == _lib.F32 else 2
+
+
+_TORCH_NAMES = {"torch.float32": _lib.F32, "torch.float16": _lib.F16, "torch.bfloat16": _lib.BF16,
+                "torch.int32": "int32", "torch.int64": "int64"}
+
+
+def _holds(name: str, obj, need: int, kind=None) -> None:
+    """Refuses a buffer whose size is known and too small for the call (an
+    address says nothing of its size), or a torch tensor of another type."""
+    if obj is None or isinstance(obj, int):
+        return
+    have = _TORCH_NAMES.get(str(getattr(obj, "dtype", "")))
+    if kind is not None and have is not None and have != kind:
+        raise TypeError(f"{name} is {obj.dtype}, the call says otherwise")
+    if isinstance(obj, DeviceBuffer):
+        size = obj.nbytes
+    elif hasattr(obj, "untyped_storage"):
+        size = int(obj.untyped_storage().nbytes() - obj.storage_offset() * obj.element_size())
+    else:
+        return
+    if size < need:
+        raise ValueError(f"{name} holds {size} bytes, the call needs {need}")
+
+
+def _span(rows: int, ld: int, last: int) -> int:
+    """Elements from the first to past the last of `rows` rows ld apart."""
+    return (rows - 1) * ld + last if rows > 0 else 0
+
+
+def qk_norm_rope(x, q, k, v, tokens: int, q_heads: int, kv_heads: int, head_dim: int, table, positions,
+                 rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None, eps: float = 1e-6,
+                 x_dtype="f32", out_dtype="f32", ld_x: int = 0, ld_q: int = 0, ld_k: int = 0, ld_v: int = 0,
+                 n_pos: int | None = None, stream=None) -> None:
+    """Norms of the query and key heads and rotary positions of the q|k|v rows
+    of ``x`` in one pass (frq_dev_qk_norm_rope), enqueued.
+
+    Row t of ``x`` (``ld_x`` elements apart, default the heads' width) goes to
+    ``q[t]``, ``k[t]`` and ``v[t]`` (``v`` None: x has, or keeps, its v); ``rot``
+    elements of each head turn (default all) by ``table[positions[t]]``
+    (:func:`flatrun_amd.attention.rope_table`; ``n_pos`` rows, taken from its
+    size where that is known); ``q_norm`` / ``k_norm``: fp32 weights or None."""
+    hd, t = int(head_dim), int(tokens)
+    rot = hd if rot is None else int(rot)
+    lq, lk, lv = int(ld_q) or q_heads * hd, int(ld_k) or kv_heads * hd, int(ld_v) or kv_heads * hd
+    width = (q_heads + (1 if v is None else 2) * kv_heads) * hd
+    lx = int(ld_x) or width
+    xs, os_ = _vsize(x_dtype), _vsize(out_dtype)
+    xi, oi = vtype_id(x_dtype), vtype_id(out_dtype)
+    if n_pos is None:
+        n_pos = _nbytes(table) // (4 * rot) if rot and table is not None else 0
+    _holds("x", x, xs * _span(t, lx, width), xi)
+    for name, buf, ld, heads in (("q", q, lq, q_heads), ("k", k, lk, kv_heads), ("v", v, lv, kv_heads)):
+        _holds(name, buf, os_ * _span(t, ld, heads * hd), oi)
+    _holds("table", table, 4 * int(n_pos) * rot, _lib.F32)
+    _holds("positions", positions, 4 * t, "int32")
+    _holds("q_norm", q_norm, 4 * hd, _lib.F32)
+    _holds("k_norm", k_norm, 4 * hd, _lib.F32)
+    check(lib().frq_dev_qk_norm_rope(xi, _addr(x), lx, oi, _addr(q), lq, _addr(k), lk, _addr(v), lv, t, int(q_heads),
+                                     int(kv_heads), hd, rot, int(bool(interleaved)), _addr(table), int(n_pos),
+                                     _addr(positions), _addr(q_norm), _addr(k_norm), float(eps), _stream(stream)))
+
+
+def kv4_bytes(pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of a 4-bit paged cache (frq_kv4_bytes); needs no GPU."""
+    n = ctypes.c_size_t()
+    check(lib().frq_kv4_bytes(int(pages), int(page_tokens), int(kv_heads), int(head_dim), ctypes.byref(n)))
+    return int(n.value)
+
+
+def _kv4_args(cache, k, v, slots, tokens, dtype, ld_k, ld_v):
+    width = cache.kv_heads * cache.head_dim
+    lk, lv = int(ld_k) or width, int(ld_v) or width
+    ti, size = vtype_id(dtype), _vsize(dtype)
+    _holds("k", k, size * _span(int(tokens), lk, width), ti)
+    _holds("v", v, size * _span(int(tokens), lv, width), ti)
+    _holds("slots", slots, 8 * int(tokens), "int64")
+    return (_addr(cache), cache.nbytes, cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, ti, _addr(k), lk,
+            _addr(v), lv, _addr(slots), int(tokens))
+
+
+def kv4_write(cache, k, v, slots, tokens: int, dtype="f32", ld_k: int = 0, ld_v: int = 0, stream=None) -> None:
+    """Quantise ``tokens`` tokens' heads into the slots (int64, on the device)
+    of a :class:`flatrun_amd.attention.KVCache4`, enqueued (frq_dev_kv4_write)."""
+    check(lib().frq_dev_kv4_write(*_kv4_args(cache, k, v, slots, tokens, dtype, ld_k, ld_v), _stream(stream)))
+
+
+def kv4_read(cache, k, v, slots, tokens: int, dtype="f32", ld_k: int = 0, ld_v: int = 0, stream=None) -> None:
+    """The values at the slots of a :class:`flatrun_amd.attention.KVCache4`
+    into k and v, enqueued (frq_dev_kv4_read)."""
+    check(lib().frq_dev_kv4_read(*_kv4_args(cache, k, v, slots, tokens, dtype, ld_k, ld_v), _stream(stream)))
+
+
+def attn_decode(q, cache, table, lens, out, batch: int, q_heads: int, max_len: int, dtype="f32",
+                scale: float | None = None, ld_q: int = 0, ld_out: int = 0, ld_table: int = 0, stream=None) -> None:
+    """out[b] = attention of query token q[b] over the first lens[b] tokens of
+    its sequence in a :class:`flatrun_amd.attention.KVCache4`, enqueued
+    (frq_dev_attn_decode).
+
+    ``table``: int32 page ids, one row per sequence (``ld_table`` apart,
+    default what ``max_len`` tokens need, or a 2-d tensor's own row stride);
+    ``lens``: int32; no length exceeds ``max_len``. ``scale`` defaults to
+    1 / sqrt(head_dim)."""
+    hd, b = cache.head_dim, int(batch)
+    lq, lo = int(ld_q) or q_heads * hd, int(ld_out) or q_heads * hd
+    per = (int(max_len) + cache.page_tokens - 1) // cache.page_tokens
+    lt = int(ld_table)
+    if not lt:
+        lt = int(table.stride(0)) if getattr(table, "ndim", 0) == 2 and hasattr(table, "stride") else per
+    ti, size = vtype_id(dtype), _vsize(dtype)
+    _holds("q", q, size * _span(b, lq, q_heads * hd), ti)
+    _holds("out", out, size * _span(b, lo, q_heads * hd), ti)
+    _holds("table", table, 4 * _span(b, lt, per), "int32")
+    _holds("lens", lens, 4 * b, "int32")
+    check(lib().frq_dev_attn_decode(ti, _addr(q), lq, _addr(cache), cache.nbytes, cache.pages, cache.page_tokens,
+                                    cache.kv_heads, hd, _addr(table), lt, _addr(lens), int(max_len), _addr(out), lo, b,
+                                    int(q_heads), hd ** -0.5 if scale is None else float(scale), _stream(stream)))
+
+
+def attn_prefill(q, k, v, out, cu_q, cu_k, seqs: int, tokens_q: int, tokens_k: int, q_heads: int, kv_heads: int,
+                 head_dim: int, max_q: int, max_k: int, causal: bool = True, dtype="bf16", out_dtype=None,
+                 scale: float | None = None, ld_q: int = 0, ld_k: int = 0, ld_v: int = 0, ld_out: int = 0, hs_q: int = 0,
+                 hs_k: int = 0, hs_v: int = 0, hs_out: int = 0, stream=None) -> None:
+    """Attention over ``seqs`` packed sequences (frq_dev_attn_prefill),
+    enqueued: the queries [cu_q[s], cu_q[s + 1]) over the keys [cu_k[s],
+    cu_k[s + 1]) (int32 on the device, seqs + 1 of each), causal from the last
+    key back. Tokens are ``ld_*`` elements apart (default all heads side by
+    side) and heads ``hs_*`` (default head_dim). ``dtype`` "bf16" or "f16";
+    ``out_dtype`` the same (default) or "f32"."""
+    hd, tq, tk = int(head_dim), int(tokens_q), int(tokens_k)
+    out_dtype = dtype if out_dtype is None else out_dtype
+    hq, hk, hv, ho = (int(h) or hd for h in (hs_q, hs_k, hs_v, hs_out))
+    lq, lo = int(ld_q) or q_heads * hd, int(ld_out) or q_heads * hd
+    lk, lv = int(ld_k) or kv_heads * hd, int(ld_v) or kv_heads * hd
+    for name, buf, rows, ld, hs, heads, ty in (("q", q, tq, lq, hq, q_heads, dtype), ("k", k, tk, lk, hk, kv_heads, dtype),
+                                               ("v", v, tk, lv, hv, kv_heads, dtype),
+                                               ("out", out, tq, lo, ho, q_heads, out_dtype)):
+        _holds(name, buf, _vsize(ty) * (_span(rows, ld, _span(heads, hs, hd)) if rows else 0), vtype_id(ty))
+    _holds("cu_q", cu_q, 4 * (int(seqs) + 1), "int32")
+    _holds("cu_k", cu_k, 4 * (int(seqs) + 1), "int32")
+    check(lib().frq_dev_attn_prefill(vtype_id(dtype), _addr(q), lq, hq, _addr(k), lk, hk, _addr(v), lv, hv,
+                                     vtype_id(out_dtype), _addr(out), lo, ho, _addr(cu_q), _addr(cu_k), int(seqs), tq, tk,
+                                     int(max_q), int(max_k), int(q_heads), int(kv_heads), hd, int(bool(causal)),
+                                     hd ** -0.5 if scale is None else float(scale), _stream(stream)))

@@ -58,6 +58,8 @@ typedef enum {
 
 enum { FRQ_Q4_0 = 2, FRQ_Q5_0 = 6, FRQ_Q5_1 = 7, FRQ_Q8_0 = 8, FRQ_Q4_K = 12, FRQ_Q5_K = 13, FRQ_Q6_K = 14,
        FRQ_Q1_0 = 41 };
+/* Activation types of the attention step, GGML type ids too. */
+enum { FRQ_F32 = 0, FRQ_F16 = 1, FRQ_BF16 = 30 };
 
 /* ---------------------------------------------------------------- general */
 
@@ -389,6 +391,81 @@ int frq_dev_gemv_swiglu(int qtype_gate, const void* w_gate, size_t gate_bytes, i
 /* 1 if frq_dev_gemv_swiglu runs these two matrices and the activation as one
  * launch at batch 1, else 0. */
 int frq_gemv_swiglu_fusable(int qtype_gate, const void* w_gate, int qtype_up, const void* w_up, int64_t k);
+
+/* --------------------------------------- a decoder block's attention step
+ * What runs between the q|k|v projection and the o projection; the reference
+ * does it in NumPy per layer (attention, RoPE and head norms of
+ * model/qwen2.py:1520-1624) and keeps K and V in fp32 (runtime/kv_cache.py).
+ * Types are FRQ_F32 / FRQ_F16 / FRQ_BF16; ld_* are the strides from a token to
+ * the next and hs_* from a head to the next, in elements; every row 16-byte
+ * aligned. Arithmetic is fp32 or better with one rounding when stored, except
+ * where said. Lengths, positions, slots and pages are device arrays that the
+ * host cannot check: the kernels do, as said for each. */
+
+/* Norms of the query and key heads and rotary positions, one pass. Row t of x
+ * holds q_heads, kv_heads (k) and, unless v is null, kv_heads (v) heads of
+ * head_dim elements (a multiple of 8 up to 256). With q_norm / k_norm (fp32
+ * [head_dim], 16-byte aligned, or null): y = x / sqrt(mean(x^2) + eps) * w per
+ * head. Then in the first `rot` elements (even, 0 for none) each pair (a, b) --
+ * (i, i + rot/2), or (2i, 2i + 1) with `interleaved` -- becomes (a c - b s,
+ * b c + a s), (c, s) = table[position][i], table fp32 [n_pos][rot/2][2]
+ * (positions and table are not read where rot is 0). v is copied. A position outside [0, n_pos) gives a row of NaN. q, k and v may be
+ * x's own heads (same type and strides), not overlap x otherwise. */
+int frq_dev_qk_norm_rope(int x_type, const void* x, int64_t ld_x, int out_type, void* q, int64_t ld_q, void* k,
+                         int64_t ld_k, void* v, int64_t ld_v, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                         int64_t head_dim, int64_t rot, int interleaved, const float* table, int64_t n_pos,
+                         const int32_t* positions, const float* q_norm, const float* k_norm, float eps, void* stream);
+
+/* A paged cache of keys and values in 4 bits: `pages` pages of page_tokens
+ * tokens (a multiple of 32 up to 4096), kv_heads heads of head_dim (64, 128 or
+ * 256). 32 channels of a head of a token share a scale d = fp16(-e / 8), e the
+ * element of largest magnitude (the first of equals), |d| held to 65504, and
+ * keep code = round_even(x / d) + 8 held to [0, 15]: the value d (code - 8) of
+ * a Q4_0 block. A block with an inf or a NaN reads back as NaN. 4.5 bits an
+ * element; the order of the bytes is the library's own (write and read are the
+ * way in and out). frq_kv4_bytes: the size of such a cache. */
+int frq_kv4_bytes(int64_t pages, int64_t page_tokens, int64_t kv_heads, int64_t head_dim, size_t* bytes);
+/* Token t's heads k[t], v[t] into slot slots[t] = page * page_tokens + place.
+ * A slot outside the cache is skipped (-1 for padding); the slots of a call
+ * are distinct. */
+int frq_dev_kv4_write(void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens, int64_t kv_heads,
+                      int64_t head_dim, int type, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
+                      const int64_t* slots, int64_t tokens, void* stream);
+/* The values at slots[t] into k[t], v[t]: zeros for a negative slot, NaN for
+ * one past the cache. */
+int frq_dev_kv4_read(const void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens, int64_t kv_heads,
+                     int64_t head_dim, int type, void* k, int64_t ld_k, void* v, int64_t ld_v, const int64_t* slots,
+                     int64_t tokens, void* stream);
+
+/* One query token per sequence against the cache: out[b, h] = sum over
+ * t < lens[b] of softmax(scale q[b, h] . k_t) v_t with the values the cache
+ * holds, query heads h / (q_heads / kv_heads) to a key head. Sequence b's token
+ * t is in page table[b * ld_table + t / page_tokens]. fp32 precision
+ * throughout (q and the weights enter the products as two fp16 parts, 22
+ * bits). lens[b] = 0: zeros. lens[b] > max_len or a page outside the cache:
+ * NaN. Long sequences are split over workgroups, whose partial results (4
+ * (head_dim + 2) bytes per query head and split) use the stream's scratch and
+ * are joined in a fixed order; the split depends on max_len and the shapes
+ * only. */
+int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
+                        int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
+                        const int32_t* lens, int64_t max_len, void* out, int64_t ld_out, int64_t batch, int64_t q_heads,
+                        float scale, void* stream);
+
+/* Attention over packed sequences: sequence s has the queries [cu_q[s],
+ * cu_q[s + 1]) and the keys [cu_k[s], cu_k[s + 1]) (int32, seqs + 1 of each,
+ * within tokens_q and tokens_k; no sequence longer than max_q and max_k).
+ * Query i of a sequence sees its keys j <= i + (keys - queries) where causal,
+ * else all; one that sees none gives zeros. Values of keys that a query does
+ * not see never reach it, infinities and NaN included. Inputs F16 or BF16 (one
+ * type), scores and sums fp32, the softmax weights rounded to the inputs' type
+ * for their product with v; out of that type or F32. head_dim 64, 128 or 256.
+ * A sequence whose offsets leave the buffers is not computed. */
+int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
+                         const void* v, int64_t ld_v, int64_t hs_v, int out_type, void* out, int64_t ld_out,
+                         int64_t hs_out, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tokens_q,
+                         int64_t tokens_k, int64_t max_q, int64_t max_k, int64_t q_heads, int64_t kv_heads,
+                         int64_t head_dim, int causal, float scale, void* stream);
 
 /* ------------------------------------------- memory, streams and events
  * Thin wrappers so a ctypes caller needs no other HIP binding. Streams are
