@@ -24,9 +24,11 @@ namespace {
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
 using f32x16 = float __attribute__((ext_vector_type(16)));
 
-constexpr int kWaves = 4, kKeys = 64, kRows = 32 * kWaves;
+constexpr int kKeys = 64;             // keys of a step
 
 template <int TYPE>
 __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
@@ -43,15 +45,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return (uint32_t)Val<TYPE>::one(a) | ((uint32_t)Val<TYPE>::one(b) << 16);
 }
 
-// Whether one of eight 16-bit values is an inf or a NaN.
+// The halves of w that are an inf or a NaN, as a mask of ones.
 template <int TYPE>
-__device__ __forceinline__ bool any_special(uint4 v) {
+__device__ __forceinline__ uint32_t specials(uint32_t w) {
     constexpr uint32_t e = TYPE == kTypeBF16 ? 0x7F80u : 0x7C00u;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool r = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r |= (w[i] & e) == e || ((w[i] >> 16) & e) == e;
-    return r;
+    return ((w & e) == e ? 0xFFFFu : 0u) | (((w >> 16) & e) == e ? 0xFFFF0000u : 0u);
 }
 
 template <int TYPE>
@@ -60,39 +58,76 @@ __device__ __forceinline__ float widen(uint16_t b) {
     return f16_bits_to_f32(b);
 }
 
+// Where 16-byte piece p of row r lies in a tile of rows of CH pieces. A wave
+// reads K as 16 rows of one piece at a time and V as 4 rows of 4 pieces; with
+// the row's low bits on the piece's high ones both touch every bank once.
+template <int CH>
+__device__ __forceinline__ int swizzle(int r) {
+    if constexpr (CH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
 // Four keys of one column: the 16 lanes of a block point at the 16 groups of
 // four columns of four rows (lane 4r + c: row r, columns 4c .. 4c + 3), lane i
 // gets column i.
-__device__ __forceinline__ uint2 read_column4(const uint16_t* p) {
-    const s16x4 v =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)const_cast<uint16_t*>(p));
+using lds_bytes = __attribute__((address_space(3))) const char*;
+__device__ __forceinline__ uint2 read_column4(lds_bytes p) {
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
     return __builtin_bit_cast(uint2, v);
 }
+__device__ __forceinline__ uint4 read_row8(lds_bytes p) {
+    const u32x4 v = *(__attribute__((address_space(3))) const u32x4*)p;
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
 
-template <int TYPE, int OUT, int D>
-__global__ void __launch_bounds__(64 * kWaves) attn_prefill_kernel(PrefillArgs a) {
-    constexpr int NK = D / 16, ND = D / 32, CH = D / 8;          // k-steps, column tiles, 16-byte pieces of a row
-    __shared__ __attribute__((aligned(16))) uint16_t sk[kKeys * D], sv[kKeys * D];
+// Asynchronous copy of a tile of kKeys rows (`rows` of them present, the others
+// become zeros) to LDS, 16 bytes a lane and step, swizzled on the way.
+template <int D, int WAVES>
+__device__ __forceinline__ void stage(const uint16_t* src, int64_t ld, int rows, uint16_t* tile) {
+    constexpr int CH = D / 8, kSteps = kKeys * CH / (64 * WAVES);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t bytes = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * ld + D) * 2) : 0u;
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(src, bytes);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const int first = (i * WAVES + wave) * 64;
+        const int at = first + lane, row = at / CH, piece = (at % CH) ^ swizzle<CH>(row);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + first * 8), 16,
+                                                 (int)(row * (uint32_t)(ld * 2) + piece * 16), 0, 0, 0);
+    }
+}
+
+template <int TYPE, int OUT, int D, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_kernel(PrefillArgs a) {
+    constexpr int NK = D / 16, ND = D / 32, CH = D / 8;          // k-steps, column tiles, 16-byte pieces of a row
+    constexpr int kRows = 32 * WAVES;
+    // Two buffers of a K and a V tile, used in turn. Objects of their own and a
+    // step's code for each, so that the compiler sees that a read of one need
+    // not wait for the copies into the other.
+    constexpr int kTile = kKeys * D;
+    __shared__ __attribute__((aligned(16))) uint16_t lk0[kTile], lv0[kTile], lk1[kTile], lv1[kTile];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 31, h = lane >> 5;
     int64_t id = blockIdx.x;
-    const int head = (int)(id % a.q_heads);
+    // neighbouring workgroups go to different XCDs: give each its own key head
+    const int hr = (int)(id % a.q_heads);
+    const int kvh = (int)(hr % a.kv_heads);
+    const int head = (int)(kvh * (a.q_heads / a.kv_heads) + hr / a.kv_heads);
     id /= a.q_heads;
     const int seq = (int)(id % a.seqs);
     const int64_t qb = a.q_blocks - 1 - id / a.seqs;             // the longest rows first
     const int64_t q0 = a.cu_q[seq], k0 = a.cu_k[seq];
     const int64_t nq = a.cu_q[seq + 1] - q0, nk = a.cu_k[seq + 1] - k0;
     if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k || qb * kRows >= nq) return;
-    const int64_t past = nk - nq;
-    const int64_t i0 = qb * kRows + 32 * wave;                   // the wave's first query
-    const int64_t qi = i0 + ln;                                  // the lane's
-    int64_t end = nk;                                            // keys that the workgroup needs
+    const int past = (int)(nk - nq);
+    const int i0 = (int)qb * kRows + 32 * wave;                  // the wave's first query
+    const int qi = i0 + ln;                                      // the lane's
+    int end = (int)nk;                                           // keys that the workgroup needs
     if (a.causal) {
         const int64_t e = (qb + 1) * kRows + past;
-        end = e < nk ? e : nk;
+        end = (int)(e < nk ? e : nk);
     }
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + (q0 + (qi < nq ? qi : nq - 1)) * a.ld_q + head * a.hs_q;
-    const int64_t kvh = head / (a.q_heads / a.kv_heads);
     const uint16_t* kp = static_cast<const uint16_t*>(a.k) + k0 * a.ld_k + kvh * a.hs_k;
     const uint16_t* vp = static_cast<const uint16_t*>(a.v) + k0 * a.ld_v + kvh * a.hs_v;
 
@@ -104,23 +139,33 @@ __global__ void __launch_bounds__(64 * kWaves) attn_prefill_kernel(PrefillArgs a
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = -__builtin_inff(), l = 0.f;
+    float m = -__builtin_inff(), nref = 0.f, l = 0.f;            // reference, minus it (0 while there is none), sum
     const float c = a.scale * 1.4426950408889634f;
+    const int lim = a.causal && qi + past < nk - 1 ? qi + past : (int)nk - 1;    // the lane's last key
 
-    for (int64_t kt = 0; kt < end; kt += kKeys) {
-        __syncthreads();
-        for (int at = threadIdx.x; at < kKeys * CH; at += 64 * kWaves) {
-            const int r = at / CH, p = at % CH;
-            const bool on = kt + r < nk;                         // rows past the sequence are zeros
-            const uint4 z = make_uint4(0, 0, 0, 0);
-            const int to = r * D + 8 * (p ^ (r & (CH - 1)));
-            *reinterpret_cast<uint4*>(sk + to) = on ? *reinterpret_cast<const uint4*>(kp + (kt + r) * a.ld_k + 8 * p) : z;
-            *reinterpret_cast<uint4*>(sv + to) = on ? *reinterpret_cast<const uint4*>(vp + (kt + r) * a.ld_v + 8 * p) : z;
+    // The lane's places in a tile. K: row ln, piece h; the other pieces are an
+    // exclusive-or away, the other rows a constant. V: keys 4h + (lane % 16) / 4
+    // and 8 further, columns 4 (lane % 4) and 16 for odd blocks of lanes.
+    const int r4 = (lane & 15) >> 2, x4 = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    const int kat = ln * D * 2 + 16 * (h ^ swizzle<CH>(ln));
+    const int vat0 = (4 * h + r4) * D * 2 + 16 * (x4 ^ swizzle<CH>(4 * h + r4)) + 8 * (lane & 1);
+    const int vat1 = (4 * h + r4 + 8) * D * 2 + 16 * (x4 ^ swizzle<CH>(4 * h + r4 + 8)) + 8 * (lane & 1);
+
+    if (end > 0) {
+        stage<D, WAVES>(kp, a.ld_k, (int)nk, lk0);
+        stage<D, WAVES>(vp, a.ld_v, (int)nk, lv0);
+    }
+    auto step = [&](int kt, uint16_t* ck, uint16_t* cv, uint16_t* tk, uint16_t* tv) __attribute__((always_inline)) {
+        // this tile is there, and everyone is done with the other buffer
+        __builtin_amdgcn_s_waitcnt(0x0F70);                      // vmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        const lds_bytes sk = (lds_bytes)ck, sv = (lds_bytes)cv;
+        if (kt + kKeys < end) {
+            const int left = (int)nk - kt - kKeys;
+            stage<D, WAVES>(kp + (int64_t)(kt + kKeys) * a.ld_k, a.ld_k, left < kKeys ? left : kKeys, tk);
+            stage<D, WAVES>(vp + (int64_t)(kt + kKeys) * a.ld_v, a.ld_v, left < kKeys ? left : kKeys, tv);
         }
-        __syncthreads();
-        const int64_t limit = a.causal ? qi + past : nk - 1;     // the lane's last key
-        const int64_t lim = limit < nk - 1 ? limit : nk - 1;
-        if (a.causal && kt > i0 + 31 + past) continue;           // nothing here for the wave
+        if (a.causal && kt > i0 + 31 + past) return;             // nothing here for the wave
         const bool masked = kt + kKeys > nk || (a.causal && kt + kKeys - 1 > i0 + past);
         f32x16 st[2];
 #pragma unroll
@@ -129,79 +174,97 @@ __global__ void __launch_bounds__(64 * kWaves) attn_prefill_kernel(PrefillArgs a
             for (int i = 0; i < 16; ++i) st[t][i] = 0.f;
 #pragma unroll
             for (int s = 0; s < NK; ++s) {
-                const int r = 32 * t + ln;
-                const uint4 kf = *reinterpret_cast<const uint4*>(sk + r * D + 8 * ((2 * s + h) ^ (r & (CH - 1))));
-                st[t] = mfma<TYPE>(kf, qf[s], st[t]);
+                st[t] = mfma<TYPE>(read_row8(sk + (kat ^ (32 * s)) + 32 * t * D * 2), qf[s], st[t]);
             }
         }
+        bool special = false;
         if (masked) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (kt + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > lim) st[t][i] = -__builtin_inff();
+            // values that a zero weight would not take out
+            uint32_t any = 0;
+            for (int at = lane; at < kKeys * CH; at += 64) {
+                const uint4 w = read_row8(sv + 16 * at);
+                any |= specials<TYPE>(w.x) | specials<TYPE>(w.y) | specials<TYPE>(w.z) | specials<TYPE>(w.w);
+            }
+            special = __builtin_amdgcn_ballot_w64(any != 0) != 0;
         }
         float top = st[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, st[t][i]);
-        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-        const float mn = __builtin_fmaxf(m, top * c);
-        const float ref = mn == -__builtin_inff() ? 0.f : mn;
-        const float keep = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        l *= keep;
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * c;
+        // the reference follows the maximum only when it is 2^8 behind: sums
+        // and weights have the room, and the rescaling is rare
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
+            const float mn = __builtin_fmaxf(m, top);
+            const float keep = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            nref = mn == -__builtin_inff() ? 0.f : -mn;
+            l *= keep;
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= keep;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                st[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][i], c, -ref));
-                l += st[t][i];
-            }
+                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+        }
+        uint4 pf[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const f32x16& p = st[s >> 1];
-            const int b = 8 * (s & 1);
-            uint4 pf;
-            pf.x = pack2<TYPE>(p[b + 0], p[b + 1]);
-            pf.y = pack2<TYPE>(p[b + 2], p[b + 3]);
-            pf.z = pack2<TYPE>(p[b + 4], p[b + 5]);
-            pf.w = pack2<TYPE>(p[b + 6], p[b + 7]);
-            const int key = 16 * s + 4 * h + ((lane & 15) >> 2);
+            float p[8];
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const int col = 32 * d + (lane & 16) + 4 * (lane & 3);
-                const uint2 lo = read_column4(sv + key * D + 8 * ((col / 8) ^ (key & (CH - 1))) + (col & 7));
-                const uint2 hi = read_column4(sv + (key + 8) * D + 8 * ((col / 8) ^ ((key + 8) & (CH - 1))) + (col & 7));
-                const uint4 vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                if (masked && __builtin_amdgcn_ballot_w64(any_special<TYPE>(vf))) {
-                    // an inf or NaN among these values: keys that the mask takes must not meet it
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + e], c, nref));
+                l += p[e];
+            }
+            pf[s] = make_uint4(pack2<TYPE>(p[0], p[1]), pack2<TYPE>(p[2], p[3]), pack2<TYPE>(p[4], p[5]),
+                               pack2<TYPE>(p[6], p[7]));
+        }
+        auto products = [&](auto clean) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        // key 16 s + e is element e of the step: held by the half (e >> 2) & 1
-                        const float mine = p[b + (e & 3) + 4 * (e >> 3)];
-                        const float other = __shfl_xor(mine, 32);
-                        const float w = ((e >> 2) & 1) == h ? mine : other;
-                        const int kr = 16 * s + e;
-                        if (kt + kr <= lim) {
+            for (int s = 0; s < 4; ++s) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int cc = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
-                                const uint16_t vb = sv[kr * D + 8 * ((cc / 8) ^ (kr & (CH - 1))) + (cc & 7)];
-                                o[d][i] = __builtin_fmaf(w, widen<TYPE>(vb), o[d][i]);
-                            }
-                        }
-                    }
-                } else {
-                    o[d] = mfma<TYPE>(vf, pf, o[d]);
+                for (int d = 0; d < ND; ++d) {
+                    const uint2 lo = read_column4(sv + (vat0 ^ (64 * d)) + 16 * s * D * 2);
+                    const uint2 hi = read_column4(sv + (vat1 ^ (64 * d)) + 16 * s * D * 2);
+                    uint4 vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    if constexpr (decltype(clean)::value)
+                        vf = make_uint4(vf.x & ~specials<TYPE>(vf.x), vf.y & ~specials<TYPE>(vf.y),
+                                        vf.z & ~specials<TYPE>(vf.z), vf.w & ~specials<TYPE>(vf.w));
+                    o[d] = mfma<TYPE>(vf, pf[s], o[d]);
                 }
             }
+        };
+        if (!special) {
+            products(Int<0>{});
+        } else {
+            // an inf or a NaN among the values: out of the product, and to
+            // the queries that see its key as it is (every weight is positive)
+            products(Int<1>{});
+            for (int kr = 0; kr < kKeys; ++kr) {
+                const int row = kr * D * 2 + 8 * h, turned = 16 * swizzle<CH>(kr);
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        // four columns 32 d + 2 i + 4 h
+                        const u32x2 w = *(__attribute__((address_space(3))) const u32x2*)(sv + row + ((64 * d + 4 * i) ^ turned));
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t b = w[e >> 1] >> (16 * (e & 1)) & 0xFFFFu;
+                            if (kt + kr <= lim && (specials<TYPE>(b) & 0xFFFFu)) o[d][i + e] += widen<TYPE>((uint16_t)b);
+                        }
+                    }
+            }
         }
+    };
+    for (int kt = 0; kt < end; kt += 2 * kKeys) {
+        step(kt, lk0, lv0, lk1, lv1);
+        if (kt + kKeys < end) step(kt + kKeys, lk1, lv1, lk0, lv0);
     }
     l += __shfl_xor(l, 32);
     if (qi >= nq) return;
@@ -214,27 +277,32 @@ __global__ void __launch_bounds__(64 * kWaves) attn_prefill_kernel(PrefillArgs a
         for (int i = 0; i < 16; ++i) out[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)] = O::one(l == 0.f ? 0.f : o[d][i] * inv);
 }
 
+template <int TYPE, int OUT, int D, int WAVES>
+hipError_t launch_one(PrefillArgs a, hipStream_t stream) {
+    a.q_blocks = (a.max_q + 32 * WAVES - 1) / (32 * WAVES);
+    attn_prefill_kernel<TYPE, OUT, D, WAVES><<<(unsigned)(a.q_blocks * a.seqs * a.q_heads), 64 * WAVES, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
 template <int TYPE, int OUT>
-hipError_t launch_typed(const PrefillArgs& a, unsigned grid, hipStream_t stream) {
+hipError_t launch_typed(const PrefillArgs& a, hipStream_t stream) {
+    const bool wide = a.max_q > 1024;
     switch (a.head_dim) {
-        case 64: attn_prefill_kernel<TYPE, OUT, 64><<<grid, 64 * kWaves, 0, stream>>>(a); break;
-        case 128: attn_prefill_kernel<TYPE, OUT, 128><<<grid, 64 * kWaves, 0, stream>>>(a); break;
-        case 256: attn_prefill_kernel<TYPE, OUT, 256><<<grid, 64 * kWaves, 0, stream>>>(a); break;
+        case 64: return wide ? launch_one<TYPE, OUT, 64, 8>(a, stream) : launch_one<TYPE, OUT, 64, 4>(a, stream);
+        case 128: return wide ? launch_one<TYPE, OUT, 128, 8>(a, stream) : launch_one<TYPE, OUT, 128, 4>(a, stream);
+        case 256: return launch_one<TYPE, OUT, 256, 4>(a, stream);
         default: return hipErrorInvalidValue;
     }
-    return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_attn_prefill(PrefillArgs a, hipStream_t stream) {
-    a.q_blocks = (a.max_q + kRows - 1) / kRows;
-    const unsigned grid = (unsigned)(a.q_blocks * a.seqs * a.q_heads);
     if (a.type == kTypeBF16)
-        return a.out_type == kTypeF32 ? launch_typed<kTypeBF16, kTypeF32>(a, grid, stream)
-                                      : launch_typed<kTypeBF16, kTypeBF16>(a, grid, stream);
-    return a.out_type == kTypeF32 ? launch_typed<kTypeF16, kTypeF32>(a, grid, stream)
-                                  : launch_typed<kTypeF16, kTypeF16>(a, grid, stream);
+        return a.out_type == kTypeF32 ? launch_typed<kTypeBF16, kTypeF32>(a, stream)
+                                      : launch_typed<kTypeBF16, kTypeBF16>(a, stream);
+    return a.out_type == kTypeF32 ? launch_typed<kTypeF16, kTypeF32>(a, stream)
+                                  : launch_typed<kTypeF16, kTypeF16>(a, stream);
 }
 
 }  // namespace frq
