@@ -23,6 +23,8 @@ namespace {
 
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
 using s16x4 = short __attribute__((ext_vector_type(4)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
@@ -42,7 +44,30 @@ __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
 
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    return (uint32_t)Val<TYPE>::one(a) | ((uint32_t)Val<TYPE>::one(b) << 16);
+    if constexpr (TYPE == kTypeBF16) {
+        const bf16x2 v = {(__bf16)a, (__bf16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    } else {
+        const f16x2 v = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+}
+
+// The larger of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float half_max(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_fmaxf(__builtin_bit_cast(float, r[0]), __builtin_bit_cast(float, r[1]));
+}
+
+// acc + both halves of a pair of weights, as they are rounded.
+template <int TYPE>
+__device__ __forceinline__ float add_pair(uint32_t w, float acc) {
+    if constexpr (TYPE == kTypeBF16) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), (bf16x2){(__bf16)1.f, (__bf16)1.f}, acc, false);
+    } else {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), (f16x2){(_Float16)1.f, (_Float16)1.f}, acc, false);
+    }
 }
 
 // The halves of w that are an inf or a NaN, as a mask of ones.
@@ -105,6 +130,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     // step's code for each, so that the compiler sees that a read of one need
     // not wait for the copies into the other.
     constexpr int kTile = kKeys * D;
+    __shared__ int special_at;
     __shared__ __attribute__((aligned(16))) uint16_t lk0[kTile], lv0[kTile], lk1[kTile], lv1[kTile];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 31, h = lane >> 5;
@@ -151,13 +177,14 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     const int vat0 = (4 * h + r4) * D * 2 + 16 * (x4 ^ swizzle<CH>(4 * h + r4)) + 8 * (lane & 1);
     const int vat1 = (4 * h + r4 + 8) * D * 2 + 16 * (x4 ^ swizzle<CH>(4 * h + r4 + 8)) + 8 * (lane & 1);
 
+    if (threadIdx.x == 0) special_at = 0;
     if (end > 0) {
         stage<D, WAVES>(kp, a.ld_k, (int)nk, lk0);
         stage<D, WAVES>(vp, a.ld_v, (int)nk, lv0);
     }
     auto step = [&](int kt, uint16_t* ck, uint16_t* cv, uint16_t* tk, uint16_t* tv) __attribute__((always_inline)) {
         // this tile is there, and everyone is done with the other buffer
-        __builtin_amdgcn_s_waitcnt(0x0F70);                      // vmcnt(0)
+        __builtin_amdgcn_s_waitcnt(0x0070);                      // vmcnt(0), lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         const lds_bytes sk = (lds_bytes)ck, sv = (lds_bytes)cv;
         if (kt + kKeys < end) {
@@ -165,39 +192,56 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
             stage<D, WAVES>(kp + (int64_t)(kt + kKeys) * a.ld_k, a.ld_k, left < kKeys ? left : kKeys, tk);
             stage<D, WAVES>(vp + (int64_t)(kt + kKeys) * a.ld_v, a.ld_v, left < kKeys ? left : kKeys, tv);
         }
+        // A zero weight does not take an inf or a NaN out of a product: where
+        // the mask cuts through the tile, such values leave it and are added
+        // below for the queries that see their keys.
+        const bool cut = a.causal && kt + kKeys - 1 > (int)qb * kRows + past;
+        if (cut) {
+            bool any = false;
+            for (int at = threadIdx.x; at < kKeys * CH; at += 64 * WAVES) {
+                u32x4 w = reinterpret_cast<const u32x4*>(cv)[at];
+                const u32x4 s = {specials<TYPE>(w[0]), specials<TYPE>(w[1]), specials<TYPE>(w[2]), specials<TYPE>(w[3])};
+                if (s[0] | s[1] | s[2] | s[3]) {
+                    any = true;
+                    reinterpret_cast<u32x4*>(cv)[at] = w & ~s;
+                }
+            }
+            if (any) special_at = kt + 1;
+            __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+        }
         if (a.causal && kt > i0 + 31 + past) return;             // nothing here for the wave
         const bool masked = kt + kKeys > nk || (a.causal && kt + kKeys - 1 > i0 + past);
         f32x16 st[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st[t][i] = 0.f;
+        for (int s = 0; s < NK; ++s)
 #pragma unroll
-            for (int s = 0; s < NK; ++s) {
+            for (int t = 0; t < 2; ++t)
                 st[t] = mfma<TYPE>(read_row8(sk + (kat ^ (32 * s)) + 32 * t * D * 2), qf[s], st[t]);
-            }
+        // four reads ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int s = 0; s < 2 * NK - 4; ++s) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        bool special = false;
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         if (masked) {
+            const int left = lim - kt - 4 * h;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (kt + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > lim) st[t][i] = -__builtin_inff();
-            // values that a zero weight would not take out
-            uint32_t any = 0;
-            for (int at = lane; at < kKeys * CH; at += 64) {
-                const uint4 w = read_row8(sv + 16 * at);
-                any |= specials<TYPE>(w.x) | specials<TYPE>(w.y) | specials<TYPE>(w.z) | specials<TYPE>(w.w);
-            }
-            special = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+                    if (32 * t + 8 * (i >> 2) + (i & 3) > left) st[t][i] = -__builtin_inff();
         }
         float top = st[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, st[t][i]);
-        top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * c;
+        top = half_max(top) * c;
         // the reference follows the maximum only when it is 2^8 behind: sums
         // and weights have the room, and the rescaling is rare
         if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
@@ -216,48 +260,33 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         for (int s = 0; s < 4; ++s) {
             float p[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 8; ++e)
                 p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + e], c, nref));
-                l += p[e];
-            }
             pf[s] = make_uint4(pack2<TYPE>(p[0], p[1]), pack2<TYPE>(p[2], p[3]), pack2<TYPE>(p[4], p[5]),
                                pack2<TYPE>(p[6], p[7]));
+            l = add_pair<TYPE>(pf[s].x, l);
+            l = add_pair<TYPE>(pf[s].y, l);
+            l = add_pair<TYPE>(pf[s].z, l);
+            l = add_pair<TYPE>(pf[s].w, l);
         }
-        auto products = [&](auto clean) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
+        for (int s = 0; s < 4; ++s) {
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const uint2 lo = read_column4(sv + (vat0 ^ (64 * d)) + 16 * s * D * 2);
-                    const uint2 hi = read_column4(sv + (vat1 ^ (64 * d)) + 16 * s * D * 2);
-                    uint4 vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                    if constexpr (decltype(clean)::value)
-                        vf = make_uint4(vf.x & ~specials<TYPE>(vf.x), vf.y & ~specials<TYPE>(vf.y),
-                                        vf.z & ~specials<TYPE>(vf.z), vf.w & ~specials<TYPE>(vf.w));
-                    o[d] = mfma<TYPE>(vf, pf[s], o[d]);
-                }
+            for (int d = 0; d < ND; ++d) {
+                const uint2 lo = read_column4(sv + (vat0 ^ (64 * d)) + 16 * s * D * 2);
+                const uint2 hi = read_column4(sv + (vat1 ^ (64 * d)) + 16 * s * D * 2);
+                o[d] = mfma<TYPE>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[s], o[d]);
             }
-        };
-        if (!special) {
-            products(Int<0>{});
-        } else {
-            // an inf or a NaN among the values: out of the product, and to
-            // the queries that see its key as it is (every weight is positive)
-            products(Int<1>{});
-            for (int kr = 0; kr < kKeys; ++kr) {
-                const int row = kr * D * 2 + 8 * h, turned = 16 * swizzle<CH>(kr);
+        }
+        if (cut && special_at == kt + 1) {
+            for (int kr = 0; kr < kKeys && kt + kr < nk; ++kr) {
+                const uint16_t* row = vp + (int64_t)(kt + kr) * a.ld_v + 4 * h;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        // four columns 32 d + 2 i + 4 h
-                        const u32x2 w = *(__attribute__((address_space(3))) const u32x2*)(sv + row + ((64 * d + 4 * i) ^ turned));
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t b = w[e >> 1] >> (16 * (e & 1)) & 0xFFFFu;
-                            if (kt + kr <= lim && (specials<TYPE>(b) & 0xFFFFu)) o[d][i + e] += widen<TYPE>((uint16_t)b);
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const uint16_t b = row[32 * d + 8 * (i >> 2) + (i & 3)];
+                        if (kt + kr <= lim && (specials<TYPE>(b) & 0xFFFFu)) o[d][i] += widen<TYPE>(b);
                     }
             }
         }
