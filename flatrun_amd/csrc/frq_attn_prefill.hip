@@ -134,14 +134,15 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     __shared__ __attribute__((aligned(16))) uint16_t lk0[kTile], lv0[kTile], lk1[kTile], lv1[kTile];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 31, h = lane >> 5;
-    int64_t id = blockIdx.x;
     // neighbouring workgroups go to different XCDs: give each its own key head
-    const int hr = (int)(id % a.q_heads);
-    const int kvh = (int)(hr % a.kv_heads);
-    const int head = (int)(kvh * (a.q_heads / a.kv_heads) + hr / a.kv_heads);
-    id /= a.q_heads;
-    const int seq = (int)(id % a.seqs);
-    const int64_t qb = a.q_blocks - 1 - id / a.seqs;             // the longest rows first
+    uint32_t id = blockIdx.x;
+    const uint32_t hr = id % (uint32_t)a.q_heads;
+    const int kvh = (int)(hr % (uint32_t)a.kv_heads);
+    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
+    const int head = kvh * group + (int)(hr / (uint32_t)a.kv_heads);
+    id /= (uint32_t)a.q_heads;
+    const int seq = (int)(id % (uint32_t)a.seqs);
+    const int64_t qb = a.q_blocks - 1 - id / (uint32_t)a.seqs;   // the longest rows first
     const int64_t q0 = a.cu_q[seq], k0 = a.cu_k[seq];
     const int64_t nq = a.cu_q[seq + 1] - q0, nk = a.cu_k[seq + 1] - k0;
     if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k || qb * kRows >= nq) return;
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         }
         if (a.causal && kt > i0 + 31 + past) return;             // nothing here for the wave
         const bool masked = kt + kKeys > nk || (a.causal && kt + kKeys - 1 > i0 + past);
+        __builtin_amdgcn_s_setprio(1);                           // a wave at its products goes first
         f32x16 st[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.f;
@@ -228,6 +230,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        __builtin_amdgcn_s_setprio(0);
         if (masked) {
             const int left = lim - kt - 4 * h;
 #pragma unroll
@@ -281,12 +284,18 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         if (cut && special_at == kt + 1) {
             for (int kr = 0; kr < kKeys && kt + kr < nk; ++kr) {
                 const uint16_t* row = vp + (int64_t)(kt + kr) * a.ld_v + 4 * h;
+                const bool seen = kt + kr <= lim;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint16_t b = row[32 * d + 8 * (i >> 2) + (i & 3)];
-                        if (kt + kr <= lim && (specials<TYPE>(b) & 0xFFFFu)) o[d][i] += widen<TYPE>(b);
+                    for (int i = 0; i < 16; i += 4) {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(row + 32 * d + 2 * i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t b = w[e >> 1] >> (16 * (e & 1)) & 0xFFFFu;
+                            if (seen && (specials<TYPE>(b) & 0xFFFFu)) o[d][i + e] += widen<TYPE>((uint16_t)b);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
             }
         }
@@ -303,7 +312,16 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) out[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)] = O::one(l == 0.f ? 0.f : o[d][i] * inv);
+        for (int i = 0; i < 16; i += 4) {                        // columns 32 d + 2 i + 4 h and the next three
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = l == 0.f ? 0.f : o[d][i + e] * inv;
+            if constexpr (OUT == kTypeF32)
+                *reinterpret_cast<float4*>(out + 32 * d + 2 * i + 4 * h) = make_float4(x[0], x[1], x[2], x[3]);
+            else
+                *reinterpret_cast<uint2*>(out + 32 * d + 2 * i + 4 * h) =
+                    make_uint2(pack2<OUT>(x[0], x[1]), pack2<OUT>(x[2], x[3]));
+        }
 }
 
 template <int TYPE, int OUT, int D, int WAVES>
@@ -315,7 +333,10 @@ hipError_t launch_one(PrefillArgs a, hipStream_t stream) {
 
 template <int TYPE, int OUT>
 hipError_t launch_typed(const PrefillArgs& a, hipStream_t stream) {
-    const bool wide = a.max_q > 1024;
+#ifndef WIDE
+#define WIDE 2048
+#endif
+    const bool wide = a.max_q > WIDE;
     switch (a.head_dim) {
         case 64: return wide ? launch_one<TYPE, OUT, 64, 8>(a, stream) : launch_one<TYPE, OUT, 64, 4>(a, stream);
         case 128: return wide ? launch_one<TYPE, OUT, 128, 8>(a, stream) : launch_one<TYPE, OUT, 128, 4>(a, stream);
