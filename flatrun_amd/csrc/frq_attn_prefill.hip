@@ -57,7 +57,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ float half_max(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x);
     const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return __builtin_fmaxf(__builtin_bit_cast(float, r[0]), __builtin_bit_cast(float, r[1]));
+    const uint32_t low = r[0], high = r[1];
+    return __builtin_fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
 }
 
 // acc + both halves of a pair of weights, as they are rounded.

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvArgs a) {
     const KvAt at = kv_at(a, slot, h, NG);
     const int g = sub >> 2, j = sub & 3;
     if ((sub & 3) == 0)
-        *reinterpret_cast<uint16_t*>(at.tile + (is_v ? kv_vs_off(NG) : kv_ks_off(NG)) + (at.t * NG + g) * 2) =
+        *reinterpret_cast<uint16_t*>(at.tile + (is_v ? kv_vs_off(NG) : kv_ks_off(NG)) + kv_scale(at.t, g, NG)) =
             (uint16_t)scale;
     if (!is_v) {
         uint32_t w = 0;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvArgs a) {
         const KvAt at = kv_at(a, slot, h, NG);
         const int g = sub >> 2, j = sub & 3, u = at.t >> 4;
         const float d = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(
-            at.tile + (is_v ? kv_vs_off(NG) : kv_ks_off(NG)) + (at.t * NG + g) * 2));
+            at.tile + (is_v ? kv_vs_off(NG) : kv_ks_off(NG)) + kv_scale(at.t, g, NG)));
         if (!is_v) {
             const uint32_t w = *reinterpret_cast<const uint32_t*>(at.tile + kv_word(u * NG + g, 16 * j + (at.t & 15)));
 #pragma unroll
