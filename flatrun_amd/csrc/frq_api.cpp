@@ -1271,7 +1271,9 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
     if (int rc = kv4_checks("attn_decode", cache, cache_bytes, pages, page_tokens, kv_heads, head_dim)) return rc;
     if (!in_range(batch, 0, (int64_t)1 << 20) || !in_range(q_heads, 1, kMaxHeads) || q_heads % kv_heads)
         return fail(FRQ_ERR_SHAPE, "attn_decode: q_heads must be a multiple of kv_heads, the batch up to 2^20");
-    if (!in_range(max_len, 0, kMaxTokens - 64) || !in_range(ld_table, (max_len + page_tokens - 1) / page_tokens, kMaxLd))
+    if (!in_range(max_len, 0, (int64_t)1 << 29))
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_decode: max_len beyond 2^29");
+    if (!in_range(ld_table, (max_len + page_tokens - 1) / page_tokens, kMaxLd))
         return fail(FRQ_ERR_SHAPE, "attn_decode: a row of the page table is shorter than max_len");
     if (!in_range(ld_q, q_heads * head_dim, kMaxLd) || !in_range(ld_out, q_heads * head_dim, kMaxLd))
         return fail(FRQ_ERR_SHAPE, "attn_decode: a row stride is shorter than its heads");
@@ -1282,8 +1284,9 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
         ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(lens)) & 3))
         return fail(FRQ_ERR_ALIGN, "attn_decode: q and out rows must be 16-byte aligned, table and lens 4-byte");
     frq::DecodeArgs a{type,  q,        ld_q, cache,   pages, page_tokens, kv_heads, head_dim, table, ld_table, lens,
-                      max_len, out,    ld_out, batch, q_heads, scale,     0,        0,        nullptr, nullptr};
-    frq::plan_attn_decode(&a);
+                      max_len, out,    ld_out, batch, q_heads, scale,     0,        0,        nullptr};
+    if (!frq::plan_attn_decode(&a))
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_decode: batch, heads and max_len together beyond 2^31 tiles of 32 tokens");
     hipStream_t s = static_cast<hipStream_t>(stream);
     float* part;
     uint32_t* cnt;

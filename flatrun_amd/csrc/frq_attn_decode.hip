@@ -9,8 +9,8 @@
 // the rest, 22 bits together). q is put under a power of two per head that
 // brings its largest element to [2^13, 2^14), so that the rest stays a normal
 // number. A block of K has its scale on the product of one instruction; the
-// scale of V goes into the weights, which stand under 2^(6 - E) with E the
-// exponent of the largest |scale| seen, so that tiny and huge values keep
+// scale of V goes into the weights, which stand under 2^(4 - E), 2^E four times
+// the largest |scale| of the first tile, so that tiny and huge values keep
 // their bits: out = sum / sum, the power cancels.
 //
 // A wave takes 32 tokens a step. S = q K^T gives a lane one token of each half
@@ -21,8 +21,11 @@
 // 2^8 ahead, so sums are rarely rescaled and the maximum over lanes is rarely
 // taken. The next step's tile is loaded while this one is worked on.
 //
-// Each wave walks its own tiles; the waves of a workgroup meet in LDS at the
-// end, and a sequence split over workgroups in a second, small kernel.
+// The tiles of all sequences and key heads, one after another, are shared out
+// evenly over the workgroups, whatever the lengths are; the four waves of a
+// workgroup take its tiles in turn and meet in LDS. A row that several
+// workgroups worked on is joined, in their order, by a second, small kernel.
+// Short sequences have one workgroup per sequence and key head, and no joining.
 #include "frq_kernels.h"
 #include "frq_kv4.h"
 
@@ -34,6 +37,10 @@ using half8v = _Float16 __attribute__((ext_vector_type(8)));
 using float4v = float __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
+constexpr int kPad = 16;               // see Line
+constexpr int kShareMin = 8;           // places of a workgroup, two tiles for each wave
+constexpr int kWhole = 8;              // tiles up to which a workgroup takes all of a pair
+constexpr int kGroups = 512;           // two workgroups of 33 KiB and 183 registers a lane on each of 256 CUs
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
@@ -64,307 +71,452 @@ __device__ __forceinline__ float row_max(float x) {
     return x;
 }
 
-// A tile as a lane holds it.
+// Codes and scales of a tile as a lane holds them: words p of the codes, and
+// of the scales words u NG/2 + g/2.
 template <int NG>
-struct Tile {
-    uint32_t kw[2 * NG], vw[2 * NG], ks[NG], vs[NG];     // ks, vs: words u NG/2 + g/2
-    __device__ __forceinline__ void load(const uint8_t* t, int lane) {
+struct Half {
+    uint32_t code[2 * NG], scale[NG];
+    __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales, int lane) {
 #pragma unroll
         for (int p = 0; p < 2 * NG; p += 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(t + kv_word(p, lane));
-            const uint4 y = *reinterpret_cast<const uint4*>(t + kv_vc_off(NG) + kv_word(p, lane));
-            kw[p] = x.x; kw[p + 1] = x.y; kw[p + 2] = x.z; kw[p + 3] = x.w;
-            vw[p] = y.x; vw[p + 1] = y.y; vw[p + 2] = y.z; vw[p + 3] = y.w;
+            const uint4 x = *reinterpret_cast<const uint4*>(codes + kv_word(p, lane));
+            code[p] = x.x; code[p + 1] = x.y; code[p + 2] = x.z; code[p + 3] = x.w;
         }
-        const uint8_t* k = t + kv_ks_off(NG) + kv_scale(lane & 15, 0, NG);
-        const uint8_t* v = t + kv_vs_off(NG) + kv_scale(lane & 15, 0, NG);
+        scales += kv_scale(lane & 15, 0, NG);
 #pragma unroll
         for (int p = 0; p < NG; p += 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(k + 4 * p), y = *reinterpret_cast<const uint2*>(v + 4 * p);
-            ks[p] = x.x; ks[p + 1] = x.y;
-            vs[p] = y.x; vs[p + 1] = y.y;
+            const uint2 x = *reinterpret_cast<const uint2*>(scales + 4 * p);
+            scale[p] = x.x; scale[p + 1] = x.y;
         }
     }
+    __device__ __forceinline__ _Float16 scale_of(int u, int g) const {
+        const int at = u * NG + g;
+        return half_of(scale[at / 2], at & 1);
+    }
 };
-
 using lds_bytes = __attribute__((address_space(3))) char*;
 using short4v = short __attribute__((ext_vector_type(4)));
 using uint2v = uint32_t __attribute__((ext_vector_type(2)));
+
+// Lengths and pages do not change under the kernel: read through the constant
+// address space, so that uniform reads are scalar ones, which neither wait for
+// the tiles that are on their way nor make what follows a vector value.
+using const_ints = const __attribute__((address_space(4))) int32_t*;
+__device__ __forceinline__ const_ints constant(const int32_t* p) { return (const_ints)(uintptr_t)p; }
+
+// The length that counts: 0 for none, -1 for one that is not what the caller
+// said (longer than max_len, or no cache to hold it), whose row is NaN.
+__device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
+    const int len = constant(a.lens)[b];
+    return len <= 0 ? 0 : len > a.max_len || a.pages == 0 ? -1 : len;
+}
+__device__ __forceinline__ int tiles_in(int len) { return len > 0 ? (int)((uint32_t)(len + kKvTile - 1) / kKvTile) : 0; }
+
+__device__ __forceinline__ int places_in(int len) { return len > 0 ? tiles_in(len) + kPad : 0; }
+
+// x summed over the lanes up to and with this one.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // within rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row 0 into 1, 2 into 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // rows 0, 1 into 2, 3
+    return x;
+}
+
+// What every workgroup works out of the lengths. The pairs (a key head, eight
+// query heads) of all sequences stand in one line, a sequence's side by side,
+// each as many places long as it has tiles and kPad more at its front: what
+// starting and ending a pair costs in tiles' time (64 sequences of 1 .. 8192
+// tokens, 8 key heads: 117 us without, 93 with 8, 87 with 16 or 24). The lengths
+// of 64 sequences at a time are in the lanes. The host keeps the whole line below 2^31.
+struct Line {
+    int total, share;   // places of all, and of a workgroup
+    int from;           // the sequence of lane 0
+    int len, upto;      // the lane's length, and the places of a pair up to its end from `from` on
+    __device__ __forceinline__ void read(const DecodeArgs& a, int at, int lane) {
+        from = at;
+        len = at + lane < a.batch ? length_of(a, at + lane) : 0;
+        upto = wave_scan(places_in(len));
+    }
+    __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ int before(int k) const { return k ? __builtin_amdgcn_readlane(upto, k - 1) : 0; }
+    __device__ __forceinline__ void open(const DecodeArgs& a, int pairs, int lane) {
+        read(a, 0, lane);
+        int sum = all();
+        for (int at = 64; at < a.batch; at += 64) {
+            read(a, at, lane);
+            sum += all();
+        }
+        if (a.batch > 64) read(a, 0, lane);
+        total = sum * pairs;
+        share = (int)(((uint32_t)total + (uint32_t)a.groups - 1) / (uint32_t)a.groups);
+        share = share < kShareMin ? kShareMin : share;
+    }
+};
 
 template <int TYPE, int NG>
 __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kernel(DecodeArgs a) {
     using T = Val<TYPE>;
     constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG);
-    // the waves' weights [group][token][row] while tiles last, then their results
-    constexpr int kOut = kWaves * 8 * D * 4, kP = kWaves * NG * 1024;
-    __shared__ __attribute__((aligned(16))) char sh[kOut > kP ? kOut : kP];
-    __shared__ float sh_m[kWaves][8], sh_l[kWaves][8];
+    // the waves' weights [group][token][row], and their results
+    __shared__ __attribute__((aligned(16))) char sh_p[kWaves * NG * 1024];
+    __shared__ float sh_o[kWaves * 8 * D], sh_m[kWaves][8], sh_l[kWaves][8];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, j = lane >> 4;
     const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
-    const uint32_t chunks = (uint32_t)(group + 7) / 8;
-    uint32_t id = blockIdx.x;
-    const int split = (int)(id % (uint32_t)a.splits);
-    id /= (uint32_t)a.splits;
-    const int hc = chunks == 1 ? 0 : (int)(id % chunks);
-    id /= chunks;
-    const int kvh = (int)(id % (uint32_t)a.kv_heads);
-    const int64_t b = id / (uint32_t)a.kv_heads;
-
-    const int64_t want = a.lens[b];
-    bool bad = want > a.max_len || (want > 0 && a.pages == 0);       // not what the caller said: NaN
-    const int len = want < 0 || bad ? 0 : (int)want;
-    const int tiles = (len + kKvTile - 1) / kKvTile;
-    const int first = split * a.chunk_tiles;
-    const int last = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
-    const int rows = group - 8 * hc < 8 ? group - 8 * hc : 8;        // query heads here
-    if (first >= last && split > 0) {                                // nothing of the sequence: the join skips it
-        return;
-    }
-
-    // this wave's tiles, their pages one ahead
+    const int chunks = (group + 7) / 8, pairs = (int)a.kv_heads * chunks;
     const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
-    const int32_t* table = a.table + b * a.ld_table;
-    const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
     const int64_t page_bytes = a.kv_heads * (int64_t)page_tiles * kTile;
-    auto tile_at = [&](int tile) {
-        const uint32_t pg = (uint32_t)tile / page_tiles, in = (uint32_t)tile - pg * page_tiles;
-        int64_t page = table[pg];
-        if (page < 0 || page >= a.pages) {
-            bad = true;
-            page = 0;
-        }
-        return heads + page * page_bytes + (int64_t)in * kTile;
-    };
-    int tile = first + wave;
-    Tile<NG> even, odd;
-    if (tile < last) even.load(tile_at(tile), lane);
 
-    // q: row n holds head n / 2, the value or (n odd) the rest
-    half8v qf[NG];
-    float rs;
-    {
-        const int row = n >> 1;
-        float x[NG][8], top = 0.f;
-        bool special = false;
-        const typename T::Elem* qp = static_cast<const typename T::Elem*>(a.q) + b * a.ld_q +
-                                     ((int64_t)kvh * group + 8 * hc + (row < rows ? row : 0)) * D;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            T::load8(qp + 32 * g + 8 * j, x[g]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float m = __builtin_fabsf(x[g][c]);
-                special |= !(m < __builtin_inff());
-                top = __builtin_fmaxf(top, m);
-            }
+    // this workgroup's tiles: [at, end) of the line, or all of one pair
+    Line line;
+    int at = 0, end = 0, begin = 0, k = 0, b, pair, first = 0, last = 0, len, tiles;
+    const bool shared = a.groups != 0;
+    if (!shared) {
+        b = (int)(blockIdx.x / (uint32_t)pairs);
+        pair = (int)(blockIdx.x - (uint32_t)b * (uint32_t)pairs);
+        len = length_of(a, b);
+        last = tiles = tiles_in(len);
+    } else {
+        line.open(a, pairs, lane);
+        at = (int)blockIdx.x * line.share;
+        if ((uint32_t)at >= (uint32_t)line.total) return;
+        end = line.total - at < line.share ? line.total : at + line.share;
+        // the sequence that `at` is in: lane k of those in hand
+        while (begin + line.all() * pairs <= at) {
+            begin += line.all() * pairs;
+            line.read(a, line.from + 64, lane);
         }
-        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-        special |= __shfl_xor((int)special, 16) != 0;
-        special |= __shfl_xor((int)special, 32) != 0;
-        int e = 0;
-        if (top > 0.f && !special) (void)frexpf(top, &e);            // top in [2^(e-1), 2^e)
-        const int up = 14 - e, u1 = up / 2, u2 = up - u1;            // up is -114 .. 162
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float v = x[g][c] * pow2(u1) * pow2(u2);
-                const _Float16 hi = (_Float16)v;
-                qf[g][c] = n & 1 ? (_Float16)(v - (float)hi) : hi;
-            }
-        }
-        rs = special ? __builtin_nanf("") : a.scale * kLog2e * pow2(-u1) * pow2(-u2);
+        k = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(begin + line.upto * pairs > at));
     }
-    // of the lane's two heads 2j and 2j + 1: rows 4j .. 4j + 3 of both products
-    const float rs2[2] = {__shfl(rs, 4 * j), __shfl(rs, 4 * j + 2)};
-    float ref[2] = {-__builtin_inff(), -__builtin_inff()}, l[2] = {0.f, 0.f};
-    int ev = -24;                                                    // E
-    float4v o[2 * NG];
-#pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) o[i] = float4v{0, 0, 0, 0};
-
-    const lds_bytes sp = (lds_bytes)sh + wave * (NG * 1024);
+    const lds_bytes sp = (lds_bytes)sh_p + wave * (NG * 1024);
     const lds_bytes sp_to = sp + n * 32 + j * 8, sp_from = sp + lane * 8;
 
-    auto step = [&](Tile<NG>& t, int tile) __attribute__((always_inline)) {
-        // scores of tokens n and 16 + n for heads 2j, 2j + 1
-        float s[2][2];
+    for (;;) {
+        if (shared) {                                                // tiles [first, last) of a pair of sequence b
+            b = line.from + k;
+            len = __builtin_amdgcn_readlane(line.len, k);
+            tiles = tiles_in(len);
+            const int in = at - begin - line.before(k) * pairs, places = tiles + kPad;
+            pair = (int)((uint32_t)in / (uint32_t)places);
+            first = in - pair * places - kPad;
+            last = end - at < tiles - first ? first + (end - at) : tiles;
+            at += last - first;
+            if (last <= 0) break;                                    // all of it padding
+            first = first > 0 ? first : 0;
+        }
+        bool bad = len < 0;
+        const int kvh = chunks == 1 ? pair : pair / chunks, hc = chunks == 1 ? 0 : pair - kvh * chunks;
+        const int rows = group - 8 * hc < 8 ? group - 8 * hc : 8;    // query heads here
+        const const_ints table = constant(a.table) + (int64_t)b * a.ld_table;
+        const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
+        // Pages are looked up a step before their tile is asked for. Past the last
+        // tile that one is asked for again: with loads that may not have been
+        // issued in flight, the compiler would wait for the ones after them too.
+        auto page_index = [&](int tile) { return (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36); };
+        auto look_up = [&](int tile) { return table[page_index(tile < last ? tile : last - 1)]; };
+        auto address = [&](int tile, int page) {
+            if ((uint32_t)page >= (uint64_t)a.pages) {
+                bad = true;
+                page = 0;
+            }
+            tile = tile < last ? tile : last - 1;
+            const uint32_t in = (uint32_t)tile - page_index(tile) * page_tiles;
+            return heads + page * page_bytes + (int64_t)in * kTile;
+        };
+        int tile = first + wave;
+        Half<NG> k0, v0, k1, v1;                                     // this tile and the wave's next one
+        auto fetch_k = [&](Half<NG>& k, const uint8_t* t) { k.load(t, t + kv_ks_off(NG), lane); };
+        auto fetch_v = [&](Half<NG>& v, const uint8_t* t) { v.load(t + kv_vc_off(NG), t + kv_vs_off(NG), lane); };
+        int page = 0;
+        auto start = [&]() __attribute__((always_inline)) {
+            const int p0 = look_up(tile), p1 = look_up(tile + kWaves);
+            page = look_up(tile + 2 * kWaves);
+            const uint8_t* t0 = address(tile, p0);
+            const uint8_t* t1 = address(tile + kWaves, p1);
+            fetch_k(k0, t0);                                         // in the order of their use
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_v(v0, t0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_k(k1, t1);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_v(v1, t1);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (tile < last) start();
+
+        // q: row n holds head n / 2, the value or (n odd) the rest
+        half8v qf[NG];
+        float rs;
+        {
+            const int row = n >> 1;
+            float x[NG][8];
+            uint32_t top = 0;                                        // bits of the largest |q|; inf and NaN above all
+            const typename T::Elem* qp = static_cast<const typename T::Elem*>(a.q) + (int64_t)b * a.ld_q +
+                                         ((int64_t)kvh * group + 8 * hc + (row < rows ? row : 0)) * D;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < NG; ++g) T::load8(qp + 32 * g + 8 * j, x[g]);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint32_t m = __builtin_bit_cast(uint32_t, x[g][c]) & 0x7FFFFFFFu;
+                    top = top > m ? top : m;
+                }
+            uint32_t other = __shfl_xor(top, 16);
+            top = top > other ? top : other;
+            other = __shfl_xor(top, 32);
+            top = top > other ? top : other;
+            const int up = top ? 140 - (int)(top >> 23) : 0;         // the largest to [2^13, 2^14)
+            const float part = n & 1 ? -1.f : 0.f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const uint32_t w = t.kw[u * NG + g];
-                const half8v kf = join(low_pair(w), high_pair(w), low_pair(w >> 8), high_pair(w >> 8));
-                const float4v c = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[g], kf, float4v{0, 0, 0, 0}, 0, 0, 0);
-                const int at = u * NG + g;
-                const float d = (float)half_of(t.ks[at / 2], at & 1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(c[i], d, acc[i]);
+                for (int c = 0; c < 8; ++c) {
+                    const float y = __builtin_ldexpf(x[g][c], up);
+                    const _Float16 hi = (_Float16)y;
+                    qf[g][c] = (_Float16)__builtin_fmaf((float)hi, part, y);
+                }
             }
-            s[u][0] = (acc[0] + acc[1]) * rs2[0];
-            s[u][1] = (acc[2] + acc[3]) * rs2[1];
+            rs = top >= 0x7F800000u ? __builtin_nanf("") : __builtin_ldexpf(a.scale * kLog2e, -up);
         }
-        const int left = len - tile * kKvTile;                       // valid tokens from here
-        if (left < kKvTile) {
+        // of the lane's two heads 2j and 2j + 1: rows 4j .. 4j + 3 of both products
+        const float rs2[2] = {__shfl(rs, 4 * j), __shfl(rs, 4 * j + 2)};
+        // what the lane's heads have in LDS: reference and sum of weights
+        float held_ref[2] = {-__builtin_inff(), -__builtin_inff()}, held_l[2] = {0.f, 0.f};
+        bool held = false;
+
+        while (tile < last) {
+        float ref[2] = {-__builtin_inff(), -__builtin_inff()}, l[2] = {0.f, 0.f};
+        int ev = 0;                                                  // E
+        int fresh = 1;
+        float4v o[2 * NG];
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) o[i] = float4v{0, 0, 0, 0};
+        if (held) start();                                           // once more from this tile
+
+        // one tile; false if it does not fit the reference
+        auto step = [&](Half<NG>& k, Half<NG>& v) __attribute__((always_inline)) {
+            const uint8_t* next = address(tile + 2 * kWaves, page);
+            page = look_up(tile + 3 * kWaves);
+            // scores of tokens n and 16 + n for heads 2j, 2j + 1
+            float s[2][2];
+            float4v c[2][NG];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t w = k.code[u * NG + g];
+                    const half8v kf = join(low_pair(w), high_pair(w), low_pair(w >> 8), high_pair(w >> 8));
+                    c[u][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[g], kf, float4v{0, 0, 0, 0}, 0, 0, 0);
+                    // products under way before one is waited for, and no more
+                    // operands at a time than the registers have room for
+                    if ((u * NG + g) % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                if (16 * u + n >= left) {
-                    s[u][0] = s[u][1] = -__builtin_inff();
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int p = 0; p < NG / 2; ++p) t.vs[u * (NG / 2) + p] = 0;
+                for (int g = 0; g < NG; ++g) {
+                    const float d = (float)k.scale_of(u, g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(c[u][g][i], d, acc[i]);
+                }
+                s[u][0] = (acc[0] + acc[1]) * rs2[0];
+                s[u][1] = (acc[2] + acc[3]) * rs2[1];
+            }
+            fetch_k(k, next);                              // these registers are free again
+            const int left = len - tile * kKvTile;                   // valid tokens from here
+            if (__builtin_expect(left < kKvTile, 0)) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (16 * u + n >= left) {
+                        s[u][0] = s[u][1] = -__builtin_inff();
+#pragma unroll
+                        for (int p = 0; p < NG / 2; ++p) v.scale[u * (NG / 2) + p] = 0;
+                    }
+                }
+            }
+            auto weigh = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[u][0] - ref[0]), p1 = __builtin_amdgcn_exp2f(s[u][1] - ref[1]);
+                    l[0] += p0;
+                    l[1] += p1;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float d = (float)v.scale_of(u, g);
+                        const _Float16 h0 = (_Float16)__builtin_fmaf(p0, d, 0.f), h1 = (_Float16)__builtin_fmaf(p1, d, 0.f);
+                        const _Float16 r0 = (_Float16)__builtin_fmaf(p0, d, -(float)h0), r1 = (_Float16)__builtin_fmaf(p1, d, -(float)h1);
+                        const half2v x = {h0, r0}, y = {h1, r1};
+                        *(__attribute__((address_space(3))) uint2v*)(sp_to + g * 1024 + u * 512) =
+                            uint2v{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                using tr = __attribute__((address_space(3))) short4v*;
+                uint2v px[NG], py[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    px[g] = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(sp_from + g * 1024)));
+                    py[g] = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(sp_from + g * 1024 + 512)));
+                }
+                __builtin_amdgcn_sched_barrier(0);                       // V is unpacked while they come
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t w0 = v.code[2 * g], w1 = v.code[2 * g + 1];
+                    const half8v va = join(low_pair(w0), low_pair(w0 >> 8), low_pair(w1), low_pair(w1 >> 8));
+                    const half8v vb = join(high_pair(w0), high_pair(w0 >> 8), high_pair(w1), high_pair(w1 >> 8));
+                    const half8v pf = join(pair_of(px[g][0]), pair_of(px[g][1]), pair_of(py[g][0]), pair_of(py[g][1]));
+                    o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, va, o[2 * g], 0, 0, 0);
+                    o[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, vb, o[2 * g + 1], 0, 0, 0);
+                    if (g % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                }
+                fetch_v(v, next);
+            };
+            // a score 2^8 past its reference's maximum, or a scale past E?
+            uint32_t big = 0;
+#pragma unroll
+            for (int p = 0; p < NG; ++p) {
+                const uint32_t w = v.scale[p] & 0x7FFF7FFFu;
+                using us2 = unsigned short __attribute__((ext_vector_type(2)));
+                big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, big), __builtin_bit_cast(us2, w)));
+            }
+            const float b0 = (float)half_of(big, 0), b1 = (float)half_of(big, 1);
+            const float t0 = __builtin_fmaxf(s[0][0], s[1][0]), t1 = __builtin_fmaxf(s[0][1], s[1][1]);
+            asm("" : "+s"(fresh));                                 // no copy of the step for the first tile
+            if (__builtin_expect(fresh != 0, 0)) {
+                float top = 0.f;                                     // of the scales that are numbers
+#pragma unroll
+                for (int p = 0; p < 2 * NG; ++p) {
+                    const float y = __builtin_fabsf((float)half_of(v.scale[p / 2], p & 1));
+                    top = y < __builtin_inff() ? __builtin_fmaxf(top, y) : top;
+                }
+                top = row_max(top);                                  // every row of lanes holds all tokens
+                const int et = top > 0.f ? __builtin_amdgcn_frexp_expf(top) + 1 : -22;
+                ev = __builtin_amdgcn_readfirstlane(et);
+                ref[0] = row_max(t0) + (float)(ev - 4);
+                ref[1] = row_max(t1) + (float)(ev - 4);
+                fresh = 0;
+            } else {
+                const float cap = pow2(ev + 1), room = (float)(12 - ev);
+                const bool past = (int)(t0 > ref[0] + room) | (int)(t1 > ref[1] + room) | (int)!(b0 < cap) | (int)!(b1 < cap);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(past) != 0, 0)) return false;
+            }
+            weigh();
+            __builtin_amdgcn_wave_barrier();
+            tile += kWaves;
+            return true;
+        };
+        while (tile < last && step(k0, v0) && tile < last && step(k1, v1)) {
+        }
+        // into LDS, under the larger of the references
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float both = __builtin_fmaxf(held_ref[i], ref[i]), base = both == -__builtin_inff() ? 0.f : both;
+            const float fo = __builtin_amdgcn_exp2f(held_ref[i] - base), fn = __builtin_amdgcn_exp2f(ref[i] - base);
+            held_l[i] = held_l[i] * fo + l[i] * fn;
+            held_ref[i] = both;
+            float* to = sh_o + (wave * 8 + 2 * j + i) * D + n;
+#pragma unroll
+            for (int c = 0; c < 2 * NG; ++c) {
+                const float x = (o[c][2 * i] + o[c][2 * i + 1]) * fn;
+                to[16 * c] = held ? to[16 * c] * fo + x : x;
+            }
+        }
+        held = true;
+        }
+        if (__builtin_amdgcn_ballot_w64(bad)) held_l[0] = held_l[1] = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int w = 1; w <= 8; w <<= 1) held_l[i] += __shfl_xor(held_l[i], w);
+            if (n == 0) {
+                sh_m[wave][2 * j + i] = held_ref[i];
+                sh_l[wave][2 * j + i] = held_l[i];
+            }
+        }
+        __syncthreads();
+        // a row that is whole here is done, else its part goes to the joining: to
+        // one place if it began before this workgroup, to another if it began here
+        const bool whole = first == 0 && last == tiles;
+        float* part = a.part + (2 * (int64_t)blockIdx.x + (first == 0)) * 8 * (D + 2);
+        for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) {
+            const int r = i / D, c = i - r * D;
+            float mm = sh_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh_m[w][r]);
+            const float base = mm == -__builtin_inff() ? 0.f : mm;
+            float sum = 0.f, val = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sh_m[w][r] - base);
+                sum += f * sh_l[w][r];
+                val += f > 0.f ? f * sh_o[(w * 8 + r) * D + c] : 0.f;    // a wave without tiles wrote none
+            }
+            if (whole) {
+                const int64_t h = (int64_t)kvh * group + 8 * hc + r;
+                static_cast<typename T::Elem*>(a.out)[(int64_t)b * a.ld_out + h * D + c] = T::one(sum == 0.f ? 0.f : val / sum);
+            } else {
+                part[r * D + c] = val;
+                if (c == 0) {
+                    part[8 * D + 2 * r] = mm;
+                    part[8 * D + 2 * r + 1] = sum;
                 }
             }
         }
-        // a score 2^8 past its reference's maximum, or a scale past E?
-        uint32_t big = 0;
-#pragma unroll
-        for (int p = 0; p < NG; ++p) {
-            const uint32_t w = t.vs[p] & 0x7FFF7FFFu;
-            using us2 = unsigned short __attribute__((ext_vector_type(2)));
-            big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, big), __builtin_bit_cast(us2, w)));
-        }
-        const float cap = pow2(ev + 1);
-        const float b0 = (float)half_of(big, 0), b1 = (float)half_of(big, 1);
-        const float t0 = __builtin_fmaxf(s[0][0], s[1][0]), t1 = __builtin_fmaxf(s[0][1], s[1][1]);
-        const float room = (float)(14 - ev);                         // ref = maximum - 6 + E
-        if (__builtin_amdgcn_ballot_w64(t0 > ref[0] + room || t1 > ref[1] + room || !(b0 < cap) || !(b1 < cap))) {
-            float top = 0.f;                                         // of the scales that are numbers
-#pragma unroll
-            for (int p = 0; p < 2 * NG; ++p) {
-                const float v = __builtin_fabsf((float)half_of(t.vs[p / 2], p & 1));
-                top = v < __builtin_inff() ? __builtin_fmaxf(top, v) : top;
+        if (!shared || at >= end) break;
+        if (last == tiles && pair == pairs - 1) {                    // on to the next sequence that has any
+            uint64_t more = __builtin_amdgcn_ballot_w64(line.len > 0) >> k >> 1;
+            while (more == 0) {
+                begin += line.all() * pairs;
+                line.read(a, line.from + 64, lane);
+                k = -1;
+                more = __builtin_amdgcn_ballot_w64(line.len > 0);
             }
-            top = row_max(top);
-            int e = ev;
-            if (top >= cap) {
-                (void)frexpf(top, &e);
-                --e;
-            }
-            const float up = (float)(e - ev);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float now = row_max(i ? t1 : t0) - 6.f + (float)e;
-                const float r = __builtin_fmaxf(ref[i] + up, now);
-                const float keep = r == ref[i] ? 1.f : __builtin_amdgcn_exp2f(ref[i] - r);
-                ref[i] = r;
-                l[i] *= keep;
-#pragma unroll
-                for (int c = 0; c < 2 * NG; ++c) {
-                    o[c][2 * i] *= keep;
-                    o[c][2 * i + 1] *= keep;
-                }
-            }
-            ev = e;
+            k += 1 + (int)__builtin_ctzll(more);
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float p0 = __builtin_amdgcn_exp2f(s[u][0] - ref[0]), p1 = __builtin_amdgcn_exp2f(s[u][1] - ref[1]);
-            l[0] += p0;
-            l[1] += p1;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const int at = u * NG + g;
-                const float d = (float)half_of(t.vs[at / 2], at & 1);
-                const _Float16 h0 = (_Float16)__builtin_fmaf(p0, d, 0.f), h1 = (_Float16)__builtin_fmaf(p1, d, 0.f);
-                const _Float16 r0 = (_Float16)__builtin_fmaf(p0, d, -(float)h0), r1 = (_Float16)__builtin_fmaf(p1, d, -(float)h1);
-                const half2v x = {h0, r0}, y = {h1, r1};
-                *(__attribute__((address_space(3))) uint2v*)(sp_to + g * 1024 + u * 512) =
-                    uint2v{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            using tr = __attribute__((address_space(3))) short4v*;
-            const uint2v x = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(sp_from + g * 1024)));
-            const uint2v y = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr)(sp_from + g * 1024 + 512)));
-            const half8v pf = join(pair_of(x[0]), pair_of(x[1]), pair_of(y[0]), pair_of(y[1]));
-            const uint32_t w0 = t.vw[2 * g], w1 = t.vw[2 * g + 1];
-            const half8v va = join(low_pair(w0), low_pair(w0 >> 8), low_pair(w1), low_pair(w1 >> 8));
-            const half8v vb = join(high_pair(w0), high_pair(w0 >> 8), high_pair(w1), high_pair(w1 >> 8));
-            o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, va, o[2 * g], 0, 0, 0);
-            o[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, vb, o[2 * g + 1], 0, 0, 0);
-        }
-        __builtin_amdgcn_wave_barrier();
-    };
-    while (tile < last) {
-        if (tile + kWaves < last) odd.load(tile_at(tile + kWaves), lane);
-        step(even, tile);
-        tile += kWaves;
-        if (tile >= last) break;
-        if (tile + kWaves < last) even.load(tile_at(tile + kWaves), lane);
-        step(odd, tile);
-        tile += kWaves;
-    }
-    // join the lanes' sums, then the waves
-    if (__builtin_amdgcn_ballot_w64(bad)) l[0] = l[1] = __builtin_nanf("");
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int k = 1; k <= 8; k <<= 1) l[i] += __shfl_xor(l[i], k);
-        if (n == 0) {
-            sh_m[wave][2 * j + i] = ref[i];
-            sh_l[wave][2 * j + i] = l[i];
-        }
-    }
-    __syncthreads();
-    float* sh_o = reinterpret_cast<float*>(sh);
-#pragma unroll
-    for (int c = 0; c < 2 * NG; ++c) {
-        sh_o[(wave * 8 + 2 * j) * D + 16 * c + n] = o[c][0] + o[c][1];
-        sh_o[(wave * 8 + 2 * j + 1) * D + 16 * c + n] = o[c][2] + o[c][3];
-    }
-    __syncthreads();
-    const bool whole = a.splits == 1;
-    for (int at = threadIdx.x; at < rows * D; at += 64 * kWaves) {
-        const int r = at / D, c = at - r * D;
-        float mm = sh_m[0][r];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh_m[w][r]);
-        const float base = mm == -__builtin_inff() ? 0.f : mm;
-        float sum = 0.f, val = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sh_m[w][r] - base);
-            sum += f * sh_l[w][r];
-            val += f * sh_o[(w * 8 + r) * D + c];
-        }
-        const int64_t h = (int64_t)kvh * group + 8 * hc + r;
-        if (whole) {
-            static_cast<typename T::Elem*>(a.out)[b * a.ld_out + h * D + c] = T::one(sum == 0.f ? 0.f : val / sum);
-        } else {
-            const int64_t part = (b * a.q_heads + h) * a.splits + split;
-            a.part_o[part * D + c] = val;
-            if (c == 0) {
-                a.part_ml[2 * part] = mm;
-                a.part_ml[2 * part + 1] = sum;
-            }
-        }
+        __syncthreads();                                             // the next results go to the same place
     }
 }
 
-// out = the splits of a row, joined in their order: 256 / (D / 4) splits at a
-// time, four columns a thread, then over those.
+// Rows that more than one workgroup worked on, joined in their order, and rows
+// that none did: 256 / (D / 4) parts at a time, four columns a thread.
 template <int TYPE, int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(DecodeArgs a) {
     using T = Val<TYPE>;
     constexpr int kCols = D / 4, kAt = 256 / kCols;
-    __shared__ float part[kAt][D], sums[kAt];
-    const int64_t r = blockIdx.x;
-    const int64_t b = (uint32_t)r / (uint32_t)a.q_heads, h = r - b * a.q_heads;
-    const int64_t want = a.lens[b];
-    const int tiles = want > a.max_len || want < 0 || a.pages == 0 ? 0 : (int)((want + kKvTile - 1) / kKvTile);
-    int used = (tiles + a.chunk_tiles - 1) / a.chunk_tiles;
-    used = used < 1 ? 1 : used;                                      // split 0 speaks for an empty row
-    const float* ml = a.part_ml + 2 * r * a.splits;
+    __shared__ float vals[kAt][D], sums[kAt];
+    const int lane = threadIdx.x & 63;
+    const uint32_t b = blockIdx.x / (uint32_t)a.q_heads, h = blockIdx.x - b * (uint32_t)a.q_heads;
+    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads), chunks = (group + 7) / 8;
+    const int pairs = (int)a.kv_heads * chunks, kvh = (int)h / group, in = (int)h - kvh * group;
+    const int pair = kvh * chunks + in / 8, row = in & 7;
+    typename T::Elem* out = static_cast<typename T::Elem*>(a.out) + b * a.ld_out + (int64_t)h * D;
+    const int len = length_of(a, (int)b), tiles = tiles_in(len);
+    if (tiles == 0) {
+        if (threadIdx.x < D) out[threadIdx.x] = T::one(len < 0 ? __builtin_nanf("") : 0.f);
+        return;
+    }
+    Line line;
+    line.open(a, pairs, lane);
+    int start = pair * (tiles + kPad) + kPad;                        // of its first tile
+    while ((int)b - line.from >= 64) {
+        start += line.all() * pairs;
+        line.read(a, line.from + 64, lane);
+    }
+    start += line.before((int)b - line.from) * pairs;
+    const uint32_t w0 = (uint32_t)start / (uint32_t)line.share, w1 = (uint32_t)(start + tiles - 1) / (uint32_t)line.share;
+    if (w0 == w1) return;                                            // one workgroup's: done
+    const int used = (int)(w1 - w0) + 1;
+    auto part = [&](int s) { return a.part + (2 * (int64_t)(w0 + s) + (s == 0)) * 8 * (D + 2); };
     float mm = -__builtin_inff();
-    for (int s = threadIdx.x & 63; s < used; s += 64) mm = __builtin_fmaxf(mm, ml[2 * s]);
+    for (int s = lane; s < used; s += 64) mm = __builtin_fmaxf(mm, part(s)[8 * D + 2 * row]);
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) mm = __builtin_fmaxf(mm, __shfl_xor(mm, i));
     const float base = mm == -__builtin_inff() ? 0.f : mm;
@@ -373,56 +525,56 @@ __global__ void __launch_bounds__(256) attn_join_kernel(DecodeArgs a) {
     float sum = 0.f;
 #pragma unroll 4
     for (int s = at; s < used; s += kAt) {
-        const float4 o = *reinterpret_cast<const float4*>(a.part_o + (r * a.splits + s) * D + 4 * c);
-        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - base);
-        sum = __builtin_fmaf(f, ml[2 * s + 1], sum);
+        const float* p = part(s);
+        const float4 o = *reinterpret_cast<const float4*>(p + row * D + 4 * c);
+        const float f = __builtin_amdgcn_exp2f(p[8 * D + 2 * row] - base);
+        sum = __builtin_fmaf(f, p[8 * D + 2 * row + 1], sum);
         val.x = __builtin_fmaf(f, o.x, val.x);
         val.y = __builtin_fmaf(f, o.y, val.y);
         val.z = __builtin_fmaf(f, o.z, val.z);
         val.w = __builtin_fmaf(f, o.w, val.w);
     }
-    *reinterpret_cast<float4*>(&part[at][4 * c]) = val;
+    *reinterpret_cast<float4*>(&vals[at][4 * c]) = val;
     if (c == 0) sums[at] = sum;
     __syncthreads();
     if (threadIdx.x < D) {
         float v = 0.f, t = 0.f;
 #pragma unroll
         for (int i = 0; i < kAt; ++i) {
-            v += part[i][threadIdx.x];
+            v += vals[i][threadIdx.x];
             t += sums[i];
         }
-        static_cast<typename T::Elem*>(a.out)[b * a.ld_out + h * D + threadIdx.x] = T::one(t == 0.f ? 0.f : v / t);
+        out[threadIdx.x] = T::one(t == 0.f ? 0.f : v / t);
     }
 }
 
 }  // namespace
 
-void plan_attn_decode(DecodeArgs* a) {
+bool plan_attn_decode(DecodeArgs* a) {
     const int64_t tiles = (a->max_len + kKvTile - 1) / kKvTile;
-    const int64_t group = a->q_heads / a->kv_heads, base = a->batch * a->kv_heads * ((group + 7) / 8);
-    int64_t splits = (1024 + base - 1) / base;
-    const int64_t most = (tiles + kWaves - 1) / kWaves;
-    splits = splits > most ? most : splits;
-    splits = splits < 1 ? 1 : splits;
-    a->chunk_tiles = (int)((tiles + splits - 1) / splits);
-    a->splits = (int)(tiles ? (tiles + a->chunk_tiles - 1) / a->chunk_tiles : 1);
+    const int64_t group = a->q_heads / a->kv_heads, pairs = a->batch * a->kv_heads * ((group + 7) / 8);
+    if (pairs * (tiles + kPad + 1) >= ((int64_t)1 << 31) - (1 << 20)) return false;
+    const int64_t most = (pairs * (tiles + kPad) + kShareMin - 1) / kShareMin;
+    a->groups = tiles <= kWhole ? 0 : (int)(most < kGroups ? most : kGroups);
+    return true;
 }
 
 size_t attn_decode_scratch(const DecodeArgs& a) {
-    return a.splits == 1 ? 0 : sizeof(float) * (size_t)(a.batch * a.q_heads * a.splits) * (size_t)(a.head_dim + 2);
+    return sizeof(float) * (size_t)a.groups * 2 * 8 * (size_t)(a.head_dim + 2);
 }
 
 hipError_t launch_attn_decode(DecodeArgs a, float* scratch, hipStream_t stream) {
-    const int64_t group = a.q_heads / a.kv_heads;
-    const int64_t grid = a.batch * a.kv_heads * ((group + 7) / 8) * a.splits;
-    a.part_o = scratch;
-    a.part_ml = scratch ? scratch + a.batch * a.q_heads * a.splits * a.head_dim : nullptr;
+    const int64_t group = a.q_heads / a.kv_heads, pairs = a.batch * a.kv_heads * ((group + 7) / 8);
+    const unsigned grid = (unsigned)(a.groups ? a.groups : pairs);
+    const uint64_t page_tiles = (uint64_t)a.page_tokens / kKvTile;
+    a.per_page = ((uint64_t)1 << 36) / page_tiles + 1;
+    a.part = scratch;
     return with_type(a.type, [&](auto ty) {
         constexpr int kT = decltype(ty)::value;
         const auto run = [&](auto ng) {
             constexpr int kN = decltype(ng)::value;
-            attn_decode_kernel<kT, kN><<<(unsigned)grid, 64 * kWaves, 0, stream>>>(a);
-            if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
+            attn_decode_kernel<kT, kN><<<grid, 64 * kWaves, 0, stream>>>(a);
+            if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.groups == 0) return e;
             attn_join_kernel<kT, 32 * kN><<<(unsigned)(a.batch * a.q_heads), 256, 0, stream>>>(a);
             return hipGetLastError();
         };

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         // the mask cuts through the tile, such values leave it and are added
         // below for the queries that see their keys.
         const bool cut = a.causal && kt + kKeys - 1 > (int)qb * kRows + past;
-        if (cut) {
+        if (__builtin_expect(cut, 0)) {
             bool any = false;
             for (int at = threadIdx.x; at < kKeys * CH; at += 64 * WAVES) {
                 u32x4 w = reinterpret_cast<const u32x4*>(cv)[at];
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         __builtin_amdgcn_s_setprio(0);
-        if (masked) {
+        if (__builtin_expect(masked, 0)) {
             const int left = lim - kt - 4 * h;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         top = half_max(top) * c;
         // the reference follows the maximum only when it is 2^8 behind: sums
         // and weights have the room, and the rescaling is rare
-        if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0, 0)) {
             const float mn = __builtin_fmaxf(m, top);
             const float keep = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
                 o[d] = mfma<TYPE>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[s], o[d]);
             }
         }
-        if (cut && special_at == kt + 1) {
+        if (__builtin_expect(cut && special_at == kt + 1, 0)) {
             for (int kr = 0; kr < kKeys && kt + kr < nk; ++kr) {
                 const uint16_t* row = vp + (int64_t)(kt + kr) * a.ld_v + 4 * h;
                 const bool seen = kt + kr <= lim;

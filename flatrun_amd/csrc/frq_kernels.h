@@ -308,10 +308,11 @@ struct DecodeArgs {
     int64_t ld_out;
     int64_t batch, q_heads;
     float scale;
-    int splits, chunk_tiles;     // plan_attn_decode
-    float *part_o, *part_ml;     // set by the launcher
+    int groups;                  // plan_attn_decode: workgroups that share the tiles, 0 for one per sequence and key head
+    uint64_t per_page;           // set by the launcher: 2^36 / tiles of a page, rounded up
+    float* part;
 };
-void plan_attn_decode(DecodeArgs* a);
+bool plan_attn_decode(DecodeArgs* a);     // false: more tiles than the kernels count
 size_t attn_decode_scratch(const DecodeArgs& a);
 hipError_t launch_attn_decode(DecodeArgs a, float* scratch, hipStream_t stream);
 

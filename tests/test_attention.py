@@ -66,7 +66,7 @@ REFUSED = [
     (decode, dict(q=0), _lib.ERR_INVALID),
     (decode, dict(table=0), _lib.ERR_INVALID),
     (decode, dict(q_heads=5), _lib.ERR_SHAPE),
-    (decode, dict(max_len=-1), _lib.ERR_SHAPE),
+    (decode, dict(max_len=-1), _lib.ERR_UNSUPPORTED),
     (decode, dict(ld_table=1), _lib.ERR_SHAPE),
     (decode, dict(ld_q=500), _lib.ERR_SHAPE),
     (decode, dict(batch=-1), _lib.ERR_SHAPE),
