@@ -1176,7 +1176,7 @@ int frq_dev_qk_norm_rope(int x_type, const void* x, int64_t ld_x, int out_type, 
     int64_t xs, os;
     if (!val_type(x_type, &xs) || !val_type(out_type, &os))
         return fail(FRQ_ERR_INVALID, "qk_norm_rope: types are F32, F16 or BF16, got %d and %d", x_type, out_type);
-    if (!in_range(tokens, 0, kMaxTokens) || !in_range(q_heads, 1, kMaxHeads) || !in_range(kv_heads, 1, kMaxHeads))
+    if (!in_range(tokens, 0, (int64_t)1 << 30) || !in_range(q_heads, 1, kMaxHeads) || !in_range(kv_heads, 1, kMaxHeads))
         return fail(FRQ_ERR_SHAPE, "qk_norm_rope: tokens or heads out of range");
     if (head_dim < 8 || head_dim > 256 || head_dim % 8)
         return fail(FRQ_ERR_UNSUPPORTED, "qk_norm_rope: head size %lld is not a multiple of 8 up to 256", (long long)head_dim);
@@ -1195,7 +1195,6 @@ int frq_dev_qk_norm_rope(int x_type, const void* x, int64_t ld_x, int out_type, 
     if ((reinterpret_cast<uintptr_t>(table) & 7) || (reinterpret_cast<uintptr_t>(positions) & 3) ||
         ((reinterpret_cast<uintptr_t>(q_norm) | reinterpret_cast<uintptr_t>(k_norm)) & 15))
         return fail(FRQ_ERR_ALIGN, "qk_norm_rope: table 8-byte, positions 4-byte, norm weights 16-byte aligned");
-    if (tokens * heads > ((int64_t)1 << 34)) return fail(FRQ_ERR_UNSUPPORTED, "qk_norm_rope: too many heads for a launch");
     frq::RopeArgs a{x_type, out_type, x,      ld_x, q,           k,     v,     ld_q,      ld_k,   ld_v,   tokens, q_heads,
                     kv_heads, head_dim, rot, interleaved != 0, table, n_pos, positions, q_norm, k_norm, eps};
     FRQ_HIP(frq::launch_qk_norm_rope(a, static_cast<hipStream_t>(stream)));
@@ -1224,6 +1223,7 @@ int frq_kv4_bytes(int64_t pages, int64_t page_tokens, int64_t kv_heads, int64_t 
                     (long long)page_tokens);
     if (head_dim != 64 && head_dim != 128 && head_dim != 256)
         return fail(FRQ_ERR_UNSUPPORTED, "kv4: head size %lld is not 64, 128 or 256", (long long)head_dim);
+    if (pages * (page_tokens / 32) >= ((int64_t)1 << 32)) return fail(FRQ_ERR_UNSUPPORTED, "kv4: 2^37 tokens or more");
     *bytes = (size_t)pages * (size_t)kv_heads * (size_t)(page_tokens / 32) * (size_t)(head_dim / 32 * 1152);
     return FRQ_OK;
 }
@@ -1241,7 +1241,7 @@ static int kv4_move(const char* what, bool write, void* cache, size_t cache_byte
     if (!k || !v || !slots) return fail(FRQ_ERR_INVALID, "null buffer");
     if (!rows_aligned(k, ld_k, size) || !rows_aligned(v, ld_v, size) || (reinterpret_cast<uintptr_t>(slots) & 7))
         return fail(FRQ_ERR_ALIGN, "%s: k and v rows must be 16-byte aligned, slots 8-byte", what);
-    if (tokens * kv_heads > ((int64_t)1 << 33)) return fail(FRQ_ERR_UNSUPPORTED, "%s: too many heads for a launch", what);
+    if (tokens * kv_heads >= ((int64_t)1 << 30)) return fail(FRQ_ERR_UNSUPPORTED, "%s: too many heads for a launch", what);
     frq::KvArgs a{cache, pages, page_tokens, kv_heads, head_dim, type, k, v, ld_k, ld_v, slots, tokens};
     hipStream_t s = static_cast<hipStream_t>(stream);
     FRQ_HIP(write ? frq::launch_kv_write(a, s) : frq::launch_kv_read(a, s));

@@ -423,39 +423,59 @@ def silu_mul(gateup, out, rows: int, inter: int, ld_in: int = 0, ld_out: int = 0
 
 # ------------------------------------------------- a block's attention step
 
+_VTYPE_OF = {**{n: i for n, i in _lib.VTYPES.items()}, **{i: i for i in _lib.VTYPES.values()}}
+
+
 def vtype_id(t) -> int:
     """Type id of activations: "f32", "f16" or "bf16" (or the id itself)."""
-    if isinstance(t, str):
-        if t.lower() not in _lib.VTYPES:
-            raise ValueError(f"activations are f32, f16 or bf16, not {t!r}")
-        return _lib.VTYPES[t.lower()]
-    return int(t)
+    i = _VTYPE_OF.get(t)
+    if i is None:
+        if isinstance(t, str):
+            i = _VTYPE_OF.get(t.lower())
+            if i is None:
+                raise ValueError(f"activations are f32, f16 or bf16, not {t!r}")
+            return i
+        return int(t)
+    return i
 
 
-def _vsize(t) -> int:
-    return 4 if vtype_id(t) == _lib.F32 else 2
+_I32, _I64 = "int32", "int64"
+_KINDS: dict = {}              # dtype object -> type id or integer kind (filled as dtypes are met)
 
 
-_TORCH_NAMES = {"torch.float32": _lib.F32, "torch.float16": _lib.F16, "torch.bfloat16": _lib.BF16,
-                "torch.int32": "int32", "torch.int64": "int64"}
+def _kind_of(dtype):
+    kind = {"torch.float32": _lib.F32, "torch.float16": _lib.F16, "torch.bfloat16": _lib.BF16, "torch.int32": _I32,
+            "torch.int64": _I64}.get(str(dtype), str(dtype))
+    _KINDS[dtype] = kind
+    return kind
 
 
-def _holds(name: str, obj, need: int, kind=None) -> None:
-    """Refuses a buffer whose size is known and too small for the call (an
-    address says nothing of its size), or a torch tensor of another type."""
-    if obj is None or isinstance(obj, int):
-        return
-    have = _TORCH_NAMES.get(str(getattr(obj, "dtype", "")))
-    if kind is not None and have is not None and have != kind:
-        raise TypeError(f"{name} is {obj.dtype}, the call says otherwise")
-    if isinstance(obj, DeviceBuffer):
-        size = obj.nbytes
-    elif hasattr(obj, "untyped_storage"):
-        size = int(obj.untyped_storage().nbytes() - obj.storage_offset() * obj.element_size())
-    else:
-        return
-    if size < need:
-        raise ValueError(f"{name} holds {size} bytes, the call needs {need}")
+def _operand(name: str, obj, need: int, kind) -> int:
+    """Address of a device operand that holds `need` bytes of `kind`. Refuses a
+    buffer whose size is known and too small, and a tensor of another type (an
+    address says nothing of either)."""
+    if obj is None:
+        return 0
+    t = type(obj)
+    if t is int:
+        return obj
+    if t is DeviceBuffer:
+        if obj.nbytes < need:
+            raise ValueError(f"{name} holds {obj.nbytes} bytes, the call needs {need}")
+        return obj.ptr
+    dtype = getattr(obj, "dtype", None)
+    if dtype is not None and hasattr(obj, "untyped_storage"):
+        have = _KINDS.get(dtype)
+        if have is None:
+            have = _kind_of(dtype)
+        if have != kind:
+            raise TypeError(f"{name} is {dtype}, the call says otherwise")
+        if obj.nbytes < need:              # a strided view reaches further than its own elements
+            size = int(obj.untyped_storage().nbytes() - obj.storage_offset() * obj.element_size())
+            if size < need:
+                raise ValueError(f"{name} holds {size} bytes, the call needs {need}")
+        return obj.data_ptr()
+    return _addr(obj)
 
 
 def _span(rows: int, ld: int, last: int) -> int:
@@ -477,23 +497,20 @@ def qk_norm_rope(x, q, k, v, tokens: int, q_heads: int, kv_heads: int, head_dim:
     size where that is known); ``q_norm`` / ``k_norm``: fp32 weights or None."""
     hd, t = int(head_dim), int(tokens)
     rot = hd if rot is None else int(rot)
-    lq, lk, lv = int(ld_q) or q_heads * hd, int(ld_k) or kv_heads * hd, int(ld_v) or kv_heads * hd
-    width = (q_heads + (1 if v is None else 2) * kv_heads) * hd
-    lx = int(ld_x) or width
-    xs, os_ = _vsize(x_dtype), _vsize(out_dtype)
+    nq, nk = q_heads * hd, kv_heads * hd
+    lq, lk, lv = ld_q or nq, ld_k or nk, ld_v or nk
+    width = nq + (nk if v is None else 2 * nk)
+    lx = ld_x or width
     xi, oi = vtype_id(x_dtype), vtype_id(out_dtype)
+    xs, os_ = (4 if xi == 0 else 2), (4 if oi == 0 else 2)
     if n_pos is None:
         n_pos = _nbytes(table) // (4 * rot) if rot and table is not None else 0
-    _holds("x", x, xs * _span(t, lx, width), xi)
-    for name, buf, ld, heads in (("q", q, lq, q_heads), ("k", k, lk, kv_heads), ("v", v, lv, kv_heads)):
-        _holds(name, buf, os_ * _span(t, ld, heads * hd), oi)
-    _holds("table", table, 4 * int(n_pos) * rot, _lib.F32)
-    _holds("positions", positions, 4 * t, "int32")
-    _holds("q_norm", q_norm, 4 * hd, _lib.F32)
-    _holds("k_norm", k_norm, 4 * hd, _lib.F32)
-    check(lib().frq_dev_qk_norm_rope(xi, _addr(x), lx, oi, _addr(q), lq, _addr(k), lk, _addr(v), lv, t, int(q_heads),
-                                     int(kv_heads), hd, rot, int(bool(interleaved)), _addr(table), int(n_pos),
-                                     _addr(positions), _addr(q_norm), _addr(k_norm), float(eps), _stream(stream)))
+    check(lib().frq_dev_qk_norm_rope(
+        xi, _operand("x", x, xs * _span(t, lx, width), xi), lx, oi, _operand("q", q, os_ * _span(t, lq, nq), oi), lq,
+        _operand("k", k, os_ * _span(t, lk, nk), oi), lk, _operand("v", v, os_ * _span(t, lv, nk), oi), lv, t, q_heads,
+        kv_heads, hd, rot, 1 if interleaved else 0, _operand("table", table, 4 * n_pos * rot, _lib.F32), n_pos,
+        _operand("positions", positions, 4 * t, _I32), _operand("q_norm", q_norm, 4 * hd, _lib.F32),
+        _operand("k_norm", k_norm, 4 * hd, _lib.F32), eps, _stream(stream)))
 
 
 def kv4_bytes(pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> int:
@@ -504,14 +521,13 @@ def kv4_bytes(pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> int
 
 
 def _kv4_args(cache, k, v, slots, tokens, dtype, ld_k, ld_v):
-    width = cache.kv_heads * cache.head_dim
-    lk, lv = int(ld_k) or width, int(ld_v) or width
-    ti, size = vtype_id(dtype), _vsize(dtype)
-    _holds("k", k, size * _span(int(tokens), lk, width), ti)
-    _holds("v", v, size * _span(int(tokens), lv, width), ti)
-    _holds("slots", slots, 8 * int(tokens), "int64")
-    return (_addr(cache), cache.nbytes, cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, ti, _addr(k), lk,
-            _addr(v), lv, _addr(slots), int(tokens))
+    width, t = cache.kv_heads * cache.head_dim, int(tokens)
+    lk, lv = ld_k or width, ld_v or width
+    ti = vtype_id(dtype)
+    size = 4 if ti == 0 else 2
+    return (cache.data_ptr(), cache.nbytes, cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, ti,
+            _operand("k", k, size * _span(t, lk, width), ti), lk, _operand("v", v, size * _span(t, lv, width), ti), lv,
+            _operand("slots", slots, 8 * t, _I64), t)
 
 
 def kv4_write(cache, k, v, slots, tokens: int, dtype="f32", ld_k: int = 0, ld_v: int = 0, stream=None) -> None:
@@ -536,20 +552,18 @@ def attn_decode(q, cache, table, lens, out, batch: int, q_heads: int, max_len: i
     default what ``max_len`` tokens need, or a 2-d tensor's own row stride);
     ``lens``: int32; no length exceeds ``max_len``. ``scale`` defaults to
     1 / sqrt(head_dim)."""
-    hd, b = cache.head_dim, int(batch)
-    lq, lo = int(ld_q) or q_heads * hd, int(ld_out) or q_heads * hd
-    per = (int(max_len) + cache.page_tokens - 1) // cache.page_tokens
-    lt = int(ld_table)
-    if not lt:
-        lt = int(table.stride(0)) if getattr(table, "ndim", 0) == 2 and hasattr(table, "stride") else per
-    ti, size = vtype_id(dtype), _vsize(dtype)
-    _holds("q", q, size * _span(b, lq, q_heads * hd), ti)
-    _holds("out", out, size * _span(b, lo, q_heads * hd), ti)
-    _holds("table", table, 4 * _span(b, lt, per), "int32")
-    _holds("lens", lens, 4 * b, "int32")
-    check(lib().frq_dev_attn_decode(ti, _addr(q), lq, _addr(cache), cache.nbytes, cache.pages, cache.page_tokens,
-                                    cache.kv_heads, hd, _addr(table), lt, _addr(lens), int(max_len), _addr(out), lo, b,
-                                    int(q_heads), hd ** -0.5 if scale is None else float(scale), _stream(stream)))
+    hd, b, n = cache.head_dim, int(batch), int(max_len)
+    nq = q_heads * hd
+    lq, lo = ld_q or nq, ld_out or nq
+    per = (n + cache.page_tokens - 1) // cache.page_tokens
+    lt = ld_table or (table.stride(0) if getattr(table, "ndim", 0) == 2 and hasattr(table, "stride") else per)
+    ti = vtype_id(dtype)
+    size = 4 if ti == 0 else 2
+    check(lib().frq_dev_attn_decode(
+        ti, _operand("q", q, size * _span(b, lq, nq), ti), lq, cache.data_ptr(), cache.nbytes, cache.pages,
+        cache.page_tokens, cache.kv_heads, hd, _operand("table", table, 4 * _span(b, lt, per), _I32), lt,
+        _operand("lens", lens, 4 * b, _I32), n, _operand("out", out, size * _span(b, lo, nq), ti), lo, b, q_heads,
+        hd ** -0.5 if scale is None else scale, _stream(stream)))
 
 
 def attn_prefill(q, k, v, out, cu_q, cu_k, seqs: int, tokens_q: int, tokens_k: int, q_heads: int, kv_heads: int,
@@ -562,18 +576,16 @@ def attn_prefill(q, k, v, out, cu_q, cu_k, seqs: int, tokens_q: int, tokens_k: i
     key back. Tokens are ``ld_*`` elements apart (default all heads side by
     side) and heads ``hs_*`` (default head_dim). ``dtype`` "bf16" or "f16";
     ``out_dtype`` the same (default) or "f32"."""
-    hd, tq, tk = int(head_dim), int(tokens_q), int(tokens_k)
-    out_dtype = dtype if out_dtype is None else out_dtype
-    hq, hk, hv, ho = (int(h) or hd for h in (hs_q, hs_k, hs_v, hs_out))
-    lq, lo = int(ld_q) or q_heads * hd, int(ld_out) or q_heads * hd
-    lk, lv = int(ld_k) or kv_heads * hd, int(ld_v) or kv_heads * hd
-    for name, buf, rows, ld, hs, heads, ty in (("q", q, tq, lq, hq, q_heads, dtype), ("k", k, tk, lk, hk, kv_heads, dtype),
-                                               ("v", v, tk, lv, hv, kv_heads, dtype),
-                                               ("out", out, tq, lo, ho, q_heads, out_dtype)):
-        _holds(name, buf, _vsize(ty) * (_span(rows, ld, _span(heads, hs, hd)) if rows else 0), vtype_id(ty))
-    _holds("cu_q", cu_q, 4 * (int(seqs) + 1), "int32")
-    _holds("cu_k", cu_k, 4 * (int(seqs) + 1), "int32")
-    check(lib().frq_dev_attn_prefill(vtype_id(dtype), _addr(q), lq, hq, _addr(k), lk, hk, _addr(v), lv, hv,
-                                     vtype_id(out_dtype), _addr(out), lo, ho, _addr(cu_q), _addr(cu_k), int(seqs), tq, tk,
-                                     int(max_q), int(max_k), int(q_heads), int(kv_heads), hd, int(bool(causal)),
-                                     hd ** -0.5 if scale is None else float(scale), _stream(stream)))
+    hd, tq, tk, n = int(head_dim), int(tokens_q), int(tokens_k), int(seqs)
+    ti = vtype_id(dtype)
+    oi = ti if out_dtype is None else vtype_id(out_dtype)
+    hq, hk, hv, ho = hs_q or hd, hs_k or hd, hs_v or hd, hs_out or hd
+    nq, nk = q_heads * hd, kv_heads * hd
+    lq, lk, lv, lo = ld_q or nq, ld_k or nk, ld_v or nk, ld_out or nq
+    check(lib().frq_dev_attn_prefill(
+        ti, _operand("q", q, 2 * _span(tq, lq, _span(q_heads, hq, hd)), ti), lq, hq,
+        _operand("k", k, 2 * _span(tk, lk, _span(kv_heads, hk, hd)), ti), lk, hk,
+        _operand("v", v, 2 * _span(tk, lv, _span(kv_heads, hv, hd)), ti), lv, hv, oi,
+        _operand("out", out, (4 if oi == 0 else 2) * _span(tq, lo, _span(q_heads, ho, hd)), oi), lo, ho,
+        _operand("cu_q", cu_q, 4 * (n + 1), _I32), _operand("cu_k", cu_k, 4 * (n + 1), _I32), n, tq, tk, int(max_q),
+        int(max_k), q_heads, kv_heads, hd, 1 if causal else 0, hd ** -0.5 if scale is None else scale, _stream(stream)))
