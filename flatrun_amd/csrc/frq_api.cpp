@@ -1322,11 +1322,11 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
         !rows_aligned(out, ld_out, os) || hs_q % 8 || hs_k % 8 || hs_v % 8 || (hs_out * os) % 16 ||
         ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) & 3))
         return fail(FRQ_ERR_ALIGN, "attn_prefill: every head's row must be 16-byte aligned, the offsets 4-byte");
-    if ((max_q + 127) / 128 * seqs > ((int64_t)1 << 31) / q_heads - 1)
+    if (((max_q + 31) / 32 + 8) * seqs > ((int64_t)1 << 31) / q_heads - 1)
         return fail(FRQ_ERR_UNSUPPORTED, "attn_prefill: more blocks than a launch takes");
     frq::PrefillArgs a{type, out_type, q,    k,    v,        ld_q,     hs_q,  ld_k,    hs_k,     ld_v,     hs_v,   out,
                        ld_out, hs_out, cu_q, cu_k, seqs, tokens_q, tokens_k, max_q, q_heads, kv_heads, head_dim, causal != 0,
-                       scale, 0};
+                       scale, 0, 0};
     FRQ_HIP(frq::launch_attn_prefill(a, static_cast<hipStream_t>(stream)));
     return FRQ_OK;
 }

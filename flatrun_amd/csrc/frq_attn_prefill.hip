@@ -9,12 +9,15 @@
 // weights are rounded to the inputs' type for the second product, as their
 // values are (the error that leaves is below the inputs' own rounding).
 //
-// A workgroup takes 128 queries of one head, a wave 32, and walks keys 64 at a
-// time through LDS. The products are S^T = K Q^T and O^T = V^T P^T: a lane then
-// holds one query's scores in both, the maximum and sum need one exchange
-// between the wave's halves, and P^T is in the registers the second product
-// reads, with the keys in the order in which S^T left them; V^T comes from the
-// row-major tile by transposing LDS reads.
+// A wave takes 32 queries of one head; the waves of a workgroup (4 or 8) the
+// heads that share a key head, then the next 32 queries, so that short
+// sequences waste little and one copy of a key tile serves all. Keys are walked
+// 64 at a time through LDS, the next tile's copy in flight. The products are
+// S^T = K Q^T and O^T = V^T P^T: a lane then holds one query's scores in both,
+// the maximum and sum need one exchange between the wave's halves, and P^T is
+// in the registers the second product reads, with the keys in the order in
+// which S^T left them; V^T comes from the row-major tile by transposing LDS
+// reads.
 #include "frq_kernels.h"
 #include "frq_vals.h"
 
@@ -126,7 +129,6 @@ __device__ __forceinline__ void stage(const uint16_t* src, int64_t ld, int rows,
 template <int TYPE, int OUT, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_kernel(PrefillArgs a) {
     constexpr int NK = D / 16, ND = D / 32, CH = D / 8;          // k-steps, column tiles, 16-byte pieces of a row
-    constexpr int kRows = 32 * WAVES;
     // Two buffers of a K and a V tile, used in turn. Objects of their own and a
     // step's code for each, so that the compiler sees that a read of one need
     // not wait for the copies into the other.
@@ -137,22 +139,25 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     const int ln = lane & 31, h = lane >> 5;
     // neighbouring workgroups go to different XCDs: give each its own key head
     uint32_t id = blockIdx.x;
-    const uint32_t hr = id % (uint32_t)a.q_heads;
-    const int kvh = (int)(hr % (uint32_t)a.kv_heads);
+    const int kvh = (int)(id % (uint32_t)a.kv_heads);
     const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
-    const int head = kvh * group + (int)(hr / (uint32_t)a.kv_heads);
-    id /= (uint32_t)a.q_heads;
-    const int seq = (int)(id % (uint32_t)a.seqs);
-    const int64_t qb = a.q_blocks - 1 - id / (uint32_t)a.seqs;   // the longest rows first
+    id /= (uint32_t)a.kv_heads;
+    const uint32_t most = (uint32_t)a.blocks, seqs = (uint32_t)a.seqs;
+    const int seq = (int)(a.together ? id % seqs : id / most);
+    const int block = (int)(most - 1 - (a.together ? id / seqs : id % most));    // the longest rows first
     const int64_t q0 = a.cu_q[seq], k0 = a.cu_k[seq];
     const int64_t nq = a.cu_q[seq + 1] - q0, nk = a.cu_k[seq + 1] - k0;
-    if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k || qb * kRows >= nq) return;
+    const int first = (int)((uint32_t)(block * WAVES) / (uint32_t)group) * 32;   // the workgroup's first query
+    if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k || first >= nq) return;
     const int past = (int)(nk - nq);
-    const int i0 = (int)qb * kRows + 32 * wave;                  // the wave's first query
+    // a wave's 32 queries of one head: the heads that share the key head side by side
+    const uint32_t unit = (uint32_t)(block * WAVES + wave);
+    const int i0 = (int)(unit / (uint32_t)group) * 32;           // the wave's first query
+    const int head = kvh * group + (int)(unit % (uint32_t)group);
     const int qi = i0 + ln;                                      // the lane's
     int end = (int)nk;                                           // keys that the workgroup needs
     if (a.causal) {
-        const int64_t e = (qb + 1) * kRows + past;
+        const int64_t e = (int64_t)((uint32_t)(block * WAVES + WAVES - 1) / (uint32_t)group) * 32 + 32 + past;
         end = (int)(e < nk ? e : nk);
     }
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + (q0 + (qi < nq ? qi : nq - 1)) * a.ld_q + head * a.hs_q;
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         // A zero weight does not take an inf or a NaN out of a product: where
         // the mask cuts through the tile, such values leave it and are added
         // below for the queries that see their keys.
-        const bool cut = a.causal && kt + kKeys - 1 > (int)qb * kRows + past;
+        const bool cut = a.causal && kt + kKeys - 1 > first + past;
         if (__builtin_expect(cut, 0)) {
             bool any = false;
             for (int at = threadIdx.x; at < kKeys * CH; at += 64 * WAVES) {
@@ -212,7 +217,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
             __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
         }
-        if (a.causal && kt > i0 + 31 + past) return;             // nothing here for the wave
+        if (i0 >= nq || (a.causal && kt > i0 + 31 + past)) return;   // nothing here for the wave
         const bool masked = kt + kKeys > nk || (a.causal && kt + kKeys - 1 > i0 + past);
         __builtin_amdgcn_s_setprio(1);                           // a wave at its products goes first
         f32x16 st[2];
@@ -327,19 +332,26 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
 
 template <int TYPE, int OUT, int D, int WAVES>
 hipError_t launch_one(PrefillArgs a, hipStream_t stream) {
-    a.q_blocks = (a.max_q + 32 * WAVES - 1) / (32 * WAVES);
-    attn_prefill_kernel<TYPE, OUT, D, WAVES><<<(unsigned)(a.q_blocks * a.seqs * a.q_heads), 64 * WAVES, 0, stream>>>(a);
+    a.blocks = ((a.max_q + 31) / 32 * (a.q_heads / a.kv_heads) + WAVES - 1) / WAVES;
+    const int64_t grid = a.blocks * a.seqs * a.kv_heads;
+    // Workgroups that all run at once go from the longest rows of any sequence to
+    // the shortest (16 sequences of 512, 14 heads of 64: 20 us against 24); more
+    // of them sequence by sequence, whose keys then stay in the L2 caches (24 of
+    // 17 to 1500 tokens after up to 1200, 32 heads of 128: 521 us against 605).
+    a.together = grid <= 1024;
+    attn_prefill_kernel<TYPE, OUT, D, WAVES><<<(unsigned)grid, 64 * WAVES, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 template <int TYPE, int OUT>
 hipError_t launch_typed(const PrefillArgs& a, hipStream_t stream) {
-#ifndef WIDE
-#define WIDE 2048
-#endif
-    const bool wide = a.max_q > WIDE;
+    // Eight waves share a key tile on long prompts of 128-wide heads (4096 tokens,
+    // 32 heads: 143 us against 156); four leave fewer idle on short ones (333
+    // tokens: 13 against 17) and suit 64-wide heads, whose bound is the
+    // exponentials (8192 tokens, 14 heads: 164 against 177).
+    const bool wide = a.max_q > 1024;
     switch (a.head_dim) {
-        case 64: return wide ? launch_one<TYPE, OUT, 64, 8>(a, stream) : launch_one<TYPE, OUT, 64, 4>(a, stream);
+        case 64: return launch_one<TYPE, OUT, 64, 4>(a, stream);
         case 128: return wide ? launch_one<TYPE, OUT, 128, 8>(a, stream) : launch_one<TYPE, OUT, 128, 4>(a, stream);
         case 256: return launch_one<TYPE, OUT, 256, 4>(a, stream);
         default: return hipErrorInvalidValue;

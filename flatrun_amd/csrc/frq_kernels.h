@@ -327,7 +327,8 @@ struct PrefillArgs {
     int64_t q_heads, kv_heads, head_dim;
     int causal;
     float scale;
-    int64_t q_blocks;            // set by the launcher
+    int64_t blocks;              // set by the launcher: workgroups of the longest sequence and a key head,
+    int together;                // and whether sequences take turns in the order of the grid
 };
 hipError_t launch_attn_prefill(PrefillArgs a, hipStream_t stream);
 

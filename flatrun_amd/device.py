@@ -463,17 +463,18 @@ def _operand(name: str, obj, need: int, kind) -> int:
         if obj.nbytes < need:
             raise ValueError(f"{name} holds {obj.nbytes} bytes, the call needs {need}")
         return obj.ptr
-    dtype = getattr(obj, "dtype", None)
-    if dtype is not None and hasattr(obj, "untyped_storage"):
-        have = _KINDS.get(dtype)
-        if have is None:
-            have = _kind_of(dtype)
-        if have != kind:
-            raise TypeError(f"{name} is {dtype}, the call says otherwise")
-        if obj.nbytes < need:              # a strided view reaches further than its own elements
-            size = int(obj.untyped_storage().nbytes() - obj.storage_offset() * obj.element_size())
-            if size < need:
-                raise ValueError(f"{name} holds {size} bytes, the call needs {need}")
+    try:
+        if _KINDS[obj.dtype] == kind and obj.nbytes >= need:
+            return obj.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    if hasattr(obj, "dtype") and hasattr(obj, "untyped_storage"):
+        if _kind_of(obj.dtype) != kind:
+            raise TypeError(f"{name} is {obj.dtype}, the call says otherwise")
+        # a strided view reaches further than its own elements
+        size = int(obj.untyped_storage().nbytes() - obj.storage_offset() * obj.element_size())
+        if size < need:
+            raise ValueError(f"{name} holds {size} bytes, the call needs {need}")
         return obj.data_ptr()
     return _addr(obj)
 
