@@ -40,8 +40,8 @@ __device__ __forceinline__ uint32_t quad(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, true);
 }
 
-// Codes of eight channels 8 sub .. 8 sub + 7 of a block, nibble i for channel
-// i, and the block's scale, from its four lanes.
+// Codes of eight channels 8 sub .. 8 sub + 7 of a block, channel i's in nibble
+// i/2 + 4 (i%2), and the block's scale, from its four lanes.
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], int sub, uint32_t& scale) {
     float hi = x[0], lo = x[0], odd = 0.f;
 #pragma unroll
@@ -74,15 +74,19 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], int sub, uint
     const float d = f16_bits_to_f32(bits), r = 1.0f / d;
     const bool none = bad || d == 0.f;
     scale = bad ? 0x7E00u : d == 0.f ? 0u : bits;
-    uint32_t word = 0;
+    uint32_t word = 0, over = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         // x / d, correctly rounded: r is, and one correction of x r leaves the
         // nearest quotient (Markstein's theorem)
         const float q = x[i] * r, y = __builtin_fmaf(__builtin_fmaf(-q, d, x[i]), r, q);
-        const int c = (int)__builtin_amdgcn_fmed3f(rintf(y), -8.f, 7.f) + 8;
-        word |= (uint32_t)c << (4 * i);
+        // 1.5 2^23 + 8 puts the code, rounded to even, into the lowest bits
+        const float c = __builtin_amdgcn_fmed3f(y, -8.f, 7.f) + 12582920.f;
+        const int at = 4 * (i / 2 + 4 * (i % 2));
+        word += __builtin_bit_cast(uint32_t, c) << at;
+        over += 0x4B400000u << at;
     }
+    word -= over;
     return none ? 0x88888888u : word;
 }
 
@@ -95,20 +99,18 @@ __device__ __forceinline__ void put(uint8_t* tile, int t, int sub, bool is_v, co
     if (j == 0)
         *reinterpret_cast<uint16_t*>(tile + (is_v ? kv_vs_off(NG) : kv_ks_off(NG)) + kv_scale(t, g, NG)) = (uint16_t)scale;
     if (!is_v) {
-        // nibbles 0 2 4 6 1 3 5 7
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (c >> (4 * i) & 15u) << (4 * (i / 2 + 4 * (i % 2)));
-        *reinterpret_cast<uint32_t*>(tile + kv_word(u * NG + g, 16 * j + (t & 15))) = w;
+        *reinterpret_cast<uint32_t*>(tile + kv_word(u * NG + g, 16 * j + (t & 15))) = c;
     } else {
         // channels 8j + i of the block: n = 8 (j % 2) + i, the upper half (j >= 2) in the high nibbles
         const int tj = (t & 15) >> 2, byte = (t & 1) * 2 + ((t & 3) >> 1);
         const uint32_t up = quad<0x4E>(c);
+        const uint32_t even = (c & 0x0F0F0F0Fu) | (up << 4 & 0xF0F0F0F0u);         // channels 0 4 1 5
+        const uint32_t odd = (c >> 4 & 0x0F0F0F0Fu) | (up & 0xF0F0F0F0u);          // channels 2 6 3 7
         if (j < 2) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 tile[kv_vc_off(NG) + kv_word(2 * g + u, 16 * tj + 8 * j + i) + byte] =
-                    (uint8_t)((c >> (4 * i) & 15u) | (up >> (4 * i) & 15u) << 4);
+                    (uint8_t)((i & 2 ? odd : even) >> (8 * ((i >> 2) + 2 * (i & 1))));
         }
     }
 }
@@ -183,31 +185,52 @@ __global__ void __launch_bounds__(256) kv_tile_kernel(KvArgs a) {
     const bool whole = s0 >= 0 && s0 + kKvTile <= slots && s0 % kKvTile == 0 &&
                        __builtin_amdgcn_ballot_w64(own != s0 + mine) == 0;
     uint4* tile = whole ? reinterpret_cast<uint4*>(kv_at(a, s0, h, NG).tile) : nullptr;
-    if (!WRITE && whole) {
-        for (int i = threadIdx.x; i < kv_tile_bytes(NG) / 16; i += 256) reinterpret_cast<uint4*>(image)[i] = tile[i];
-        __syncthreads();
+    const int64_t at0 = (int64_t)h * NG * 32 + sub * 8;
+    typename T::Elem* rows[2] = {static_cast<typename T::Elem*>(a.k) + at0, static_cast<typename T::Elem*>(a.v) + at0};
+    const int64_t ld[2] = {a.ld_k, a.ld_v};
+    const int t0 = (int)threadIdx.x / kLanes;
+    if (whole) {
+        if constexpr (WRITE) {
+            float x[2][kKvTile / kPer][8];                           // all loads under way before the first is waited for
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+                for (int i = 0; i < kKvTile / kPer; ++i) T::load8(rows[kv] + (first + t0 + i * kPer) * ld[kv], x[kv][i]);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+                for (int i = 0; i < kKvTile / kPer; ++i) put<NG>(image, t0 + i * kPer, sub, kv == 1, x[kv][i]);
+            __syncthreads();
+            for (int i = threadIdx.x; i < kv_tile_bytes(NG) / 16; i += 256) tile[i] = reinterpret_cast<const uint4*>(image)[i];
+        } else {
+            for (int i = threadIdx.x; i < kv_tile_bytes(NG) / 16; i += 256) reinterpret_cast<uint4*>(image)[i] = tile[i];
+            __syncthreads();
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+                for (int i = 0; i < kKvTile / kPer; ++i) {
+                    float x[8];
+                    get<NG>(image, t0 + i * kPer, sub, kv == 1, x);
+                    T::store8(rows[kv] + (first + t0 + i * kPer) * ld[kv], x);
+                }
+        }
+        return;
     }
+    for (int t = t0; t < count; t += kPer) {
+        const int64_t slot = a.slots[first + t];
+        const bool there = slot >= 0 && slot < slots;
+        const KvAt place = kv_at(a, there ? slot : 0, h, NG);
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        typename T::Elem* rows = static_cast<typename T::Elem*>(kv ? a.v : a.k) + (int64_t)h * NG * 32 + sub * 8;
-        const int64_t ld = kv ? a.ld_v : a.ld_k;
-#pragma unroll
-        for (int at = 0; at < kKvTile; at += kPer) {
-            const int t = at + (int)threadIdx.x / kLanes;
-            if (t >= count) continue;
+        for (int kv = 0; kv < 2; ++kv) {
+            typename T::Elem* row = rows[kv] + (first + t) * ld[kv];
             float x[8];
-            typename T::Elem* row = rows + (first + t) * ld;
-            const int64_t slot = whole ? s0 + t : a.slots[first + t];
-            const bool there = slot >= 0 && slot < slots;
             if constexpr (WRITE) {
                 if (!there) continue;
                 T::load8(row, x);
-                const KvAt to = whole ? KvAt{image, t} : kv_at(a, slot, h, NG);
-                put<NG>(to.tile, to.t, sub, kv == 1, x);
+                put<NG>(place.tile, place.t, sub, kv == 1, x);
             } else {
                 if (there) {
-                    const KvAt from = whole ? KvAt{image, t} : kv_at(a, slot, h, NG);
-                    get<NG>(from.tile, from.t, sub, kv == 1, x);
+                    get<NG>(place.tile, place.t, sub, kv == 1, x);
                 } else {
                     const float fill = slot < 0 ? 0.f : __builtin_nanf("");
 #pragma unroll
@@ -216,10 +239,6 @@ __global__ void __launch_bounds__(256) kv_tile_kernel(KvArgs a) {
                 T::store8(row, x);
             }
         }
-    }
-    if (WRITE && whole) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kv_tile_bytes(NG) / 16; i += 256) tile[i] = reinterpret_cast<const uint4*>(image)[i];
     }
 }
 

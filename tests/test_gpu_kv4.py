@@ -62,6 +62,27 @@ def test_appending_a_token_at_a_time_equals_writing_at_once(frq):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("start,n,page", [(0, 320, 32), (64, 300, 64), (13, 299, 96), (32, 257, 256)])
+@pytest.mark.parametrize("d,src", [(64, "f32"), (128, "bf16"), (256, "f16")])
+def test_runs_of_slots(frq, start, n, page, d, src):
+    """Prompts: slots one after another, from a tile's start and from within."""
+    h, pages = 2, -(-(start + n) // page) + 1
+    c = KVCache4(pages, page, h, d)
+    fill = heads(pages * page, h, d, "f32", 3)
+    c.write(fill.cuda(), fill.cuda(), dev(np.arange(pages * page)), pages * page)
+    k, v = heads(n, h, d, src, 4), heads(n, h, d, src, 5)
+    slots = np.arange(start, start + n)
+    c.write(k.cuda(), v.cuda(), dev(slots), n, dtype=src)
+    one = [np.concatenate([f64(x) for x in part]) for part in zip(*(read(c, [i]) for i in range(pages * page)))]
+    want = [block4(f64(fill)) for _ in range(2)]
+    for w, x in zip(want, (k, v)):
+        w[start:start + n] = block4(f64(x))
+    for a, b, w in zip(one, read(c, np.arange(pages * page)), want):
+        assert np.array_equal(a, w) and np.array_equal(f64(b), w)
+    for a, w in zip(read(c, slots), want):
+        assert np.array_equal(f64(a), w[start:start + n])
+
+
 def test_edges(frq):
     x = torch.zeros((12, 1, 64))
     x[0, 0, 3], x[0, 0, 9] = 5.0, -5.0             # the first of equals gives the sign
