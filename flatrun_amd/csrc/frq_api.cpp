@@ -1314,6 +1314,8 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
     const int64_t strides[8] = {ld_q, hs_q, ld_k, hs_k, ld_v, hs_v, ld_out, hs_out};
     for (int64_t s : strides)
         if (!in_range(s, head_dim, kMaxLd)) return fail(FRQ_ERR_SHAPE, "attn_prefill: a stride is shorter than a head");
+    if (ld_k >= (int64_t)1 << 24 || ld_v >= (int64_t)1 << 24)    // offsets inside a tile of 64 keys are 32-bit
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_prefill: keys or values 2^24 elements or more apart");
     if (!(scale > 0.f && scale < __builtin_inff())) return fail(FRQ_ERR_INVALID, "attn_prefill: scale must be positive");
     if (seqs == 0 || max_q == 0) return FRQ_OK;
     if (!q || !out || !cu_q || !cu_k || (tokens_k && (!k || !v))) return fail(FRQ_ERR_INVALID, "null buffer");

@@ -110,7 +110,8 @@ __device__ __forceinline__ uint4 read_row8(lds_bytes p) {
 }
 
 // Asynchronous copy of a tile of kKeys rows (`rows` of them present, the others
-// become zeros) to LDS, 16 bytes a lane and step, swizzled on the way.
+// become zeros) to LDS, 16 bytes a lane and step, swizzled on the way. The host
+// keeps a tile's bytes, kKeys rows of ld, below 2^31.
 template <int D, int WAVES>
 __device__ __forceinline__ void stage(const uint16_t* src, int64_t ld, int rows, uint16_t* tile) {
     constexpr int CH = D / 8, kSteps = kKeys * CH / (64 * WAVES);
@@ -186,8 +187,9 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
 
     if (threadIdx.x == 0) special_at = 0;
     if (end > 0) {
-        stage<D, WAVES>(kp, a.ld_k, (int)nk, lk0);
-        stage<D, WAVES>(vp, a.ld_v, (int)nk, lv0);
+        const int rows = nk < kKeys ? (int)nk : kKeys;
+        stage<D, WAVES>(kp, a.ld_k, rows, lk0);
+        stage<D, WAVES>(vp, a.ld_v, rows, lv0);
     }
     auto step = [&](int kt, uint16_t* ck, uint16_t* cv, uint16_t* tk, uint16_t* tv) __attribute__((always_inline)) {
         // this tile is there, and everyone is done with the other buffer

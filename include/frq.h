@@ -443,10 +443,13 @@ int frq_dev_kv4_read(const void* cache, size_t cache_bytes, int64_t pages, int64
  * t is in page table[b * ld_table + t / page_tokens]. fp32 precision
  * throughout (q and the weights enter the products as two fp16 parts, 22
  * bits). lens[b] = 0: zeros. lens[b] > max_len or a page outside the cache:
- * NaN. Long sequences are split over workgroups, whose partial results (4
- * (head_dim + 2) bytes per query head and split) use the stream's scratch and
- * are joined in a fixed order; the split depends on max_len and the shapes
- * only. */
+ * NaN. Where sequences are long their tiles are shared out evenly over at most
+ * 512 workgroups, whose partial results (two sets of 8 (head_dim + 2) floats a
+ * workgroup) use the stream's scratch and are joined in a fixed order. The
+ * division follows from lens, max_len and the shapes: the same call gives the
+ * same bits, but a sequence's last bits may change with its neighbours'
+ * lengths. max_len up to 2^29, and batch, key heads and tiles together below
+ * 2^31. */
 int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
                         int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
                         const int32_t* lens, int64_t max_len, void* out, int64_t ld_out, int64_t batch, int64_t q_heads,
@@ -460,7 +463,8 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
  * not see never reach it, infinities and NaN included. Inputs F16 or BF16 (one
  * type), scores and sums fp32, the softmax weights rounded to the inputs' type
  * for their product with v; out of that type or F32. head_dim 64, 128 or 256.
- * A sequence whose offsets leave the buffers is not computed. */
+ * ld_k and ld_v below 2^24. A sequence whose offsets leave the buffers is not
+ * computed. */
 int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
                          const void* v, int64_t ld_v, int64_t hs_v, int out_type, void* out, int64_t ld_out,
                          int64_t hs_out, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tokens_q,

@@ -82,6 +82,8 @@ REFUSED = [
     (prefill, dict(hs_k=64), _lib.ERR_SHAPE),
     (prefill, dict(head_dim=96), _lib.ERR_UNSUPPORTED),
     (prefill, dict(ld_v=257), _lib.ERR_ALIGN),
+    (prefill, dict(ld_k=1 << 24), _lib.ERR_UNSUPPORTED),
+    (prefill, dict(ld_v=1 << 24), _lib.ERR_UNSUPPORTED),
     (prefill, dict(hs_q=132), _lib.ERR_ALIGN),
     (prefill, dict(q=0x10002), _lib.ERR_ALIGN),
 ]
