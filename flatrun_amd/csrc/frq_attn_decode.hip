@@ -197,7 +197,10 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
         k = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(begin + line.upto * pairs > at));
     }
     const lds_bytes sp = (lds_bytes)sh_p + wave * (NG * 1024);
-    const lds_bytes sp_to = sp + n * 32 + j * 8, sp_from = sp + lane * 8;
+    // a token's row of weights, its pieces in an order by which half a wave's
+    // writes touch every bank once
+    const int row = lane >> 2;
+    const lds_bytes sp_to = sp + n * 32 + (j ^ (n >> 3 << 1)) * 8, sp_from = sp + row * 32 + ((lane & 3) ^ (row >> 3 << 1)) * 8;
 
     for (;;) {
         if (shared) {                                                // tiles [first, last) of a pair of sequence b
