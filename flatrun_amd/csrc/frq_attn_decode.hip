@@ -163,10 +163,10 @@ struct Line {
 template <int TYPE, int NG>
 __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kernel(DecodeArgs a) {
     using T = Val<TYPE>;
-    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG);
+    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRow = D + 8;   // 16 banks from the row of the next j
     // the waves' weights [group][token][row], and their results
     __shared__ __attribute__((aligned(16))) char sh_p[kWaves * NG * 1024];
-    __shared__ float sh_o[kWaves * 8 * D], sh_m[kWaves][8], sh_l[kWaves][8];
+    __shared__ float sh_o[kWaves * 8 * kRow], sh_m[kWaves][8], sh_l[kWaves][8];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, j = lane >> 4;
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
             const float fo = __builtin_amdgcn_exp2f(held_ref[i] - base), fn = __builtin_amdgcn_exp2f(ref[i] - base);
             held_l[i] = held_l[i] * fo + l[i] * fn;
             held_ref[i] = both;
-            float* to = sh_o + (wave * 8 + 2 * j + i) * D + n;
+            float* to = sh_o + (wave * 8 + 2 * j + i) * kRow + n;
 #pragma unroll
             for (int c = 0; c < 2 * NG; ++c) {
                 const float x = (o[c][2 * i] + o[c][2 * i + 1]) * fn;
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
             for (int w = 0; w < kWaves; ++w) {
                 const float f = __builtin_amdgcn_exp2f(sh_m[w][r] - base);
                 sum += f * sh_l[w][r];
-                val += f > 0.f ? f * sh_o[(w * 8 + r) * D + c] : 0.f;    // a wave without tiles wrote none
+                val += f > 0.f ? f * sh_o[(w * 8 + r) * kRow + c] : 0.f;    // a wave without tiles wrote none
             }
             if (whole) {
                 const int64_t h = (int64_t)kvh * group + 8 * hc + r;
