@@ -17,15 +17,27 @@
 // and both numbers of two heads, so scores, weights and their scales need no
 // other lane; the weights pass through LDS, a wave's own part of it, to stand
 // as the second product's operand (transposing reads). The reference that the
-// exponentials are taken from follows the running maximum only when that is
-// 2^8 ahead, so sums are rarely rescaled and the maximum over lanes is rarely
-// taken. The next step's tile is loaded while this one is worked on.
+// exponentials are taken from, and E, are those of a wave's first tile. A tile
+// whose scores pass the reference by more than 2^8, or whose scales pass E, ends
+// the run: sums and reference go to LDS, where runs and later waves are joined
+// under the larger one, and the wave starts anew from that tile. So the loop
+// has no rescaling and no maximum over lanes. Two tiles are on their way while
+// one is worked on, 9.2 KB a wave at 128 channels.
 //
 // The tiles of all sequences and key heads, one after another, are shared out
 // evenly over the workgroups, whatever the lengths are; the four waves of a
 // workgroup take its tiles in turn and meet in LDS. A row that several
-// workgroups worked on is joined, in their order, by a second, small kernel.
+// workgroups worked on is joined, in their order, by a second, small kernel
+// (joined by the last workgroup to finish instead, the release between XCDs
+// costs what the launch does: 131072 tokens 42 us, 64 ragged sequences the same).
 // Short sequences have one workgroup per sequence and key head, and no joining.
+//
+// 131072 tokens of 8 key heads of 128, 32 query heads: 35 us and 4.6 for the
+// joining, 151 MB at 4.3 TB/s (reads alone reach 6.1): 4 us until the first tile
+// is there, 2 for the end, the rest at 5.2 TB/s. 64 sequences of 1 to 8192
+// tokens: 69 and 6 us, 4.6 TB/s; vector instructions (unpacking, weights) are
+// then issued 53 % of the time, the matrix cores work 11 %. 16 sequences of
+// 2000 to 4096, 4 key heads: 15 and 4 us, of which the loads are a third.
 #include "frq_kernels.h"
 #include "frq_kv4.h"
 

@@ -18,6 +18,16 @@
 // in the registers the second product reads, with the keys in the order in
 // which S^T left them; V^T comes from the row-major tile by transposing LDS
 // reads.
+//
+// 16384 tokens of 32 heads of 128 over 8, causal, bf16: 1.9 to 2.0 ms, 1.1 to
+// 1.16 PFLOP/s, where a large plain product reaches 1.35: the matrix cores are
+// busy 58 % of the time and vector instructions 39 %, at the 1.86 GHz that the
+// power leaves; the LDS 30 %, without conflicts. 24 sequences of 17 to 1500
+// tokens after up to 1200: 444 us, 845 TFLOP/s, matrix cores 41 %, 2.07 GHz: a
+// workgroup's start and end, its two tiles cut by the mask and what its 18 tiles
+// round up to. Workgroups that stay and take the next block of queries from a
+// queue, its tile loaded ahead, gave 435 there, nothing on the long prompt and
+// 13.7 against 12.7 us on a short one.
 #include "frq_kernels.h"
 #include "frq_vals.h"
 

@@ -16,9 +16,10 @@ The projections are frq_dev_gemv_group / frq_dev_gemv launches (fp32
 contract, 1e-5 of fp64); gate, up and SiLU·mul are frq_dev_gemv_swiglu (one
 launch for a Q4_K pair at batch 1, the grouped launch and frq_dev_silu_mul
 otherwise, same bits); all on one stream.
-Attention, RoPE, norms and residuals are not quantized matvecs; the caller
-supplies them as functions on device buffers (or does them itself between
-:meth:`qkv`, :meth:`o` and :meth:`mlp`).
+Attention, norms and residuals are not quantized matvecs; the caller supplies
+them as functions on device buffers (or does them itself between :meth:`qkv`,
+:meth:`o` and :meth:`mlp`). :class:`flatrun_amd.attention.BlockAttention` is
+such a function for the attention, rotary positions and 4-bit cache included.
 
 o_proj is a projection like the others here. In the reference its native
 branch never runs: o's weight comes from ``_fetch_linear_with_quant`` ->
