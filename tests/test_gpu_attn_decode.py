@@ -197,3 +197,64 @@ def test_graph_replays(frq):
         assert torch.equal(replay, out)
     s.check(f64(out))
     g.destroy()
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d", [
+    ([0] * 70 + [1400, 0, 1, 33] + [0] * 64 + [1000], 4, 2, 64),     # empty stretches longer than a wave's lanes
+    ([1500, 7, 0, 901], 24, 1, 128),                                 # three chunks of query heads to a key head
+    ([1000, 1, 1203], 8, 4, 256),
+    ([3] * 30 + [2200] + [40] * 33, 8, 8, 64),                       # a pair at least for every workgroup
+    ([0, 0, 950], 14, 2, 128),
+])
+def test_sequences_that_share_the_workgroups(frq, lens, hq, hkv, d):
+    s = Setup(lens, hq, hkv, d, 32, seed=len(lens) + d)
+    got = s.run()
+    assert np.all(got[np.array(lens) == 0] == 0)
+    s.check(got)
+    assert np.array_equal(got, s.run())
+
+
+def test_growth_and_special_values_in_shared_sequences(frq):
+    """References that are outgrown, bad lengths, pages and values where rows
+    are joined from several workgroups."""
+    s = Setup([2000, 1200, 0, 1300], 8, 2, 64, 32, seed=11)
+    s.v[:2000] *= np.exp(np.linspace(-9, 9, 2000))[:, None, None].astype(np.float32)
+    s.k[2000:3200] *= np.linspace(0.01, 6, 1200)[:, None, None].astype(np.float32)
+    s.cache.write(dev(s.k), dev(s.v), dev(s.slots), 4500)
+    clean = s.run()
+    s.check(clean)
+    s.q[0, 5, 3] = float("nan")
+    got = s.run()
+    assert np.isnan(got[0, 5]).all()
+    got[0, 5] = clean[0, 5]
+    assert np.array_equal(got, clean)
+    s = Setup([2000, 1200, 0, 1300], 8, 2, 64, 32, seed=12)
+    clean = s.run()
+    s.table[0, 60] = s.cache.pages                           # of its last tiles
+    got = s.run()
+    assert np.isnan(got[0]).all() and np.array_equal(got[1:], clean[1:])
+    got = s.run(max_len=1999)
+    assert np.isnan(got[0]).all() and np.all(got[2] == 0) and np.isfinite(got[1:]).all()
+
+
+def test_offsets_past_32_bits(frq):
+    """A cache of 5 GiB, the sequence's pages at its end."""
+    c = KVCache4(1200, 4096, 8, 128)
+    g = torch.Generator().manual_seed(13)
+    k, v, q = (torch.randn((n, h, 128), generator=g) for n, h in ((300, 8), (300, 8), (1, 16)))
+    t = np.arange(300)
+    page = np.where(t < 100, 1199, 1100)                     # places 3996 .. 4095 of one page, then of another
+    place = np.where(t < 100, 3996 + t, t - 100)
+    pad = np.arange(3996)
+    c.write(dev(np.zeros((3996, 8, 128), np.float32)), dev(np.zeros((3996, 8, 128), np.float32)), dev(1199 * 4096 + pad), 3996)
+    c.write(k.cuda(), v.cuda(), dev((page * 4096 + place).astype(np.int64)), 300)
+    out = torch.zeros((1, 16, 128), device="cuda")
+    device.attn_decode(q.cuda(), c, dev(np.array([[1199, 1100]], np.int32)), dev(np.array([4296], np.int32)), out, 1, 16,
+                       4296)
+    torch.cuda.synchronize()
+    kk, vv = (np.concatenate([np.zeros((3996, 8, 128)), block4(f64(x))]) for x in (k, v))
+    got = f64(out)
+    for h in range(16):
+        want, mag, size = attend(f64(q)[:, h], kk[:, h // 2], vv[:, h // 2], 128 ** -0.5, np.array([4295]))
+        assert np.all(np.abs(got[:, h] - want) <= fp32_bound(mag, size, 4296, 128)), h
+    c.close()

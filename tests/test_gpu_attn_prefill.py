@@ -164,3 +164,39 @@ def test_offsets_that_leave_the_buffers_are_not_computed(frq):
     s.cu[1] = dev(np.array([0, 20, 40, 61], np.int32))
     got = s.run()
     assert np.array_equal(got[:40], clean[:40]) and np.all(got[40:] == 5.0)
+
+
+def test_offsets_past_32_bits(frq):
+    """Keys and values 2 MiB apart: 2100 of them span more than 2^32 bytes, and
+    a tile of 64 more than 2^26."""
+    s = Setup([70], [2100], 2, 1, 64, seed=9)
+    clean = s.run()
+    ld = 1 << 20
+    wide = torch.empty(2099 * ld + 128, dtype=torch.bfloat16, device="cuda")
+    rows = torch.as_strided(wide, (2100, 128), (ld, 1))
+    rows[:, :64] = s.k[:, 0].cuda()
+    rows[:, 64:] = s.v[:, 0].cuda()
+    out = torch.zeros((70, 2, 64), dtype=torch.bfloat16, device="cuda")
+    device.attn_prefill(s.q.cuda(), wide.data_ptr(), wide.data_ptr() + 128, out, *s.cu, 1, 70, 2100, 2, 1, 64, 70, 2100,
+                        ld_k=ld, ld_v=ld)
+    torch.cuda.synchronize()
+    assert np.array_equal(f64(out), clean)
+
+
+@pytest.mark.parametrize("nq,nk,hq,hkv", [([1100, 40, 0, 513], [1100, 700, 9, 600], 4, 2), ([1030], [1090], 12, 4),
+                                          ([1025, 1], [1025, 1], 5, 1)])
+def test_long_packed_heads_of_128(frq, nq, nk, hq, hkv):
+    """More than 1024 queries: eight waves to a key tile."""
+    s = Setup(nq, nk, hq, hkv, 128, seed=sum(nq))
+    s.check(s.run(), heads=range(0, hq, 3))
+
+
+def test_special_values_in_masked_places_of_long_prompts(frq):
+    s = Setup([1100], [1100], 4, 1, 128, seed=10)
+    clean = s.run()
+    s.v[1040, 0, 5], s.v[1041, 0, 6] = float("inf"), float("nan")
+    got = s.run()
+    assert np.array_equal(got[:1040], clean[:1040])
+    assert np.all(got[1040:, :, 5] == np.inf) and np.isnan(got[1041:, :, 6]).all()
+    got[1040:, :, 5:7] = clean[1040:, :, 5:7]
+    assert np.array_equal(got, clean)
