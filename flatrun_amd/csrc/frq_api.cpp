@@ -1327,7 +1327,7 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
     if (((max_q + 31) / 32 + 8) * seqs > ((int64_t)1 << 31) / q_heads - 1)
         return fail(FRQ_ERR_UNSUPPORTED, "attn_prefill: more blocks than a launch takes");
     frq::PrefillArgs a{type, out_type, q,    k,    v,        ld_q,     hs_q,  ld_k,    hs_k,     ld_v,     hs_v,   out,
-                       ld_out, hs_out, cu_q, cu_k, seqs, tokens_q, tokens_k, max_q, q_heads, kv_heads, head_dim, causal != 0,
+                       ld_out, hs_out, cu_q, cu_k, seqs, tokens_q, tokens_k, max_q, max_k, q_heads, kv_heads, head_dim, causal != 0,
                        scale, 0, 0};
     FRQ_HIP(frq::launch_attn_prefill(a, static_cast<hipStream_t>(stream)));
     return FRQ_OK;

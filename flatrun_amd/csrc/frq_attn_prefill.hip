@@ -11,8 +11,10 @@
 //
 // A wave takes 32 queries of one head; the waves of a workgroup (4 or 8) the
 // heads that share a key head, then the next 32 queries, so that short
-// sequences waste little and one copy of a key tile serves all. Keys are walked
-// 64 at a time through LDS, the next tile's copy in flight. The products are
+// sequences waste little and one copy of a key tile serves all. Where there are
+// few queries two waves share them, each with every other tile, and join at the
+// end. Keys are walked 64 (then 128) at a time through LDS, the next copy in
+// flight. The products are
 // S^T = K Q^T and O^T = V^T P^T: a lane then holds one query's scores in both,
 // the maximum and sum need one exchange between the wave's halves, and P^T is
 // in the registers the second product reads, with the keys in the order in
@@ -137,15 +139,17 @@ __device__ __forceinline__ void stage(const uint16_t* src, int64_t ld, int rows,
     }
 }
 
-template <int TYPE, int OUT, int D, int WAVES>
+template <int TYPE, int OUT, int D, int WAVES, int SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_kernel(PrefillArgs a) {
+    constexpr int kUnits = WAVES / SPLIT;                        // of 32 queries of a head
     constexpr int NK = D / 16, ND = D / 32, CH = D / 8;          // k-steps, column tiles, 16-byte pieces of a row
     // Two buffers of a K and a V tile, used in turn. Objects of their own and a
     // step's code for each, so that the compiler sees that a read of one need
     // not wait for the copies into the other.
     constexpr int kTile = kKeys * D;
     __shared__ int special_at;
-    __shared__ __attribute__((aligned(16))) uint16_t lk0[kTile], lv0[kTile], lk1[kTile], lv1[kTile];
+    __shared__ __attribute__((aligned(16))) uint16_t lk0[SPLIT * kTile], lv0[SPLIT * kTile];
+    __shared__ __attribute__((aligned(16))) uint16_t lk1[SPLIT * kTile], lv1[SPLIT * kTile];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 31, h = lane >> 5;
     // neighbouring workgroups go to different XCDs: give each its own key head
@@ -158,17 +162,18 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     const int block = (int)(most - 1 - (a.together ? id / seqs : id % most));    // the longest rows first
     const int64_t q0 = a.cu_q[seq], k0 = a.cu_k[seq];
     const int64_t nq = a.cu_q[seq + 1] - q0, nk = a.cu_k[seq + 1] - k0;
-    const int first = (int)((uint32_t)(block * WAVES) / (uint32_t)group) * 32;   // the workgroup's first query
+    const int first = (int)((uint32_t)(block * kUnits) / (uint32_t)group) * 32;   // the workgroup's first query
     if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k || first >= nq) return;
     const int past = (int)(nk - nq);
     // a wave's 32 queries of one head: the heads that share the key head side by side
-    const uint32_t unit = (uint32_t)(block * WAVES + wave);
+    const int part = SPLIT > 1 ? wave / kUnits : 0;              // which of SPLIT tiles at a time is the wave's
+    const uint32_t unit = (uint32_t)(block * kUnits + (SPLIT > 1 ? wave % kUnits : wave));
     const int i0 = (int)(unit / (uint32_t)group) * 32;           // the wave's first query
     const int head = kvh * group + (int)(unit % (uint32_t)group);
     const int qi = i0 + ln;                                      // the lane's
     int end = (int)nk;                                           // keys that the workgroup needs
     if (a.causal) {
-        const int64_t e = (int64_t)((uint32_t)(block * WAVES + WAVES - 1) / (uint32_t)group) * 32 + 32 + past;
+        const int64_t e = (int64_t)((uint32_t)(block * kUnits + kUnits - 1) / (uint32_t)group) * 32 + 32 + past;
         end = (int)(e < nk ? e : nk);
     }
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + (q0 + (qi < nq ? qi : nq - 1)) * a.ld_q + head * a.hs_q;
@@ -196,40 +201,42 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     const int vat1 = (4 * h + r4 + 8) * D * 2 + 16 * (x4 ^ swizzle<CH>(4 * h + r4 + 8)) + 8 * (lane & 1);
 
     if (threadIdx.x == 0) special_at = 0;
-    if (end > 0) {
-        const int rows = nk < kKeys ? (int)nk : kKeys;
-        stage<D, WAVES>(kp, a.ld_k, rows, lk0);
-        stage<D, WAVES>(vp, a.ld_v, rows, lv0);
-    }
-    auto step = [&](int kt, uint16_t* ck, uint16_t* cv, uint16_t* tk, uint16_t* tv) __attribute__((always_inline)) {
+    auto stage_all = [&](int kt, uint16_t* tk, uint16_t* tv) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < SPLIT; ++x) {
+            const int left = (int)nk - kt - x * kKeys, rows = left < kKeys ? left : kKeys;
+            stage<D, WAVES>(kp + (int64_t)(kt + x * kKeys) * a.ld_k, a.ld_k, rows, tk + x * kTile);
+            stage<D, WAVES>(vp + (int64_t)(kt + x * kKeys) * a.ld_v, a.ld_v, rows, tv + x * kTile);
+        }
+    };
+    constexpr int kStep = SPLIT * kKeys;
+    if (end > 0) stage_all(0, lk0, lv0);
+    auto step = [&](int at, uint16_t* ck, uint16_t* cv, uint16_t* tk, uint16_t* tv) __attribute__((always_inline)) {
         // this tile is there, and everyone is done with the other buffer
         __builtin_amdgcn_s_waitcnt(0x0070);                      // vmcnt(0), lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
-        const lds_bytes sk = (lds_bytes)ck, sv = (lds_bytes)cv;
-        if (kt + kKeys < end) {
-            const int left = (int)nk - kt - kKeys;
-            stage<D, WAVES>(kp + (int64_t)(kt + kKeys) * a.ld_k, a.ld_k, left < kKeys ? left : kKeys, tk);
-            stage<D, WAVES>(vp + (int64_t)(kt + kKeys) * a.ld_v, a.ld_v, left < kKeys ? left : kKeys, tv);
-        }
+        const lds_bytes sk = (lds_bytes)ck + part * (2 * kTile), sv = (lds_bytes)cv + part * (2 * kTile);
+        if (at + kStep < end) stage_all(at + kStep, tk, tv);
         // A zero weight does not take an inf or a NaN out of a product: where
         // the mask cuts through the tile, such values leave it and are added
         // below for the queries that see their keys.
-        const bool cut = a.causal && kt + kKeys - 1 > first + past;
+        const bool cut = a.causal && at + kStep - 1 > first + past;
         if (__builtin_expect(cut, 0)) {
             bool any = false;
-            for (int at = threadIdx.x; at < kKeys * CH; at += 64 * WAVES) {
-                u32x4 w = reinterpret_cast<const u32x4*>(cv)[at];
+            for (int i = threadIdx.x; i < kStep * CH; i += 64 * WAVES) {
+                u32x4 w = reinterpret_cast<const u32x4*>(cv)[i];
                 const u32x4 s = {specials<TYPE>(w[0]), specials<TYPE>(w[1]), specials<TYPE>(w[2]), specials<TYPE>(w[3])};
                 if (s[0] | s[1] | s[2] | s[3]) {
                     any = true;
-                    reinterpret_cast<u32x4*>(cv)[at] = w & ~s;
+                    reinterpret_cast<u32x4*>(cv)[i] = w & ~s;
                 }
             }
-            if (any) special_at = kt + 1;
+            if (any) special_at = at + 1;
             __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
         }
-        if (i0 >= nq || (a.causal && kt > i0 + 31 + past)) return;   // nothing here for the wave
+        const int kt = at + part * kKeys;
+        if (i0 >= nq || (SPLIT > 1 && kt >= nk) || (a.causal && kt > i0 + 31 + past)) return;   // nothing here for the wave
         const bool masked = kt + kKeys > nk || (a.causal && kt + kKeys - 1 > i0 + past);
         __builtin_amdgcn_s_setprio(1);                           // a wave at its products goes first
         f32x16 st[2];
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
                 o[d] = mfma<TYPE>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[s], o[d]);
             }
         }
-        if (__builtin_expect(cut && special_at == kt + 1, 0)) {
+        if (__builtin_expect(cut && special_at == at + 1, 0)) {
             for (int kr = 0; kr < kKeys && kt + kr < nk; ++kr) {
                 const uint16_t* row = vp + (int64_t)(kt + kr) * a.ld_v + 4 * h;
                 const bool seen = kt + kr <= lim;
@@ -318,11 +325,44 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
             }
         }
     };
-    for (int kt = 0; kt < end; kt += 2 * kKeys) {
-        step(kt, lk0, lv0, lk1, lv1);
-        if (kt + kKeys < end) step(kt + kKeys, lk1, lv1, lk0, lv0);
+    for (int at = 0; at < end; at += 2 * kStep) {
+        step(at, lk0, lv0, lk1, lv1);
+        if (at + kStep < end) step(at + kStep, lk1, lv1, lk0, lv0);
     }
     l += __shfl_xor(l, 32);
+    if constexpr (SPLIT == 2) {
+        // the second half's sums to the first, in the place of the tiles
+        __shared__ float sh_m[kUnits][32], sh_l[kUnits][32];
+        const int u = wave % kUnits;
+        float4* held = reinterpret_cast<float4*>((u < 2 ? lk0 : lv0) + (u & 1) * kTile) + lane;
+        __syncthreads();
+        if (part == 1) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    held[16 * (16 * d + i)] = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+            if (h == 0) {
+                sh_m[u][ln] = m;
+                sh_l[u][ln] = l;
+            }
+        }
+        __syncthreads();
+        if (part == 1) return;
+        const float m1 = sh_m[u][ln], both = __builtin_fmaxf(m, m1), base = both == -__builtin_inff() ? 0.f : both;
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
+        l = l * f0 + sh_l[u][ln] * f1;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 x = held[16 * (16 * d + i)];
+                o[d][i] = o[d][i] * f0 + x.x * f1;
+                o[d][i + 1] = o[d][i + 1] * f0 + x.y * f1;
+                o[d][i + 2] = o[d][i + 2] * f0 + x.z * f1;
+                o[d][i + 3] = o[d][i + 3] * f0 + x.w * f1;
+            }
+    }
     if (qi >= nq) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     using O = Val<OUT>;
@@ -342,30 +382,42 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         }
 }
 
-template <int TYPE, int OUT, int D, int WAVES>
+template <int TYPE, int OUT, int D, int WAVES, int SPLIT>
 hipError_t launch_one(PrefillArgs a, hipStream_t stream) {
-    a.blocks = ((a.max_q + 31) / 32 * (a.q_heads / a.kv_heads) + WAVES - 1) / WAVES;
+    constexpr int kUnits = WAVES / SPLIT;
+    a.blocks = ((a.max_q + 31) / 32 * (a.q_heads / a.kv_heads) + kUnits - 1) / kUnits;
     const int64_t grid = a.blocks * a.seqs * a.kv_heads;
     // Workgroups that all run at once go from the longest rows of any sequence to
     // the shortest (16 sequences of 512, 14 heads of 64: 20 us against 24); more
     // of them sequence by sequence, whose keys then stay in the L2 caches (24 of
     // 17 to 1500 tokens after up to 1200, 32 heads of 128: 521 us against 605).
     a.together = grid <= 1024;
-    attn_prefill_kernel<TYPE, OUT, D, WAVES><<<(unsigned)grid, 64 * WAVES, 0, stream>>>(a);
+    attn_prefill_kernel<TYPE, OUT, D, WAVES, SPLIT><<<(unsigned)grid, 64 * WAVES, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 template <int TYPE, int OUT>
 hipError_t launch_typed(const PrefillArgs& a, hipStream_t stream) {
-    // Eight waves share a key tile on long prompts of 128-wide heads (4096 tokens,
-    // 32 heads: 143 us against 156); four leave fewer idle on short ones (333
-    // tokens: 13 against 17) and suit 64-wide heads, whose bound is the
-    // exponentials (8192 tokens, 14 heads: 164 against 177).
-    const bool wide = a.max_q > 1024;
+    // Where every wave's 32 queries have a SIMD of their own to spare, two waves
+    // share them, a tile each at a time: with at most 512 such units in workgroups
+    // of four waves, with at most 1024 of eight (1024 tokens, 14 heads of 64: 12.8
+    // us against 20.1; 1000 after 1000, 32 heads of 128: 41.5 against 47.6; 100
+    // after 1500, twice: 30.0 against 35.2; 384, 16 heads: 12.9 against 13.5). Below
+    // 384 keys the joining costs what it gains (333: 13.3 both, 128: 11.6, 11.0).
+    // Else eight waves share a key tile on long prompts of 128-wide heads (4096
+    // tokens, 32 heads: 143 us against 156); four leave fewer idle on short ones
+    // and suit 64-wide heads, whose bound is the exponentials (8192 tokens, 14
+    // heads: 164 against 177).
+    const int64_t units = (a.max_q + 31) / 32 * a.q_heads * a.seqs;
+    const bool half = a.max_k >= 384 && units <= 1024, little = units <= 512;
     switch (a.head_dim) {
-        case 64: return launch_one<TYPE, OUT, 64, 4>(a, stream);
-        case 128: return wide ? launch_one<TYPE, OUT, 128, 8>(a, stream) : launch_one<TYPE, OUT, 128, 4>(a, stream);
-        case 256: return launch_one<TYPE, OUT, 256, 4>(a, stream);
+        case 64:
+            if (half) return little ? launch_one<TYPE, OUT, 64, 4, 2>(a, stream) : launch_one<TYPE, OUT, 64, 8, 2>(a, stream);
+            return launch_one<TYPE, OUT, 64, 4, 1>(a, stream);
+        case 128:
+            if (half) return little ? launch_one<TYPE, OUT, 128, 4, 2>(a, stream) : launch_one<TYPE, OUT, 128, 8, 2>(a, stream);
+            return a.max_q > 1024 ? launch_one<TYPE, OUT, 128, 8, 1>(a, stream) : launch_one<TYPE, OUT, 128, 4, 1>(a, stream);
+        case 256: return launch_one<TYPE, OUT, 256, 4, 1>(a, stream);
         default: return hipErrorInvalidValue;
     }
 }

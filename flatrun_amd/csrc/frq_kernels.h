@@ -323,7 +323,7 @@ struct PrefillArgs {
     void* out;
     int64_t ld_out, hs_out;
     const int32_t *cu_q, *cu_k;
-    int64_t seqs, tokens_q, tokens_k, max_q;
+    int64_t seqs, tokens_q, tokens_k, max_q, max_k;
     int64_t q_heads, kv_heads, head_dim;
     int causal;
     float scale;

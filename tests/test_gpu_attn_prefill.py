@@ -200,3 +200,30 @@ def test_special_values_in_masked_places_of_long_prompts(frq):
     assert np.all(got[1040:, :, 5] == np.inf) and np.isnan(got[1041:, :, 6]).all()
     got[1040:, :, 5:7] = clean[1040:, :, 5:7]
     assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("nq,nk,hq,hkv,d,causal", [
+    ([384], [384], 2, 1, 64, True), ([33, 1, 0, 200], [640, 385, 3, 200], 4, 2, 128, True),
+    ([40, 450], [449, 300], 2, 2, 64, False), ([300, 20], [400, 0], 6, 2, 128, False),
+    ([700], [700], 28, 4, 128, True), ([900, 31], [1000, 64], 14, 2, 64, True),
+    ([200] * 7, [390] * 7, 32, 8, 128, True), ([1100], [1100], 32, 8, 128, True),
+])
+def test_few_queries_and_many(frq, nq, nk, hq, hkv, d, causal):
+    """Tiles of a unit shared by two waves, in workgroups of four and of eight,
+    and enough units that none are."""
+    s = Setup(nq, nk, hq, hkv, d, seed=sum(nk) + d)
+    got = s.run(causal=causal)
+    s.check(got, causal=causal, heads=range(0, hq, max(1, hq // 4)))
+    assert np.array_equal(got, s.run(causal=causal))
+
+
+def test_peaked_rows_whose_tiles_two_waves_share(frq):
+    """The reference rises from tile to tile, or is far apart in the two halves."""
+    s = Setup([100], [900], 4, 2, 64, seed=11, qmul=6.0)
+    s.k *= torch.linspace(0.1, 6, 900)[:, None, None].to(s.k.dtype)
+    s.check(s.run())
+    s = Setup([100], [900], 4, 2, 128, seed=12, qmul=6.0)
+    s.k[64:128] *= 8                                         # one tile of the second half outweighs the rest
+    s.check(s.run())
+    s.k[:64] *= 30
+    s.check(s.run())
