@@ -142,6 +142,12 @@ __device__ __forceinline__ void stage(const uint16_t* src, int64_t ld, int rows,
 template <int TYPE, int OUT, int D, int WAVES, int SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_kernel(PrefillArgs a) {
     constexpr int kUnits = WAVES / SPLIT;                        // of 32 queries of a head
+    // Operands read four products ahead of their use in the order of the source:
+    // heads of 256, which the compiler's order serves one by one (4096 tokens, 8
+    // heads: 141 us against 183), and whole tiles of 64 (14 heads, 8192 tokens: 152
+    // against 165; 24 packed sequences: 125 against 120). For the others its own
+    // order is as good or 2 to 3 % better.
+    constexpr bool kAhead = D == 256 || (D == 64 && SPLIT == 1);
     constexpr int NK = D / 16, ND = D / 32, CH = D / 8;          // k-steps, column tiles, 16-byte pieces of a row
     // Two buffers of a K and a V tile, used in turn. Objects of their own and a
     // step's code for each, so that the compiler sees that a read of one need
@@ -242,19 +248,32 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         f32x16 st[2];
 #pragma unroll
         for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.f;
+        if constexpr (kAhead) {
+            auto row = [&](int x) { return read_row8(sk + (kat ^ (32 * (x >> 1))) + 32 * (x & 1) * D * 2); };
+            uint4 ahead[4];
 #pragma unroll
-        for (int s = 0; s < NK; ++s)
+            for (int x = 0; x < 4; ++x) ahead[x] = row(x);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-                st[t] = mfma<TYPE>(read_row8(sk + (kat ^ (32 * s)) + 32 * t * D * 2), qf[s], st[t]);
-        // four reads ahead of the products
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            for (int x = 0; x < 2 * NK; ++x) {
+                st[x & 1] = mfma<TYPE>(ahead[x & 3], qf[x >> 1], st[x & 1]);
+                if (x + 4 < 2 * NK) ahead[x & 3] = row(x + 4);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
 #pragma unroll
-        for (int s = 0; s < 2 * NK - 4; ++s) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            for (int s = 0; s < NK; ++s)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    st[t] = mfma<TYPE>(read_row8(sk + (kat ^ (32 * s)) + 32 * t * D * 2), qf[s], st[t]);
+            // four reads ahead of the products
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int s = 0; s < 2 * NK - 4; ++s) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         __builtin_amdgcn_s_setprio(0);
         if (__builtin_expect(masked, 0)) {
             const int left = lim - kt - 4 * h;
@@ -297,13 +316,30 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
             l = add_pair<TYPE>(pf[s].z, l);
             l = add_pair<TYPE>(pf[s].w, l);
         }
+        if constexpr (kAhead) {
+            auto columns = [&](int x) {
+                const int at = 16 * (x / ND) * D * 2, d = 64 * (x % ND);
+                const uint2 lo = read_column4(sv + (vat0 ^ d) + at), hi = read_column4(sv + (vat1 ^ d) + at);
+                return make_uint4(lo.x, lo.y, hi.x, hi.y);
+            };
+            uint4 ahead[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+            for (int x = 0; x < 4; ++x) ahead[x] = columns(x);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const uint2 lo = read_column4(sv + (vat0 ^ (64 * d)) + 16 * s * D * 2);
-                const uint2 hi = read_column4(sv + (vat1 ^ (64 * d)) + 16 * s * D * 2);
-                o[d] = mfma<TYPE>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[s], o[d]);
+            for (int x = 0; x < 4 * ND; ++x) {
+                o[x % ND] = mfma<TYPE>(ahead[x & 3], pf[x / ND], o[x % ND]);
+                if (x + 4 < 4 * ND) ahead[x & 3] = columns(x + 4);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const uint2 lo = read_column4(sv + (vat0 ^ (64 * d)) + 16 * s * D * 2);
+                    const uint2 hi = read_column4(sv + (vat1 ^ (64 * d)) + 16 * s * D * 2);
+                    o[d] = mfma<TYPE>(make_uint4(lo.x, lo.y, hi.x, hi.y), pf[s], o[d]);
+                }
             }
         }
         if (__builtin_expect(cut && special_at == at + 1, 0)) {
@@ -402,12 +438,15 @@ hipError_t launch_typed(const PrefillArgs& a, hipStream_t stream) {
     // share them, a tile each at a time: with at most 512 such units in workgroups
     // of four waves, with at most 1024 of eight (1024 tokens, 14 heads of 64: 12.8
     // us against 20.1; 1000 after 1000, 32 heads of 128: 41.5 against 47.6; 100
-    // after 1500, twice: 30.0 against 35.2; 384, 16 heads: 12.9 against 13.5). Below
-    // 384 keys the joining costs what it gains (333: 13.3 both, 128: 11.6, 11.0).
-    // Else eight waves share a key tile on long prompts of 128-wide heads (4096
-    // tokens, 32 heads: 143 us against 156); four leave fewer idle on short ones
-    // and suit 64-wide heads, whose bound is the exponentials (8192 tokens, 14
-    // heads: 164 against 177).
+    // after 1500, twice: 27.5 against 35.2; 384, 16 heads: 12.0 against 13.5). Below
+    // 384 keys the joining costs what it gains (333: 13.3 both, 128: 11.6, 11.0),
+    // and with more units the waves are there without it (512, four times, 28 heads:
+    // 26.0 against 20.7).
+    // Else eight waves share a key tile on long prompts of 128-wide heads (32 heads,
+    // 4096 tokens: 145 us against 154; 8192: 502 against 522; packed sequences the
+    // same); four leave fewer idle where there are few rounds of workgroups (2048
+    // tokens: 54 against 62, 2500: 68 against 76) and suit 64-wide heads, whose bound
+    // is the exponentials (8192 tokens, 14 heads: 164 against 177).
     const int64_t units = (a.max_q + 31) / 32 * a.q_heads * a.seqs;
     const bool half = a.max_k >= 384 && units <= 1024, little = units <= 512;
     switch (a.head_dim) {
@@ -416,7 +455,7 @@ hipError_t launch_typed(const PrefillArgs& a, hipStream_t stream) {
             return launch_one<TYPE, OUT, 64, 4, 1>(a, stream);
         case 128:
             if (half) return little ? launch_one<TYPE, OUT, 128, 4, 2>(a, stream) : launch_one<TYPE, OUT, 128, 8, 2>(a, stream);
-            return a.max_q > 1024 ? launch_one<TYPE, OUT, 128, 8, 1>(a, stream) : launch_one<TYPE, OUT, 128, 4, 1>(a, stream);
+            return a.max_q > 1024 && units > 3200 ? launch_one<TYPE, OUT, 128, 8, 1>(a, stream) : launch_one<TYPE, OUT, 128, 4, 1>(a, stream);
         case 256: return launch_one<TYPE, OUT, 256, 4, 1>(a, stream);
         default: return hipErrorInvalidValue;
     }

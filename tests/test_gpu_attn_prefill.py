@@ -207,6 +207,7 @@ def test_special_values_in_masked_places_of_long_prompts(frq):
     ([40, 450], [449, 300], 2, 2, 64, False), ([300, 20], [400, 0], 6, 2, 128, False),
     ([700], [700], 28, 4, 128, True), ([900, 31], [1000, 64], 14, 2, 64, True),
     ([200] * 7, [390] * 7, 32, 8, 128, True), ([1100], [1100], 32, 8, 128, True),
+    ([1030, 40, 700, 5], [1030, 90, 700, 5], 32, 8, 128, True),
 ])
 def test_few_queries_and_many(frq, nq, nk, hq, hkv, d, causal):
     """Tiles of a unit shared by two waves, in workgroups of four and of eight,
