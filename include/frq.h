@@ -463,6 +463,8 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
  * not see never reach it, infinities and NaN included. Inputs F16 or BF16 (one
  * type), scores and sums fp32, the softmax weights rounded to the inputs' type
  * for their product with v; out of that type or F32. head_dim 64, 128 or 256.
+ * The same call gives the same bits; how the work is divided follows from
+ * seqs, max_q, max_k and the heads, and with it the last bits of a sum.
  * ld_k and ld_v below 2^24. A sequence whose offsets leave the buffers is not
  * computed. */
 int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
