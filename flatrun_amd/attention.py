@@ -216,12 +216,12 @@ class BlockAttention:
         c = self.cache
         slots = np.concatenate([table[i, np.arange(n) // c.page_tokens].astype(np.int64) * c.page_tokens
                                 + np.arange(n) % c.page_tokens for i, n in enumerate(a + b for a, b in zip(past, counts))])
-        size = 2 * p["tokens_k"] * c.kv_heads * c.head_dim
+        size = 2 * p["tokens_k"] * c.kv_heads * c.head_dim   # whole rows of 64 elements and more: K and V stay aligned
         want = 2 * size + slots.nbytes
         if self._ctx is None or self._ctx.nbytes < want:
             self._ctx = device.DeviceBuffer(want)
-        p["ctx_slots"], p["ctx_k"], p["ctx_v"] = self._ctx.ptr, self._ctx.ptr + slots.nbytes, self._ctx.ptr + slots.nbytes + size
-        _lib.check(_lib.lib().frq_memcpy_h2d(self._ctx.ptr, slots.ctypes.data, slots.nbytes))
+        p["ctx_k"], p["ctx_v"], p["ctx_slots"] = (self._ctx.ptr + i * size for i in range(3))
+        _lib.check(_lib.lib().frq_memcpy_h2d(p["ctx_slots"], slots.ctypes.data, slots.nbytes))
 
     def __call__(self, qkv, rows: int):
         p, c = self._plan, self.cache

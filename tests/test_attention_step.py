@@ -1,0 +1,77 @@
+"""BlockAttention on host memory: plans, pages, buffers and the order of its
+calls, every row of every step against 64-bit attention over all that its
+sequence has seen. What the cache rounds (4 bits) is rounded in the reference
+too; bf16 heads of prompts are given their rounding."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from attn_host import Buffer, Stream, host, view    # noqa: F401  (host: fixture)
+from attn_ref import attend, block4, rope
+from flatrun_amd import device
+from flatrun_amd.attention import BlockAttention, KVCache4, Sequence, rope_table
+
+HQ, HKV, D = 4, 2, 64
+WIDTH = (HQ + 2 * HKV) * D
+
+
+class Model:
+    """Layers of random q|k|v rows and what each has to answer."""
+
+    def __init__(self, layers=1, pages=12, page=32, max_rows=160, max_seqs=4, max_context=200, n_pos=256):
+        rng = np.random.default_rng(layers)
+        self.table = rope_table(D, n_pos)
+        self.norms = [[(1 + 0.2 * rng.standard_normal(D)).astype(np.float32) for _ in range(2)] for _ in range(layers)]
+        self.rng, self.seen = rng, [{} for _ in range(layers)]
+        self.stream, self.steps, self.caches = Stream(), [], []
+        kw = dict(max_rows=max_rows, max_seqs=max_seqs, max_context=max_context, stream=self.stream)
+        up = device.DeviceBuffer.from_host
+        for wq, wk in self.norms:
+            self.caches.append(KVCache4(pages, page, HKV, D))
+            self.steps.append(BlockAttention(self.caches[-1], HQ, up(self.table), n_pos, q_norm=up(wq), k_norm=up(wk), **kw))
+
+    def step(self, new):
+        start = {s: s.length for s in new}
+        self.steps[0].plan(new)
+        n = sum(new.values())
+        for i, one in enumerate(self.steps):
+            qkv = self.rng.standard_normal((n, WIDTH)).astype(np.float32)
+            got = one(device.DeviceBuffer.from_host(qkv), n).to_host(np.float32)[:n * HQ * D].reshape(n, HQ, D)
+            self.check(i, new, start, qkv.reshape(n, -1, D), got)
+
+    def check(self, layer, new, start, x, got):
+        at = 0
+        for s, n in new.items():
+            pos = np.arange(start[s], start[s] + n)
+            (q, k, v), _ = rope(x[at:at + n], HQ, HKV, D, D, False, self.table[pos], *self.norms[layer])
+            kv = self.seen[layer].setdefault(s, [np.zeros((0, HKV, D))] * 2)
+            kv[:] = [np.concatenate([a, b]) for a, b in zip(kv, (k, v))]
+            for h in range(HQ):
+                g = h // (HQ // HKV)
+                one = n == 1
+                kk, vv = ([block4(np.float32(a)) for a in kv] if one or start[s] else kv)
+                want, mag, _ = attend(q[:, h], kk[:, g], vv[:, g], D ** -0.5, pos)
+                # one token: fp32 heads against the cache's own values. A prompt: q, k and v rounded to bf16, 2^-9 each
+                # of scores of some units and of the values
+                err = np.linalg.norm(got[at:at + n, h] - want) / np.linalg.norm(mag)
+                assert err <= (2.0 ** -18 if one else 1.2e-2), (layer, n, start[s], h, err)
+            at += n
+
+
+@pytest.mark.parametrize("chunks", [(45, 40), (2, 3), (33, 64, 4), (31, 7)])
+def test_chunks_of_any_total(host, chunks):
+    """A chunk's context and new keys together may be an odd number."""
+    m, s = Model(), Sequence()
+    for n in chunks:
+        m.step({s: n})
+    assert s.length == sum(chunks) and len(s.pages) == -(-s.length // 32)
+
+
+def test_a_context_buffer_that_grows(host):
+    m = Model()
+    a, b = Sequence(), Sequence()
+    m.step({a: 3, b: 6})
+    m.step({a: 4, b: 2})
+    m.step({b: 97, a: 12})
