@@ -75,3 +75,18 @@ def test_a_context_buffer_that_grows(host):
     m.step({a: 3, b: 6})
     m.step({a: 4, b: 2})
     m.step({b: 97, a: 12})
+
+
+def test_a_tokens_entry_does_not_depend_on_its_step(host):
+    """The same rows as one prompt, as chunks and one at a time: the same values in the cache."""
+    x = np.random.default_rng(5).standard_normal((40, WIDTH)).astype(np.float32)
+    held = []
+    for cuts in ((40,), (7, 33), (1,) * 40, (20, 1, 19)):
+        m, s, at = Model(), Sequence(), 0
+        for n in cuts:
+            m.steps[0].plan({s: n})
+            m.steps[0](device.DeviceBuffer.from_host(x[at:at + n]), n)
+            at += n
+        store = host.held[m.caches[0]]
+        held.append(np.stack([np.stack(store[s.pages[t // 32] * 32 + t % 32]) for t in range(40)]))
+    assert all(np.array_equal(held[0], h) for h in held[1:])
