@@ -124,20 +124,29 @@ class KVCache4:
 
 
 class Sequence:
-    """A sequence's place in the caches: its pages (the same ids in every
-    layer's cache that it uses) and its length."""
+    """A sequence's place in a model's caches: its length and its pages, which
+    have the same ids in every layer's cache. ``cache`` is the one that handed
+    them out, the first layer's."""
 
     def __init__(self):
         self.pages: list[int] = []
         self.length = 0
+        self.cache: KVCache4 | None = None
 
 
 class BlockAttention:
     """The attention step of one decoder block over its :class:`KVCache4`.
 
-    ``plan(new)`` fixes the step: ``new`` maps each sequence of the batch, in
-    the order of the rows of qkv, to its number of new tokens; it takes pages
-    for them and uploads positions, slots, lengths and the page table. Then
+    The blocks of a model share one plan: the first layer's has buffers and
+    hands out pages, the others are made with ``first=`` that one, on the same
+    stream and with caches of their own of the same shape. They use its
+    buffers, so a layer's output is read before the next layer is enqueued, as
+    ``DecoderProjections.forward`` on one stream does.
+
+    ``plan(new)``, on the first layer and once per step, fixes the step for all:
+    ``new`` maps each sequence of the batch, in the order of the rows of qkv, to
+    its number of new tokens; it takes pages for them and uploads positions,
+    slots, lengths and the page table. Then, layer by layer,
     ``attention(qkv, rows)`` -- what ``DecoderProjections.forward`` calls --
     enqueues the step on the stream and returns fp32 rows for the o
     projection:
@@ -154,14 +163,20 @@ class BlockAttention:
     ``plan`` waits for the stream's earlier steps before it reuses its
     buffers."""
 
-    def __init__(self, cache: KVCache4, q_heads: int, table, n_pos: int, max_rows: int, max_seqs: int, max_context: int,
-                 rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None, eps: float = 1e-6,
-                 stream=None):
+    def __init__(self, cache: KVCache4, q_heads: int, table, n_pos: int, max_rows: int = 0, max_seqs: int = 0,
+                 max_context: int = 0, rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None,
+                 eps: float = 1e-6, stream=None, first: BlockAttention | None = None):
         if q_heads % cache.kv_heads:
             raise ValueError("q_heads must be a multiple of the cache's kv_heads")
         self.cache, self.q_heads, self.table, self.n_pos = cache, int(q_heads), table, int(n_pos)
         self.rot, self.interleaved, self.eps = rot, interleaved, eps
         self.q_norm, self.k_norm, self.stream = q_norm, k_norm, stream
+        self._first = first
+        if first is not None:
+            self._share(first, max_rows, max_seqs, max_context)
+            return
+        if min(int(max_rows), int(max_seqs), int(max_context)) < 1:
+            raise ValueError("max_rows, max_seqs and max_context must be at least 1")
         self.max_rows, self.max_seqs, self.max_context = int(max_rows), int(max_seqs), int(max_context)
         self.max_pages = -(-self.max_context // cache.page_tokens)
         d, hkv, r = cache.head_dim, cache.kv_heads, self.max_rows
@@ -173,9 +188,28 @@ class BlockAttention:
         self._ctx = None                     # K and V of a chunk's context, made when a prompt first needs it
         self._plan = None
 
+    def _share(self, first: BlockAttention, *sizes) -> None:
+        c, f = self.cache, first.cache
+        if first._first is not None:
+            raise ValueError("first must be the layer that plans")
+        if (c.pages, c.page_tokens, c.kv_heads, c.head_dim) != (f.pages, f.page_tokens, f.kv_heads, f.head_dim) or c is f:
+            raise ValueError("the layers' caches must have the same shape, and be one per layer")
+        if self.q_heads != first.q_heads or self.n_pos < first.n_pos:
+            raise ValueError("the layers must have the same heads and tables of as many positions")
+        if device._stream(self.stream or first.stream) != device._stream(first.stream) or any(sizes):
+            raise ValueError("the stream, max_rows, max_seqs and max_context are those of the first layer")
+        self.stream = first.stream
+        self.q, self.k, self.v, self.out, self._slots = first.q, first.k, first.v, first.out, first._slots
+        self.max_rows, self.max_seqs, self.max_context = first.max_rows, first.max_seqs, first.max_context
+        self.max_pages = first.max_pages
+
     def plan(self, new: dict) -> None:
+        if self._first is not None:
+            raise ValueError("the first layer plans the step for all of them")
         seqs, counts = list(new), [int(n) for n in new.values()]
         rows, c = sum(counts), self.cache
+        if any(s.cache not in (None, c) for s in seqs):
+            raise ValueError("a sequence is planned by the first layer of its model only (BlockAttention's first=)")
         if not seqs or len(seqs) > self.max_seqs or rows > self.max_rows or min(counts) < 1:
             raise ValueError(f"a step takes 1..{self.max_seqs} sequences and {self.max_rows} rows, a token at least each")
         if max(s.length + n for s, n in zip(seqs, counts)) > min(self.max_context, self.n_pos):
@@ -185,6 +219,7 @@ class BlockAttention:
         table = np.zeros((len(seqs), self.max_pages), np.int32)
         slots, positions = [], []
         for i, (s, n) in enumerate(zip(seqs, counts)):
+            s.cache = c
             for _ in range(max(0, need[i])):
                 s.pages.append(ids.pop())
             table[i, :len(s.pages)] = s.pages
@@ -227,7 +262,7 @@ class BlockAttention:
         _lib.check(_lib.lib().frq_memcpy_h2d(p["ctx_slots"], slots.ctypes.data, slots.nbytes))
 
     def __call__(self, qkv, rows: int):
-        p, c = self._plan, self.cache
+        p, c = (self._first or self)._plan, self.cache
         if p is None or rows != p["rows"]:
             raise ValueError("plan() this step's rows first")
         d, hkv, hq, s = c.head_dim, c.kv_heads, self.q_heads, self.stream
@@ -256,6 +291,9 @@ class BlockAttention:
         return self.out
 
     def close(self) -> None:
+        """Frees the buffers, once for all layers: on the first."""
+        if self._first is not None:
+            return
         for b in (self.q, self.k, self.v, self.out, self._ints, self._slots, self._ctx):
             if b is not None:
                 b.free()

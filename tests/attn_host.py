@@ -70,7 +70,7 @@ class Lib:
 
 
 class Stream:
-    waits = 0
+    waits, cuda_stream = 0, 5
 
     def synchronize(self):
         self.waits += 1

@@ -30,7 +30,8 @@ class Model:
         up = device.DeviceBuffer.from_host
         for wq, wk in self.norms:
             self.caches.append(KVCache4(pages, page, HKV, D))
-            self.steps.append(BlockAttention(self.caches[-1], HQ, up(self.table), n_pos, q_norm=up(wq), k_norm=up(wk), **kw))
+            more = {"first": self.steps[0]} if self.steps else kw
+            self.steps.append(BlockAttention(self.caches[-1], HQ, up(self.table), n_pos, q_norm=up(wq), k_norm=up(wk), **more))
 
     def step(self, new):
         start = {s: s.length for s in new}
@@ -90,3 +91,38 @@ def test_a_tokens_entry_does_not_depend_on_its_step(host):
         store = host.held[m.caches[0]]
         held.append(np.stack([np.stack(store[s.pages[t // 32] * 32 + t % 32]) for t in range(40)]))
     assert all(np.array_equal(held[0], h) for h in held[1:])
+
+
+def test_layers_share_a_plan(host):
+    """A prompt, a chunk and single tokens through three layers, each with its own cache; one plan a step."""
+    m = Model(layers=3)
+    a, b = Sequence(), Sequence()
+    for i, new in enumerate(({a: 45, b: 7}, {a: 40}, {a: 1, b: 1}, {b: 30, a: 2}, {a: 1, b: 1})):
+        m.step(new)
+        assert m.stream.waits == i + 1
+    assert (a.length, b.length) == (89, 39) and (len(a.pages), len(b.pages)) == (3, 2)
+    assert len(set(a.pages + b.pages)) == 5 and len(m.caches[0]._free) == 12 - 5
+
+
+def test_a_sequence_has_one_planner(host):
+    """Layers that each plan a sequence would advance it twice: refused, nothing changed."""
+    m, s = Model(), Sequence()
+    table = device.DeviceBuffer.from_host(m.table)
+    other = BlockAttention(KVCache4(12, 32, HKV, D), HQ, table, 256, max_rows=160, max_seqs=4, max_context=200,
+                           stream=m.stream)
+    m.step({s: 40})
+    pages = list(s.pages)
+    with pytest.raises(ValueError):
+        other.plan({Sequence(): 2, s: 1})
+    assert s.length == 40 and s.pages == pages and len(other.cache._free) == 12
+    more = BlockAttention(KVCache4(12, 32, HKV, D), HQ, table, 256, first=m.steps[0])
+    with pytest.raises(ValueError):
+        more.plan({s: 1})
+    m.step({s: 1})
+    for cache, kw in ((KVCache4(11, 32, HKV, D), {}), (KVCache4(12, 64, HKV, D), {}), (KVCache4(12, 32, 1, D), {}),
+                      (m.caches[0], {}), (KVCache4(12, 32, HKV, D), dict(stream=7)),
+                      (KVCache4(12, 32, HKV, D), dict(max_rows=10)), (KVCache4(12, 32, HKV, D), dict(first=more))):
+        with pytest.raises(ValueError):
+            BlockAttention(cache, HQ, table, 256, **{"first": m.steps[0], **kw})
+    with pytest.raises(ValueError):
+        BlockAttention(KVCache4(12, 32, HKV, D), HQ, table, 256)
