@@ -153,12 +153,9 @@ class BlockAttention:
 
     * one new token per sequence: norms and rotary positions in fp32, the
       token into the cache, attn_decode against it;
-    * prompts: the heads as bf16 and attn_prefill on them; where a sequence has
-      tokens in the cache already (a prompt in chunks), all its keys, new ones
-      too, are what the cache reads back.
-
-    The cache quantises fp32 heads in every step, so a token's entry does not
-    depend on what else its step held.
+    * prompts: the heads as bf16, into the cache, and attn_prefill on them;
+      where a sequence has tokens in the cache already (a prompt in chunks),
+      all its keys, new ones too, are what the cache reads back.
 
     ``plan`` waits for the stream's earlier steps before it reuses its
     buffers."""
@@ -267,22 +264,15 @@ class BlockAttention:
             raise ValueError("plan() this step's rows first")
         d, hkv, hq, s = c.head_dim, c.kv_heads, self.q_heads, self.stream
         kind = "f32" if p["single"] else "bf16"
-        x, width, nk = device._addr(qkv), (hq + 2 * hkv) * d, hkv * d
-        turn = dict(rot=self.rot, interleaved=self.interleaved, eps=self.eps, n_pos=self.n_pos, stream=s)
-        k16, v16 = self.k.ptr, self.k.ptr + 2 * rows * nk        # of a prompt; self.v then holds its fp32 keys
-        device.qk_norm_rope(qkv, self.q, self.k, self.v if p["single"] else v16, rows, hq, hkv, d, self.table,
-                            p["positions"], q_norm=self.q_norm, k_norm=self.k_norm, out_dtype=kind, **turn)
+        device.qk_norm_rope(qkv, self.q, self.k, self.v, rows, hq, hkv, d, self.table, p["positions"], rot=self.rot,
+                            interleaved=self.interleaved, q_norm=self.q_norm, k_norm=self.k_norm, eps=self.eps,
+                            out_dtype=kind, n_pos=self.n_pos, stream=s)
+        c.write(self.k, self.v, self._slots, rows, dtype=kind, stream=s)
         if p["single"]:
-            c.write(self.k, self.v, self._slots, rows, stream=s)
             device.attn_decode(self.q, c, p["table"], p["lens"], self.out, p["batch"], hq, p["max_len"],
                                ld_table=self.max_pages, stream=s)
             return self.out
-        # The keys once more for the cache, in fp32: the operator's "query heads" here. Its one "key head", the first
-        # of v, goes to rows of out, which the attention overwrites.
-        device.qk_norm_rope(x + 4 * hq * d, self.v, self.out, None, rows, hkv, 1, d, self.table, p["positions"],
-                            q_norm=self.k_norm, ld_x=width, ld_k=hq * d, **turn)
-        c.write(self.v, x + 4 * (hq + hkv) * d, self._slots, rows, ld_v=width, stream=s)
-        k, v, tk, cu_k = k16, v16, rows, p["cu_q"]
+        k, v, tk, cu_k = self.k, self.v, rows, p["cu_q"]
         if p["context"]:
             k, v, tk, cu_k = p["ctx_k"], p["ctx_v"], p["tokens_k"], p["cu_k"]
             c.read(k, v, p["ctx_slots"], tk, dtype="bf16", stream=s)

