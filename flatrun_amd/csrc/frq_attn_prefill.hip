@@ -400,7 +400,9 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
             }
     }
     if (qi >= nq) return;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    // No weight at all: zeros for a query without keys; where its keys all score
+    // -inf the softmax is 0 / 0.
+    const float inv = 1.0f / l, none = lim < 0 ? 0.f : __builtin_nanf("");
     using O = Val<OUT>;
     typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (q0 + qi) * a.ld_out + head * a.hs_out;
 #pragma unroll
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
         for (int i = 0; i < 16; i += 4) {                        // columns 32 d + 2 i + 4 h and the next three
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = l == 0.f ? 0.f : o[d][i + e] * inv;
+            for (int e = 0; e < 4; ++e) x[e] = l == 0.f ? none : o[d][i + e] * inv;
             if constexpr (OUT == kTypeF32)
                 *reinterpret_cast<float4*>(out + 32 * d + 2 * i + 4 * h) = make_float4(x[0], x[1], x[2], x[3]);
             else

@@ -228,3 +228,22 @@ def test_peaked_rows_whose_tiles_two_waves_share(frq):
     s.check(s.run())
     s.k[:64] *= 30
     s.check(s.run())
+
+
+@pytest.mark.parametrize("nq,nk,at,d", [([100], [100], 0, 64), ([100], [100], 40, 128), ([70, 20], [500, 20], 69, 64),
+                                        ([40], [30], 10, 256)])
+def test_queries_whose_keys_all_score_minus_infinity(frq, nq, nk, at, d):
+    """A softmax of nothing but -inf is 0 / 0; zeros are for queries that see no key."""
+    s = Setup(nq, nk, 2, 1, d, seed=14)
+    clean = s.run(out_dtype="f32")
+    s.q[at, 1, 7] = float("inf")
+    s.k[:, 0, 7] = -s.k[:, 0, 7].abs() - 0.125
+    want = s.run(out_dtype="f32")                            # of the other queries, with these keys
+    assert np.isnan(want[at, 1]).all()
+    s.q[at, 1, 7] = 1.0
+    other = s.run(out_dtype="f32")
+    other[at, 1], want[at, 1] = 0, 0
+    assert np.array_equal(other, want) and np.isfinite(clean).all()
+    if nk[0] < nq[0]:                                        # no key at all: zeros, also for a query with an inf
+        s.q[3, 1, 7] = float("inf")
+        assert np.all(s.run()[:nq[0] - nk[0]] == 0)
