@@ -151,11 +151,15 @@ class BlockAttention:
     enqueues the step on the stream and returns fp32 rows for the o
     projection:
 
-    * one new token per sequence: norms and rotary positions in fp32, the
+    * one new token of a sequence: norms and rotary positions in fp32, the
       token into the cache, attn_decode against it;
     * prompts: the heads as bf16, into the cache, and attn_prefill on them;
-      where a sequence has tokens in the cache already (a prompt in chunks),
-      all its keys, new ones too, are what the cache reads back.
+      where a prompt has tokens in the cache already (it comes in chunks), all
+      its keys, new ones too, are what the cache reads back.
+
+    A step may hold both; what a sequence gets does not depend on its
+    neighbours (but for the last bits of sums). Single tokens that stand side
+    by side in ``new`` share their launches.
 
     ``plan`` waits for the stream's earlier steps before it reuses its
     buffers."""
@@ -225,8 +229,13 @@ class BlockAttention:
             slots.append(table[i, t // c.page_tokens].astype(np.int64) * c.page_tokens + t % c.page_tokens)
         past = [s.length for s in seqs]
         lens = np.array([p + n for p, n in zip(past, counts)], np.int32)
+        single = [n == 1 for n in counts]
+        context = any(p and not one for p, one in zip(past, single))
+        # keys of the prompts' attention; a single token beside them has none, or, where the rows themselves are the
+        # keys, its own: attn_decode overwrites what comes of it
+        keys = np.where(single, 0, lens) if context else np.array(counts)
         cu_q = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
-        cu_k = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        cu_k = np.concatenate([[0], np.cumsum(keys)]).astype(np.int32)
         ints = np.concatenate([np.concatenate(positions).astype(np.int32), lens, cu_q, cu_k, table.reshape(-1)])
         if self.stream is not None:
             self.stream.synchronize()        # earlier steps still read these buffers
@@ -238,19 +247,25 @@ class BlockAttention:
         check(lib.frq_memcpy_h2d(self._slots.ptr, sl.ctypes.data, sl.nbytes))
         b, at = len(seqs), self._ints.ptr
         p = {"rows": rows, "batch": b, "positions": at, "lens": at + 4 * rows, "cu_q": at + 4 * (rows + b),
-             "cu_k": at + 4 * (rows + 2 * b + 1), "table": at + 4 * (rows + 3 * b + 2), "max_len": int(lens.max()),
-             "max_q": max(counts), "single": max(counts) == 1, "tokens_k": int(lens.sum()), "context": any(past)}
-        if not p["single"] and p["context"]:
-            self._plan_context(p, table, past, counts, cu_q, cu_k)
+             "cu_k": at + 4 * (rows + 2 * b + 1), "table": at + 4 * (rows + 3 * b + 2), "max_q": max(counts),
+             "max_k": int(keys.max()), "tokens_k": int(keys.sum()), "prompts": not all(single), "context": context,
+             "max_len": max([int(n) for n, one in zip(lens, single) if one], default=0), "tokens": []}
+        for i in range(b):                   # runs of single tokens: (sequence, row, count)
+            if single[i] and i and single[i - 1]:
+                p["tokens"][-1][2] += 1
+            elif single[i]:
+                p["tokens"].append([i, int(cu_q[i]), 1])
+        if context:
+            self._plan_context(p, table, keys)
         for s, n in zip(seqs, counts):
             s.length += n
         self._plan = p
 
-    def _plan_context(self, p: dict, table, past, counts, cu_q, cu_k) -> None:
-        """Slots of every key of the batch, context and new, in packed order."""
+    def _plan_context(self, p: dict, table, keys) -> None:
+        """Slots of every key of the prompts, context and new, in packed order."""
         c = self.cache
         slots = np.concatenate([table[i, np.arange(n) // c.page_tokens].astype(np.int64) * c.page_tokens
-                                + np.arange(n) % c.page_tokens for i, n in enumerate(a + b for a, b in zip(past, counts))])
+                                + np.arange(n) % c.page_tokens for i, n in enumerate(keys)])
         size = 2 * p["tokens_k"] * c.kv_heads * c.head_dim   # whole rows of 64 elements and more: K and V stay aligned
         want = 2 * size + slots.nbytes
         if self._ctx is None or self._ctx.nbytes < want:
@@ -262,23 +277,38 @@ class BlockAttention:
         p, c = (self._first or self)._plan, self.cache
         if p is None or rows != p["rows"]:
             raise ValueError("plan() this step's rows first")
-        d, hkv, hq, s = c.head_dim, c.kv_heads, self.q_heads, self.stream
-        kind = "f32" if p["single"] else "bf16"
-        device.qk_norm_rope(qkv, self.q, self.k, self.v, rows, hq, hkv, d, self.table, p["positions"], rot=self.rot,
-                            interleaved=self.interleaved, q_norm=self.q_norm, k_norm=self.k_norm, eps=self.eps,
-                            out_dtype=kind, n_pos=self.n_pos, stream=s)
-        c.write(self.k, self.v, self._slots, rows, dtype=kind, stream=s)
-        if p["single"]:
-            device.attn_decode(self.q, c, p["table"], p["lens"], self.out, p["batch"], hq, p["max_len"],
-                               ld_table=self.max_pages, stream=s)
-            return self.out
-        k, v, tk, cu_k = self.k, self.v, rows, p["cu_q"]
-        if p["context"]:
-            k, v, tk, cu_k = p["ctx_k"], p["ctx_v"], p["tokens_k"], p["cu_k"]
-            c.read(k, v, p["ctx_slots"], tk, dtype="bf16", stream=s)
-        device.attn_prefill(self.q, k, v, self.out, p["cu_q"], cu_k, p["batch"], rows, tk, hq, hkv, d, max_q=p["max_q"],
-                            max_k=min(p["max_len"], tk), out_dtype="f32", stream=s)
+        if p["prompts"]:
+            self._prompts(p, qkv)
+        for seq, row, count in p["tokens"]:
+            self._tokens(p, qkv, seq, row, count)
         return self.out
+
+    def _heads(self, p: dict, qkv, row: int, count: int, dtype: str) -> None:
+        """q, k and v of `count` rows from `row` on, the new tokens into the cache."""
+        c, slots = self.cache, (self._first or self)._slots
+        width = (self.q_heads + 2 * c.kv_heads) * c.head_dim
+        device.qk_norm_rope(qkv if row == 0 else device._addr(qkv) + 4 * row * width, self.q, self.k, self.v, count,
+                            self.q_heads, c.kv_heads, c.head_dim, self.table, p["positions"] + 4 * row, rot=self.rot,
+                            interleaved=self.interleaved, q_norm=self.q_norm, k_norm=self.k_norm, eps=self.eps,
+                            out_dtype=dtype, n_pos=self.n_pos, stream=self.stream)
+        c.write(self.k, self.v, slots.ptr + 8 * row, count, dtype=dtype, stream=self.stream)
+
+    def _prompts(self, p: dict, qkv) -> None:
+        c, rows, s = self.cache, p["rows"], self.stream
+        self._heads(p, qkv, 0, rows, "bf16")
+        k, v, cu_k = self.k, self.v, p["cu_q"]
+        if p["context"]:
+            k, v, cu_k = p["ctx_k"], p["ctx_v"], p["cu_k"]
+            c.read(k, v, p["ctx_slots"], p["tokens_k"], dtype="bf16", stream=s)
+        device.attn_prefill(self.q, k, v, self.out, p["cu_q"], cu_k, p["batch"], rows, p["tokens_k"], self.q_heads,
+                            c.kv_heads, c.head_dim, max_q=p["max_q"], max_k=p["max_k"], out_dtype="f32", stream=s)
+
+    def _tokens(self, p: dict, qkv, seq: int, row: int, count: int) -> None:
+        c, s = self.cache, self.stream
+        self._heads(p, qkv, row, count, "f32")
+        device.attn_decode(self.q, c, p["table"] + 4 * seq * self.max_pages, p["lens"] + 4 * seq,
+                           self.out.ptr + 4 * row * self.q_heads * c.head_dim, count, self.q_heads, p["max_len"],
+                           ld_table=self.max_pages, stream=s)
 
     def close(self) -> None:
         """Frees the buffers, once for all layers: on the first."""

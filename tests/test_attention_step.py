@@ -115,3 +115,51 @@ def test_a_sequence_has_one_planner(host):
             BlockAttention(cache, HQ, table, 256, **{"first": m.steps[0], **kw})
     with pytest.raises(ValueError):
         BlockAttention(KVCache4(12, 32, HKV, D), HQ, table, 256)
+
+
+MIXED = [(0, 1, 30, 1), (1, 30, 1, 1), (30, 1, 1, 12), (1, 1, 1, 9)]
+
+
+@pytest.mark.parametrize("past", [(40, 33, 0, 5), (0, 40, 31, 0), (2, 2, 2, 2)])
+@pytest.mark.parametrize("new", MIXED)
+def test_single_tokens_beside_prompts(host, past, new):
+    """fp32 and the cache for single tokens, bf16 for prompts, whatever stands beside them and in which order."""
+    m, seqs = Model(layers=2, max_rows=200), [Sequence() for _ in past]
+    for s, n in zip(seqs, past):
+        if n:
+            m.step({s: n})
+    m.step({s: n for s, n in zip(seqs, new) if n})
+    m.step({s: 1 for s in seqs})
+
+
+def test_a_tokens_result_does_not_depend_on_its_neighbours(host):
+    rng = np.random.default_rng(5)
+    x = [rng.standard_normal((n, WIDTH)).astype(np.float32) for n in (45, 1, 1, 30)]
+    got = []
+    for beside in (False, True):
+        m, a, b = Model(), Sequence(), Sequence()
+        outs = []
+        for i in range(3):
+            new, at, qkv = {a: len(x[i])}, 0, x[i]
+            if beside and i:
+                new, qkv, at = ({b: 30, a: 1}, np.concatenate([x[3], x[i]]), 30)
+            m.steps[0].plan(new)
+            out = m.steps[0](device.DeviceBuffer.from_host(qkv), len(qkv)).to_host(np.float32)
+            outs.append(out[at * HQ * D:len(qkv) * HQ * D])
+        store = host.held[m.caches[0]]
+        got.append(outs + [np.stack(store[a.pages[t // 32] * 32 + t % 32]) for t in range(47)])
+    assert all(np.array_equal(p, q) for p, q in zip(*got))
+
+
+def test_launches_of_a_step(host):
+    """Single tokens side by side go together; a step of one kind has no launch of the other."""
+    m, seqs = Model(), [Sequence() for _ in range(4)]
+    m.step({seqs[0]: 3, seqs[1]: 5})
+    assert [c[0] for c in host.calls] == ["rope", "write", "prefill"]
+    host.calls.clear()
+    m.step({s: 1 for s in seqs})
+    assert [c[0] for c in host.calls] == ["rope", "write", "decode"] and host.calls[-1][1] == 4
+    host.calls.clear()
+    m.step({seqs[0]: 1, seqs[1]: 1, seqs[2]: 4, seqs[3]: 1})
+    assert [c[0] for c in host.calls] == ["rope", "write", "read", "prefill"] + ["rope", "write", "decode"] * 2
+    assert [c[1] for c in host.calls if c[0] == "decode"] == [2, 1] and host.calls[3][3] == 5    # keys: the prompt's only
