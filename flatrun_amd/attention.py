@@ -154,10 +154,11 @@ class BlockAttention:
     * one new token of a sequence: norms and rotary positions in fp32, the
       token into the cache, attn_decode against it;
     * prompts: the heads as bf16, into the cache, and attn_prefill on them;
-      where a prompt has tokens in the cache already (it comes in chunks), all
-      its keys, new ones too, are what the cache reads back.
+      where a prompt of the step has tokens in the cache already (it comes in
+      chunks), all keys of the step's prompts, new ones too, are what the cache
+      reads back.
 
-    A step may hold both; what a sequence gets does not depend on its
+    A step may hold both; what a single token gets does not depend on its
     neighbours (but for the last bits of sums). Single tokens that stand side
     by side in ``new`` share their launches.
 

@@ -45,7 +45,7 @@ class Model:
             self.check(i, new, start, qkv.reshape(n, -1, D), got)
 
     def check(self, layer, new, start, x, got):
-        at = 0
+        at, context = 0, any(start[s] and n > 1 for s, n in new.items())
         for s, n in new.items():
             pos = np.arange(start[s], start[s] + n)
             (q, k, v), _ = rope(x[at:at + n], HQ, HKV, D, D, False, self.table[pos], *self.norms[layer])
@@ -56,10 +56,10 @@ class Model:
             kv[:] = [np.concatenate([a, b]) for a, b in zip(kv, (k, v))]
             for h in range(HQ):
                 g = h // (HQ // HKV)
-                kk, vv = ([block4(np.float32(a)) for a in kv] if one or start[s] else kv)
+                kk, vv = ([block4(np.float32(a)) for a in kv] if one or context else kv)
                 want, mag, _ = attend(q[:, h], kk[:, g], vv[:, g], D ** -0.5, pos)
                 # one token: fp32 heads against the cache's own values. A prompt: q and what the cache reads back
-                # rounded to bf16, 2^-9 each of scores of some units and of the values
+                # rounded to bf16, some 2^-9.5 in the mean of scores of some units and of the values
                 err = np.linalg.norm(got[at:at + n, h] - want) / np.linalg.norm(mag)
                 assert err <= (2.0 ** -18 if one else 1.2e-2), (layer, n, start[s], h, err)
             at += n
@@ -79,7 +79,7 @@ def test_a_context_buffer_that_grows(host):
     a, b = Sequence(), Sequence()
     m.step({a: 3, b: 6})
     m.step({a: 4, b: 2})
-    m.step({b: 97, a: 12})
+    m.step({b: 97, a: 12, Sequence(): 21})     # one that the cache held nothing of reads it back too
 
 
 def test_layers_share_a_plan(host):
