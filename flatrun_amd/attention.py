@@ -163,7 +163,12 @@ class BlockAttention:
     by side in ``new`` share their launches.
 
     ``plan`` waits for the stream's earlier steps before it reuses its
-    buffers."""
+    buffers.
+
+    A step of single tokens can be captured in a graph and replayed after later
+    plans of as many sequences. Its launches keep the longest length that they
+    were made for: give ``plan`` a ``max_len`` that the replays will not pass
+    (default: the longest sequence of this step, past which a replay gives NaN)."""
 
     def __init__(self, cache: KVCache4, q_heads: int, table, n_pos: int, max_rows: int = 0, max_seqs: int = 0,
                  max_context: int = 0, rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None,
@@ -205,7 +210,7 @@ class BlockAttention:
         self.max_rows, self.max_seqs, self.max_context = first.max_rows, first.max_seqs, first.max_context
         self.max_pages = first.max_pages
 
-    def plan(self, new: dict) -> None:
+    def plan(self, new: dict, max_len: int | None = None) -> None:
         if self._first is not None:
             raise ValueError("the first layer plans the step for all of them")
         seqs, counts = list(new), [int(n) for n in new.values()]
@@ -216,6 +221,8 @@ class BlockAttention:
             raise ValueError(f"a step takes 1..{self.max_seqs} sequences and {self.max_rows} rows, a token at least each")
         if max(s.length + n for s, n in zip(seqs, counts)) > min(self.max_context, self.n_pos):
             raise ValueError("a sequence would pass max_context or the rotary table")
+        if max_len is not None and not max(s.length + n for s, n in zip(seqs, counts)) <= max_len <= self.max_context:
+            raise ValueError("max_len is from the step's longest sequence to max_context")
         need = [-(-(s.length + n) // c.page_tokens) - len(s.pages) for s, n in zip(seqs, counts)]
         ids = c.take(sum(max(0, n) for n in need))
         table = np.zeros((len(seqs), self.max_pages), np.int32)
@@ -250,7 +257,7 @@ class BlockAttention:
         p = {"rows": rows, "batch": b, "positions": at, "lens": at + 4 * rows, "cu_q": at + 4 * (rows + b),
              "cu_k": at + 4 * (rows + 2 * b + 1), "table": at + 4 * (rows + 3 * b + 2), "max_q": max(counts),
              "max_k": int(keys.max()), "tokens_k": int(keys.sum()), "prompts": not all(single), "context": context,
-             "max_len": max([int(n) for n, one in zip(lens, single) if one], default=0), "tokens": []}
+             "max_len": max_len or max([int(n) for n, one in zip(lens, single) if one], default=0), "tokens": []}
         for i in range(b):                   # runs of single tokens: (sequence, row, count)
             if single[i] and i and single[i - 1]:
                 p["tokens"][-1][2] += 1

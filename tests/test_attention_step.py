@@ -35,9 +35,9 @@ class Model:
             more = {"first": self.steps[0]} if self.steps else kw
             self.steps.append(BlockAttention(self.caches[-1], HQ, up(self.table), n_pos, q_norm=up(wq), k_norm=up(wk), **more))
 
-    def step(self, new):
+    def step(self, new, **kw):
         start = {s: s.length for s in new}
-        self.steps[0].plan(new)
+        self.steps[0].plan(new, **kw)
         n = sum(new.values())
         for i, one in enumerate(self.steps):
             qkv = self.rng.standard_normal((n, WIDTH)).astype(np.float32)
@@ -163,3 +163,16 @@ def test_launches_of_a_step(host):
     m.step({seqs[0]: 1, seqs[1]: 1, seqs[2]: 4, seqs[3]: 1})
     assert [c[0] for c in host.calls] == ["rope", "write", "read", "prefill"] + ["rope", "write", "decode"] * 2
     assert [c[1] for c in host.calls if c[0] == "decode"] == [2, 1] and host.calls[3][3] == 5    # keys: the prompt's only
+
+
+def test_the_length_that_a_captured_step_is_made_for(host):
+    m, s = Model(), Sequence()
+    m.step({s: 40})
+    m.step({s: 1})
+    assert host.calls[-1][:3] == ("decode", 1, 41)
+    m.step({s: 1}, max_len=200)
+    assert host.calls[-1][:3] == ("decode", 1, 200)
+    for bad in (42, 201, 0, -1):
+        with pytest.raises(ValueError):
+            m.steps[0].plan({s: 1}, max_len=bad)
+    assert s.length == 42

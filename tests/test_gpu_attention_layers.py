@@ -90,3 +90,36 @@ def test_layers_chunks_and_mixed_steps(frq, page):
     steps[0].close()
     for cache in caches:
         cache.close()
+
+
+def test_a_captured_step_of_single_tokens(frq):
+    """Captured once, replayed after later plans while the sequences grow: the eager step's bits every time."""
+    cache, stream = KVCache4(60, 32, HKV, D), device.Stream()
+    table = device.DeviceBuffer.from_host(rope_table(D, 2048))
+    step = BlockAttention(cache, HQ, table, 2048, max_rows=96, max_seqs=2, max_context=1600, stream=stream)
+    seqs = [Sequence(), Sequence()]
+    qkv = device.DeviceBuffer(4 * 96 * WIDTH)
+    rng = np.random.default_rng(1)
+    upload(qkv, rng.standard_normal(67 * WIDTH).astype(np.float32))
+    step.plan({seqs[0]: 60, seqs[1]: 7})
+    step(qkv, 67)
+    stream.synchronize()
+    graph = None
+    for i in range(70):                                      # over two page ends, the longest from 61 to 130
+        upload(qkv, rng.standard_normal(2 * WIDTH).astype(np.float32))
+        step.plan({s: 1 for s in seqs}, max_len=1600)
+        if graph is None:
+            step(qkv, 2)                                     # the scratch of this shape is there
+            stream.synchronize()
+            with device.Graph.capture(stream) as graph:
+                step(qkv, 2)
+        graph.launch(stream)
+        stream.synchronize()
+        got = step.out.to_host(np.float32)[:2 * HQ * D]
+        step(qkv, 2)
+        stream.synchronize()
+        assert np.isfinite(got).all() and np.array_equal(got, step.out.to_host(np.float32)[:2 * HQ * D]), i
+    assert seqs[0].length == 130
+    graph.destroy()
+    step.close()
+    cache.close()
