@@ -5,24 +5,28 @@
 // The cache is read as it is held, once for up to eight query heads that share
 // a key head. Both products run on v_mfma_f32_16x16x32_f16 with fp32 precision:
 // the codes c - 8 are exact fp16 integers, and q and the softmax weights go in
-// as two fp16 numbers each, rows 2h and 2h + 1 of the product (the value and
-// the rest, 22 bits together). q is put under a power of two per head that
-// brings its largest element to [2^13, 2^14), so that the rest stays a normal
-// number. A block of K has its scale on the product of one instruction; the
-// scale of V goes into the weights, which stand under 2^(4 - E), 2^E four times
-// the largest |scale| of the first tile, so that tiny and huge values keep
-// their bits: out = sum / sum, the power cancels.
+// as two fp16 numbers each, rows 2h and 2h + 1 of the product: the value and the
+// rest, 22 bits together. The rests stand 2^12 higher and their rows' sums are
+// taken back at the end, so that the parts hold small numbers too: fp16 steps of
+// 2^-24 become 2^-36 (without that, tokens at 2^-24 of a large one's weight were
+// off by a tenth each). q is put under a power of two per head that brings its
+// largest element to [2^13, 2^14). A block of K has its scale on the product of
+// one instruction; the scale of V goes into the weights. Each group of 32
+// channels has sums of its own and so a power of two of its own, 2^(5 - E), 2^E
+// twice to four times the largest |scale| of the first tile's tokens in the
+// group: a weight times a scale is kept to 22 bits, or to 2^-40 of the reference's
+// weight times the largest scale where that is coarser.
 //
 // A wave takes 32 tokens a step. S = q K^T gives a lane one token of each half
 // and both numbers of two heads, so scores, weights and their scales need no
 // other lane; the weights pass through LDS, a wave's own part of it, to stand
 // as the second product's operand (transposing reads). The reference that the
 // exponentials are taken from, and E, are those of a wave's first tile. A tile
-// whose scores pass the reference by more than 2^8, or whose scales pass E, ends
-// the run: sums and reference go to LDS, where runs and later waves are joined
-// under the larger one, and the wave starts anew from that tile. So the loop
-// has no rescaling and no maximum over lanes. Two tiles are on their way while
-// one is worked on, 9.2 KB a wave at 128 channels.
+// whose scores pass the reference by more than 2^8, or whose scales reach
+// 2^(E + 1) in a group, ends the run: sums and reference go to LDS, where runs
+// and later waves are joined under the larger one, and the wave starts anew from
+// that tile. So the loop has no rescaling and no maximum over lanes. Two tiles
+// are on their way while one is worked on, 9.2 KB a wave at 128 channels.
 //
 // The tiles of all sequences and key heads, one after another, are shared out
 // evenly over the workgroups, whatever the lengths are; the four waves of a
@@ -58,6 +62,8 @@ constexpr int kShareMin = 8;           // places of a workgroup, two tiles for e
 constexpr int kWhole = 28, kWholeMany = 64;
 constexpr int kGroups = 512;           // two workgroups of 33 KiB and 183 registers a lane on each of 256 CUs
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRest = 4096;          // the rests stand 2^12 higher than the values
+constexpr int kTop = 5;                // of the exponents that weights stand under, see the head of the file
 
 // Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
 // 0x6400 | n is 1024 + n; under the mask 0xF0 it is 1024 + 16 n.
@@ -79,6 +85,11 @@ __device__ __forceinline__ _Float16 half_of(uint32_t w, int hi) {
 
 // 2^e as a float, e in the normal range.
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); }
+
+// kRest / p, p a power of two: exponents (127 + 12 - e) + (127 + e) are 254 + 12.
+__device__ __forceinline__ float over_pow2(float p) {
+    return __builtin_bit_cast(float, ((254u + 12u) << 23) - __builtin_bit_cast(uint32_t, p));
+}
 
 // The largest of x over the 16 lanes of a row.
 __device__ __forceinline__ float row_max(float x) {
@@ -290,14 +301,14 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
             other = __shfl_xor(top, 32);
             top = top > other ? top : other;
             const int up = top ? 140 - (int)(top >> 23) : 0;         // the largest to [2^13, 2^14)
-            const float part = n & 1 ? -1.f : 0.f;
+            const float part = n & 1 ? -kRest : 0.f, gain = n & 1 ? kRest : 1.f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const float y = __builtin_ldexpf(x[g][c], up);
                     const _Float16 hi = (_Float16)y;
-                    qf[g][c] = (_Float16)__builtin_fmaf((float)hi, part, y);
+                    qf[g][c] = (_Float16)__builtin_fmaf((float)hi, part, y * gain);
                 }
             }
             rs = top >= 0x7F800000u ? __builtin_nanf("") : __builtin_ldexpf(a.scale * kLog2e, -up);
@@ -310,7 +321,12 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
 
         while (tile < last) {
         float ref[2] = {-__builtin_inff(), -__builtin_inff()}, l[2] = {0.f, 0.f};
-        int ev = 0;                                                  // E
+        float under[NG];                                             // 2^(kTop - E) kRest of each group
+        uint32_t cap[NG / 2];                                        // the largest |scale| bits that fit, of two groups
+#pragma unroll
+        for (int g = 0; g < NG; ++g) under[g] = 1.f;
+#pragma unroll
+        for (int p = 0; p < NG / 2; ++p) cap[p] = 0;
         int fresh = 1;
         float4v o[2 * NG];
 #pragma unroll
@@ -344,8 +360,8 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(c[u][g][i], d, acc[i]);
                 }
-                s[u][0] = (acc[0] + acc[1]) * rs2[0];
-                s[u][1] = (acc[2] + acc[3]) * rs2[1];
+                s[u][0] = __builtin_fmaf(acc[1], 1 / kRest, acc[0]) * rs2[0];
+                s[u][1] = __builtin_fmaf(acc[3], 1 / kRest, acc[2]) * rs2[1];
             }
             fetch_k(k, next);                              // these registers are free again
             const int left = len - tile * kKvTile;                   // valid tokens from here
@@ -367,9 +383,9 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
                     l[1] += p1;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        const float d = (float)v.scale_of(u, g);
-                        const _Float16 h0 = (_Float16)__builtin_fmaf(p0, d, 0.f), h1 = (_Float16)__builtin_fmaf(p1, d, 0.f);
-                        const _Float16 r0 = (_Float16)__builtin_fmaf(p0, d, -(float)h0), r1 = (_Float16)__builtin_fmaf(p1, d, -(float)h1);
+                        const float d = __builtin_fmaf((float)v.scale_of(u, g), under[g], 0.f), y0 = p0 * d, y1 = p1 * d;
+                        const _Float16 h0 = (_Float16)__builtin_fmaf(y0, 1 / kRest, 0.f), h1 = (_Float16)__builtin_fmaf(y1, 1 / kRest, 0.f);
+                        const _Float16 r0 = (_Float16)__builtin_fmaf((float)h0, -kRest, y0), r1 = (_Float16)__builtin_fmaf((float)h1, -kRest, y1);
                         const half2v x = {h0, r0}, y = {h1, r1};
                         *(__attribute__((address_space(3))) uint2v*)(sp_to + g * 1024 + u * 512) =
                             uint2v{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
@@ -398,33 +414,47 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
                 }
                 fetch_v(v, next);
             };
-            // a score 2^8 past its reference's maximum, or a scale past E?
-            uint32_t big = 0;
+            // a score 2^8 past its reference, or a scale past its group's E?
+            using us2 = unsigned short __attribute__((ext_vector_type(2)));
+            us2 big[NG / 2], over = {0, 0};
 #pragma unroll
-            for (int p = 0; p < NG; ++p) {
-                const uint32_t w = v.scale[p] & 0x7FFF7FFFu;
-                using us2 = unsigned short __attribute__((ext_vector_type(2)));
-                big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, big), __builtin_bit_cast(us2, w)));
+            for (int p = 0; p < NG / 2; ++p) {
+                big[p] = __builtin_elementwise_max(__builtin_bit_cast(us2, v.scale[p] & 0x7FFF7FFFu),
+                                                   __builtin_bit_cast(us2, v.scale[NG / 2 + p] & 0x7FFF7FFFu));
+                over |= __builtin_elementwise_sub_sat(big[p], __builtin_bit_cast(us2, cap[p]));
             }
-            const float b0 = (float)half_of(big, 0), b1 = (float)half_of(big, 1);
             const float t0 = __builtin_fmaxf(s[0][0], s[1][0]), t1 = __builtin_fmaxf(s[0][1], s[1][1]);
             asm("" : "+s"(fresh));                                 // no copy of the step for the first tile
             if (__builtin_expect(fresh != 0, 0)) {
-                float top = 0.f;                                     // of the scales that are numbers
 #pragma unroll
-                for (int p = 0; p < 2 * NG; ++p) {
-                    const float y = __builtin_fabsf((float)half_of(v.scale[p / 2], p & 1));
-                    top = y < __builtin_inff() ? __builtin_fmaxf(top, y) : top;
+                for (int p = 0; p < NG / 2; ++p) {
+                    us2 top = {0, 0};                                // of the scales that are numbers
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const us2 x = __builtin_bit_cast(us2, v.scale[u * (NG / 2) + p] & 0x7FFF7FFFu);
+                        top = __builtin_elementwise_max(top, (us2){x[0] < 0x7C00 ? x[0] : (unsigned short)0, x[1] < 0x7C00 ? x[1] : (unsigned short)0});
+                    }
+#pragma unroll
+                    for (int i = 1; i <= 8; i <<= 1)                 // every row of lanes holds all tokens
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, __shfl_xor(__builtin_bit_cast(uint32_t, top), i)));
+                    const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top));
+                    uint32_t caps[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        // 2^E from twice to four times the largest, scales below 2^(E + 1) fit
+                        const uint32_t h = i ? w >> 16 : w & 0xFFFFu;
+                        const int e = h ? __builtin_amdgcn_frexp_expf((float)half_of(h, 0)) + 1 : -22;
+                        const int ev = __builtin_amdgcn_readfirstlane(e);
+                        under[2 * p + i] = pow2(kTop + 12 - ev);
+                        caps[i] = ev >= 15 ? 0x7BFFu : ev >= -15 ? ((uint32_t)(ev + 16) << 10) - 1 : (1u << (ev + 25)) - 1;
+                    }
+                    cap[p] = caps[0] | caps[1] << 16;
                 }
-                top = row_max(top);                                  // every row of lanes holds all tokens
-                const int et = top > 0.f ? __builtin_amdgcn_frexp_expf(top) + 1 : -22;
-                ev = __builtin_amdgcn_readfirstlane(et);
-                ref[0] = row_max(t0) + (float)(ev - 4);
-                ref[1] = row_max(t1) + (float)(ev - 4);
+                ref[0] = row_max(t0);
+                ref[1] = row_max(t1);
                 fresh = 0;
             } else {
-                const float cap = pow2(ev + 1), room = (float)(12 - ev);
-                const bool past = (int)(t0 > ref[0] + room) | (int)(t1 > ref[1] + room) | (int)!(b0 < cap) | (int)!(b1 < cap);
+                const bool past = (int)(t0 - ref[0] > 8.f) | (int)(t1 - ref[1] > 8.f) | (int)(__builtin_bit_cast(uint32_t, over) != 0);
                 if (__builtin_expect(__builtin_amdgcn_ballot_w64(past) != 0, 0)) return false;
             }
             weigh();
@@ -449,7 +479,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
             float* to = sh_o + (wave * 8 + 2 * j + i) * kRow + n;
 #pragma unroll
             for (int c = 0; c < 2 * NG; ++c) {
-                const float x = (o[c][2 * i] + o[c][2 * i + 1]) * fn;
+                const float x = __builtin_fmaf(o[c][2 * i + 1], 1 / kRest, o[c][2 * i]) * over_pow2(under[c / 2]) * fn;
                 to[16 * c] = held ? to[16 * c] * fo + x : x;
             }
         }

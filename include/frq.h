@@ -441,8 +441,11 @@ int frq_dev_kv4_read(const void* cache, size_t cache_bytes, int64_t pages, int64
  * t < lens[b] of softmax(scale q[b, h] . k_t) v_t with the values the cache
  * holds, query heads h / (q_heads / kv_heads) to a key head. Sequence b's token
  * t is in page table[b * ld_table + t / page_tokens]. fp32 precision
- * throughout (q and the weights enter the products as two fp16 parts, 22
- * bits). lens[b] = 0: zeros. lens[b] > max_len or a page outside the cache:
+ * throughout: q and the weights enter the products as two fp16 parts. A weight
+ * times a block's scale is kept to 22 bits, or to 2^-40 of the largest weight
+ * times the largest scale of those channels (of some stretch of the sequence)
+ * where that is coarser; an element of q to 22 bits, or 2^-48 of its head's
+ * largest. lens[b] = 0: zeros. lens[b] > max_len or a page outside the cache:
  * NaN. Where sequences are long their tiles are shared out evenly over at most
  * 512 workgroups, whose partial results (two sets of 8 (head_dim + 2) floats a
  * workgroup) use the stream's scratch and are joined in a fixed order. The
