@@ -450,8 +450,9 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
                     }
                     cap[p] = caps[0] | caps[1] << 16;
                 }
-                ref[0] = row_max(t0);
-                ref[1] = row_max(t1);
+                // where all scores are -inf, below everything, so that they count nothing
+                ref[0] = __builtin_fmaxf(row_max(t0), -3.4028235e38f);
+                ref[1] = __builtin_fmaxf(row_max(t1), -3.4028235e38f);
                 fresh = 0;
             } else {
                 const bool past = (int)(t0 - ref[0] > 8.f) | (int)(t1 - ref[1] > 8.f) | (int)(__builtin_bit_cast(uint32_t, over) != 0);
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_decode_kern
             }
             if (whole) {
                 const int64_t h = (int64_t)kvh * group + 8 * hc + r;
-                static_cast<typename T::Elem*>(a.out)[(int64_t)b * a.ld_out + h * D + c] = T::one(sum == 0.f ? 0.f : val / sum);
+                static_cast<typename T::Elem*>(a.out)[(int64_t)b * a.ld_out + h * D + c] = T::one(len == 0 ? 0.f : val / sum);
             } else {
                 part[r * D + c] = val;
                 if (c == 0) {
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(DecodeArgs a) {
             v += vals[i][threadIdx.x];
             t += sums[i];
         }
-        out[threadIdx.x] = T::one(t == 0.f ? 0.f : v / t);
+        out[threadIdx.x] = T::one(v / t);
     }
 }
 

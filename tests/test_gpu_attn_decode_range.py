@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from attn_ref import dev
+from attn_ref import block4, dev
 from test_gpu_attn_decode import Setup
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +67,20 @@ def test_same_bits_every_time(frq):
     s.v[..., :32] *= 1e-4
     write(s)
     assert np.array_equal(s.run(), s.run())
+
+
+@pytest.mark.parametrize("n,low", [(100, 40), (100, 99), (5000, 700), (5000, 4999)])
+def test_tokens_whose_scores_overflow(frq, n, low):
+    """-inf in fp32: no weight, wherever it stands, as the definition has it; NaN where nothing else is left."""
+    s = Setup([n, 20], 8, 2, 64, 32, seed=26, spare=0)
+    s.q[0] = 0
+    s.q[0, :, 0] = 3e38
+    s.k[:n, :, :32] = 0
+    s.k[:low, :, 0] = -1000.0
+    write(s)
+    got = s.run()
+    v = block4(s.v[low:n]).repeat(4, axis=1)                 # equal weights of the others
+    assert np.all(np.abs(got[0] - v.mean(0)) <= (2.0 ** -20 + 8 * n ** 0.5 * 2.0 ** -24) * np.abs(v).mean(0))
+    s.k[:n, :, 0] = -1000.0
+    write(s)
+    assert np.isnan(s.run()[0]).all() and np.array_equal(s.run()[1], got[1])
