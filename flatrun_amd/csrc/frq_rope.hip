@@ -42,12 +42,7 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(RopeArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
             float4 v = make_float4(1.f, 0.f, 1.f, 0.f);
-            if (at + i + 3 < rot) {
-                v = *reinterpret_cast<const float4*>(row + at + i);
-            } else if (at + i + 1 < rot) {
-                v.x = row[at + i];
-                v.y = row[at + i + 1];
-            }
+            if (at + i < rot) v = *reinterpret_cast<const float4*>(row + at + i);    // rot is a multiple of 4
             cs[h][i] = v.x;
             cs[h][i + 1] = v.y;
             cs[h][i + 2] = v.z;
@@ -83,10 +78,11 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(RopeArgs a) {
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
                         const float p = x[k][i], q = x[k][i + 1], c = cs[k][i], s = cs[k][i + 1];
-                        x[k][i] = __builtin_fmaf(p, c, -(q * s));
-                        x[k][i + 1] = __builtin_fmaf(q, c, p * s);
+                        const bool turn = k * (D / 2) + 8 * sub + i < rot;    // else they pass: 0 times an inf is a NaN
+                        x[k][i] = turn ? __builtin_fmaf(p, c, -(q * s)) : p;
+                        x[k][i + 1] = turn ? __builtin_fmaf(q, c, p * s) : q;
                     }
-            } else {
+            } else if (rot) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float p = x[0][i], q = x[1][i], c = cs[i >> 2][(2 * i) & 7], s = cs[i >> 2][((2 * i) & 7) + 1];
