@@ -450,10 +450,25 @@ def _kind_of(dtype):
     return kind
 
 
-def _operand(name: str, obj, need: int, kind) -> int:
+def _rows_of(obj, ld: int, hs: int) -> bool:
+    """Whether a strided tensor lies as the call describes it: elements side by
+    side, in rows ld or heads hs apart."""
+    dims: list = []
+    for n, step in zip(reversed(obj.shape), reversed(obj.stride())):
+        if n == 1:
+            continue
+        if dims and step == dims[-1][0] * dims[-1][1]:
+            dims[-1] = (n * dims[-1][0], dims[-1][1])       # one run with the dimension inside it
+        else:
+            dims.append((n, step))
+    return not dims or (dims[0][1] == 1 and all(step > 0 and step in (ld, hs) for _, step in dims[1:]))
+
+
+def _operand(name: str, obj, need: int, kind, ld: int = 0, hs: int = 0) -> int:
     """Address of a device operand that holds `need` bytes of `kind`. Refuses a
-    buffer whose size is known and too small, and a tensor of another type (an
-    address says nothing of either)."""
+    buffer whose size is known and too small, and a tensor of another type, in
+    host memory, or of strides other than the call's (an address says nothing of
+    either)."""
     if obj is None:
         return 0
     t = type(obj)
@@ -464,7 +479,7 @@ def _operand(name: str, obj, need: int, kind) -> int:
             raise ValueError(f"{name} holds {obj.nbytes} bytes, the call needs {need}")
         return obj.ptr
     try:
-        if _KINDS[obj.dtype] == kind and obj.nbytes >= need:
+        if _KINDS[obj.dtype] == kind and obj.nbytes >= need and obj.is_cuda and obj.is_contiguous():
             return obj.data_ptr()
     except (AttributeError, KeyError):
         pass
@@ -475,6 +490,10 @@ def _operand(name: str, obj, need: int, kind) -> int:
         size = int(obj.untyped_storage().nbytes() - obj.storage_offset() * obj.element_size())
         if size < need:
             raise ValueError(f"{name} holds {size} bytes, the call needs {need}")
+        if not obj.is_contiguous() and not _rows_of(obj, ld, hs):
+            raise ValueError(f"{name} has strides {tuple(obj.stride())}, the call takes its rows {ld or 1} elements apart")
+        if not obj.is_cuda and not obj.is_pinned():
+            raise ValueError(f"{name} is in host memory")
         return obj.data_ptr()
     return _addr(obj)
 
@@ -507,8 +526,8 @@ def qk_norm_rope(x, q, k, v, tokens: int, q_heads: int, kv_heads: int, head_dim:
     if n_pos is None:
         n_pos = _nbytes(table) // (4 * rot) if rot and table is not None else 0
     check(lib().frq_dev_qk_norm_rope(
-        xi, _operand("x", x, xs * _span(t, lx, width), xi), lx, oi, _operand("q", q, os_ * _span(t, lq, nq), oi), lq,
-        _operand("k", k, os_ * _span(t, lk, nk), oi), lk, _operand("v", v, os_ * _span(t, lv, nk), oi), lv, t, q_heads,
+        xi, _operand("x", x, xs * _span(t, lx, width), xi, lx), lx, oi, _operand("q", q, os_ * _span(t, lq, nq), oi, lq), lq,
+        _operand("k", k, os_ * _span(t, lk, nk), oi, lk), lk, _operand("v", v, os_ * _span(t, lv, nk), oi, lv), lv, t, q_heads,
         kv_heads, hd, rot, 1 if interleaved else 0, _operand("table", table, 4 * n_pos * rot, _lib.F32), n_pos,
         _operand("positions", positions, 4 * t, _I32), _operand("q_norm", q_norm, 4 * hd, _lib.F32),
         _operand("k_norm", k_norm, 4 * hd, _lib.F32), eps, _stream(stream)))
@@ -527,7 +546,7 @@ def _kv4_args(cache, k, v, slots, tokens, dtype, ld_k, ld_v):
     ti = vtype_id(dtype)
     size = 4 if ti == 0 else 2
     return (cache.data_ptr(), cache.nbytes, cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, ti,
-            _operand("k", k, size * _span(t, lk, width), ti), lk, _operand("v", v, size * _span(t, lv, width), ti), lv,
+            _operand("k", k, size * _span(t, lk, width), ti, lk), lk, _operand("v", v, size * _span(t, lv, width), ti, lv), lv,
             _operand("slots", slots, 8 * t, _I64), t)
 
 
@@ -561,9 +580,9 @@ def attn_decode(q, cache, table, lens, out, batch: int, q_heads: int, max_len: i
     ti = vtype_id(dtype)
     size = 4 if ti == 0 else 2
     check(lib().frq_dev_attn_decode(
-        ti, _operand("q", q, size * _span(b, lq, nq), ti), lq, cache.data_ptr(), cache.nbytes, cache.pages,
-        cache.page_tokens, cache.kv_heads, hd, _operand("table", table, 4 * _span(b, lt, per), _I32), lt,
-        _operand("lens", lens, 4 * b, _I32), n, _operand("out", out, size * _span(b, lo, nq), ti), lo, b, q_heads,
+        ti, _operand("q", q, size * _span(b, lq, nq), ti, lq), lq, cache.data_ptr(), cache.nbytes, cache.pages,
+        cache.page_tokens, cache.kv_heads, hd, _operand("table", table, 4 * _span(b, lt, per), _I32, lt), lt,
+        _operand("lens", lens, 4 * b, _I32), n, _operand("out", out, size * _span(b, lo, nq), ti, lo), lo, b, q_heads,
         hd ** -0.5 if scale is None else scale, _stream(stream)))
 
 
@@ -584,9 +603,9 @@ def attn_prefill(q, k, v, out, cu_q, cu_k, seqs: int, tokens_q: int, tokens_k: i
     nq, nk = q_heads * hd, kv_heads * hd
     lq, lk, lv, lo = ld_q or nq, ld_k or nk, ld_v or nk, ld_out or nq
     check(lib().frq_dev_attn_prefill(
-        ti, _operand("q", q, 2 * _span(tq, lq, _span(q_heads, hq, hd)), ti), lq, hq,
-        _operand("k", k, 2 * _span(tk, lk, _span(kv_heads, hk, hd)), ti), lk, hk,
-        _operand("v", v, 2 * _span(tk, lv, _span(kv_heads, hv, hd)), ti), lv, hv, oi,
-        _operand("out", out, (4 if oi == 0 else 2) * _span(tq, lo, _span(q_heads, ho, hd)), oi), lo, ho,
+        ti, _operand("q", q, 2 * _span(tq, lq, _span(q_heads, hq, hd)), ti, lq, hq), lq, hq,
+        _operand("k", k, 2 * _span(tk, lk, _span(kv_heads, hk, hd)), ti, lk, hk), lk, hk,
+        _operand("v", v, 2 * _span(tk, lv, _span(kv_heads, hv, hd)), ti, lv, hv), lv, hv, oi,
+        _operand("out", out, (4 if oi == 0 else 2) * _span(tq, lo, _span(q_heads, ho, hd)), oi, lo, ho), lo, ho,
         _operand("cu_q", cu_q, 4 * (n + 1), _I32), _operand("cu_k", cu_k, 4 * (n + 1), _I32), n, tq, tk, int(max_q),
         int(max_k), q_heads, kv_heads, hd, 1 if causal else 0, hd ** -0.5 if scale is None else scale, _stream(stream)))
