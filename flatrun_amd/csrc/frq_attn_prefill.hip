@@ -139,8 +139,10 @@ __device__ __forceinline__ void stage(const uint16_t* src, int64_t ld, int rows,
     }
 }
 
+// Waves to a SIMD: 64-wide heads in workgroups of eight fit two of those on a CU
+// with 128 registers a lane, which the compiler passes if it is not told.
 template <int TYPE, int OUT, int D, int WAVES, int SPLIT>
-__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_kernel(PrefillArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : D == 64 && WAVES == 8 ? 4 : 2) attn_prefill_kernel(PrefillArgs a) {
     constexpr int kUnits = WAVES / SPLIT;                        // of 32 queries of a head
     // Operands read four products ahead of their use in the order of the source:
     // heads of 256, which the compiler's order serves one by one (4096 tokens, 8
@@ -169,7 +171,16 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attn_prefill_ker
     const int64_t q0 = a.cu_q[seq], k0 = a.cu_k[seq];
     const int64_t nq = a.cu_q[seq + 1] - q0, nk = a.cu_k[seq + 1] - k0;
     const int first = (int)((uint32_t)(block * kUnits) / (uint32_t)group) * 32;   // the workgroup's first query
-    if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k || first >= nq) return;
+    if (q0 < 0 || k0 < 0 || nk < 0 || q0 + nq > a.tokens_q || k0 + nk > a.tokens_k) return;
+    if (nq > a.max_q) {                                          // more queries than the grid is made for: NaN
+        using O = Val<OUT>;
+        for (int64_t i = block; i < nq; i += most) {
+            typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (q0 + i) * a.ld_out + (int64_t)kvh * group * a.hs_out;
+            for (int e = threadIdx.x; e < group * D; e += 64 * WAVES) out[e / D * a.hs_out + e % D] = O::one(__builtin_nanf(""));
+        }
+        return;
+    }
+    if (first >= nq) return;
     const int past = (int)(nk - nq);
     // a wave's 32 queries of one head: the heads that share the key head side by side
     const int part = SPLIT > 1 ? wave / kUnits : 0;              // which of SPLIT tiles at a time is the wave's

@@ -469,7 +469,7 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
  * The same call gives the same bits; how the work is divided follows from
  * seqs, max_q, max_k and the heads, and with it the last bits of a sum.
  * ld_k and ld_v below 2^24. A sequence whose offsets leave the buffers is not
- * computed. */
+ * computed; one with more queries than max_q gives NaN. */
 int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
                          const void* v, int64_t ld_v, int64_t hs_v, int out_type, void* out, int64_t ld_out,
                          int64_t hs_out, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tokens_q,

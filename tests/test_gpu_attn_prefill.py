@@ -247,3 +247,17 @@ def test_queries_whose_keys_all_score_minus_infinity(frq, nq, nk, at, d):
     if nk[0] < nq[0]:                                        # no key at all: zeros, also for a query with an inf
         s.q[3, 1, 7] = float("inf")
         assert np.all(s.run()[:nq[0] - nk[0]] == 0)
+
+
+@pytest.mark.parametrize("most", [20, 64, 129])
+@pytest.mark.parametrize("d,hq,hkv", [(64, 6, 2), (128, 4, 4)])
+def test_sequences_longer_than_max_q_are_nan(frq, most, d, hq, hkv):
+    """All their rows, and only theirs."""
+    s = Setup([130, 20, 700, 0, 300], [130, 20, 700, 5, 500], hq, hkv, d, seed=15)
+    clean = s.run()
+    out = torch.full((1170, hq, d), 5.0, dtype=torch.bfloat16, device="cuda")
+    device.attn_prefill(s.q.cuda(), s.k.cuda(), s.v.cuda(), out[:1150], *s.cu, 5, 1150, 1355, hq, hkv, d, most, 700)
+    torch.cuda.synchronize()
+    got = f64(out)
+    assert np.isnan(got[:130]).all() and np.isnan(got[150:1150]).all() and np.all(got[1150:] == 5)
+    s.check(np.concatenate([clean[:130], got[130:150], clean[150:]]))
