@@ -1241,7 +1241,9 @@ static int kv4_move(const char* what, bool write, void* cache, size_t cache_byte
     if (!k || !v || !slots) return fail(FRQ_ERR_INVALID, "null buffer");
     if (!rows_aligned(k, ld_k, size) || !rows_aligned(v, ld_v, size) || (reinterpret_cast<uintptr_t>(slots) & 7))
         return fail(FRQ_ERR_ALIGN, "%s: k and v rows must be 16-byte aligned, slots 8-byte", what);
-    if (tokens * kv_heads >= ((int64_t)1 << 30)) return fail(FRQ_ERR_UNSUPPORTED, "%s: too many heads for a launch", what);
+    // a launch has fewer than 2^32 threads; 256 for a head of 32 tokens
+    if ((tokens + 31) / 32 * kv_heads >= ((int64_t)1 << 24))
+        return fail(FRQ_ERR_UNSUPPORTED, "%s: too many heads for a launch", what);
     frq::KvArgs a{cache, pages, page_tokens, kv_heads, head_dim, type, k, v, ld_k, ld_v, slots, tokens};
     hipStream_t s = static_cast<hipStream_t>(stream);
     FRQ_HIP(write ? frq::launch_kv_write(a, s) : frq::launch_kv_read(a, s));
@@ -1286,7 +1288,7 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
     frq::DecodeArgs a{type,  q,        ld_q, cache,   pages, page_tokens, kv_heads, head_dim, table, ld_table, lens,
                       max_len, out,    ld_out, batch, q_heads, scale,     0,        0,        nullptr};
     if (!frq::plan_attn_decode(&a))
-        return fail(FRQ_ERR_UNSUPPORTED, "attn_decode: batch, heads and max_len together beyond 2^31 tiles of 32 tokens");
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_decode: batch, heads and max_len together beyond 2^31 tiles of 32 tokens or a launch");
     hipStream_t s = static_cast<hipStream_t>(stream);
     float* part;
     uint32_t* cnt;
@@ -1324,7 +1326,8 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
         !rows_aligned(out, ld_out, os) || hs_q % 8 || hs_k % 8 || hs_v % 8 || (hs_out * os) % 16 ||
         ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) & 3))
         return fail(FRQ_ERR_ALIGN, "attn_prefill: every head's row must be 16-byte aligned, the offsets 4-byte");
-    if (((max_q + 31) / 32 + 8) * seqs > ((int64_t)1 << 31) / q_heads - 1)
+    // a launch has fewer than 2^32 threads: 64 for 32 queries of a head, in workgroups of up to 8 such
+    if ((max_q + 31) / 32 * (q_heads / kv_heads) + 7 >= ((int64_t)1 << 26) / (seqs * kv_heads))
         return fail(FRQ_ERR_UNSUPPORTED, "attn_prefill: more blocks than a launch takes");
     frq::PrefillArgs a{type, out_type, q,    k,    v,        ld_q,     hs_q,  ld_k,    hs_k,     ld_v,     hs_v,   out,
                        ld_out, hs_out, cu_q, cu_k, seqs, tokens_q, tokens_k, max_q, max_k, q_heads, kv_heads, head_dim, causal != 0,

@@ -611,7 +611,8 @@ bool plan_attn_decode(DecodeArgs* a) {
     if (pairs * (tiles + kPad + 1) >= ((int64_t)1 << 31) - (1 << 20)) return false;
     const int64_t most = (pairs * (tiles + kPad) + kShareMin - 1) / kShareMin;
     a->groups = tiles <= (pairs < kGroups ? kWhole : kWholeMany) ? 0 : (int)(most < kGroups ? most : kGroups);
-    return true;
+    // a launch has fewer than 2^32 threads: 256 for a pair, or for a row that is joined
+    return (a->groups ? a->batch * a->q_heads : pairs) < ((int64_t)1 << 24);
 }
 
 size_t attn_decode_scratch(const DecodeArgs& a) {

@@ -312,7 +312,7 @@ struct DecodeArgs {
     uint64_t per_page;           // set by the launcher: 2^36 / tiles of a page, rounded up
     float* part;
 };
-bool plan_attn_decode(DecodeArgs* a);     // false: more tiles than the kernels count
+bool plan_attn_decode(DecodeArgs* a);     // false: more tiles than the kernels count, or than a launch takes
 size_t attn_decode_scratch(const DecodeArgs& a);
 hipError_t launch_attn_decode(DecodeArgs a, float* scratch, hipStream_t stream);
 

@@ -181,9 +181,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeArgs a, int lanes
     if (on) O::store8(dst, x);
 }
 
-}  // namespace
-
-hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t stream) {
+hipError_t launch_tokens(const RopeArgs& a, hipStream_t stream) {
     int lanes = 1;
     while (lanes * 8 < a.head_dim) lanes *= 2;
     const unsigned heads = (unsigned)(a.q_heads + (a.v ? 2 : 1) * a.kv_heads), tokens = (unsigned)a.tokens;
@@ -212,6 +210,24 @@ hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t stream) {
             return hipGetLastError();
         });
     });
+}
+
+}  // namespace
+
+hipError_t launch_qk_norm_rope(const RopeArgs& all, hipStream_t stream) {
+    constexpr int64_t kMost = (int64_t)1 << 23;        // tokens of 256 threads: a launch has fewer than 2^32
+    RopeArgs a = all;
+    const int64_t xs = a.x_type == kTypeF32 ? 4 : 2, os = a.out_type == kTypeF32 ? 4 : 2;
+    for (int64_t at = 0; at < all.tokens; at += kMost) {
+        a.tokens = all.tokens - at < kMost ? all.tokens - at : kMost;
+        a.x = static_cast<const char*>(all.x) + at * a.ld_x * xs;
+        a.q = static_cast<char*>(all.q) + at * a.ld_q * os;
+        a.k = static_cast<char*>(all.k) + at * a.ld_k * os;
+        if (all.v) a.v = static_cast<char*>(all.v) + at * a.ld_v * os;
+        if (all.positions) a.positions = all.positions + at;
+        if (const hipError_t e = launch_tokens(a, stream); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace frq

@@ -427,7 +427,7 @@ int frq_dev_qk_norm_rope(int x_type, const void* x, int64_t ld_x, int out_type, 
 int frq_kv4_bytes(int64_t pages, int64_t page_tokens, int64_t kv_heads, int64_t head_dim, size_t* bytes);
 /* Token t's heads k[t], v[t] into slot slots[t] = page * page_tokens + place.
  * A slot outside the cache is skipped (-1 for padding); the slots of a call
- * are distinct. */
+ * are distinct. A write or read takes fewer than 2^24 heads of 32 tokens. */
 int frq_dev_kv4_write(void* cache, size_t cache_bytes, int64_t pages, int64_t page_tokens, int64_t kv_heads,
                       int64_t head_dim, int type, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
                       const int64_t* slots, int64_t tokens, void* stream);
@@ -451,8 +451,8 @@ int frq_dev_kv4_read(const void* cache, size_t cache_bytes, int64_t pages, int64
  * workgroup) use the stream's scratch and are joined in a fixed order. The
  * division follows from lens, max_len and the shapes: the same call gives the
  * same bits, but a sequence's last bits may change with its neighbours'
- * lengths. max_len up to 2^29, and batch, key heads and tiles together below
- * 2^31. */
+ * lengths. max_len up to 2^29, batch, key heads and tiles together below 2^31,
+ * and batch times q_heads below 2^24. */
 int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
                         int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
                         const int32_t* lens, int64_t max_len, void* out, int64_t ld_out, int64_t batch, int64_t q_heads,
@@ -468,7 +468,8 @@ int frq_dev_attn_decode(int type, const void* q, int64_t ld_q, const void* cache
  * for their product with v; out of that type or F32. head_dim 64, 128 or 256.
  * The same call gives the same bits; how the work is divided follows from
  * seqs, max_q, max_k and the heads, and with it the last bits of a sum.
- * ld_k and ld_v below 2^24. A sequence whose offsets leave the buffers is not
+ * ld_k and ld_v below 2^24, and fewer than 2^26 blocks of 32 queries of a head
+ * if every sequence had max_q. A sequence whose offsets leave the buffers is not
  * computed; one with more queries than max_q gives NaN. */
 int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, const void* k, int64_t ld_k, int64_t hs_k,
                          const void* v, int64_t ld_v, int64_t hs_v, int out_type, void* out, int64_t ld_out,

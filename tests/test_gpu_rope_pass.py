@@ -32,3 +32,18 @@ def test_elements_past_the_turned_part(frq, d, part, inter, bad):
         lo = rot if i < 2 else 0
         assert torch.equal(torch.nan_to_num(got[:, lo:], nan=7e7), torch.nan_to_num(x[:, i, lo:], nan=7e7))
         assert torch.isfinite(got[:, :lo]).all()
+
+
+def test_more_tokens_than_one_launch_takes(frq):
+    """2^24 workgroups of 256 threads are one too many."""
+    n, d = (1 << 24) + 3, 8
+    row = torch.randn((1 << 12, 2 * d)).bfloat16()
+    x = row.cuda().repeat((n >> 12) + 1, 1)[:n].contiguous()
+    q, k = (torch.zeros((n, d), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table, pos = dev(rope_table(d, 4096)), torch.arange(n, dtype=torch.int32, device="cuda") % 4096
+    device.qk_norm_rope(x, q, k, None, n, 1, 1, d, table, pos, x_dtype="bf16", out_dtype="bf16")
+    torch.cuda.synchronize()
+    for t in (q, k):
+        assert torch.isfinite(t[:4096]).all() and t[:4096].abs().sum() > 0
+        assert torch.equal(t[:n >> 12 << 12].view(-1, 4096, d), t[:4096].expand(n >> 12, 4096, d))
+        assert torch.equal(t[n >> 12 << 12:], t[:3])
