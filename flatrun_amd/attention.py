@@ -245,11 +245,13 @@ class BlockAttention:
         cu_q = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         cu_k = np.concatenate([[0], np.cumsum(keys)]).astype(np.int32)
         ints = np.concatenate([np.concatenate(positions).astype(np.int32), lens, cu_q, cu_k, table.reshape(-1)])
-        if self.stream is not None:
-            self.stream.synchronize()        # earlier steps still read these buffers
-        else:
-            device.synchronize()
         lib, check = _lib.lib(), _lib.check
+        if self.stream is None:              # earlier steps still read these buffers
+            device.synchronize()
+        elif hasattr(self.stream, "synchronize"):
+            self.stream.synchronize()
+        else:                                # a stream's handle
+            check(lib.frq_stream_synchronize(device._stream(self.stream)))
         check(lib.frq_memcpy_h2d(self._ints.ptr, ints.ctypes.data, ints.nbytes))
         sl = np.concatenate(slots)
         check(lib.frq_memcpy_h2d(self._slots.ptr, sl.ctypes.data, sl.nbytes))

@@ -12,7 +12,7 @@ import torch
 
 from attn_host import Buffer, Stream, host, view    # noqa: F401  (host: fixture)
 from attn_ref import attend, block4, rope
-from flatrun_amd import device
+from flatrun_amd import _lib, device
 from flatrun_amd.attention import BlockAttention, KVCache4, Sequence, rope_table
 
 HQ, HKV, D = 4, 2, 64
@@ -176,3 +176,11 @@ def test_the_length_that_a_captured_step_is_made_for(host):
         with pytest.raises(ValueError):
             m.steps[0].plan({s: 1}, max_len=bad)
     assert s.length == 42
+
+
+def test_a_stream_given_by_its_handle(host):
+    table = device.DeviceBuffer.from_host(rope_table(D, 64))
+    step = BlockAttention(KVCache4(2, 32, HKV, D), HQ, table, 64, max_rows=8, max_seqs=2, max_context=64, stream=7)
+    more = BlockAttention(KVCache4(2, 32, HKV, D), HQ, table, 64, first=step)
+    step.plan({Sequence(): 3})
+    assert more.stream == 7 and _lib.lib().waits == [7]
