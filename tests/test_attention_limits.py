@@ -14,7 +14,7 @@ class Cache:
 
     def __init__(self, pages, kv_heads):
         self.pages, self.kv_heads = pages, kv_heads
-        self.nbytes = device.kv4_bytes(pages, 32, kv_heads, 64)
+        self.nbytes = pages * kv_heads * 32 * 2 * 64 * 9 // 16      # no call while tests are collected: torch loads first
 
     def data_ptr(self):
         return 0x10000
