@@ -44,9 +44,10 @@ def _stream(s) -> int:
         return 0
     if isinstance(s, Stream):
         return s.handle
-    if hasattr(s, "cuda_stream"):
-        return int(s.cuda_stream)
-    return int(s)
+    try:
+        return s.cuda_stream             # torch's
+    except AttributeError:
+        return int(s)
 
 
 class DeviceBuffer:
@@ -498,11 +499,6 @@ def _operand(name: str, obj, need: int, kind, ld: int = 0, hs: int = 0) -> int:
     return _addr(obj)
 
 
-def _span(rows: int, ld: int, last: int) -> int:
-    """Elements from the first to past the last of `rows` rows ld apart."""
-    return (rows - 1) * ld + last if rows > 0 else 0
-
-
 def qk_norm_rope(x, q, k, v, tokens: int, q_heads: int, kv_heads: int, head_dim: int, table, positions,
                  rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None, eps: float = 1e-6,
                  x_dtype="f32", out_dtype="f32", ld_x: int = 0, ld_q: int = 0, ld_k: int = 0, ld_v: int = 0,
@@ -526,8 +522,8 @@ def qk_norm_rope(x, q, k, v, tokens: int, q_heads: int, kv_heads: int, head_dim:
     if n_pos is None:
         n_pos = _nbytes(table) // (4 * rot) if rot and table is not None else 0
     check(lib().frq_dev_qk_norm_rope(
-        xi, _operand("x", x, xs * _span(t, lx, width), xi, lx), lx, oi, _operand("q", q, os_ * _span(t, lq, nq), oi, lq), lq,
-        _operand("k", k, os_ * _span(t, lk, nk), oi, lk), lk, _operand("v", v, os_ * _span(t, lv, nk), oi, lv), lv, t, q_heads,
+        xi, _operand("x", x, xs * ((t - 1) * lx + width), xi, lx), lx, oi, _operand("q", q, os_ * ((t - 1) * lq + nq), oi, lq), lq,
+        _operand("k", k, os_ * ((t - 1) * lk + nk), oi, lk), lk, _operand("v", v, os_ * ((t - 1) * lv + nk), oi, lv), lv, t, q_heads,
         kv_heads, hd, rot, 1 if interleaved else 0, _operand("table", table, 4 * n_pos * rot, _lib.F32), n_pos,
         _operand("positions", positions, 4 * t, _I32), _operand("q_norm", q_norm, 4 * hd, _lib.F32),
         _operand("k_norm", k_norm, 4 * hd, _lib.F32), eps, _stream(stream)))
@@ -546,7 +542,7 @@ def _kv4_args(cache, k, v, slots, tokens, dtype, ld_k, ld_v):
     ti = vtype_id(dtype)
     size = 4 if ti == 0 else 2
     return (cache.data_ptr(), cache.nbytes, cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, ti,
-            _operand("k", k, size * _span(t, lk, width), ti, lk), lk, _operand("v", v, size * _span(t, lv, width), ti, lv), lv,
+            _operand("k", k, size * ((t - 1) * lk + width), ti, lk), lk, _operand("v", v, size * ((t - 1) * lv + width), ti, lv), lv,
             _operand("slots", slots, 8 * t, _I64), t)
 
 
@@ -580,9 +576,9 @@ def attn_decode(q, cache, table, lens, out, batch: int, q_heads: int, max_len: i
     ti = vtype_id(dtype)
     size = 4 if ti == 0 else 2
     check(lib().frq_dev_attn_decode(
-        ti, _operand("q", q, size * _span(b, lq, nq), ti, lq), lq, cache.data_ptr(), cache.nbytes, cache.pages,
-        cache.page_tokens, cache.kv_heads, hd, _operand("table", table, 4 * _span(b, lt, per), _I32, lt), lt,
-        _operand("lens", lens, 4 * b, _I32), n, _operand("out", out, size * _span(b, lo, nq), ti, lo), lo, b, q_heads,
+        ti, _operand("q", q, size * ((b - 1) * lq + nq), ti, lq), lq, cache.data_ptr(), cache.nbytes, cache.pages,
+        cache.page_tokens, cache.kv_heads, hd, _operand("table", table, 4 * ((b - 1) * lt + per), _I32, lt), lt,
+        _operand("lens", lens, 4 * b, _I32), n, _operand("out", out, size * ((b - 1) * lo + nq), ti, lo), lo, b, q_heads,
         hd ** -0.5 if scale is None else scale, _stream(stream)))
 
 
@@ -603,9 +599,9 @@ def attn_prefill(q, k, v, out, cu_q, cu_k, seqs: int, tokens_q: int, tokens_k: i
     nq, nk = q_heads * hd, kv_heads * hd
     lq, lk, lv, lo = ld_q or nq, ld_k or nk, ld_v or nk, ld_out or nq
     check(lib().frq_dev_attn_prefill(
-        ti, _operand("q", q, 2 * _span(tq, lq, _span(q_heads, hq, hd)), ti, lq, hq), lq, hq,
-        _operand("k", k, 2 * _span(tk, lk, _span(kv_heads, hk, hd)), ti, lk, hk), lk, hk,
-        _operand("v", v, 2 * _span(tk, lv, _span(kv_heads, hv, hd)), ti, lv, hv), lv, hv, oi,
-        _operand("out", out, (4 if oi == 0 else 2) * _span(tq, lo, _span(q_heads, ho, hd)), oi, lo, ho), lo, ho,
+        ti, _operand("q", q, 2 * ((tq - 1) * lq + (q_heads - 1) * hq + hd) if tq else 0, ti, lq, hq), lq, hq,
+        _operand("k", k, 2 * ((tk - 1) * lk + (kv_heads - 1) * hk + hd) if tk else 0, ti, lk, hk), lk, hk,
+        _operand("v", v, 2 * ((tk - 1) * lv + (kv_heads - 1) * hv + hd) if tk else 0, ti, lv, hv), lv, hv, oi,
+        _operand("out", out, (4 if oi == 0 else 2) * ((tq - 1) * lo + (q_heads - 1) * ho + hd) if tq else 0, oi, lo, ho), lo, ho,
         _operand("cu_q", cu_q, 4 * (n + 1), _I32), _operand("cu_k", cu_k, 4 * (n + 1), _I32), n, tq, tk, int(max_q),
         int(max_k), q_heads, kv_heads, hd, 1 if causal else 0, hd ** -0.5 if scale is None else scale, _stream(stream)))

@@ -55,3 +55,10 @@ def test_strides_that_are_not_the_calls(call, kw):
 def test_rows_of_a_view(shape, strides, ld, hs, fits):
     t = torch.as_strided(torch.zeros(1 << 14), shape, strides)
     assert device._rows_of(t, ld, hs) == fits
+
+
+def test_no_rows_need_no_bytes():
+    """Whatever their strides are."""
+    none = torch.zeros((2, 0, 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="host memory"):
+        prefill(k=none, tokens_k=0, max_k=0, ld_k=128, hs_k=1 << 20)
