@@ -36,12 +36,16 @@
 // costs what the launch does: 131072 tokens 42 us, 64 ragged sequences the same).
 // Short sequences have one workgroup per sequence and key head, and no joining.
 //
-// 131072 tokens of 8 key heads of 128, 32 query heads: 35 us and 4.6 for the
-// joining, 151 MB at 4.3 TB/s (reads alone reach 6.1): 4 us until the first tile
-// is there, 2 for the end, the rest at 5.2 TB/s. 64 sequences of 1 to 8192
-// tokens: 69 and 6 us, 4.6 TB/s; vector instructions (unpacking, weights) are
-// then issued 53 % of the time, the matrix cores work 11 %. 16 sequences of
-// 2000 to 4096, 4 key heads: 15 and 4 us, of which the loads are a third.
+// 131072 tokens of 8 key heads of 128, 32 query heads: 37 us and 4.6 for the
+// joining, 151 MB at 4.1 TB/s (reads alone reach 6.1): 4 us until the first tile
+// is there, 2 for the end, the rest at 4.9 TB/s. 64 sequences of 1 to 8192
+// tokens: 73 and 6 us, 4.3 TB/s; vector instructions (unpacking, weights) are
+// then issued 55 % of the time, the matrix cores work 11 %. 16 sequences of
+// 2000 to 4096, 4 key heads: 16 and 4 us, of which the loads are a third. Powers
+// of two by channel group and the raised rests are 24 of a tile's 144 vector
+// instructions, 2 us of the first case; 256-wide heads, one wave to a SIMD, take
+// a tenth longer by them (32768 tokens, 8 heads over 4: 34.7 us against 31.2).
+// The comparisons further down were measured without them.
 #include "frq_kernels.h"
 #include "frq_kv4.h"
 
@@ -60,7 +64,9 @@ constexpr int kShareMin = 8;           // places of a workgroup, two tiles for e
 // 13), and with at least one for every workgroup (64 sequences of 8 key heads,
 // up to 63 tiles: 28.7 against 33.1; up to 256: 104 against 79).
 constexpr int kWhole = 28, kWholeMany = 64;
-constexpr int kGroups = 512;           // two workgroups of 33 KiB and 183 registers a lane on each of 256 CUs
+// Two workgroups on each of 256 CUs at 128 channels (34 KB, 193 registers a
+// lane); at 64 a CU would hold three, at 256 it holds one, and they run in turn.
+constexpr int kGroups = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRest = 4096;          // the rests stand 2^12 higher than the values
 constexpr int kTop = 5;                // of the exponents that weights stand under, see the head of the file
