@@ -128,6 +128,11 @@ SIGNATURES: dict[str, list] = {
                             _i64, _c.c_float, _vp],
     "frq_dev_attn_prefill": [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp,
                              _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _c.c_float, _vp],
+    "frq_dev_attn_chunk": [_i32, _vp, _i64, _vp, _sz, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                           _i32, _vp, _i64, _i64, _c.c_float, _vp],
+    "frq_dev_add_rms_norm": [_i32, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _c.c_float, _i32, _vp, _i64, _i64, _i64, _vp],
+    "frq_dev_sample": [_i32, _vp, _i64, _i64, _i64, _vp, _c.c_float, _vp, _i64, _vp, _c.c_float, _vp, _c.c_float, _vp, _vp, _vp,
+                       _vp],
     "frq_set_device": [_i32],
     "frq_malloc": [_c.POINTER(_vp), _sz],
     "frq_free": [_vp],

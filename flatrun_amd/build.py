@@ -39,6 +39,7 @@ SOURCES = ["frq_dequant.hip", "frq_gemv.hip", "frq_gemv_mx.hip", "frq_gemv_sk.hi
            "frq_gemm_pair.hip",
            "frq_noalloc.hip", "frq_act.hip",
            "frq_rope.hip", "frq_kv4.hip", "frq_attn_decode.hip", "frq_attn_prefill.hip",
+           "frq_attn_chunk.hip", "frq_norm.hip", "frq_sample.hip",
            "frq_api.cpp"]
 ARCH = os.environ.get("FRQ_OFFLOAD_ARCH", "gfx950")
 
@@ -69,7 +70,7 @@ def _flags() -> list[str]:
 # Attention: sums of the matrix instructions stay in ordinary registers, which the
 # softmax between two products reads (640 tokens of 16 heads: 15.1 us against 16.3;
 # 100 after 1500, twice: 27.5 against 30.5; long prompts the same).
-EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("frq_attn_decode.hip", "frq_attn_prefill.hip")}
+EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in ("frq_attn_decode.hip", "frq_attn_prefill.hip", "frq_attn_chunk.hip")}
 
 
 def _compile(src: Path, obj: Path, asm: bool) -> None:

@@ -1336,6 +1336,98 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
     return FRQ_OK;
 }
 
+int frq_dev_attn_chunk(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
+                       int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
+                       const int32_t* lens, const int32_t* cu_q, int64_t seqs, int64_t tokens_q, int64_t max_q,
+                       int64_t max_len, int out_type, void* out, int64_t ld_out, int64_t q_heads, float scale, void* stream) {
+    if ((type != FRQ_F16 && type != FRQ_BF16) || (out_type != type && out_type != FRQ_F32))
+        return fail(FRQ_ERR_INVALID, "attn_chunk: queries are F16 or BF16, the output the same or F32, got %d and %d", type, out_type);
+    if (int rc = kv4_checks("attn_chunk", cache, cache_bytes, pages, page_tokens, kv_heads, head_dim)) return rc;
+    if (!in_range(seqs, 0, (int64_t)1 << 20) || !in_range(tokens_q, 0, kMaxTokens - 256) || !in_range(max_q, 0, tokens_q))
+        return fail(FRQ_ERR_SHAPE, "attn_chunk: sequences or queries out of range");
+    if (!in_range(q_heads, 1, kMaxHeads) || q_heads % kv_heads)
+        return fail(FRQ_ERR_SHAPE, "attn_chunk: q_heads must be a multiple of kv_heads");
+    if (!in_range(max_len, 0, (int64_t)1 << 29)) return fail(FRQ_ERR_UNSUPPORTED, "attn_chunk: max_len beyond 2^29");
+    if (!in_range(ld_table, (max_len + page_tokens - 1) / page_tokens, kMaxLd))
+        return fail(FRQ_ERR_SHAPE, "attn_chunk: a row of the page table is shorter than max_len");
+    if (!in_range(ld_q, q_heads * head_dim, kMaxLd) || !in_range(ld_out, q_heads * head_dim, kMaxLd))
+        return fail(FRQ_ERR_SHAPE, "attn_chunk: a row stride is shorter than its heads");
+    if (!(scale > 0.f && scale < __builtin_inff())) return fail(FRQ_ERR_INVALID, "attn_chunk: scale must be positive");
+    if (seqs == 0 || max_q == 0) return FRQ_OK;
+    if (!q || !out || !lens || !cu_q || (!table && max_len)) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (!rows_aligned(q, ld_q, 2) || !rows_aligned(out, ld_out, out_type == FRQ_F32 ? 4 : 2) ||
+        ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(lens) | reinterpret_cast<uintptr_t>(cu_q)) & 3))
+        return fail(FRQ_ERR_ALIGN, "attn_chunk: q and out rows must be 16-byte aligned, table, lens and cu_q 4-byte");
+    // rows (queries of a head) are counted in 31 bits
+    if (max_q * (q_heads / kv_heads) >= ((int64_t)1 << 31) - 256)
+        return fail(FRQ_ERR_UNSUPPORTED, "attn_chunk: more rows of a key head than 2^31");
+    frq::ChunkArgs a{type,   out_type, q,     ld_q,    cache, pages,  page_tokens, kv_heads, head_dim, table, ld_table, lens, cu_q, seqs,
+                     tokens_q, max_q,  max_len, out, ld_out, q_heads, scale,       0,        0,        0,     0,        0,    nullptr};
+    if (!frq::plan_attn_chunk(&a)) return fail(FRQ_ERR_UNSUPPORTED, "attn_chunk: more blocks than a launch takes");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    float* part;
+    uint32_t* cnt;
+    std::lock_guard<std::mutex> lk(g_sk_mu);
+    if (int rc = sk_scratch_locked(s, frq::attn_chunk_scratch(a), 0, &part, &cnt)) return rc;
+    FRQ_HIP(frq::launch_attn_chunk(a, part, s));
+    return FRQ_OK;
+}
+
+// -------------------------------------- between blocks, and the next token
+int frq_dev_add_rms_norm(int x_type, const void* x, int64_t ld_x, int res_type, const void* residual, int64_t ld_res,
+                         void* sum, int64_t ld_sum, const float* weight, float eps, int out_type, void* out,
+                         int64_t ld_out, int64_t rows, int64_t hidden, void* stream) {
+    int64_t xs, rs, os;
+    const bool q8 = out_type == FRQ_Q8_0;
+    if (!val_type(x_type, &xs) || !val_type(res_type, &rs) || (!val_type(out_type, &os) && !q8))
+        return fail(FRQ_ERR_INVALID, "add_rms_norm: types are F32, F16 or BF16, the output's Q8_0 too, got %d, %d and %d", x_type,
+                    res_type, out_type);
+    if (!in_range(rows, 0, kMaxTokens) || !in_range(hidden, 1, (int64_t)1 << 24))
+        return fail(FRQ_ERR_SHAPE, "add_rms_norm: rows or hidden size out of range");
+    if (!in_range(ld_x, hidden, kMaxLd) || (residual && !in_range(ld_res, hidden, kMaxLd)) ||
+        (sum && !in_range(ld_sum, hidden, kMaxLd)) || !in_range(ld_out, hidden, kMaxLd))
+        return fail(FRQ_ERR_SHAPE, "add_rms_norm: a row stride is shorter than a row");
+    if (q8 && (hidden % 32 || ld_out % 32))
+        return fail(FRQ_ERR_SHAPE, "add_rms_norm: rows of Q8_0 blocks are multiples of 32 elements");
+    if (sum && !residual) return fail(FRQ_ERR_INVALID, "add_rms_norm: a sum without a residual");
+    if (!(eps >= 0.f && eps < __builtin_inff())) return fail(FRQ_ERR_INVALID, "add_rms_norm: eps must not be negative");
+    if (rows == 0) return FRQ_OK;
+    if (!x || !out) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (sum == out) return fail(FRQ_ERR_INVALID, "add_rms_norm: sum and out are the same rows");
+    if (reinterpret_cast<uintptr_t>(x) % xs || reinterpret_cast<uintptr_t>(residual) % rs ||
+        reinterpret_cast<uintptr_t>(sum) % rs || reinterpret_cast<uintptr_t>(out) % (q8 ? 2 : os) ||
+        reinterpret_cast<uintptr_t>(weight) % 4)
+        return fail(FRQ_ERR_ALIGN, "add_rms_norm: a buffer is not aligned to its type");
+    frq::NormArgs a{x_type, res_type, out_type, x, ld_x, residual, ld_res, sum, ld_sum, weight, eps, out, ld_out, rows, hidden};
+    FRQ_HIP(frq::launch_add_rms_norm(a, static_cast<hipStream_t>(stream)));
+    return FRQ_OK;
+}
+
+int frq_dev_sample(int type, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* u,
+                   float temperature, const float* temperatures, int64_t top_k, const int32_t* top_ks, float top_p,
+                   const float* top_ps, float min_p, const float* min_ps, int32_t* tokens, float* probs, void* stream) {
+    int64_t size;
+    if (!val_type(type, &size)) return fail(FRQ_ERR_INVALID, "sample: the type is F32, F16 or BF16, got %d", type);
+    if (!in_range(rows, 0, (int64_t)1 << 20)) return fail(FRQ_ERR_SHAPE, "sample: rows out of range");
+    if (!in_range(vocab, 1, (int64_t)1 << 20)) return fail(FRQ_ERR_UNSUPPORTED, "sample: 1 to 2^20 logits a row");
+    if (!in_range(ld, vocab, kMaxLd)) return fail(FRQ_ERR_SHAPE, "sample: a row stride is shorter than a row");
+    if ((!temperatures && !(temperature >= 0.f && temperature < __builtin_inff())) ||
+        (!top_ps && !(top_p >= 0.f && top_p <= 1.f)) || (!min_ps && !(min_p >= 0.f && min_p <= 1.f)) ||
+        (!top_ks && top_k < 0))
+        return fail(FRQ_ERR_INVALID, "sample: temperature and top_k must not be negative, top_p and min_p lie in [0, 1]");
+    if (rows == 0) return FRQ_OK;
+    if (!logits || !u || !tokens) return fail(FRQ_ERR_INVALID, "null buffer");
+    if (reinterpret_cast<uintptr_t>(logits) % size ||
+        ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(temperatures) | reinterpret_cast<uintptr_t>(top_ks) |
+          reinterpret_cast<uintptr_t>(top_ps) | reinterpret_cast<uintptr_t>(min_ps) | reinterpret_cast<uintptr_t>(tokens) |
+          reinterpret_cast<uintptr_t>(probs)) & 3))
+        return fail(FRQ_ERR_ALIGN, "sample: a buffer is not aligned to its type");
+    frq::SampleArgs a{type, logits, ld, rows, vocab, u, temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks,
+                      tokens, probs, 0};
+    FRQ_HIP(frq::launch_sample(a, static_cast<hipStream_t>(stream)));
+    return FRQ_OK;
+}
+
 int frq_set_device(int device) { FRQ_HIP(hipSetDevice(device)); return FRQ_OK; }
 int frq_malloc(void** ptr, size_t bytes) {
     if (!ptr) return fail(FRQ_ERR_INVALID, "null ptr");

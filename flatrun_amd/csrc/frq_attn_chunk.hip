@@ -1,0 +1,509 @@
+// Attention of chunks of new tokens against the 4-bit paged cache (frq_kv4.h),
+// which holds the new tokens' keys too: of a sequence with n queries and length
+// len, query i sees the keys j <= i + len - n,
+//   S[i, j] = scale q_i . k_j,  out_i = sum_j softmax(S)[i, j] v_j.
+//
+// The queries of the heads that share a key head stand side by side as rows,
+// 16 to a column tile of v_mfma_f32_16x16x32_f16. The products are
+// S^T = K Q^T and O^T = V^T P^T: the cache's tiles lie in the order of both left
+// operands, so that a lane unpacks what it loaded and nothing of K or V passes
+// through LDS; and S^T leaves a lane the eight tokens of a query that are its
+// k-slots in P^T. No value goes to another lane until the end.
+//
+// Numbers: k and v are code times scale, rounded to fp16 (2^-12 of themselves);
+// q stands under a power of two per row that makes its 8 (bf16) or 11 (fp16)
+// bits exact down to 2^-28 of the row's largest; weights are fp16 numbers under
+// 2^5, at most 2^12 (2^-12 of themselves, or 2^-30 of the row's largest), summed
+// as they are rounded; scores, maxima and sums are fp32. A tile with a scale
+// beyond 8188, whose values pass fp16, is worked on at an eighth of its values.
+#include "frq_kernels.h"
+#include "frq_kv4.h"
+
+namespace frq {
+namespace {
+
+using half2v = _Float16 __attribute__((ext_vector_type(2)));
+using half8v = _Float16 __attribute__((ext_vector_type(8)));
+using float4v = float __attribute__((ext_vector_type(4)));
+using us2 = unsigned short __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kUnder = 5.f, kLag = 7.f;      // of the weights' powers of two: see the head of the file
+constexpr float kInf = __builtin_inff();
+
+// Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
+// 0x6400 | n is 1024 + n; under the mask 0xF0 it is 1024 + 16 n.
+__device__ __forceinline__ half2v low_pair(uint32_t w) {
+    const half2v x = __builtin_bit_cast(half2v, vand_or(w, 0x000F000Fu, 0x64006400u));
+    return x - (half2v){1032, 1032};
+}
+__device__ __forceinline__ half2v high_pair(uint32_t w) {
+    const half2v x = __builtin_bit_cast(half2v, vand_or(w, 0x00F000F0u, 0x64006400u));
+    return __builtin_elementwise_fma(x, (half2v){0.0625f16, 0.0625f16}, (half2v){-72, -72});
+}
+__device__ __forceinline__ half8v join(half2v a, half2v b, half2v c, half2v d) {
+    return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ half2v pair_of(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ uint32_t bits_of(half2v x) { return __builtin_bit_cast(uint32_t, x); }
+// (half h of a, half h of b)
+__device__ __forceinline__ half2v halves(uint32_t a, uint32_t b, int h) {
+    return pair_of(__builtin_amdgcn_perm(b, a, h ? 0x07060302u : 0x05040100u));
+}
+
+// The largest of x over the four lanes that hold a query.
+__device__ __forceinline__ float quad_max(float x) {
+    x = __builtin_fmaxf(x, __shfl_xor(x, 16));
+    return __builtin_fmaxf(x, __shfl_xor(x, 32));
+}
+
+using const_ints = const __attribute__((address_space(4))) int32_t*;
+__device__ __forceinline__ const_ints constant(const int32_t* p) { return (const_ints)(uintptr_t)p; }
+
+// What a sequence and a workgroup's rows of it come to.
+struct Span {
+    int64_t q0;                // first query
+    int nq, len, past;
+    bool bad;                  // not what the caller said: NaN
+    __device__ __forceinline__ bool read(const ChunkArgs& a, int seq) {
+        const const_ints cu = constant(a.cu_q);
+        q0 = cu[seq];
+        const int64_t n = (int64_t)cu[seq + 1] - q0;
+        len = constant(a.lens)[seq];
+        len = len < 0 ? 0 : len;
+        if (q0 < 0 || n <= 0 || q0 + n > a.tokens_q) return false;
+        nq = (int)n;
+        bad = n > a.max_q || len > a.max_len || (len > 0 && a.pages == 0);
+        past = len - nq;
+        return true;
+    }
+    // keys that rows up to `row` see, `group` rows to a token
+    __device__ __forceinline__ int keys(int row, int group) const {
+        const int i = row / group, e = past + (i < nq ? i : nq - 1) + 1;
+        return e < 0 ? 0 : e;
+    }
+};
+
+template <int TYPE, int OUT, int NG, int R>
+__global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) attn_chunk_kernel(ChunkArgs a) {
+    using T = Val<TYPE>;
+    using O = Val<OUT>;
+    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 16 * R;
+    __shared__ __attribute__((aligned(16))) float sh_o[2][R * 2 * NG][64][4];
+    __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, j = lane >> 4;
+    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
+    uint32_t id = blockIdx.x;
+    const int split = (int)(id % (uint32_t)a.splits);
+    id /= (uint32_t)a.splits;
+    const int kvh = (int)(id % (uint32_t)a.kv_heads);
+    id /= (uint32_t)a.kv_heads;
+    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
+    Span sp;
+    if (!sp.read(a, seq)) return;
+    if (sp.bad) {
+        if (split) return;
+        for (int64_t i = block; i < sp.nq; i += a.blocks) {
+            typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)kvh * group * D;
+            for (int e = threadIdx.x; e < group * D; e += 64 * kWaves) out[e] = O::one(__builtin_nanf(""));
+        }
+        return;
+    }
+    const int row0 = block * kRows, rows = sp.nq * group;
+    if (row0 >= rows) return;
+    const int end = sp.keys(row0 + kRows - 1, group);                // keys that the workgroup's rows see
+    const int tiles = (end + kKvTile - 1) / kKvTile;
+    const int first = split * (int)a.share;
+    const int last = tiles < first + (int)a.share ? tiles : first + (int)a.share;
+    if (first >= tiles && split) return;                             // nothing here: the joining knows
+    const int whole = sp.keys(row0, group);                          // keys below this one every row sees
+
+    // the lane's rows, one of each column tile: queries, and the last key they see
+    half8v qf[R][NG];
+    float rs[R], m[R], nref[R], l[R];
+    int lim[R];
+#pragma unroll
+    for (int c = 0; c < R; ++c) {
+        int row = row0 + 16 * c + n;
+        row = row < rows ? row : rows - 1;
+        const int i = row / group;
+        lim[c] = sp.past + i;
+        const typename T::Elem* q = static_cast<const typename T::Elem*>(a.q) + (sp.q0 + i) * a.ld_q +
+                                    (int64_t)(kvh * group + row - i * group) * D;
+        float x[NG][8];
+        uint32_t top = 0;                                            // bits of the largest |q|; inf and NaN above all
+#pragma unroll
+        for (int g = 0; g < NG; ++g) T::load8(q + 32 * g + 8 * j, x[g]);
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t b = __builtin_bit_cast(uint32_t, x[g][e]) & 0x7FFFFFFFu;
+                top = top > b ? top : b;
+            }
+        uint32_t other = __shfl_xor(top, 16);
+        top = top > other ? top : other;
+        other = __shfl_xor(top, 32);
+        top = top > other ? top : other;
+        const int up = top ? 140 - (int)(top >> 23) : 0;             // the largest to [2^13, 2^14)
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qf[c][g][e] = (_Float16)__builtin_ldexpf(x[g][e], up);
+        rs[c] = top >= 0x7F800000u ? __builtin_nanf("") : __builtin_ldexpf(a.scale * kLog2e, -up);
+        m[c] = -kInf;
+        nref[c] = 0.f;
+        l[c] = 0.f;
+    }
+    float4v o[R][2 * NG];
+#pragma unroll
+    for (int c = 0; c < R; ++c)
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) o[c][i] = float4v{0, 0, 0, 0};
+
+    const const_ints table = constant(a.table) + (int64_t)seq * a.ld_table;
+    const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
+    const int64_t page_bytes = a.kv_heads * (int64_t)page_tiles * kTile;
+    const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
+    bool bad = false;
+    auto address = [&](int tile) {
+        const uint32_t in = (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36);
+        int page = table[in];
+        if ((uint32_t)page >= (uint64_t)a.pages) {
+            bad = true;
+            page = 0;
+        }
+        return heads + page * page_bytes + (int64_t)((uint32_t)tile - in * page_tiles) * kTile;
+    };
+
+    for (int tile = first + wave; tile < last; tile += kWaves) {
+        const uint8_t* at = address(tile);
+        uint32_t kc[2 * NG], ks[NG], vc[2 * NG], vs[4][NG], flat = 0;
+#pragma unroll
+        for (int p = 0; p < 2 * NG; p += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(at + kv_word(p, lane));
+            kc[p] = x.x; kc[p + 1] = x.y; kc[p + 2] = x.z; kc[p + 3] = x.w;
+            const uint4 y = *reinterpret_cast<const uint4*>(at + kv_vc_off(NG) + kv_word(p, lane));
+            vc[p] = y.x; vc[p + 1] = y.y; vc[p + 2] = y.z; vc[p + 3] = y.w;
+        }
+#pragma unroll
+        for (int p = 0; p < NG; p += 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(at + kv_ks_off(NG) + kv_scale(n, 0, NG) + 4 * p);
+            ks[p] = x.x; ks[p + 1] = x.y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                            // tokens 4j + i and 16 more
+                const uint2 y = *reinterpret_cast<const uint2*>(at + kv_vs_off(NG) + kv_scale(4 * j + i, 0, NG) + 4 * p);
+                vs[i][p] = y.x; vs[i][p + 1] = y.y;
+            }
+        }
+        // is a scale beyond 8188, or no number?
+#pragma unroll
+        for (int p = 0; p < NG; ++p) {
+            us2 x = __builtin_bit_cast(us2, ks[p] & 0x7FFF7FFFu);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x = __builtin_elementwise_max(x, __builtin_bit_cast(us2, vs[i][p] & 0x7FFF7FFFu));
+            flat |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(x, (us2){0x6FFF, 0x6FFF}));
+        }
+        const int kt = tile * kKvTile;
+        const bool masked = kt + kKvTile > whole;
+        float up = 1.f, down = 1.f, under = kUnder;
+        uint64_t gone = 0;                                           // blocks taken out of the product
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(flat != 0) != 0, 0)) {
+            // Behind the sequence's end nothing is known, and a zero weight does
+            // not take a NaN out of a product: where rows differ in what they
+            // see, a block of V that is no number leaves the product, to be
+            // added below for the rows that see it.
+            bool any = false, big = false;
+            auto clean = [&](uint32_t& w, bool v, int token, int h) {
+                const uint32_t half = h ? 0xFFFF0000u : 0xFFFFu, s = (h ? w >> 16 : w) & 0x7FFFu;
+                const bool past_end = token >= sp.len, no = s >= 0x7C00;
+                big |= s > 0x6FFF && !past_end && !no;
+                any |= v && no && masked && !past_end;
+                if (past_end || (v && no && masked)) w &= ~half;
+            };
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const int p = (u * NG + g) / 2, h = (u * NG + g) & 1;
+                    clean(ks[p], false, kt + 16 * u + n, h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) clean(vs[i][p], true, kt + 16 * u + 4 * j + i, h);
+                }
+            gone = __builtin_amdgcn_ballot_w64(any);
+            if (__builtin_amdgcn_ballot_w64(big)) {
+                up = 8.f;
+                down = 0.125f;
+                under = kUnder + 3.f;
+#pragma unroll
+                for (int p = 0; p < NG; ++p) {
+                    ks[p] = bits_of(pair_of(ks[p]) * (half2v){0.125f16, 0.125f16});
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vs[i][p] = bits_of(pair_of(vs[i][p]) * (half2v){0.125f16, 0.125f16});
+                }
+            }
+        }
+        // the tile's operands: K of 16 tokens and 32 channels each, V of 16 channels
+        half8v kf[2][NG], vf[2 * NG];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t w = kc[u * NG + g], at2 = ks[(u * NG + g) / 2];
+                const half2v d = halves(at2, at2, (u * NG + g) & 1);
+                kf[u][g] = join(low_pair(w) * d, high_pair(w) * d, low_pair(w >> 8) * d, high_pair(w >> 8) * d);
+            }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const uint32_t w0 = vc[2 * g], w1 = vc[2 * g + 1];
+            half2v d[4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int p = (u * NG + g) / 2, h = (u * NG + g) & 1;
+                    d[2 * u + i] = halves(vs[2 * i][p], vs[2 * i + 1][p], h);
+                }
+            vf[2 * g] = join(low_pair(w0) * d[0], low_pair(w0 >> 8) * d[1], low_pair(w1) * d[2], low_pair(w1 >> 8) * d[3]);
+            vf[2 * g + 1] = join(high_pair(w0) * d[0], high_pair(w0 >> 8) * d[1], high_pair(w1) * d[2], high_pair(w1 >> 8) * d[3]);
+        }
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+            float4v s[2] = {float4v{0, 0, 0, 0}, float4v{0, 0, 0, 0}};
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u][g], qf[c][g], s[u], 0, 0, 0);
+            const float by = rs[c] * up;
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (kt + 16 * u + 4 * j + i > lim[c]) s[u][i] = -kInf;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, s[u][i]);
+            top *= by;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m[c] + kLag) != 0, 0)) {
+                // each row by its own scores alone
+                const float all = quad_max(top), mn = all > m[c] + kLag ? all : m[c];
+                const float keep = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
+                m[c] = mn;
+                nref[c] = mn == -kInf ? 0.f : -mn;
+                l[c] *= keep;
+#pragma unroll
+                for (int d = 0; d < 2 * NG; ++d) o[c][d] *= keep;
+            }
+            half2v pf[4];
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], by, nref[c] + under));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], by, nref[c] + under));
+                    const half2v p = {(_Float16)p0, (_Float16)p1};
+                    pf[2 * u + i / 2] = p;
+                    sum = __builtin_amdgcn_fdot2(p, (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
+                }
+            l[c] = __builtin_fmaf(sum, down, l[c]);
+            const half8v pv = join(pf[0], pf[1], pf[2], pf[3]);
+#pragma unroll
+            for (int d = 0; d < 2 * NG; ++d) o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pv, o[c][d], 0, 0, 0);
+        }
+        if (__builtin_expect(gone != 0, 0)) {
+            for (int t = 0; t < kKvTile && kt + t < sp.len; ++t)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint16_t b = *reinterpret_cast<const uint16_t*>(at + kv_vs_off(NG) + kv_scale(t, g, NG));
+                    if ((b & 0x7C00) == 0x7C00) {
+#pragma unroll
+                        for (int c = 0; c < R; ++c)
+                            if (kt + t <= lim[c]) o[c][2 * g] += __builtin_nanf(""), o[c][2 * g + 1] += __builtin_nanf("");
+                    }
+                }
+        }
+    }
+    if (__builtin_amdgcn_ballot_w64(bad)) {
+#pragma unroll
+        for (int c = 0; c < R; ++c) l[c] = __builtin_nanf("");
+    }
+
+    // the waves' sums, under the largest of their references: 2 and 3 to 0 and 1, 1 to 0
+#pragma unroll
+    for (int c = 0; c < R; ++c) {
+        l[c] += __shfl_xor(l[c], 16);
+        l[c] += __shfl_xor(l[c], 32);
+        if (j == 0) {
+            sh_m[wave][16 * c + n] = m[c];
+            sh_l[wave][16 * c + n] = l[c];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < R; ++c) {
+        float mm = sh_m[0][16 * c + n];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh_m[w][16 * c + n]);
+        const float base = mm == -kInf ? 0.f : mm, f = __builtin_amdgcn_exp2f(m[c] - base);
+#pragma unroll
+        for (int d = 0; d < 2 * NG; ++d) o[c][d] *= f;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum += sh_l[w][16 * c + n] * __builtin_amdgcn_exp2f(sh_m[w][16 * c + n] - base);
+        l[c] = sum;
+        m[c] = mm;
+    }
+#pragma unroll
+    for (int half = 2; half; half >>= 1) {
+        if (wave >= half && wave < 2 * half)
+#pragma unroll
+            for (int c = 0; c < R; ++c)
+#pragma unroll
+                for (int d = 0; d < 2 * NG; ++d) *reinterpret_cast<float4v*>(sh_o[wave - half][c * 2 * NG + d][lane]) = o[c][d];
+        __syncthreads();
+        if (wave < half)
+#pragma unroll
+            for (int c = 0; c < R; ++c)
+#pragma unroll
+                for (int d = 0; d < 2 * NG; ++d) o[c][d] += *reinterpret_cast<const float4v*>(sh_o[wave][c * 2 * NG + d][lane]);
+        __syncthreads();
+    }
+    if (wave) return;
+#pragma unroll
+    for (int c = 0; c < R; ++c) {
+        const int row = row0 + 16 * c + n;
+        if (row >= rows) continue;
+        if (a.splits > 1) {
+            float* part = a.part + (((int64_t)(seq * a.kv_heads + kvh) * a.blocks + block) * a.splits + split) * kRows * (D + 4) +
+                          (16 * c + n) * (D + 4);
+#pragma unroll
+            for (int d = 0; d < 2 * NG; ++d) *reinterpret_cast<float4v*>(part + 16 * d + 4 * j) = o[c][d];
+            if (j == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[c], l[c]);
+            continue;
+        }
+        // zeros for a query without keys; no weight at all elsewhere is 0 / 0
+        const int i = row / group;
+        const float inv = 1.0f / l[c];
+        typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)(kvh * group + row - i * group) * D;
+#pragma unroll
+        for (int d = 0; d < 2 * NG; ++d) {
+            typename O::Elem y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = O::one(lim[c] < 0 ? 0.f : l[c] == 0.f ? __builtin_nanf("") : o[c][d][e] * inv);
+            __builtin_memcpy(__builtin_assume_aligned(out + 16 * d + 4 * j, 4 * sizeof(y[0])), y, sizeof(y));
+        }
+    }
+}
+
+// A row's parts of all splits, joined in their order; a wave a row of D channels.
+template <int OUT, int NG>
+__global__ void __launch_bounds__(256) attn_chunk_join_kernel(ChunkArgs a, int kRows) {
+    using O = Val<OUT>;
+    constexpr int D = 32 * NG, kPer = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
+    const uint32_t unit = blockIdx.x;                                // block of a key head of a sequence
+    const uint32_t id = unit / (uint32_t)a.blocks;
+    const int block = (int)(unit % (uint32_t)a.blocks), kvh = (int)(id % (uint32_t)a.kv_heads), seq = (int)(id / (uint32_t)a.kv_heads);
+    Span sp;
+    if (!sp.read(a, seq) || sp.bad) return;
+    const int row0 = block * kRows, rows = sp.nq * group;
+    if (row0 >= rows) return;
+    const int tiles = (sp.keys(row0 + kRows - 1, group) + kKvTile - 1) / kKvTile;
+    const int share = (int)a.share, used = tiles <= share ? 1 : (tiles + share - 1) / share;
+    const float* parts = a.part + (int64_t)unit * a.splits * kRows * (D + 4);
+    for (int r = threadIdx.x >> 6; r < kRows && row0 + r < rows; r += 4) {
+        const float* p = parts + r * (D + 4);
+        const int64_t step = (int64_t)kRows * (D + 4);
+        float mm = -kInf;
+        for (int s = lane; s < used; s += 64) mm = __builtin_fmaxf(mm, p[s * step + D]);
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) mm = __builtin_fmaxf(mm, __shfl_xor(mm, i));
+        const float base = mm == -kInf ? 0.f : mm;
+        float val[kPer] = {}, sum = 0.f;
+        for (int s = 0; s < used; ++s) {
+            const float f = __builtin_amdgcn_exp2f(p[s * step + D] - base);
+            sum = __builtin_fmaf(f, p[s * step + D + 1], sum);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) val[e] = __builtin_fmaf(f, p[s * step + lane * kPer + e], val[e]);
+        }
+        const int i = (row0 + r) / group;
+        typename O::Elem* out =
+            static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)(kvh * group + row0 + r - i * group) * D + lane * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) out[e] = O::one(sp.past + i < 0 ? 0.f : val[e] / sum);
+    }
+}
+
+template <int TYPE, int OUT, int NG, int R>
+hipError_t launch_one(const ChunkArgs& a, hipStream_t stream) {
+    const int64_t units = a.seqs * a.kv_heads * a.blocks;
+    attn_chunk_kernel<TYPE, OUT, NG, R><<<(unsigned)(units * a.splits), 64 * kWaves, 0, stream>>>(a);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
+    attn_chunk_join_kernel<OUT, NG><<<(unsigned)units, 256, 0, stream>>>(a, 16 * R);
+    return hipGetLastError();
+}
+
+template <int TYPE, int OUT>
+hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
+    const auto run = [&](auto ng) {
+        constexpr int kN = decltype(ng)::value;
+        switch (a.tiles) {
+            case 1: return launch_one<TYPE, OUT, kN, 1>(a, stream);
+            case 2: return launch_one<TYPE, OUT, kN, 2>(a, stream);
+            default:
+                if constexpr (kN <= 4) return launch_one<TYPE, OUT, kN, 4>(a, stream);
+                return hipErrorInvalidValue;
+        }
+    };
+    switch (a.head_dim) {
+        case 64: return run(Int<2>{});
+        case 128: return run(Int<4>{});
+        case 256: return run(Int<8>{});
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+bool plan_attn_chunk(ChunkArgs* a) {
+    const int64_t rows = a->max_q * (a->q_heads / a->kv_heads), keys = (a->max_len + kKvTile - 1) / kKvTile;
+    a->tiles = rows <= 16 ? 1 : rows <= 32 || a->head_dim == 256 ? 2 : 4;
+    a->blocks = (rows + 16 * a->tiles - 1) / (16 * a->tiles);
+    const int64_t units = a->seqs * a->kv_heads * a->blocks;
+    if (units >= (int64_t)1 << 23) return false;                     // a launch has fewer than 2^32 threads
+    int64_t splits = units >= 512 ? 1 : (1024 + units - 1) / units;
+    const int64_t most = (keys + 4 * kWaves - 1) / (4 * kWaves);     // four tiles a wave at least
+    splits = splits < most ? splits : most;
+    splits = splits > 0 ? splits : 1;
+    a->share = (keys + splits - 1) / splits;
+    a->share = a->share > 0 ? a->share : 1;
+    a->splits = (keys + a->share - 1) / a->share;
+    a->splits = a->splits > 0 ? a->splits : 1;
+    a->per_page = ((uint64_t)1 << 36) / ((uint64_t)a->page_tokens / kKvTile) + 1;
+    return true;
+}
+
+size_t attn_chunk_scratch(const ChunkArgs& a) {
+    if (a.splits == 1) return 0;
+    return sizeof(float) * (size_t)(a.seqs * a.kv_heads * a.blocks * a.splits * 16 * a.tiles) * (size_t)(a.head_dim + 4);
+}
+
+hipError_t launch_attn_chunk(ChunkArgs a, float* scratch, hipStream_t stream) {
+    a.part = scratch;
+    if (a.type == kTypeBF16)
+        return a.out_type == kTypeF32 ? launch_typed<kTypeBF16, kTypeF32>(a, stream)
+                                      : launch_typed<kTypeBF16, kTypeBF16>(a, stream);
+    return a.out_type == kTypeF32 ? launch_typed<kTypeF16, kTypeF32>(a, stream)
+                                  : launch_typed<kTypeF16, kTypeF16>(a, stream);
+}
+
+}  // namespace frq

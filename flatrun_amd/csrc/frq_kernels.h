@@ -332,6 +332,63 @@ struct PrefillArgs {
 };
 hipError_t launch_attn_prefill(PrefillArgs a, hipStream_t stream);
 
+// Chunks of new tokens against the 4-bit cache.
+struct ChunkArgs {
+    int type, out_type;
+    const void* q;
+    int64_t ld_q;
+    const void* cache;
+    int64_t pages, page_tokens, kv_heads, head_dim;
+    const int32_t* table;
+    int64_t ld_table;
+    const int32_t *lens, *cu_q;
+    int64_t seqs, tokens_q, max_q, max_len;
+    void* out;
+    int64_t ld_out, q_heads;
+    float scale;
+    // plan_attn_chunk: column tiles of 16 rows of a workgroup, workgroups of the
+    // longest chunk and a key head, the parts its keys are split into, and the
+    // tiles of a part
+    int64_t tiles, blocks, splits, share;
+    uint64_t per_page;           // 2^36 / tiles of a page, rounded up
+    float* part;
+};
+bool plan_attn_chunk(ChunkArgs* a);       // false: more than a launch takes
+size_t attn_chunk_scratch(const ChunkArgs& a);
+hipError_t launch_attn_chunk(ChunkArgs a, float* scratch, hipStream_t stream);
+
+// The residual's addition and the norm behind it (out_type: a type above, or 8,
+// Q8_0 blocks, whose ld_out is in elements too), and the draw of a token.
+struct NormArgs {
+    int x_type, res_type, out_type;
+    const void* x;
+    int64_t ld_x;
+    const void* residual;        // null: x alone
+    int64_t ld_res;
+    void* sum;                   // null: not stored
+    int64_t ld_sum;
+    const float* weight;         // null: ones
+    float eps;
+    void* out;
+    int64_t ld_out, rows, hidden;
+};
+hipError_t launch_add_rms_norm(const NormArgs& a, hipStream_t stream);
+
+struct SampleArgs {
+    int type;
+    const void* logits;
+    int64_t ld, rows, vocab;
+    const float* u;
+    float temperature, top_p, min_p;         // where there is no array of one a row
+    int64_t top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const int32_t* top_ks;
+    int32_t* tokens;
+    float* probs;                // null: not stored
+    int frac;                    // set by the launcher: bits of a weight below 1
+};
+hipError_t launch_sample(SampleArgs a, hipStream_t stream);
+
 // Scratch a caller brings in place of the stream registry's: exchange slots
 // (zero before a launch, left zero by every launch) and split-K partials.
 struct FixedScratch {

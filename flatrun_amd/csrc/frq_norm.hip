@@ -1,0 +1,229 @@
+// The residual's addition and the root-mean-square norm behind it, one pass:
+//   h = x + r, rounded to the residual's type (the next block's residual)
+//   y = h / sqrt(mean(h^2) + eps) * w
+// y in fp32, fp16, bf16, or as Q8_0 blocks: of the fp32 values, 32 at a time,
+// d = fp16(max|y| / 127), held to 65504, and the codes round_even(y / d); a block
+// with an inf or a NaN has d = NaN.
+//
+// Sums and products are in 64 bits and rounded once: an fp32 sum of squares
+// leaves the last bit of y to the order of the sum, and with it, now and then,
+// a code of the 8-bit form. Memory bounds the kernel either way.
+//
+// A workgroup holds a row in registers, eight elements at a time a thread. Rows
+// of other sizes and alignments (and those past 16384 elements) take a second
+// kernel, which reads them twice, an element a thread.
+#include "frq_kernels.h"
+#include "frq_vals.h"
+
+namespace frq {
+namespace {
+
+constexpr int kQ8 = 8;                   // out_type: Q8_0 blocks, 34 bytes for 32 elements
+constexpr int kQ8Bytes = 34;
+
+// Sum over the workgroup, in a fixed order; part: one place a wave.
+__device__ __forceinline__ double group_sum(double x, double* part) {
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) x += __shfl_xor(x, i);
+    const int waves = blockDim.x >> 6;
+    if (waves > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = part[0];
+        for (int w = 1; w < waves; ++w) x += part[w];
+    }
+    return x;
+}
+
+// fp16(top / 127), held to 65504, and the code of y: correctly rounded quotients.
+__device__ __forceinline__ uint16_t q8_scale(float top) { return f32_to_f16_bits(__builtin_fminf(top / 127.0f, 65504.f)); }
+__device__ __forceinline__ int q8_code(float y, float d) {
+    if (d == 0.f) return 0;
+    const float q = __builtin_rintf(y / d);
+    return (int)__builtin_fminf(__builtin_fmaxf(q, -127.f), 127.f);
+}
+
+template <int TYPE>
+__device__ __forceinline__ float round_to(float x) {
+    if constexpr (TYPE == kTypeBF16) return __builtin_bit_cast(float, (uint32_t)f32_to_bf16_bits(x) << 16);
+    if constexpr (TYPE == kTypeF16) return f16_bits_to_f32(f32_to_f16_bits(x));
+    return x;
+}
+
+// Eight elements a thread, CH times.
+template <int X, int R, int OUT, int CH>
+__global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
+    using TX = Val<X>;
+    using TR = Val<R>;
+    __shared__ double part[16];
+    const int64_t row = blockIdx.x;
+    const int hidden = (int)a.hidden, step = (int)blockDim.x * 8;
+    float h[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = c * step + (int)threadIdx.x * 8;
+        if (e < hidden) TX::load8(static_cast<const typename TX::Elem*>(a.x) + row * a.ld_x + e, h[c]);
+    }
+    if (a.residual) {
+        float r[CH][8];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e = c * step + (int)threadIdx.x * 8;
+            if (e < hidden) TR::load8(static_cast<const typename TR::Elem*>(a.residual) + row * a.ld_res + e, r[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e = c * step + (int)threadIdx.x * 8;
+            if (e >= hidden) break;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[c][i] = round_to<R>(h[c][i] + r[c][i]);
+            if (a.sum) TR::store8(static_cast<typename TR::Elem*>(a.sum) + row * a.ld_sum + e, h[c]);
+        }
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        if (c * step + (int)threadIdx.x * 8 < hidden)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)h[c][i], (double)h[c][i], ss);
+    const double f = 1.0 / __builtin_sqrt(group_sum(ss, part) / (double)hidden + (double)a.eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = c * step + (int)threadIdx.x * 8;
+        if (e >= hidden) break;                          // whole blocks of 32: four lanes go together
+        float w[8], y[8];
+        if (a.weight) Val<kTypeF32>::load8(a.weight + e, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (float)((double)h[c][i] * f * (a.weight ? (double)w[i] : 1.0));
+        if constexpr (OUT == kQ8) {
+            float top = 0.f;
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                top = __builtin_fmaxf(top, __builtin_fabsf(y[i]));
+                odd |= !(__builtin_fabsf(y[i]) < __builtin_inff());
+            }
+            if (odd) top = __builtin_inff();
+            top = __builtin_fmaxf(top, __shfl_xor(top, 1));
+            top = __builtin_fmaxf(top, __shfl_xor(top, 2));
+            const uint16_t bits = top < __builtin_inff() ? q8_scale(top) : 0x7E00;
+            const float d = f16_bits_to_f32(bits);
+            uint32_t lo = 0, hi = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                lo |= (uint32_t)(q8_code(y[i], d) & 255) << (8 * i);
+                hi |= (uint32_t)(q8_code(y[4 + i], d) & 255) << (8 * i);
+            }
+            uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.out) + (row * a.ld_out + e) / 32 * kQ8Bytes);
+            const int j = threadIdx.x & 3;
+            if (j == 0) to[0] = bits;
+            to[1 + 4 * j] = (uint16_t)lo;
+            to[2 + 4 * j] = (uint16_t)(lo >> 16);
+            to[3 + 4 * j] = (uint16_t)hi;
+            to[4 + 4 * j] = (uint16_t)(hi >> 16);
+        } else {
+            using TO = Val<OUT>;
+            TO::store8(static_cast<typename TO::Elem*>(a.out) + row * a.ld_out + e, y);
+        }
+    }
+}
+
+__device__ __forceinline__ float load_one(int type, const void* p, int64_t i) {
+    if (type == kTypeF32) return static_cast<const float*>(p)[i];
+    const uint16_t b = static_cast<const uint16_t*>(p)[i];
+    return type == kTypeF16 ? f16_bits_to_f32(b) : __builtin_bit_cast(float, (uint32_t)b << 16);
+}
+__device__ __forceinline__ void store_one(int type, void* p, int64_t i, float x) {
+    if (type == kTypeF32)
+        static_cast<float*>(p)[i] = x;
+    else
+        static_cast<uint16_t*>(p)[i] = type == kTypeF16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
+}
+
+// Any size and alignment: a row twice, an element a thread; 32 lanes share a block.
+__global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
+    __shared__ double part[4];
+    const int64_t row = blockIdx.x;
+    auto sum_at = [&](int64_t e) {
+        const float x = load_one(a.x_type, a.x, row * a.ld_x + e);
+        if (!a.residual) return x;
+        const float h = x + load_one(a.res_type, a.residual, row * a.ld_res + e);
+        return a.res_type == kTypeF32 ? h : a.res_type == kTypeF16 ? round_to<kTypeF16>(h) : round_to<kTypeBF16>(h);
+    };
+    double ss = 0.0;
+    for (int64_t e = threadIdx.x; e < a.hidden; e += 256) {
+        const float h = sum_at(e);
+        if (a.sum) store_one(a.res_type, a.sum, row * a.ld_sum + e, h);
+        ss = __builtin_fma((double)h, (double)h, ss);
+    }
+    const double f = 1.0 / __builtin_sqrt(group_sum(ss, part) / (double)a.hidden + (double)a.eps);
+    for (int64_t e = threadIdx.x; e < a.hidden; e += 256) {
+        // the sum may stand where x or the residual stood
+        const float h = a.sum ? load_one(a.res_type, a.sum, row * a.ld_sum + e) : sum_at(e);
+        const float y = (float)((double)h * f * (a.weight ? (double)a.weight[e] : 1.0));
+        if (a.out_type != kQ8) {
+            store_one(a.out_type, a.out, row * a.ld_out + e, y);
+            continue;
+        }
+        float top = __builtin_fabsf(y) < __builtin_inff() ? __builtin_fabsf(y) : __builtin_inff();
+#pragma unroll
+        for (int i = 1; i < 32; i <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, i));
+        const uint16_t bits = top < __builtin_inff() ? q8_scale(top) : 0x7E00;
+        uint8_t* to = static_cast<uint8_t*>(a.out) + (row * a.ld_out + e) / 32 * kQ8Bytes;
+        if ((e & 31) == 0) *reinterpret_cast<uint16_t*>(to) = bits;
+        to[2 + (e & 31)] = (uint8_t)q8_code(y, f16_bits_to_f32(bits));
+    }
+}
+
+template <int X, int R, int OUT>
+hipError_t launch_typed(const NormArgs& a, unsigned threads, hipStream_t stream) {
+    if (a.hidden <= (int64_t)threads * 8)
+        norm_rows_kernel<X, R, OUT, 1><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+    else
+        norm_rows_kernel<X, R, OUT, 2><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+bool aligned(const void* p, int64_t ld, int type) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * (type == kTypeF32 ? 4 : 2) % 16 == 0;
+}
+
+hipError_t launch_part(const NormArgs& a, hipStream_t stream) {
+    const bool wide = a.hidden % 8 == 0 && a.hidden <= 16384 && aligned(a.x, a.ld_x, a.x_type) &&
+                      (!a.residual || aligned(a.residual, a.ld_res, a.res_type)) &&
+                      (!a.sum || aligned(a.sum, a.ld_sum, a.res_type)) && (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0 &&
+                      (a.out_type == kQ8 || aligned(a.out, a.ld_out, a.out_type));
+    if (!wide) {
+        norm_any_kernel<<<(unsigned)a.rows, 256, 0, stream>>>(a);
+        return hipGetLastError();
+    }
+    unsigned threads = 64;
+    while (threads < 1024 && (int64_t)threads * 8 < a.hidden) threads *= 2;
+    return with_type(a.x_type, [&](auto x) {
+        return with_type(a.residual ? a.res_type : kTypeF32, [&](auto r) {
+            constexpr int kX = decltype(x)::value, kR = decltype(r)::value;
+            if (a.out_type == kQ8) return launch_typed<kX, kR, kQ8>(a, threads, stream);
+            return with_type(a.out_type, [&](auto o) { return launch_typed<kX, kR, decltype(o)::value>(a, threads, stream); });
+        });
+    });
+}
+
+}  // namespace
+
+hipError_t launch_add_rms_norm(const NormArgs& all, hipStream_t stream) {
+    constexpr int64_t kMost = (int64_t)1 << 21;          // rows of 1024 threads: a launch has fewer than 2^32
+    NormArgs a = all;
+    const auto size = [](int type) { return type == kTypeF32 ? 4 : 2; };
+    for (int64_t at = 0; at < all.rows; at += kMost) {
+        a.rows = all.rows - at < kMost ? all.rows - at : kMost;
+        a.x = static_cast<const char*>(all.x) + at * a.ld_x * size(a.x_type);
+        if (a.residual) a.residual = static_cast<const char*>(all.residual) + at * a.ld_res * size(a.res_type);
+        if (a.sum) a.sum = static_cast<char*>(all.sum) + at * a.ld_sum * size(a.res_type);
+        a.out = static_cast<char*>(all.out) +
+                (a.out_type == kQ8 ? at * a.ld_out / 32 * kQ8Bytes : at * a.ld_out * size(a.out_type));
+        if (const hipError_t e = launch_part(a, stream); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace frq

@@ -440,7 +440,8 @@ def vtype_id(t) -> int:
     return i
 
 
-_I32, _I64 = "int32", "int64"
+_I32, _I64, _U8 = "int32", "int64", "torch.uint8"
+_Q8 = _lib.QTYPES["Q8_0"]
 _KINDS: dict = {}              # dtype object -> type id or integer kind (filled as dtypes are met)
 
 
@@ -605,3 +606,84 @@ def attn_prefill(q, k, v, out, cu_q, cu_k, seqs: int, tokens_q: int, tokens_k: i
         _operand("out", out, (4 if oi == 0 else 2) * ((tq - 1) * lo + (q_heads - 1) * ho + hd) if tq else 0, oi, lo, ho), lo, ho,
         _operand("cu_q", cu_q, 4 * (n + 1), _I32), _operand("cu_k", cu_k, 4 * (n + 1), _I32), n, tq, tk, int(max_q),
         int(max_k), q_heads, kv_heads, hd, 1 if causal else 0, hd ** -0.5 if scale is None else scale, _stream(stream)))
+
+
+def attn_chunk(q, cache, table, lens, cu_q, out, seqs: int, tokens_q: int, q_heads: int, max_q: int, max_len: int,
+               dtype="bf16", out_dtype=None, scale: float | None = None, ld_q: int = 0, ld_out: int = 0, ld_table: int = 0,
+               stream=None) -> None:
+    """Attention of each sequence's new tokens, the queries [cu_q[s], cu_q[s + 1])
+    (int32 on the device, seqs + 1), over the lens[s] tokens that a
+    :class:`flatrun_amd.attention.KVCache4` holds of it, the new ones among them,
+    causal from the last token back; enqueued (frq_dev_attn_chunk).
+
+    ``table``, ``lens`` and ``ld_table`` as for :func:`attn_decode`; no sequence
+    has more than ``max_q`` queries or ``max_len`` tokens. ``dtype`` "bf16" or
+    "f16"; ``out_dtype`` the same (default) or "f32"."""
+    hd, n, tq, most = cache.head_dim, int(seqs), int(tokens_q), int(max_len)
+    nq = q_heads * hd
+    lq, lo = ld_q or nq, ld_out or nq
+    per = (most + cache.page_tokens - 1) // cache.page_tokens
+    lt = ld_table or (table.stride(0) if getattr(table, "ndim", 0) == 2 and hasattr(table, "stride") else per)
+    ti = vtype_id(dtype)
+    oi = ti if out_dtype is None else vtype_id(out_dtype)
+    check(lib().frq_dev_attn_chunk(
+        ti, _operand("q", q, 2 * ((tq - 1) * lq + nq) if tq else 0, ti, lq), lq, cache.data_ptr(), cache.nbytes, cache.pages,
+        cache.page_tokens, cache.kv_heads, hd, _operand("table", table, 4 * ((n - 1) * lt + per), _I32, lt), lt,
+        _operand("lens", lens, 4 * n, _I32), _operand("cu_q", cu_q, 4 * (n + 1), _I32), n, tq, int(max_q), most, oi,
+        _operand("out", out, (4 if oi == 0 else 2) * ((tq - 1) * lo + nq) if tq else 0, oi, lo), lo, q_heads,
+        hd ** -0.5 if scale is None else scale, _stream(stream)))
+
+
+# ------------------------------ between blocks, and from logits to a token
+
+def add_rms_norm(x, out, rows: int, hidden: int, weight=None, residual=None, sum_out=None, eps: float = 1e-6, x_dtype="f32",
+                 res_dtype="f32", out_dtype="f32", ld_x: int = 0, ld_res: int = 0, ld_sum: int = 0, ld_out: int = 0,
+                 stream=None) -> None:
+    """sum_out = x + residual and out = its root-mean-square norm times
+    ``weight`` (fp32, None for ones), row by row, enqueued (frq_dev_add_rms_norm).
+
+    ``residual`` None: the norm of x alone. ``sum_out`` (of ``res_dtype``, None:
+    not kept) may be the residual itself. ``out_dtype`` "f32", "f16", "bf16" or
+    "q8_0": rows of hidden / 32 blocks of 34 bytes, as :func:`dequant` and
+    :func:`gemv` read them (a uint8 tensor or a buffer). ``ld_*``: elements from a
+    row to the next, default ``hidden``."""
+    n, h = int(rows), int(hidden)
+    lx, lr, ls, lo = ld_x or h, ld_res or h, ld_sum or h, ld_out or h
+    xi, ri = vtype_id(x_dtype), vtype_id(res_dtype)
+    q8 = out_dtype == _Q8 or (isinstance(out_dtype, str) and out_dtype.lower() == "q8_0")
+    oi = _Q8 if q8 else vtype_id(out_dtype)
+    xs, rs = (4 if xi == 0 else 2), (4 if ri == 0 else 2)
+    last = (n - 1) * lo + h
+    to = (_operand("out", out, last // 32 * 34, _U8, lo // 32 * 34) if q8
+          else _operand("out", out, (4 if oi == 0 else 2) * last, oi, lo))
+    check(lib().frq_dev_add_rms_norm(
+        xi, _operand("x", x, xs * ((n - 1) * lx + h), xi, lx), lx, ri,
+        _operand("residual", residual, rs * ((n - 1) * lr + h), ri, lr), lr,
+        _operand("sum_out", sum_out, rs * ((n - 1) * ls + h), ri, ls), ls, _operand("weight", weight, 4 * h, _lib.F32), eps, oi,
+        to, lo, n, h, _stream(stream)))
+
+
+def sample(logits, u, tokens, rows: int, vocab: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, probs=None,
+           dtype="f32", ld: int = 0, stream=None) -> None:
+    """One token (int32) per row of ``logits``, rows ``ld`` elements apart
+    (default ``vocab``), drawn with the random numbers ``u`` (fp32 in [0, 1), one a
+    row); enqueued (frq_dev_sample).
+
+    The ``top_k`` largest logits stay (0: all), of these the fewest whose
+    probabilities at ``temperature`` sum to ``top_p`` of theirs, of these the ones
+    at least ``min_p`` times as probable as the largest; temperature 0 takes the
+    largest. Each parameter is a number for all rows or a device array of one a row
+    (fp32, ``top_k`` int32). ``probs`` (fp32, None: not wanted): the tokens'
+    probabilities among those that stayed."""
+    n, v = int(rows), int(vocab)
+    lx, ti = ld or v, vtype_id(dtype)
+    one, many = [], []
+    for name, p, kind, rest in (("temperature", temperature, _lib.F32, 1.0), ("top_k", top_k, _I32, 0),
+                                ("top_p", top_p, _lib.F32, 1.0), ("min_p", min_p, _lib.F32, 0.0)):
+        number = isinstance(p, (int, float, np.integer, np.floating))
+        one.append(p if number else rest)
+        many.append(0 if number else _operand(name, p, 4 * n, kind))
+    check(lib().frq_dev_sample(
+        ti, _operand("logits", logits, (4 if ti == 0 else 2) * ((n - 1) * lx + v), ti, lx), lx, n, v,
+        _operand("u", u, 4 * n, _lib.F32), float(one[0]), many[0], int(one[1]), many[1], float(one[2]), many[2], float(one[3]), many[3],
+        _operand("tokens", tokens, 4 * n, _I32), _operand("probs", probs, 4 * n, _lib.F32), _stream(stream)))

@@ -477,6 +477,67 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
                          int64_t tokens_k, int64_t max_q, int64_t max_k, int64_t q_heads, int64_t kv_heads,
                          int64_t head_dim, int causal, float scale, void* stream);
 
+/* Chunks of new tokens against the cache, which holds their keys and values
+ * already: sequence s has the queries [cu_q[s], cu_q[s + 1]) (int32, seqs + 1,
+ * within tokens_q, no more than max_q of one sequence) and lens[s] tokens in the
+ * cache, its pages in row s of table as for attn_decode. Query i of n sees the
+ * tokens j <= i + lens[s] - n; one that sees none gives zeros. q F16 or BF16, out
+ * of that type or F32; scores and sums fp32. k and v enter the products rounded
+ * to fp16 (not to bf16 as frq_dev_kv4_read with BF16 does), q exactly (to 2^-28 of
+ * a head's largest), a softmax weight to 2^-12 of itself or 2^-30 of the row's
+ * largest; in a tile of 32 tokens with a value beyond 65504, k and v to 2^-21.
+ * No NaN in the cache reaches a query that does not see its token. lens[s] >
+ * max_len, more queries than max_q or a page outside the cache: NaN; offsets
+ * outside q: the sequence is not computed. Few rows: the keys are split over
+ * workgroups, whose results (at most 1024 + as many as there are key heads and
+ * sequences, of 64 rows) use the stream's scratch and are joined in a fixed
+ * order. The division follows from the shapes: the same call gives the same
+ * bits. max_len up to 2^29; seqs, key heads and blocks of 16 to 64 rows together
+ * below 2^23. */
+int frq_dev_attn_chunk(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
+                       int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
+                       const int32_t* lens, const int32_t* cu_q, int64_t seqs, int64_t tokens_q, int64_t max_q,
+                       int64_t max_len, int out_type, void* out, int64_t ld_out, int64_t q_heads, float scale, void* stream);
+
+/* ------------------------------- between blocks, and from logits to a token
+ * The forwarder's residual additions and norms (model/qwen2.py:1388-1773, NumPy)
+ * and its sampler (model/sampling.py), on the device. Buffers are aligned to
+ * their type; 16-byte aligned rows are read and written 16 bytes at a time.   */
+
+/* h = x + residual, rounded to the residual's type and stored in sum (null: not
+ * stored; it may be the residual's or x's own rows), then
+ * out = h / sqrt(mean(h^2) + eps) * weight for each of `rows` rows of `hidden`
+ * elements (up to 2^24). residual null: h = x. weight fp32 or null (ones). Types
+ * F32, F16 or BF16; out may be x's or the residual's rows where types and strides
+ * are the same. The norm is computed in 64 bits and rounded once. out_type
+ * FRQ_Q8_0: rows of Q8_0 blocks as frq_dev_dequant and frq_dev_gemv read them
+ * (hidden and ld_out, in elements, multiples of 32): of the fp32 values, 32 at a
+ * time, d = fp16(max|y| / 127) held to 65504, codes round_even(y / d) held to
+ * +-127; a block with an inf or a NaN has d = NaN. */
+int frq_dev_add_rms_norm(int x_type, const void* x, int64_t ld_x, int res_type, const void* residual, int64_t ld_res,
+                         void* sum, int64_t ld_sum, const float* weight, float eps, int out_type, void* out,
+                         int64_t ld_out, int64_t rows, int64_t hidden, void* stream);
+
+/* One token per row of logits (F32, F16 or BF16, vocab up to 2^20) and its
+ * probability. With w_i = exp((x_i - max x) / temperature), sorted by x and equal
+ * ones by index: the first top_k stay (0: all), of these the shortest run whose
+ * weights sum to at least top_p of theirs (1: all), of these the ones with w_i >=
+ * min_p; the largest always stays. The token is the first index at which the sum,
+ * in the order of the indices, of the weights that stayed exceeds u[row] times
+ * all of it (u in [0, 1); the caller's random numbers). probs (null: not wanted):
+ * the token's share of that sum. temperature 0: the largest logit, the lowest
+ * index of equals, probability 1. Parameters are one value for all rows or, where
+ * the array is not null, one a row: in an array a temperature that is not positive
+ * means 0, top_k below 1 all, min_p and top_p are held to [0, 1], and a NaN cuts
+ * nothing. -inf and NaN logits are never drawn; a row of nothing else gives token
+ * -1 and probability 0; where logits are inf, only those are drawn. Weights are
+ * computed in 64 bits and held to 2^-45 of the largest (2^-43 at 2^20 logits),
+ * sums are exact: tokens do not depend on how the work is divided. Some kilobytes
+ * of the stream's scratch a row. */
+int frq_dev_sample(int type, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* u,
+                   float temperature, const float* temperatures, int64_t top_k, const int32_t* top_ks, float top_p,
+                   const float* top_ps, float min_p, const float* min_ps, int32_t* tokens, float* probs, void* stream);
+
 /* ------------------------------------------- memory, streams and events
  * Thin wrappers so a ctypes caller needs no other HIP binding. Streams are
  * created at the default priority.                                         */
