@@ -52,6 +52,25 @@ __device__ __forceinline__ half2v halves(uint32_t a, uint32_t b, int h) {
     return pair_of(__builtin_amdgcn_perm(b, a, h ? 0x07060302u : 0x05040100u));
 }
 
+// A lane's share of a tile's K or V scales, to look for what is not ordinary.
+template <int NG>
+struct Flat {
+    uint32_t w[(NG + 3) / 4];
+    __device__ __forceinline__ void load(const uint8_t* scales, int lane) {
+        if constexpr (NG == 2) {
+            w[0] = reinterpret_cast<const uint16_t*>(scales)[lane];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NG / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(scales)[64 * i + lane];
+        }
+    }
+    __device__ __forceinline__ bool large() const {                  // beyond 8188, an inf or a NaN
+        us2 x = __builtin_bit_cast(us2, w[0] & 0x7FFF7FFFu);
+        if constexpr (NG == 8) x = __builtin_elementwise_max(x, __builtin_bit_cast(us2, w[1] & 0x7FFF7FFFu));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(x, (us2){0x6FFF, 0x6FFF})) != 0;
+    }
+};
+
 // The largest of x over the four lanes that hold a query.
 __device__ __forceinline__ float quad_max(float x) {
     x = __builtin_fmaxf(x, __shfl_xor(x, 16));
@@ -86,12 +105,14 @@ struct Span {
 };
 
 template <int TYPE, int OUT, int NG, int R>
-__global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) attn_chunk_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kernel(ChunkArgs a) {
     using T = Val<TYPE>;
     using O = Val<OUT>;
     constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 16 * R;
+    constexpr bool kHeld = NG * R <= 8;            // queries in registers, or in LDS
     __shared__ __attribute__((aligned(16))) float sh_o[2][R * 2 * NG][64][4];
     __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
+    half8v (*sh_q)[64] = reinterpret_cast<half8v(*)[64]>(&sh_o[0][0][0][0]);    // [R NG][64], until the sums' turn comes
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, j = lane >> 4;
@@ -121,8 +142,66 @@ __global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) 
     if (first >= tiles && split) return;                             // nothing here: the joining knows
     const int whole = sp.keys(row0, group);                          // keys below this one every row sees
 
+    const const_ints table = constant(a.table) + (int64_t)seq * a.ld_table;
+    const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
+    const int64_t page_bytes = a.kv_heads * (int64_t)page_tiles * kTile;
+    const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
+    bool bad = false;
+    // Pages are looked up a step before their tile is asked for. Past the last
+    // tile that one is asked for again: a load that may not have been issued
+    // would make the compiler wait for those after it.
+    auto page_index = [&](int tile) { return (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36); };
+    auto look_up = [&](int tile) { return table[page_index(tile < last ? tile : last - 1)]; };
+    auto address = [&](int tile, int page) {
+        if ((uint32_t)page >= (uint64_t)a.pages) {
+            bad = true;
+            page = 0;
+        }
+        tile = tile < last ? tile : last - 1;
+        const uint32_t in = (uint32_t)tile - page_index(tile) * page_tiles;
+        return heads + page * page_bytes + (int64_t)in * kTile;
+    };
+    uint32_t kc[2 * NG], ks[NG], vc[2 * NG], vs[4][NG];              // a tile's codes and scales as a lane holds them
+    Flat<NG> fk, fv;
+    auto fetch_k = [&](const uint8_t* t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < 2 * NG; p += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(t + kv_word(p, lane));
+            kc[p] = x.x; kc[p + 1] = x.y; kc[p + 2] = x.z; kc[p + 3] = x.w;
+        }
+#pragma unroll
+        for (int p = 0; p < NG; p += 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(t + kv_ks_off(NG) + kv_scale(n, 0, NG) + 4 * p);
+            ks[p] = x.x; ks[p + 1] = x.y;
+        }
+        fk.load(t + kv_ks_off(NG), lane);
+    };
+    auto fetch_v = [&](const uint8_t* t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < 2 * NG; p += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(t + kv_vc_off(NG) + kv_word(p, lane));
+            vc[p] = x.x; vc[p + 1] = x.y; vc[p + 2] = x.z; vc[p + 3] = x.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)                                  // tokens 4j + i and 16 more
+#pragma unroll
+            for (int p = 0; p < NG; p += 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(t + kv_vs_off(NG) + kv_scale(4 * j + i, 0, NG) + 4 * p);
+                vs[i][p] = x.x; vs[i][p + 1] = x.y;
+            }
+        fv.load(t + kv_vs_off(NG), lane);
+    };
+    int tile = first + wave, page = 0;
+    const uint8_t* at = nullptr;
+    if (tile < last) {
+        at = address(tile, look_up(tile));
+        page = look_up(tile + kWaves);
+        fetch_k(at);
+        fetch_v(at);
+    }
+
     // the lane's rows, one of each column tile: queries, and the last key they see
-    half8v qf[R][NG];
+    half8v qf[kHeld ? R : 1][NG];
     float rs[R], m[R], nref[R], l[R];
     int lim[R];
 #pragma unroll
@@ -150,68 +229,36 @@ __global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) 
         top = top > other ? top : other;
         const int up = top ? 140 - (int)(top >> 23) : 0;             // the largest to [2^13, 2^14)
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g) {
+            half8v y;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qf[c][g][e] = (_Float16)__builtin_ldexpf(x[g][e], up);
+            for (int e = 0; e < 8; ++e) y[e] = (_Float16)__builtin_ldexpf(x[g][e], up);
+            if constexpr (kHeld)
+                qf[c][g] = y;
+            else if (wave == c % kWaves)
+                sh_q[c * NG + g][lane] = y;
+        }
         rs[c] = top >= 0x7F800000u ? __builtin_nanf("") : __builtin_ldexpf(a.scale * kLog2e, -up);
         m[c] = -kInf;
         nref[c] = 0.f;
         l[c] = 0.f;
     }
+    if constexpr (!kHeld) __syncthreads();
     float4v o[R][2 * NG];
 #pragma unroll
     for (int c = 0; c < R; ++c)
 #pragma unroll
         for (int i = 0; i < 2 * NG; ++i) o[c][i] = float4v{0, 0, 0, 0};
 
-    const const_ints table = constant(a.table) + (int64_t)seq * a.ld_table;
-    const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
-    const int64_t page_bytes = a.kv_heads * (int64_t)page_tiles * kTile;
-    const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
-    bool bad = false;
-    auto address = [&](int tile) {
-        const uint32_t in = (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36);
-        int page = table[in];
-        if ((uint32_t)page >= (uint64_t)a.pages) {
-            bad = true;
-            page = 0;
-        }
-        return heads + page * page_bytes + (int64_t)((uint32_t)tile - in * page_tiles) * kTile;
-    };
-
-    for (int tile = first + wave; tile < last; tile += kWaves) {
-        const uint8_t* at = address(tile);
-        uint32_t kc[2 * NG], ks[NG], vc[2 * NG], vs[4][NG], flat = 0;
-#pragma unroll
-        for (int p = 0; p < 2 * NG; p += 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(at + kv_word(p, lane));
-            kc[p] = x.x; kc[p + 1] = x.y; kc[p + 2] = x.z; kc[p + 3] = x.w;
-            const uint4 y = *reinterpret_cast<const uint4*>(at + kv_vc_off(NG) + kv_word(p, lane));
-            vc[p] = y.x; vc[p + 1] = y.y; vc[p + 2] = y.z; vc[p + 3] = y.w;
-        }
-#pragma unroll
-        for (int p = 0; p < NG; p += 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(at + kv_ks_off(NG) + kv_scale(n, 0, NG) + 4 * p);
-            ks[p] = x.x; ks[p + 1] = x.y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {                            // tokens 4j + i and 16 more
-                const uint2 y = *reinterpret_cast<const uint2*>(at + kv_vs_off(NG) + kv_scale(4 * j + i, 0, NG) + 4 * p);
-                vs[i][p] = y.x; vs[i][p + 1] = y.y;
-            }
-        }
-        // is a scale beyond 8188, or no number?
-#pragma unroll
-        for (int p = 0; p < NG; ++p) {
-            us2 x = __builtin_bit_cast(us2, ks[p] & 0x7FFF7FFFu);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x = __builtin_elementwise_max(x, __builtin_bit_cast(us2, vs[i][p] & 0x7FFF7FFFu));
-            flat |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(x, (us2){0x6FFF, 0x6FFF}));
-        }
+    for (; tile < last; tile += kWaves) {
+        const uint8_t* next = address(tile + kWaves, page);
+        page = look_up(tile + 2 * kWaves);
         const int kt = tile * kKvTile;
         const bool masked = kt + kKvTile > whole;
         float up = 1.f, down = 1.f, under = kUnder;
         uint64_t gone = 0;                                           // blocks taken out of the product
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(flat != 0) != 0, 0)) {
+        // a scale beyond 8188, or no number?
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(fk.large() || fv.large()) != 0, 0)) {
             // Behind the sequence's end nothing is known, and a zero weight does
             // not take a NaN out of a product: where rows differ in what they
             // see, a block of V that is no number leaves the product, to be
@@ -246,50 +293,47 @@ __global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) 
                 }
             }
         }
-        // the tile's operands: K of 16 tokens and 32 channels each, V of 16 channels
-        half8v kf[2][NG], vf[2 * NG];
+        // scores of tokens 16u + 4j .. 4j + 3: K of 16 tokens and 32 channels at a time
+        float4v s[R][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const uint32_t w = kc[u * NG + g], at2 = ks[(u * NG + g) / 2];
-                const half2v d = halves(at2, at2, (u * NG + g) & 1);
-                kf[u][g] = join(low_pair(w) * d, high_pair(w) * d, low_pair(w >> 8) * d, high_pair(w >> 8) * d);
-            }
+        for (int c = 0; c < R; ++c) s[c][0] = s[c][1] = float4v{0, 0, 0, 0};
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const uint32_t w0 = vc[2 * g], w1 = vc[2 * g + 1];
-            half2v d[4];
+            half8v q[R];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int c = 0; c < R; ++c) {
+                if constexpr (kHeld)
+                    q[c] = qf[c][g];
+                else
+                    q[c] = sh_q[c * NG + g][lane];
+            }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int p = (u * NG + g) / 2, h = (u * NG + g) & 1;
-                    d[2 * u + i] = halves(vs[2 * i][p], vs[2 * i + 1][p], h);
-                }
-            vf[2 * g] = join(low_pair(w0) * d[0], low_pair(w0 >> 8) * d[1], low_pair(w1) * d[2], low_pair(w1 >> 8) * d[3]);
-            vf[2 * g + 1] = join(high_pair(w0) * d[0], high_pair(w0 >> 8) * d[1], high_pair(w1) * d[2], high_pair(w1 >> 8) * d[3]);
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t w = kc[u * NG + g], at2 = ks[(u * NG + g) / 2];
+                const half2v d = halves(at2, at2, (u * NG + g) & 1);
+                const half8v kf = join(low_pair(w) * d, high_pair(w) * d, low_pair(w >> 8) * d, high_pair(w >> 8) * d);
+#pragma unroll
+                for (int c = 0; c < R; ++c) s[c][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[c], s[c][u], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        fetch_k(next);                                               // these registers are free again
+        half8v pf[R];
 #pragma unroll
         for (int c = 0; c < R; ++c) {
-            float4v s[2] = {float4v{0, 0, 0, 0}, float4v{0, 0, 0, 0}};
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u][g], qf[c][g], s[u], 0, 0, 0);
             const float by = rs[c] * up;
             if (masked) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (kt + 16 * u + 4 * j + i > lim[c]) s[u][i] = -kInf;
+                        if (kt + 16 * u + 4 * j + i > lim[c]) s[c][u][i] = -kInf;
             }
-            float top = s[0][0];
+            float top = s[c][0][0];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, s[u][i]);
+                for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, s[c][u][i]);
             top *= by;
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m[c] + kLag) != 0, 0)) {
                 // each row by its own scores alone
@@ -301,23 +345,43 @@ __global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) 
 #pragma unroll
                 for (int d = 0; d < 2 * NG; ++d) o[c][d] *= keep;
             }
-            half2v pf[4];
+            half2v p[4];
             float sum = 0.f;
+            const float ref = nref[c] + under;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], by, nref[c] + under));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], by, nref[c] + under));
-                    const half2v p = {(_Float16)p0, (_Float16)p1};
-                    pf[2 * u + i / 2] = p;
-                    sum = __builtin_amdgcn_fdot2(p, (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][u][i], by, ref));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][u][i + 1], by, ref));
+                    p[2 * u + i / 2] = half2v{(_Float16)p0, (_Float16)p1};
+                    sum = __builtin_amdgcn_fdot2(p[2 * u + i / 2], (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
                 }
             l[c] = __builtin_fmaf(sum, down, l[c]);
-            const half8v pv = join(pf[0], pf[1], pf[2], pf[3]);
-#pragma unroll
-            for (int d = 0; d < 2 * NG; ++d) o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pv, o[c][d], 0, 0, 0);
+            pf[c] = join(p[0], p[1], p[2], p[3]);
         }
+        // V of 16 channels at a time
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const uint32_t w0 = vc[2 * g], w1 = vc[2 * g + 1];
+            half2v d[4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int p = (u * NG + g) / 2, h = (u * NG + g) & 1;
+                    d[2 * u + i] = halves(vs[2 * i][p], vs[2 * i + 1][p], h);
+                }
+            const half8v va = join(low_pair(w0) * d[0], low_pair(w0 >> 8) * d[1], low_pair(w1) * d[2], low_pair(w1 >> 8) * d[3]);
+            const half8v vb = join(high_pair(w0) * d[0], high_pair(w0 >> 8) * d[1], high_pair(w1) * d[2], high_pair(w1 >> 8) * d[3]);
+#pragma unroll
+            for (int c = 0; c < R; ++c) {
+                o[c][2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[c], o[c][2 * g], 0, 0, 0);
+                o[c][2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, pf[c], o[c][2 * g + 1], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        fetch_v(next);
         if (__builtin_expect(gone != 0, 0)) {
             for (int t = 0; t < kKvTile && kt + t < sp.len; ++t)
 #pragma unroll
@@ -330,6 +394,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) 
                     }
                 }
         }
+        at = next;
     }
     if (__builtin_amdgcn_ballot_w64(bad)) {
 #pragma unroll
@@ -403,44 +468,73 @@ __global__ void __launch_bounds__(64 * kWaves, NG * R >= 16 || NG == 8 ? 1 : 2) 
     }
 }
 
-// A row's parts of all splits, joined in their order; a wave a row of D channels.
-template <int OUT, int NG>
+// A row's parts of all splits, joined in their order, four columns a thread. A
+// workgroup has D / 4 threads for each of its rows (few splits), or eight (of
+// 128) such sets on the splits of one row, which meet in LDS.
+template <int OUT, int NG, bool ONE>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(ChunkArgs a, int kRows) {
     using O = Val<OUT>;
-    constexpr int D = 32 * NG, kPer = D / 64;
-    const int lane = threadIdx.x & 63;
+    constexpr int D = 32 * NG, kCols = D / 4, kSets = 256 / kCols;
+    __shared__ __attribute__((aligned(16))) float vals[ONE ? kSets : 1][D];
+    __shared__ float sums[kSets];
     const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
-    const uint32_t unit = blockIdx.x;                                // block of a key head of a sequence
+    const int col = threadIdx.x % kCols, set = threadIdx.x / kCols;
+    const uint32_t per = ONE ? (uint32_t)kRows : (uint32_t)((kRows + kSets - 1) / kSets);   // workgroups of a block
+    const uint32_t unit = blockIdx.x / per;                          // block of a key head of a sequence
+    const int r = (int)(blockIdx.x - unit * per) * (ONE ? 1 : kSets) + (ONE ? 0 : set);
     const uint32_t id = unit / (uint32_t)a.blocks;
     const int block = (int)(unit % (uint32_t)a.blocks), kvh = (int)(id % (uint32_t)a.kv_heads), seq = (int)(id / (uint32_t)a.kv_heads);
     Span sp;
     if (!sp.read(a, seq) || sp.bad) return;
-    const int row0 = block * kRows, rows = sp.nq * group;
-    if (row0 >= rows) return;
+    const int row0 = block * kRows, row = row0 + r;
+    if (row >= sp.nq * group || r >= kRows) return;                  // where ONE the whole workgroup
     const int tiles = (sp.keys(row0 + kRows - 1, group) + kKvTile - 1) / kKvTile;
     const int share = (int)a.share, used = tiles <= share ? 1 : (tiles + share - 1) / share;
-    const float* parts = a.part + (int64_t)unit * a.splits * kRows * (D + 4);
-    for (int r = threadIdx.x >> 6; r < kRows && row0 + r < rows; r += 4) {
-        const float* p = parts + r * (D + 4);
-        const int64_t step = (int64_t)kRows * (D + 4);
-        float mm = -kInf;
-        for (int s = lane; s < used; s += 64) mm = __builtin_fmaxf(mm, p[s * step + D]);
+    const int64_t step = (int64_t)kRows * (D + 4);
+    const float* p = a.part + (int64_t)unit * a.splits * step + r * (D + 4);
+    float mm = -kInf;
+    if constexpr (ONE) {
+        for (int s = threadIdx.x & 63; s < used; s += 64) mm = __builtin_fmaxf(mm, p[s * step + D]);
 #pragma unroll
         for (int i = 1; i < 64; i <<= 1) mm = __builtin_fmaxf(mm, __shfl_xor(mm, i));
-        const float base = mm == -kInf ? 0.f : mm;
-        float val[kPer] = {}, sum = 0.f;
-        for (int s = 0; s < used; ++s) {
-            const float f = __builtin_amdgcn_exp2f(p[s * step + D] - base);
-            sum = __builtin_fmaf(f, p[s * step + D + 1], sum);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) val[e] = __builtin_fmaf(f, p[s * step + lane * kPer + e], val[e]);
-        }
-        const int i = (row0 + r) / group;
-        typename O::Elem* out =
-            static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)(kvh * group + row0 + r - i * group) * D + lane * kPer;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) out[e] = O::one(sp.past + i < 0 ? 0.f : val[e] / sum);
+    } else {
+        for (int s = 0; s < used; ++s) mm = __builtin_fmaxf(mm, p[s * step + D]);
     }
+    const float base = mm == -kInf ? 0.f : mm;
+    float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = ONE ? set : 0; s < used; s += ONE ? kSets : 1) {
+        const float4 x = *reinterpret_cast<const float4*>(p + s * step + 4 * col);
+        const float2 ml = *reinterpret_cast<const float2*>(p + s * step + D);
+        const float f = __builtin_amdgcn_exp2f(ml.x - base);
+        sum = __builtin_fmaf(f, ml.y, sum);
+        val.x = __builtin_fmaf(f, x.x, val.x);
+        val.y = __builtin_fmaf(f, x.y, val.y);
+        val.z = __builtin_fmaf(f, x.z, val.z);
+        val.w = __builtin_fmaf(f, x.w, val.w);
+    }
+    if constexpr (ONE) {
+        *reinterpret_cast<float4*>(&vals[set][4 * col]) = val;
+        if (col == 0) sums[set] = sum;
+        __syncthreads();
+        if (set) return;
+#pragma unroll
+        for (int i = 1; i < kSets; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(&vals[i][4 * col]);
+            val.x += x.x;
+            val.y += x.y;
+            val.z += x.z;
+            val.w += x.w;
+            sum += sums[i];
+        }
+    }
+    const int i = row / group;
+    typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)(kvh * group + row - i * group) * D;
+    const bool none = sp.past + i < 0;
+    const typename O::Elem y[4] = {O::one(none ? 0.f : val.x / sum), O::one(none ? 0.f : val.y / sum),
+                                   O::one(none ? 0.f : val.z / sum), O::one(none ? 0.f : val.w / sum)};
+    __builtin_memcpy(__builtin_assume_aligned(out + 4 * col, 4 * sizeof(y[0])), y, sizeof(y));
 }
 
 template <int TYPE, int OUT, int NG, int R>
@@ -448,7 +542,11 @@ hipError_t launch_one(const ChunkArgs& a, hipStream_t stream) {
     const int64_t units = a.seqs * a.kv_heads * a.blocks;
     attn_chunk_kernel<TYPE, OUT, NG, R><<<(unsigned)(units * a.splits), 64 * kWaves, 0, stream>>>(a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
-    attn_chunk_join_kernel<OUT, NG><<<(unsigned)units, 256, 0, stream>>>(a, 16 * R);
+    constexpr int kSets = 256 / (8 * NG);
+    if (a.splits > 8)
+        attn_chunk_join_kernel<OUT, NG, true><<<(unsigned)(units * 16 * R), 256, 0, stream>>>(a, 16 * R);
+    else
+        attn_chunk_join_kernel<OUT, NG, false><<<(unsigned)(units * ((16 * R + kSets - 1) / kSets)), 256, 0, stream>>>(a, 16 * R);
     return hipGetLastError();
 }
 
@@ -460,7 +558,7 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
             case 1: return launch_one<TYPE, OUT, kN, 1>(a, stream);
             case 2: return launch_one<TYPE, OUT, kN, 2>(a, stream);
             default:
-                if constexpr (kN <= 4) return launch_one<TYPE, OUT, kN, 4>(a, stream);
+                if constexpr (kN <= 4) return a.tiles == 3 ? launch_one<TYPE, OUT, kN, 3>(a, stream) : launch_one<TYPE, OUT, kN, 4>(a, stream);
                 return hipErrorInvalidValue;
         }
     };
@@ -476,11 +574,11 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
 
 bool plan_attn_chunk(ChunkArgs* a) {
     const int64_t rows = a->max_q * (a->q_heads / a->kv_heads), keys = (a->max_len + kKvTile - 1) / kKvTile;
-    a->tiles = rows <= 16 ? 1 : rows <= 32 || a->head_dim == 256 ? 2 : 4;
+    a->tiles = rows <= 16 ? 1 : rows <= 32 || a->head_dim == 256 ? 2 : rows <= 48 ? 3 : 4;
     a->blocks = (rows + 16 * a->tiles - 1) / (16 * a->tiles);
     const int64_t units = a->seqs * a->kv_heads * a->blocks;
     if (units >= (int64_t)1 << 23) return false;                     // a launch has fewer than 2^32 threads
-    int64_t splits = units >= 512 ? 1 : (1024 + units - 1) / units;
+    int64_t splits = units >= 512 ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
     const int64_t most = (keys + 4 * kWaves - 1) / (4 * kWaves);     // four tiles a wave at least
     splits = splits < most ? splits : most;
     splits = splits > 0 ? splits : 1;
