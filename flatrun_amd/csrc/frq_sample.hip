@@ -5,98 +5,197 @@
 //   the sum of the weights that stayed exceeds u times all of it.
 //
 // Nothing is sorted. All three cuts take the list's lower end away, so what
-// stays is: the logits above one value, and the first few that equal it. That
-// value is found from histograms: 2048 bins of 1/64 in (max - x) / T, and below
-// them, within one bin, the bits of x, eight at a time.
+// stays is the logits above one place of the list. A histogram of the weights
+// over the depth log2(e) (max - x) / T, 2048 bins of 1/44, says which bins stay
+// whole and in which one or two the cuts lie; the logits of those, some hundreds,
+// are listed and ranked against each other. Where they are too many for the
+// list (thousands of logits within 1/44 of each other) the cuts are found from
+// the bits of x, eight at a time, in further passes over the row.
 //
-// Weights are whole numbers of 2^-kFrac: computed in 64 bits, rounded once.
-// Sums of them are exact whatever their order, so every pass sees the same
-// ones, the atomics of a histogram decide nothing, and a border lies where sums
-// in 64 bits have it. A weight below 2^-45 of the largest is nothing.
+// Weights are whole numbers of 2^-kFrac, computed in 64 bits and rounded once.
+// Sums of them are exact whatever their order: every pass sees the same ones,
+// atomics decide nothing, and a border lies where sums in 64 bits have it. In
+// fp32 one draw in some hundred would fall on the other side of a border of a
+// flat row of 10^5 logits.
+//
+// Passes over a row: its largest; the histogram (not without top_k and top_p);
+// the sums of what stays by group of 256, and the list; the group that the draw
+// falls into. One workgroup does them all where there are rows for the GPU, else
+// each pass is a launch of slices of all rows.
 #include "frq_kernels.h"
 #include "frq_vals.h"
 
 namespace frq {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 2048;                  // of 1/64 each: exp(-32) is below 2^-45
-constexpr int kStep = 256;                   // logits a wave takes at a time, four a lane
+constexpr int kBins = 2048, kPerBit = 44;    // depths up to 46.5: 2^-46 is no weight any more
 constexpr int kFrac = 44;
+constexpr int kGroup = 256;                  // logits a wave takes at a time, four a lane
+constexpr int kGroups = 4096;                // of a row, at most
+constexpr int kList = 2048;                  // logits that are ranked one by one
+constexpr int kRowThreads = 1024, kSliceThreads = 256;
+constexpr float kInf = __builtin_inff();
+using u64 = unsigned long long;
 
 // Order of x as a number, larger first; equal ones (0 and -0) alike. NaN and
 // -inf, which are never drawn, are 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
     const uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    return x > -__builtin_inff() ? k : 0u;
+    return x > -kInf ? k : 0u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) {
     return __builtin_bit_cast(float, k ^ (~(uint32_t)((int32_t)k >> 31) | 0x80000000u));
 }
+// The list's order: larger logits first, then lower indices.
+__device__ __forceinline__ u64 place_of(uint32_t key, int index) { return (u64)~key << 32 | (uint32_t)index; }
 
-// A row's parameters, the largest logit, and the weights under them.
-struct Row {
-    double per_t;                            // T, to divide by
-    float top, min_p, top_p;
-    int64_t top_k;
-    uint32_t top_key;
-    bool greedy;
-    __device__ __forceinline__ double depth(uint32_t key) const {        // (max - x) / T
-        return key == top_key ? 0.0 : ((double)top - (double)of_key(key)) / per_t;
-    }
-};
-
-__device__ __forceinline__ uint64_t wave_sum(uint64_t x) {
+__device__ __forceinline__ u64 wave_sum(u64 x) {
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) x += __shfl_xor((unsigned long long)x, i);
+    for (int i = 1; i < 64; i <<= 1) x += __shfl_xor(x, i);
     return x;
 }
-__device__ __forceinline__ uint64_t wave_scan(uint64_t x, int lane) {    // up to and with the lane's
+__device__ __forceinline__ u64 wave_scan(u64 x, int lane) {          // up to and with the lane's
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)x, i);
+        const u64 y = __shfl_up(x, i);
         if (lane >= i) x += y;
     }
     return x;
 }
 
+// Four consecutive logits; those from n on are -inf.
 template <int TYPE>
-__device__ __forceinline__ float load_logit(const void* row, int64_t i) {
-    if constexpr (TYPE == kTypeF32) return static_cast<const float*>(row)[i];
-    const uint16_t b = static_cast<const uint16_t*>(row)[i];
-    if constexpr (TYPE == kTypeF16) return f16_bits_to_f32(b);
-    return __builtin_bit_cast(float, (uint32_t)b << 16);
+__device__ __forceinline__ void load4(const void* row, int e, int n, float (&x)[4]) {
+    if (e + 4 <= n) {
+        if constexpr (TYPE == kTypeF32) {
+            __builtin_memcpy(x, static_cast<const float*>(row) + e, 16);
+        } else {
+            uint16_t b[4];
+            __builtin_memcpy(b, static_cast<const uint16_t*>(row) + e, 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[i] = TYPE == kTypeF16 ? f16_bits_to_f32(b[i]) : __builtin_bit_cast(float, (uint32_t)b[i] << 16);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = -kInf;
+        if (e + i >= n) continue;
+        if constexpr (TYPE == kTypeF32) {
+            x[i] = static_cast<const float*>(row)[e + i];
+        } else {
+            const uint16_t b = static_cast<const uint16_t*>(row)[e + i];
+            x[i] = TYPE == kTypeF16 ? f16_bits_to_f32(b) : __builtin_bit_cast(float, (uint32_t)b << 16);
+        }
+    }
 }
 
+// A row's parameters, its largest logit, and weights under it.
+struct Row {
+    double per, top, least;                  // log2(e) / T; the largest; the least weight that min_p leaves, times 2^frac
+    int frac;
+    uint32_t top_key;
+    float top_p;
+    int64_t top_k;
+    bool greedy, cut_k, cut_p;
+
+    __device__ __forceinline__ void read(const SampleArgs& a, int64_t r, uint32_t key) {
+        const float t = a.temperatures ? a.temperatures[r] : a.temperature;
+        const float least_p = a.min_ps ? a.min_ps[r] : a.min_p;
+        top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+        top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+        greedy = !(t > 0.f);
+        per = 1.4426950408889634 / (double)__builtin_fminf(t, 3.4028235e38f);
+        top_key = key;
+        top = (double)of_key(key);
+        frac = a.frac;
+        least = least_p > 0.f ? (double)__builtin_fminf(least_p, 1.f) * (double)((u64)1 << frac) : 0.0;
+        cut_k = top_k > 0 && top_k < a.vocab;
+        cut_p = top_p < 1.f;
+    }
+    // log2(e) (max - x) / T
+    __device__ __forceinline__ double depth(uint32_t key) const {
+        const double t = key == top_key ? 0.0 : (top - (double)of_key(key)) * per;
+        return __builtin_fmin(t, 60.0);
+    }
+    // 2^(frac - t), by whole steps and a polynomial of degree 9 through
+    // Chebyshev's points of [-1/2, 1/2], within 4e-14 of itself.
+    __device__ __forceinline__ double scaled(double t) const {
+        const double whole = t + 6755399441055744.0, r = t - (whole - 6755399441055744.0);     // 1.5 2^52
+        double y = -0x1.b63880a088780p-24;
+        y = __builtin_fma(y, r, 0x1.63d136366f695p-20);
+        y = __builtin_fma(y, r, -0x1.ffcb9515b5679p-17);
+        y = __builtin_fma(y, r, 0x1.4308ac85aa8a7p-13);
+        y = __builtin_fma(y, r, -0x1.5d87fe86fe7f7p-10);
+        y = __builtin_fma(y, r, 0x1.3b2ab7181b755p-7);
+        y = __builtin_fma(y, r, -0x1.c6b08d7047e52p-5);
+        y = __builtin_fma(y, r, 0x1.ebfbdff823cedp-3);
+        y = __builtin_fma(y, r, -0x1.62e42fefa39efp-1);
+        y = __builtin_fma(y, r, 1.0);
+        const int n = frac - (int)(uint32_t)__builtin_bit_cast(u64, whole);
+        return __builtin_bit_cast(double, __builtin_bit_cast(u64, y) + ((u64)(uint32_t)(n << 20) << 32));
+    }
+    // A scaled weight as a whole number, to nearest: below 2^52.
+    static __device__ __forceinline__ u64 count(double y) {
+        return __builtin_bit_cast(u64, y + 4503599627370496.0) & 0x000FFFFFFFFFFFFFull;
+    }
+    // After min_p (of the logits that the other cuts leave).
+    __device__ __forceinline__ u64 kept(double y) const { return y >= least ? count(y) : 0; }
+    static __device__ __forceinline__ int bin(double t) {            // kBins and more: no weight
+        return (int)(t * (double)kPerBit);
+    }
+    // The weight that top_p asks for of `all`: the run's sum reaches it.
+    __device__ __forceinline__ u64 wanted(u64 all) const {
+        const double want = __builtin_ceil((double)top_p * (double)all);
+        const u64 w = want >= 1.0 ? (u64)want : 1;
+        return w < all ? w : all;
+    }
+    // Every logit of depth t and less has a key of at least this.
+    __device__ __forceinline__ uint32_t floor_of(double t) const {
+        const double x = top - t / per, low = x - (__builtin_fabs(x) + __builtin_fabs(top)) * 1e-6;
+        return low > -3.4e38 ? key_of((float)low) : 1u;
+    }
+};
+
 struct Shared {
-    unsigned long long sum[kBins];
-    uint32_t count[kBins];
-    unsigned long long group[4096];          // of 256 logits
-    unsigned long long wave[kWaves];
-    uint32_t key[kWaves], index[kWaves];
-    unsigned long long before, at;           // a search's answer
+    u64 wave[16];
+    uint32_t key[16], index[16];
+    u64 before, at;                          // a search's answer
     uint32_t found;
 };
 
+// Sum over the workgroup of a value a thread.
+template <int NT>
+__device__ __forceinline__ u64 group_sum(Shared& sh, u64 x) {
+    x = wave_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = 0;
+    for (int w = 0; w < NT / 64; ++w) x += sh.wave[w];
+    return x;
+}
+
 // The first of `n` entries at which the running sum of f(i) passes `target`
 // (less than the whole): its number in sh.found, what stands before it in
-// sh.before. The whole workgroup calls.
-template <typename F>
-__device__ __forceinline__ void search(Shared& sh, int n, unsigned long long target, F&& f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (n + kThreads - 1) / kThreads;
+// sh.before, itself in sh.at. The whole workgroup calls.
+template <int NT, typename F>
+__device__ __forceinline__ void search(Shared& sh, int n, u64 target, F&& f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (n + NT - 1) / NT;
     const int from = (int)threadIdx.x * per;
-    unsigned long long mine = 0;
+    u64 mine = 0;
     for (int i = 0; i < per && from + i < n; ++i) mine += f(from + i);
-    const unsigned long long upto = wave_scan(mine, lane);
+    const u64 upto = wave_scan(mine, lane);
     __syncthreads();
     if (lane == 63) sh.wave[wave] = upto;
     __syncthreads();
-    unsigned long long base = upto - mine;
+    u64 base = upto - mine;
     for (int w = 0; w < wave; ++w) base += sh.wave[w];
     if (base <= target && target < base + mine) {
         for (int i = 0; i < per && from + i < n; ++i) {
-            const unsigned long long x = f(from + i);
+            const u64 x = f(from + i);
             if (target < base + x) {
                 sh.found = (uint32_t)(from + i);
                 sh.before = base;
@@ -109,218 +208,392 @@ __device__ __forceinline__ void search(Shared& sh, int n, unsigned long long tar
     __syncthreads();
 }
 
-// Sum over the workgroup of a value a thread.
-__device__ __forceinline__ unsigned long long group_sum(Shared& sh, unsigned long long x) {
+// Where the cuts lie: bins below `sure` stay whole; the logits of the bins
+// [p_from, p_to] (top_p's cut) and of k_bin (top_k's) are listed.
+struct Cuts {
+    int sure, p_from, p_to, k_bin;
+    u64 k_left;                              // logits of k_bin that stay
+    u64 k_before, p_before, all;             // weights below k_bin, below p_from, and of all bins
+    __device__ __forceinline__ bool listed(int b) const { return b == k_bin || (b >= p_from && b <= p_to); }
+    __device__ __forceinline__ void none() {
+        sure = kBins;
+        p_from = 1, p_to = 0, k_bin = -1;
+        k_left = k_before = p_before = all = 0;
+    }
+    // The cuts from a histogram; false if neither applies.
+    template <int NT>
+    __device__ __forceinline__ void find(Shared& sh, const Row& p, const u64* sum, const uint32_t* count) {
+        none();
+        u64 many = 0;
+        for (int i = threadIdx.x; i < kBins; i += NT) {
+            all += sum[i];
+            many += count[i];
+        }
+        all = group_sum<NT>(sh, all);
+        many = group_sum<NT>(sh, many);
+        u64 low = all, high = all;                                   // what top_k leaves lies between
+        if (p.cut_k && (u64)p.top_k < many) {
+            search<NT>(sh, kBins, (u64)p.top_k - 1, [&](int i) { return (u64)count[i]; });
+            k_bin = (int)sh.found;
+            k_left = (u64)p.top_k - sh.before;
+            low = 0;
+            for (int i = threadIdx.x; i < k_bin; i += NT) low += sum[i];
+            low = k_before = group_sum<NT>(sh, low);
+            high = low + sum[k_bin];
+            sure = k_bin;
+        }
+        if (p.cut_p && high > 0) {
+            search<NT>(sh, kBins, (low > 0 ? p.wanted(low) : 1) - 1, [&](int i) { return sum[i]; });
+            p_from = sure = (int)sh.found;
+            p_before = sh.before;
+            search<NT>(sh, kBins, p.wanted(high) - 1, [&](int i) { return sum[i]; });
+            p_to = (int)sh.found;
+        }
+    }
+    // the deepest that anything that stays or is listed can lie
+    __device__ __forceinline__ double deepest() const {
+        int b = sure - 1 > k_bin ? sure - 1 : k_bin;
+        b = b > p_to ? b : p_to;
+        return (b + 1) * (1.0 / kPerBit) + 1e-9;
+    }
+};
+
+// A listed logit: its place, and its weight below its bin.
+struct Entry {
+    u64 place, weight;
+    __device__ __forceinline__ int bin() const { return (int)(weight >> 48); }
+    __device__ __forceinline__ u64 w() const { return weight & 0xFFFFFFFFFFFFull; }
+};
+
+// Logits of the groups [from, to), wave by wave: f(index, four logits).
+template <int TYPE, int NT, typename F>
+__device__ __forceinline__ void each(const void* row, int n, int from, int to, F&& f) {
+    constexpr int kAhead = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    x = wave_sum(x);
-    __syncthreads();
-    if (lane == 0) sh.wave[wave] = x;
-    __syncthreads();
-    x = 0;
-    for (int w = 0; w < kWaves; ++w) x += sh.wave[w];
-    return x;
+    for (int g = from + wave; g < to; g += kAhead * (NT / 64)) {
+        float x[kAhead][4];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int at = g + i * (NT / 64);
+            if (at < to) load4<TYPE>(row, at * kGroup + 4 * lane, n, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int at = g + i * (NT / 64);
+            if (at < to) f(at, at * kGroup + 4 * lane, x[i]);
+        }
+    }
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs a) {
-    __shared__ Shared sh;
+// The largest of the groups, the lowest index of equals, to every thread.
+template <int TYPE, int NT>
+__device__ __forceinline__ void largest(Shared& sh, const void* row, int n, int from, int to, uint32_t& key, uint32_t& index) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r = blockIdx.x;
-    const int n = (int)a.vocab, groups = (n + kStep - 1) / kStep;
-    constexpr int kSize = TYPE == kTypeF32 ? 4 : 2;
-    const char* row = static_cast<const char*>(a.logits) + r * a.ld * kSize;
-    const double one = (double)((uint64_t)1 << a.frac);
-
-    // every logit once: f(index, key), keys of a group of 256 by one wave
-    auto each = [&](auto&& f) {
-        for (int g = wave; g < groups; g += kWaves)
+    float best = -kInf;
+    int where = -1;
+    each<TYPE, NT>(row, n, from, to, [&](int, int e, const float (&x)[4]) {
+        // a lane meets its indices in rising order: the first of equals stays
 #pragma unroll
-            for (int i = 0; i < kStep / 64; ++i) {
-                const int e = g * kStep + i * 64 + lane;
-                if (e < n) f(e, key_of(load_logit<TYPE>(row, e)));
-            }
-    };
-
-    // the largest, the lowest index of equals
-    Row p;
-    uint32_t best = 0, where = 0;
-    each([&](int e, uint32_t k) {
-        if (k > best) { best = k; where = (uint32_t)e; }
+        for (int i = 0; i < 4; ++i)
+            if (x[i] > best) best = x[i], where = e + i;
     });
+    key = key_of(best);
+    index = (uint32_t)where;
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) {
-        const uint32_t k = __shfl_xor(best, i), w = __shfl_xor(where, i);
-        if (k > best || (k == best && w < where)) { best = k; where = w; }
+        const uint32_t k = __shfl_xor(key, i), w = __shfl_xor(index, i);
+        if (k > key || (k == key && w < index)) key = k, index = w;
     }
-    if (lane == 0) { sh.key[wave] = best; sh.index[wave] = where; }
     __syncthreads();
-    best = 0, where = 0;
-    for (int w = 0; w < kWaves; ++w)
-        if (sh.key[w] > best || (sh.key[w] == best && sh.index[w] < where)) { best = sh.key[w]; where = sh.index[w]; }
-    const float t = a.temperatures ? a.temperatures[r] : a.temperature;
-    p.top_key = best;
-    p.top = of_key(best);
-    p.per_t = (double)__builtin_fminf(t, 3.4028235e38f);
-    p.greedy = !(t > 0.f);
-    p.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-    p.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-    p.min_p = a.min_ps ? a.min_ps[r] : a.min_p;
-    if (best == 0 || p.greedy) {                 // nothing to draw, or the largest
-        if (threadIdx.x == 0) {
-            a.tokens[r] = best ? (int32_t)where : -1;
-            if (a.probs) a.probs[r] = best ? 1.f : 0.f;
-        }
-        return;
-    }
-    const double min_w = p.min_p > 0.f ? (double)__builtin_fminf(p.min_p, 1.f) : 0.0;
-    const bool cut_k = p.top_k > 0 && p.top_k < n, cut_p = p.top_p < 1.f;
-    auto weight = [&](double w) { return (unsigned long long)__builtin_rint(w * one); };
-    auto weight_of = [&](uint32_t k) -> unsigned long long { return k ? weight(exp(-p.depth(k))) : 0ull; };
+    if (lane == 0) sh.key[wave] = key, sh.index[wave] = index;
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w)
+        if (sh.key[w] > key || (sh.key[w] == key && sh.index[w] < index)) key = sh.key[w], index = sh.index[w];
+}
 
-    // What stays: keys above `low`, and those equal to it up to index `last`.
-    uint32_t low = 0;
-    int last = n;
-    if (cut_k || cut_p) {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.sum[i] = 0, sh.count[i] = 0;
+// The histogram of the groups, into LDS that is zero.
+template <int TYPE, int NT>
+__device__ __forceinline__ void histogram(const Row& p, const void* row, int n, int from, int to, u64* sum, uint32_t* count) {
+    const bool sums = p.cut_p;               // top_k alone asks for no weights
+    const uint32_t least = p.floor_of((double)kBins / kPerBit);
+    each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t k = key_of(x[i]);
+            if (k < least) continue;
+            const double t = p.depth(k);
+            const int b = Row::bin(t);
+            if (b >= kBins) continue;
+            if (sums) atomicAdd(&sum[b], Row::count(p.scaled(t)));
+            if (p.cut_k) atomicAdd(&count[b], 1u);
+        }
+    });
+}
+
+// Sums of what stays for certain, by group, and the list: entries that fit in
+// kList, all of them counted.
+template <int TYPE, int NT>
+__device__ __forceinline__ void sums_and_list(const Row& p, const Cuts& c, const void* row, int n, int from, int to, u64* group,
+                                              Entry* list, uint32_t* listed) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t least = p.floor_of(c.deepest());
+    const int last = c.p_to > c.k_bin ? c.p_to : c.k_bin;            // of the bins that matter
+    each<TYPE, NT>(row, n, from, to, [&](int g, int e, const float (&x)[4]) {
+        u64 s = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t k = key_of(x[i]);
+            if (k < least || k == 0) continue;
+            const double t = p.depth(k);
+            const int b = Row::bin(t);
+            if (b >= c.sure && (b > last || !c.listed(b))) continue;
+            const double y = p.scaled(t);
+            if (b < c.sure) {
+                s += p.kept(y);
+            } else {
+                const uint32_t at = atomicAdd(listed, 1u);
+                if (at < kList) list[at] = Entry{place_of(k, e + i), Row::count(y) | (u64)b << 48};
+            }
+        }
+        if (__builtin_amdgcn_ballot_w64(s != 0)) s = wave_sum(s);
+        if (lane == 0) group[g] = s;
+    });
+}
+
+// What stays of the list: those up to `to` in its order. Their weights are added
+// to their groups.
+template <int NT>
+__device__ __forceinline__ u64 resolve(Shared& sh, const Row& p, const Cuts& c, const Entry* list, int many, u64* group) {
+    u64 kept_k = 0;
+    constexpr int kPer = kList / NT;
+    u64 before[kPer], rank[kPer];
+    for (int x = 0; x < kPer; ++x) {
+        const int i = x * NT + (int)threadIdx.x;
+        before[x] = rank[x] = 0;
+        if (i >= many) continue;
+        const Entry mine = list[i];
+        for (int o = 0; o < many; ++o) {
+            const Entry e = list[o];
+            if (e.place >= mine.place) continue;
+            const int b = e.bin();
+            if (b == c.k_bin) ++rank[x];
+            if (b >= c.p_from && b <= c.p_to) before[x] += e.w();
+        }
+        if (mine.bin() == c.k_bin && rank[x] < c.k_left) kept_k += mine.w();
+    }
+    u64 want = 0;
+    if (p.cut_p) {
+        const u64 all = c.k_bin >= 0 ? c.k_before + group_sum<NT>(sh, kept_k) : c.all;
+        want = all > 0 ? p.wanted(all) : 0;
+    }
+    u64 to = 0;
+    for (int x = 0; x < kPer; ++x) {
+        const int i = x * NT + (int)threadIdx.x;
+        if (i >= many) continue;
+        const Entry mine = list[i];
+        const int b = mine.bin();
+        const bool by_k = b != c.k_bin || rank[x] < c.k_left;
+        const bool by_p = !p.cut_p || (b >= c.p_from && b <= c.p_to && c.p_before + before[x] < want);
+        if (!by_k || !by_p) continue;
+        to = mine.place > to ? mine.place : to;
+        const uint32_t key = ~(uint32_t)(mine.place >> 32);
+        atomicAdd(&group[(uint32_t)mine.place / kGroup], p.kept(p.scaled(p.depth(key))));
+    }
+    // the largest of the workgroup's
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+        const u64 o = __shfl_xor(to, i);
+        to = o > to ? o : to;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = to;
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w) to = sh.wave[w] > to ? sh.wave[w] : to;
+    return to;
+}
+
+// The draw from the groups' sums: what stays are bins below `sure` and places up
+// to `to`. The whole workgroup calls.
+template <int TYPE, int NT>
+__device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r, const Row& p, int sure, u64 to, const void* row,
+                                     const u64* group) {
+    const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, lane = threadIdx.x & 63;
+    u64 all = 0;
+    for (int i = threadIdx.x; i < groups; i += NT) all += group[i];
+    all = group_sum<NT>(sh, all);
+    const double u = a.u[r], x = u > 0.0 ? u * (double)all : 0.0;
+    u64 target = x < (double)all ? (u64)x : all - 1;
+    target = target < all ? target : all - 1;
+    search<NT>(sh, groups, target, [&](int i) { return group[i]; });
+    if (threadIdx.x >= 64) return;
+    const int e = (int)sh.found * kGroup + 4 * lane;
+    float y[4];
+    load4<TYPE>(row, e, n, y);
+    u64 w[4], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t k = key_of(y[i]);
+        const double t = p.depth(k);
+        w[i] = k && (Row::bin(t) < sure || place_of(k, e + i) <= to) ? p.kept(p.scaled(t)) : 0;
+        mine += w[i];
+    }
+    u64 left = target - sh.before;
+    const u64 upto = wave_scan(mine, lane);
+    u64 base = upto - mine;
+    if (base <= left && left < upto) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (base <= left && left < base + w[i]) {
+                a.tokens[r] = e + i;
+                if (a.probs) a.probs[r] = (float)((double)w[i] / (double)all);
+            }
+            base += w[i];
+        }
+    }
+}
+
+// The cuts from the bits of x, for rows whose list is too long: eight bits at a
+// time within a bin, then the indices of equal ones. Returns the last place that
+// stays. `sum`, `count`: the histogram again.
+template <int TYPE, int NT>
+__device__ __noinline__ u64 border(Shared& sh, const Row& p, const void* row, int n, const u64* sum, const uint32_t* count,
+                                   u64* dsum, uint32_t* dcount, u64* group, bool by_count, u64 target, u64& upto) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = (n + kGroup - 1) / kGroup;
+    search<NT>(sh, kBins, target, [&](int i) { return by_count ? (u64)count[i] : sum[i]; });
+    const int bin = (int)sh.found;
+    target -= sh.before;
+    upto = 0;
+    for (int i = threadIdx.x; i < bin; i += NT) upto += sum[i];
+    upto = group_sum<NT>(sh, upto);
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
-        each([&](int, uint32_t k) {
-            const double d = k ? p.depth(k) : 1e9;
-            if (d < kBins / 64.0) {
-                const int b = (int)(d * 64.0);
-                atomicAdd(&sh.sum[b], weight(exp(-d)));
-                atomicAdd(&sh.count[b], 1u);
+        for (int i = threadIdx.x; i < 256; i += NT) dsum[i] = 0, dcount[i] = 0;
+        __syncthreads();
+        each<TYPE, NT>(row, n, 0, groups, [&](int, int, const float (&x)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t k = key_of(x[i]);
+                if (!k || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
+                const double t = p.depth(k);
+                if (Row::bin(t) != bin) continue;
+                const int digit = 255 - (int)(k >> shift & 255);
+                atomicAdd(&dsum[digit], Row::count(p.scaled(t)));
+                atomicAdd(&dcount[digit], 1u);
             }
         });
         __syncthreads();
-        // One border: in the order of the list, the entry at which the running
-        // count (by_count) or weight passes `target`. Leaves the entry's key in
-        // `low`, the index of the last equal one that stays in `last`, and
-        // returns the weight up to and with it.
-        unsigned long long all = 0, many = 0;
-        for (int i = threadIdx.x; i < kBins; i += kThreads) all += sh.sum[i], many += sh.count[i];
-        all = group_sum(sh, all);
-        many = group_sum(sh, many);
-        const int bins = kBins;
-        auto border = [&](bool by_count, unsigned long long target) -> unsigned long long {
-            // the bin (sh.sum and sh.count still hold the bins of depth)
-            search(sh, bins, target, [&](int i) { return by_count ? (unsigned long long)sh.count[i] : sh.sum[i]; });
-            const int bin = (int)sh.found;
-            target -= sh.before;
-            unsigned long long upto = 0;
-            for (int i = threadIdx.x; i < bin; i += kThreads) upto += sh.sum[i];
-            upto = group_sum(sh, upto);
-            // within it the bits of the key, from the top
-            __shared__ unsigned long long dsum[256];
-            __shared__ uint32_t dcount[256];
-            uint32_t prefix = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < 256; i += kThreads) dsum[i] = 0, dcount[i] = 0;
-                __syncthreads();
-                each([&](int, uint32_t k) {
-                    if (!k || (shift < 24 && (k >> (shift + 8)) != prefix)) return;
-                    const double d = p.depth(k);
-                    if (!(d < kBins / 64.0) || (int)(d * 64.0) != bin) return;
-                    const int digit = 255 - (int)(k >> shift & 255);
-                    atomicAdd(&dsum[digit], weight(exp(-d)));
-                    atomicAdd(&dcount[digit], 1u);
-                });
-                __syncthreads();
-                search(sh, 256, target, [&](int i) { return by_count ? (unsigned long long)dcount[i] : dsum[i]; });
-                const int digit = (int)sh.found;
-                target -= sh.before;
-                unsigned long long over = threadIdx.x < digit ? dsum[threadIdx.x & 255] : 0;
-                upto += group_sum(sh, over);
-                prefix = prefix << 8 | (uint32_t)(255 - digit);
-            }
-            // the equal ones: the first `extra` by index stay
-            const unsigned long long w = weight_of(prefix);
-            const unsigned long long extra = (by_count ? target : target / w) + 1;
-            low = prefix;
-            __syncthreads();
-            for (int g = wave; g < groups; g += kWaves) {
-                unsigned long long c = 0;
-                for (int i = 0; i < kStep / 64; ++i) {
-                    const int e = g * kStep + i * 64 + lane;
-                    c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(e < n && key_of(load_logit<TYPE>(row, e < n ? e : 0)) == low));
-                }
-                if (lane == 0) sh.group[g] = c;
-            }
-            __syncthreads();
-            search(sh, groups, extra - 1, [&](int i) { return sh.group[i]; });
-            {
-                const int g = (int)sh.found;
-                unsigned long long left = extra - 1 - sh.before;             // equal ones of the group before the last
-                int at = 0;
-                for (int i = 0; i < kStep / 64; ++i) {
-                    const int e = g * kStep + i * 64 + lane;
-                    const uint64_t m = __builtin_amdgcn_ballot_w64(e < n && key_of(load_logit<TYPE>(row, e < n ? e : 0)) == low);
-                    const unsigned long long c = (unsigned long long)__builtin_popcountll(m);
-                    if (left < c) {
-                        uint64_t rest = m;
-                        for (unsigned long long s = 0; s < left; ++s) rest &= rest - 1;
-                        at = g * kStep + i * 64 + (int)__builtin_ctzll(rest);
-                        break;
-                    }
-                    left -= c;
-                }
-                last = at;
-            }
-            __syncthreads();
-            return upto + extra * w;
-        };
-        if (cut_k && (unsigned long long)p.top_k < many) all = border(true, (unsigned long long)p.top_k - 1);
-        if (cut_p) {
-            const double want = __builtin_ceil((double)p.top_p * (double)all);
-            unsigned long long target = want >= 1.0 ? (unsigned long long)want : 1;
-            if (target > all) target = all;
-            border(false, target - 1);           // not past top_k's: all of the weight ends there
+        search<NT>(sh, 256, target, [&](int i) { return by_count ? (u64)dcount[i] : dsum[i]; });
+        const int digit = (int)sh.found;
+        target -= sh.before;
+        upto += group_sum<NT>(sh, (int)threadIdx.x < digit && threadIdx.x < 256 ? dsum[threadIdx.x & 255] : 0);
+        prefix = prefix << 8 | (uint32_t)(255 - digit);
+    }
+    // the equal ones: the first `extra` by index stay
+    const u64 w = Row::count(p.scaled(p.depth(prefix)));
+    const u64 extra = (by_count ? target : target / w) + 1;
+    upto += extra * w;
+    __syncthreads();
+    each<TYPE, NT>(row, n, 0, groups, [&](int g, int, const float (&x)[4]) {
+        u64 c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_of(x[i]) == prefix));
+        if (lane == 0) group[g] = c;
+    });
+    __syncthreads();
+    search<NT>(sh, groups, extra - 1, [&](int i) { return group[i]; });
+    const int g = (int)sh.found;
+    const u64 left = extra - 1 - sh.before;                          // equal ones of the group before the last
+    if (wave == 0) {
+        const int e = g * kGroup + 4 * lane;
+        float x[4];
+        load4<TYPE>(row, e, n, x);
+        u64 mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += key_of(x[i]) == prefix;
+        u64 base = wave_scan(mine, lane) - mine;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (key_of(x[i]) != prefix) continue;
+            if (base == left) sh.at = place_of(prefix, e + i);
+            ++base;
         }
     }
-    auto stays = [&](int e, uint32_t k) { return k > low || (k == low && e <= last); };
-    auto kept = [&](int e, uint32_t k) -> unsigned long long {
-        if (k == 0 || !stays(e, k)) return 0;
-        const double w = exp(-p.depth(k));
-        return w < min_w && k != p.top_key ? 0 : weight(w);
-    };
-
-    // the weights that stay, summed by group, and the draw
     __syncthreads();
-    for (int g = wave; g < groups; g += kWaves) {
-        unsigned long long s = 0;
-        for (int i = 0; i < kStep / 64; ++i) {
-            const int e = g * kStep + i * 64 + lane;
-            if (e < n) s += kept(e, key_of(load_logit<TYPE>(row, e)));
+    const u64 place = sh.at;
+    __syncthreads();
+    return place;
+}
+
+template <int TYPE, int NT>
+__device__ __noinline__ void long_way(Shared& sh, const SampleArgs& a, int64_t r, const Row& p, const void* row, const u64* sum,
+                                      const uint32_t* count, u64* dsum, uint32_t* dcount, u64* group) {
+    const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, lane = threadIdx.x & 63;
+    u64 all = 0, many = 0, to = ~(u64)0;
+    for (int i = threadIdx.x; i < kBins; i += NT) all += sum[i], many += count[i];
+    all = group_sum<NT>(sh, all);
+    many = group_sum<NT>(sh, many);
+    u64 upto = 0;
+    if (p.cut_k && (u64)p.top_k < many) {
+        to = border<TYPE, NT>(sh, p, row, n, sum, count, dsum, dcount, group, true, (u64)p.top_k - 1, upto);
+        all = upto;
+    }
+    if (p.cut_p) to = border<TYPE, NT>(sh, p, row, n, sum, count, dsum, dcount, group, false, p.wanted(all) - 1, upto);
+    __syncthreads();
+    each<TYPE, NT>(row, n, 0, groups, [&](int g, int e, const float (&x)[4]) {
+        u64 s = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t k = key_of(x[i]);
+            if (k && place_of(k, e + i) <= to) s += p.kept(p.scaled(p.depth(k)));
         }
         s = wave_sum(s);
-        if (lane == 0) sh.group[g] = s;
-    }
+        if (lane == 0) group[g] = s;
+    });
     __syncthreads();
-    unsigned long long all = 0;
-    for (int i = threadIdx.x; i < groups; i += kThreads) all += sh.group[i];
-    all = group_sum(sh, all);
-    const double u = a.u[r];
-    const double x = u > 0.0 ? u * (double)all : 0.0;
-    unsigned long long target = x < (double)all ? (unsigned long long)x : all - 1;
-    if (target > all - 1) target = all - 1;
-    search(sh, groups, target, [&](int i) { return sh.group[i]; });
-    if (wave == 0) {
-        const int g = (int)sh.found;
-        unsigned long long left = target - sh.before;
-        for (int i = 0; i < kStep / 64; ++i) {
-            const int e = g * kStep + i * 64 + lane;
-            const unsigned long long w = e < n ? kept(e, key_of(load_logit<TYPE>(row, e))) : 0, upto = wave_scan(w, lane);
-            const uint64_t m = __builtin_amdgcn_ballot_w64(left < upto);
-            if (m) {
-                if (lane == (int)__builtin_ctzll(m)) {
-                    a.tokens[r] = e;
-                    if (a.probs) a.probs[r] = (float)((double)w / (double)all);
-                }
-                break;
-            }
-            left -= __shfl((unsigned long long)upto, 63);
-        }
+    draw<TYPE, NT>(sh, a, r, p, 0, to, row, group);
+}
+
+__device__ __forceinline__ void take(const SampleArgs& a, int64_t r, uint32_t key, uint32_t index) {
+    if (threadIdx.x) return;
+    a.tokens[r] = key ? (int32_t)index : -1;
+    if (a.probs) a.probs[r] = key ? 1.f : 0.f;
+}
+
+// --------------------------------------------------- a row to a workgroup
+
+template <int TYPE>
+__global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
+    constexpr int NT = kRowThreads;
+    __shared__ Shared sh;
+    __shared__ u64 sum[kBins], group[kGroups], dsum[256];
+    __shared__ uint32_t count[kBins], dcount[256], listed;
+    __shared__ Entry list[kList];
+    const int64_t r = blockIdx.x;
+    const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup;
+    const char* row = static_cast<const char*>(a.logits) + r * a.ld * (TYPE == kTypeF32 ? 4 : 2);
+    if (threadIdx.x == 0) listed = 0;
+    for (int i = threadIdx.x; i < kBins; i += NT) sum[i] = 0, count[i] = 0;
+    uint32_t key, index;
+    largest<TYPE, NT>(sh, row, n, 0, groups, key, index);
+    Row p;
+    p.read(a, r, key);
+    if (key == 0 || p.greedy) return take(a, r, key, index);         // nothing to draw, or the largest
+    Cuts c;
+    c.none();
+    const bool cut = p.cut_k || p.cut_p;
+    if (cut) {
+        histogram<TYPE, NT>(p, row, n, 0, groups, sum, count);
+        __syncthreads();
+        c.find<NT>(sh, p, sum, count);
     }
+    sums_and_list<TYPE, NT>(p, c, row, n, 0, groups, group, list, &listed);
+    __syncthreads();
+    const int many = (int)listed;
+    if (many > kList) return long_way<TYPE, NT>(sh, a, r, p, row, sum, count, dsum, dcount, group);
+    const u64 to = many ? resolve<NT>(sh, p, c, list, many, group) : 0;
+    __syncthreads();
+    draw<TYPE, NT>(sh, a, r, p, c.sure, to, row, group);
 }
 
 }  // namespace
@@ -330,7 +603,7 @@ hipError_t launch_sample(SampleArgs a, hipStream_t stream) {
     while (((int64_t)1 << bits) < a.vocab) ++bits;
     a.frac = 62 - bits < kFrac ? 62 - bits : kFrac;          // the sum of a row stays below 2^62
     return with_type(a.type, [&](auto ty) {
-        sample_row_kernel<decltype(ty)::value><<<(unsigned)a.rows, kThreads, 0, stream>>>(a);
+        sample_row_kernel<decltype(ty)::value><<<(unsigned)a.rows, kRowThreads, 0, stream>>>(a);
         return hipGetLastError();
     });
 }
