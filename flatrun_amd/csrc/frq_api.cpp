@@ -1423,8 +1423,14 @@ int frq_dev_sample(int type, const void* logits, int64_t ld, int64_t rows, int64
           reinterpret_cast<uintptr_t>(probs)) & 3))
         return fail(FRQ_ERR_ALIGN, "sample: a buffer is not aligned to its type");
     frq::SampleArgs a{type, logits, ld, rows, vocab, u, temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks,
-                      tokens, probs, 0};
-    FRQ_HIP(frq::launch_sample(a, static_cast<hipStream_t>(stream)));
+                      tokens, probs, 0, 0, nullptr};
+    frq::plan_sample(&a);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    float* part;
+    uint32_t* cnt;
+    std::lock_guard<std::mutex> lk(g_sk_mu);
+    if (int rc = sk_scratch_locked(s, frq::sample_scratch(a), 0, &part, &cnt)) return rc;
+    FRQ_HIP(frq::launch_sample(a, part, s));
     return FRQ_OK;
 }
 

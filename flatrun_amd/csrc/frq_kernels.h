@@ -385,9 +385,12 @@ struct SampleArgs {
     const int32_t* top_ks;
     int32_t* tokens;
     float* probs;                // null: not stored
-    int frac;                    // set by the launcher: bits of a weight below 1
+    int frac, slices;            // plan_sample: bits of a weight below 1; workgroups of a row, 1 for all passes in one
+    void* scratch;
 };
-hipError_t launch_sample(SampleArgs a, hipStream_t stream);
+void plan_sample(SampleArgs* a);
+size_t sample_scratch(const SampleArgs& a);
+hipError_t launch_sample(SampleArgs a, void* scratch, hipStream_t stream);
 
 // Scratch a caller brings in place of the stream registry's: exchange slots
 // (zero before a launch, left zero by every launch) and split-K partials.

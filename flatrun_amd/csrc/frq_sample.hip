@@ -5,12 +5,13 @@
 //   the sum of the weights that stayed exceeds u times all of it.
 //
 // Nothing is sorted. All three cuts take the list's lower end away, so what
-// stays is the logits above one place of the list. A histogram of the weights
-// over the depth log2(e) (max - x) / T, 2048 bins of 1/44, says which bins stay
-// whole and in which one or two the cuts lie; the logits of those, some hundreds,
-// are listed and ranked against each other. Where they are too many for the
-// list (thousands of logits within 1/44 of each other) the cuts are found from
-// the bits of x, eight at a time, in further passes over the row.
+// stays is the logits above one place of the list. A histogram over the depth
+// log2(e) (max - x) / T, 2048 bins of 1/44, says which bins stay whole and in
+// which one or two the cuts lie; the logits of those, some hundreds, are listed
+// and ranked against each other. top_k alone decides by counts; where it leaves
+// up to kShort, all of them are listed and only they are weighed. Where a list
+// is too long (thousands of logits within 1/44 of each other) the cuts are found
+// from the bits of x, eight at a time, in further passes over the row.
 //
 // Weights are whole numbers of 2^-kFrac, computed in 64 bits and rounded once.
 // Sums of them are exact whatever their order: every pass sees the same ones,
@@ -32,7 +33,8 @@ constexpr int kBins = 2048, kPerBit = 44;    // depths up to 46.5: 2^-46 is no w
 constexpr int kFrac = 44;
 constexpr int kGroup = 256;                  // logits a wave takes at a time, four a lane
 constexpr int kGroups = 4096;                // of a row, at most
-constexpr int kList = 2048;                  // logits that are ranked one by one
+constexpr int kList = 2048;                  // logits that are listed
+constexpr int kShort = 1024;                 // top_k up to which all that stay are listed
 constexpr int kRowThreads = 1024, kSliceThreads = 256;
 constexpr float kInf = __builtin_inff();
 using u64 = unsigned long long;
@@ -95,34 +97,41 @@ __device__ __forceinline__ void load4(const void* row, int e, int n, float (&x)[
 // A row's parameters, its largest logit, and weights under it.
 struct Row {
     double per, top, least;                  // log2(e) / T; the largest; the least weight that min_p leaves, times 2^frac
+    float top32, per32;
     int frac;
-    uint32_t top_key;
     float top_p;
     int64_t top_k;
-    bool greedy, cut_k, cut_p;
+    bool greedy, cut_k, cut_p, short_list;
 
-    __device__ __forceinline__ void read(const SampleArgs& a, int64_t r, uint32_t key) {
+    __device__ __forceinline__ void read(const SampleArgs& a, int64_t r) {
         const float t = a.temperatures ? a.temperatures[r] : a.temperature;
         const float least_p = a.min_ps ? a.min_ps[r] : a.min_p;
         top_p = a.top_ps ? a.top_ps[r] : a.top_p;
         top_k = a.top_ks ? a.top_ks[r] : a.top_k;
         greedy = !(t > 0.f);
         per = 1.4426950408889634 / (double)__builtin_fminf(t, 3.4028235e38f);
-        top_key = key;
-        top = (double)of_key(key);
+        per32 = (float)(per * kPerBit);
         frac = a.frac;
         least = least_p > 0.f ? (double)__builtin_fminf(least_p, 1.f) * (double)((u64)1 << frac) : 0.0;
         cut_k = top_k > 0 && top_k < a.vocab;
         cut_p = top_p < 1.f;
+        short_list = cut_k && top_k <= kShort;
     }
-    // log2(e) (max - x) / T
-    __device__ __forceinline__ double depth(uint32_t key) const {
-        const double t = key == top_key ? 0.0 : (top - (double)of_key(key)) * per;
-        return __builtin_fmin(t, 60.0);
+    __device__ __forceinline__ void largest_is(uint32_t key) {
+        top32 = of_key(key);
+        top = (double)top32;
     }
-    // 2^(frac - t), by whole steps and a polynomial of degree 9 through
-    // Chebyshev's points of [-1/2, 1/2], within 4e-14 of itself.
-    __device__ __forceinline__ double scaled(double t) const {
+    // The bin of x, in fp32: all that is asked of it is that a smaller x has no
+    // smaller bin. kBins: no weight, or no number.
+    __device__ __forceinline__ int bin(float x) const {
+        const float d = x == top32 ? 0.f : (top32 - x) * per32;
+        return d < (float)kBins ? (int)d : kBins;
+    }
+    // 2^(frac - t), t = log2(e) (max - x) / T, by whole steps of t and a
+    // polynomial of degree 9 through Chebyshev's points of [-1/2, 1/2], within
+    // 4e-14 of itself.
+    __device__ __forceinline__ double scaled(float x) const {
+        const double t = __builtin_fmin(x == top32 ? 0.0 : (top - (double)x) * per, 60.0);
         const double whole = t + 6755399441055744.0, r = t - (whole - 6755399441055744.0);     // 1.5 2^52
         double y = -0x1.b63880a088780p-24;
         y = __builtin_fma(y, r, 0x1.63d136366f695p-20);
@@ -135,7 +144,7 @@ struct Row {
         y = __builtin_fma(y, r, -0x1.62e42fefa39efp-1);
         y = __builtin_fma(y, r, 1.0);
         const int n = frac - (int)(uint32_t)__builtin_bit_cast(u64, whole);
-        return __builtin_bit_cast(double, __builtin_bit_cast(u64, y) + ((u64)(uint32_t)(n << 20) << 32));
+        return __builtin_bit_cast(double, __builtin_bit_cast(u64, y) + ((u64)((uint32_t)n << 20) << 32));
     }
     // A scaled weight as a whole number, to nearest: below 2^52.
     static __device__ __forceinline__ u64 count(double y) {
@@ -143,19 +152,11 @@ struct Row {
     }
     // After min_p (of the logits that the other cuts leave).
     __device__ __forceinline__ u64 kept(double y) const { return y >= least ? count(y) : 0; }
-    static __device__ __forceinline__ int bin(double t) {            // kBins and more: no weight
-        return (int)(t * (double)kPerBit);
-    }
     // The weight that top_p asks for of `all`: the run's sum reaches it.
     __device__ __forceinline__ u64 wanted(u64 all) const {
         const double want = __builtin_ceil((double)top_p * (double)all);
         const u64 w = want >= 1.0 ? (u64)want : 1;
         return w < all ? w : all;
-    }
-    // Every logit of depth t and less has a key of at least this.
-    __device__ __forceinline__ uint32_t floor_of(double t) const {
-        const double x = top - t / per, low = x - (__builtin_fabs(x) + __builtin_fabs(top)) * 1e-6;
-        return low > -3.4e38 ? key_of((float)low) : 1u;
     }
 };
 
@@ -215,46 +216,50 @@ struct Cuts {
     u64 k_left;                              // logits of k_bin that stay
     u64 k_before, p_before, all;             // weights below k_bin, below p_from, and of all bins
     __device__ __forceinline__ bool listed(int b) const { return b == k_bin || (b >= p_from && b <= p_to); }
+    __device__ __forceinline__ int last() const { return p_to > k_bin ? p_to : k_bin; }
     __device__ __forceinline__ void none() {
         sure = kBins;
         p_from = 1, p_to = 0, k_bin = -1;
         k_left = k_before = p_before = all = 0;
     }
-    // The cuts from a histogram; false if neither applies.
+    template <int NT>
+    __device__ __forceinline__ void find_k(Shared& sh, const Row& p, const uint32_t* count) {
+        u64 many = 0;
+        for (int i = threadIdx.x; i < kBins; i += NT) many += count[i];
+        many = group_sum<NT>(sh, many);
+        if (!p.cut_k || (u64)p.top_k >= many) return;
+        search<NT>(sh, kBins, (u64)p.top_k - 1, [&](int i) { return (u64)count[i]; });
+        k_bin = (int)sh.found;
+        k_left = (u64)p.top_k - sh.before;
+        sure = k_bin;
+    }
+    // The bins that a short list takes, from counts alone.
+    template <int NT>
+    __device__ __forceinline__ void find_short(Shared& sh, const Row& p, const uint32_t* count) {
+        none();
+        find_k<NT>(sh, p, count);
+        p_from = 0, p_to = k_bin >= 0 ? k_bin : kBins - 1, sure = 0, k_bin = -1;
+    }
     template <int NT>
     __device__ __forceinline__ void find(Shared& sh, const Row& p, const u64* sum, const uint32_t* count) {
         none();
-        u64 many = 0;
+        find_k<NT>(sh, p, count);
+        if (!p.cut_p) return;
+        u64 low = 0;                                                 // what top_k leaves lies between low and high
         for (int i = threadIdx.x; i < kBins; i += NT) {
             all += sum[i];
-            many += count[i];
+            if (i < k_bin) low += sum[i];
         }
         all = group_sum<NT>(sh, all);
-        many = group_sum<NT>(sh, many);
-        u64 low = all, high = all;                                   // what top_k leaves lies between
-        if (p.cut_k && (u64)p.top_k < many) {
-            search<NT>(sh, kBins, (u64)p.top_k - 1, [&](int i) { return (u64)count[i]; });
-            k_bin = (int)sh.found;
-            k_left = (u64)p.top_k - sh.before;
-            low = 0;
-            for (int i = threadIdx.x; i < k_bin; i += NT) low += sum[i];
-            low = k_before = group_sum<NT>(sh, low);
-            high = low + sum[k_bin];
-            sure = k_bin;
-        }
-        if (p.cut_p && high > 0) {
-            search<NT>(sh, kBins, (low > 0 ? p.wanted(low) : 1) - 1, [&](int i) { return sum[i]; });
-            p_from = sure = (int)sh.found;
-            p_before = sh.before;
-            search<NT>(sh, kBins, p.wanted(high) - 1, [&](int i) { return sum[i]; });
-            p_to = (int)sh.found;
-        }
-    }
-    // the deepest that anything that stays or is listed can lie
-    __device__ __forceinline__ double deepest() const {
-        int b = sure - 1 > k_bin ? sure - 1 : k_bin;
-        b = b > p_to ? b : p_to;
-        return (b + 1) * (1.0 / kPerBit) + 1e-9;
+        k_before = group_sum<NT>(sh, low);
+        low = k_bin >= 0 ? k_before : all;
+        const u64 high = k_bin >= 0 ? low + sum[k_bin] : all;
+        if (high == 0) return;
+        search<NT>(sh, kBins, (low > 0 ? p.wanted(low) : 1) - 1, [&](int i) { return sum[i]; });
+        p_from = sure = (int)sh.found;
+        p_before = sh.before;
+        search<NT>(sh, kBins, p.wanted(high) - 1, [&](int i) { return sum[i]; });
+        p_to = (int)sh.found;
     }
 };
 
@@ -263,6 +268,7 @@ struct Entry {
     u64 place, weight;
     __device__ __forceinline__ int bin() const { return (int)(weight >> 48); }
     __device__ __forceinline__ u64 w() const { return weight & 0xFFFFFFFFFFFFull; }
+    __device__ __forceinline__ float value() const { return of_key(~(uint32_t)(place >> 32)); }
 };
 
 // Logits of the groups [from, to), wave by wave: f(index, four logits).
@@ -285,20 +291,28 @@ __device__ __forceinline__ void each(const void* row, int n, int from, int to, F
     }
 }
 
-// The largest of the groups, the lowest index of equals, to every thread.
+// The largest of the groups and, where asked for, the lowest index of equals, to
+// every thread.
 template <int TYPE, int NT>
-__device__ __forceinline__ void largest(Shared& sh, const void* row, int n, int from, int to, uint32_t& key, uint32_t& index) {
+__device__ __forceinline__ void largest(Shared& sh, const void* row, int n, int from, int to, bool where, uint32_t& key,
+                                        uint32_t& index) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float best = -kInf;
-    int where = -1;
-    each<TYPE, NT>(row, n, from, to, [&](int, int e, const float (&x)[4]) {
-        // a lane meets its indices in rising order: the first of equals stays
+    int at = -1;
+    if (where)
+        each<TYPE, NT>(row, n, from, to, [&](int, int e, const float (&x)[4]) {
+            // a lane meets its indices in rising order: the first of equals stays
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (x[i] > best) best = x[i], where = e + i;
-    });
+            for (int i = 0; i < 4; ++i)
+                if (x[i] > best) best = x[i], at = e + i;
+        });
+    else
+        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) best = __builtin_fmaxf(best, x[i]);
+        });
     key = key_of(best);
-    index = (uint32_t)where;
+    index = (uint32_t)at;
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) {
         const uint32_t k = __shfl_xor(key, i), w = __shfl_xor(index, i);
@@ -314,20 +328,24 @@ __device__ __forceinline__ void largest(Shared& sh, const void* row, int n, int 
 // The histogram of the groups, into LDS that is zero.
 template <int TYPE, int NT>
 __device__ __forceinline__ void histogram(const Row& p, const void* row, int n, int from, int to, u64* sum, uint32_t* count) {
-    const bool sums = p.cut_p;               // top_k alone asks for no weights
-    const uint32_t least = p.floor_of((double)kBins / kPerBit);
-    each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+    if (p.short_list)                        // counts alone
+        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t k = key_of(x[i]);
-            if (k < least) continue;
-            const double t = p.depth(k);
-            const int b = Row::bin(t);
-            if (b >= kBins) continue;
-            if (sums) atomicAdd(&sum[b], Row::count(p.scaled(t)));
-            if (p.cut_k) atomicAdd(&count[b], 1u);
-        }
-    });
+            for (int i = 0; i < 4; ++i) {
+                const int b = p.bin(x[i]);
+                if (b < kBins) atomicAdd(&count[b], 1u);
+            }
+        });
+    else
+        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = p.bin(x[i]);
+                if (b >= kBins) continue;
+                atomicAdd(&sum[b], Row::count(p.scaled(x[i])));
+                if (p.cut_k) atomicAdd(&count[b], 1u);
+            }
+        });
 }
 
 // Sums of what stays for certain, by group, and the list: entries that fit in
@@ -335,28 +353,25 @@ __device__ __forceinline__ void histogram(const Row& p, const void* row, int n, 
 template <int TYPE, int NT>
 __device__ __forceinline__ void sums_and_list(const Row& p, const Cuts& c, const void* row, int n, int from, int to, u64* group,
                                               Entry* list, uint32_t* listed) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t least = p.floor_of(c.deepest());
-    const int last = c.p_to > c.k_bin ? c.p_to : c.k_bin;            // of the bins that matter
+    const int lane = threadIdx.x & 63, last = c.last();
     each<TYPE, NT>(row, n, from, to, [&](int g, int e, const float (&x)[4]) {
         u64 s = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t k = key_of(x[i]);
-            if (k < least || k == 0) continue;
-            const double t = p.depth(k);
-            const int b = Row::bin(t);
+            const int b = p.bin(x[i]);
             if (b >= c.sure && (b > last || !c.listed(b))) continue;
-            const double y = p.scaled(t);
+            const double y = p.scaled(x[i]);
             if (b < c.sure) {
                 s += p.kept(y);
             } else {
                 const uint32_t at = atomicAdd(listed, 1u);
-                if (at < kList) list[at] = Entry{place_of(k, e + i), Row::count(y) | (u64)b << 48};
+                if (at < kList) list[at] = Entry{place_of(key_of(x[i]), e + i), Row::count(y) | (u64)b << 48};
             }
         }
-        if (__builtin_amdgcn_ballot_w64(s != 0)) s = wave_sum(s);
-        if (lane == 0) group[g] = s;
+        if (!p.short_list) {                 // else all that stays is listed
+            if (__builtin_amdgcn_ballot_w64(s != 0)) s = wave_sum(s);
+            if (lane == 0) group[g] = s;
+        }
     });
 }
 
@@ -372,6 +387,7 @@ __device__ __forceinline__ u64 resolve(Shared& sh, const Row& p, const Cuts& c, 
         before[x] = rank[x] = 0;
         if (i >= many) continue;
         const Entry mine = list[i];
+#pragma unroll 4
         for (int o = 0; o < many; ++o) {
             const Entry e = list[o];
             if (e.place >= mine.place) continue;
@@ -396,8 +412,7 @@ __device__ __forceinline__ u64 resolve(Shared& sh, const Row& p, const Cuts& c, 
         const bool by_p = !p.cut_p || (b >= c.p_from && b <= c.p_to && c.p_before + before[x] < want);
         if (!by_k || !by_p) continue;
         to = mine.place > to ? mine.place : to;
-        const uint32_t key = ~(uint32_t)(mine.place >> 32);
-        atomicAdd(&group[(uint32_t)mine.place / kGroup], p.kept(p.scaled(p.depth(key))));
+        atomicAdd(&group[(uint32_t)mine.place / kGroup], p.kept(p.scaled(mine.value())));
     }
     // the largest of the workgroup's
 #pragma unroll
@@ -432,9 +447,8 @@ __device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r,
     u64 w[4], mine = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t k = key_of(y[i]);
-        const double t = p.depth(k);
-        w[i] = k && (Row::bin(t) < sure || place_of(k, e + i) <= to) ? p.kept(p.scaled(t)) : 0;
+        const int b = p.bin(y[i]);
+        w[i] = b < sure || (b < kBins && place_of(key_of(y[i]), e + i) <= to) ? p.kept(p.scaled(y[i])) : 0;
         mine += w[i];
     }
     u64 left = target - sh.before;
@@ -452,45 +466,49 @@ __device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r,
     }
 }
 
-// The cuts from the bits of x, for rows whose list is too long: eight bits at a
-// time within a bin, then the indices of equal ones. Returns the last place that
-// stays. `sum`, `count`: the histogram again.
+// LDS of a workgroup that finishes a row.
+struct Finish {
+    u64 sum[kBins], group[kGroups], dsum[256];
+    uint32_t count[kBins], dcount[256], listed, listed2;
+    Entry list[kList], list2[kList];
+};
+
+// A cut from the bits of x, for rows whose list is too long: eight bits at a time
+// within a bin, then the indices of equal ones. Returns the last place that stays,
+// and the weight up to it.
 template <int TYPE, int NT>
-__device__ __noinline__ u64 border(Shared& sh, const Row& p, const void* row, int n, const u64* sum, const uint32_t* count,
-                                   u64* dsum, uint32_t* dcount, u64* group, bool by_count, u64 target, u64& upto) {
+__device__ __noinline__ u64 border(Shared& sh, Finish& f, const Row& p, const void* row, int n, bool by_count, u64 target, u64& upto) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = (n + kGroup - 1) / kGroup;
-    search<NT>(sh, kBins, target, [&](int i) { return by_count ? (u64)count[i] : sum[i]; });
+    search<NT>(sh, kBins, target, [&](int i) { return by_count ? (u64)f.count[i] : f.sum[i]; });
     const int bin = (int)sh.found;
     target -= sh.before;
     upto = 0;
-    for (int i = threadIdx.x; i < bin; i += NT) upto += sum[i];
+    for (int i = threadIdx.x; i < bin; i += NT) upto += f.sum[i];
     upto = group_sum<NT>(sh, upto);
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
-        for (int i = threadIdx.x; i < 256; i += NT) dsum[i] = 0, dcount[i] = 0;
+        for (int i = threadIdx.x; i < 256; i += NT) f.dsum[i] = 0, f.dcount[i] = 0;
         __syncthreads();
         each<TYPE, NT>(row, n, 0, groups, [&](int, int, const float (&x)[4]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t k = key_of(x[i]);
-                if (!k || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
-                const double t = p.depth(k);
-                if (Row::bin(t) != bin) continue;
+                if (p.bin(x[i]) != bin || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
                 const int digit = 255 - (int)(k >> shift & 255);
-                atomicAdd(&dsum[digit], Row::count(p.scaled(t)));
-                atomicAdd(&dcount[digit], 1u);
+                atomicAdd(&f.dsum[digit], Row::count(p.scaled(x[i])));
+                atomicAdd(&f.dcount[digit], 1u);
             }
         });
         __syncthreads();
-        search<NT>(sh, 256, target, [&](int i) { return by_count ? (u64)dcount[i] : dsum[i]; });
+        search<NT>(sh, 256, target, [&](int i) { return by_count ? (u64)f.dcount[i] : f.dsum[i]; });
         const int digit = (int)sh.found;
         target -= sh.before;
-        upto += group_sum<NT>(sh, (int)threadIdx.x < digit && threadIdx.x < 256 ? dsum[threadIdx.x & 255] : 0);
+        upto += group_sum<NT>(sh, (int)threadIdx.x < digit ? f.dsum[threadIdx.x & 255] : 0);
         prefix = prefix << 8 | (uint32_t)(255 - digit);
     }
     // the equal ones: the first `extra` by index stay
-    const u64 w = Row::count(p.scaled(p.depth(prefix)));
+    const u64 w = Row::count(p.scaled(of_key(prefix)));
     const u64 extra = (by_count ? target : target / w) + 1;
     upto += extra * w;
     __syncthreads();
@@ -498,14 +516,13 @@ __device__ __noinline__ u64 border(Shared& sh, const Row& p, const void* row, in
         u64 c = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) c += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_of(x[i]) == prefix));
-        if (lane == 0) group[g] = c;
+        if (lane == 0) f.group[g] = c;
     });
     __syncthreads();
-    search<NT>(sh, groups, extra - 1, [&](int i) { return group[i]; });
-    const int g = (int)sh.found;
-    const u64 left = extra - 1 - sh.before;                          // equal ones of the group before the last
+    search<NT>(sh, groups, extra - 1, [&](int i) { return f.group[i]; });
     if (wave == 0) {
-        const int e = g * kGroup + 4 * lane;
+        const u64 left = extra - 1 - sh.before;                      // equal ones of the group before the last
+        const int e = (int)sh.found * kGroup + 4 * lane;
         float x[4];
         load4<TYPE>(row, e, n, x);
         u64 mine = 0;
@@ -526,32 +543,66 @@ __device__ __noinline__ u64 border(Shared& sh, const Row& p, const void* row, in
 }
 
 template <int TYPE, int NT>
-__device__ __noinline__ void long_way(Shared& sh, const SampleArgs& a, int64_t r, const Row& p, const void* row, const u64* sum,
-                                      const uint32_t* count, u64* dsum, uint32_t* dcount, u64* group) {
+__device__ __noinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, Row p, const void* row) {
     const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, lane = threadIdx.x & 63;
-    u64 all = 0, many = 0, to = ~(u64)0;
-    for (int i = threadIdx.x; i < kBins; i += NT) all += sum[i], many += count[i];
+    p.short_list = false;                    // weights of all bins
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = 0, f.count[i] = 0;
+    __syncthreads();
+    histogram<TYPE, NT>(p, row, n, 0, groups, f.sum, f.count);
+    __syncthreads();
+    u64 all = 0, many = 0, to = ~(u64)0, upto = 0;
+    for (int i = threadIdx.x; i < kBins; i += NT) all += f.sum[i], many += f.count[i];
     all = group_sum<NT>(sh, all);
     many = group_sum<NT>(sh, many);
-    u64 upto = 0;
     if (p.cut_k && (u64)p.top_k < many) {
-        to = border<TYPE, NT>(sh, p, row, n, sum, count, dsum, dcount, group, true, (u64)p.top_k - 1, upto);
+        to = border<TYPE, NT>(sh, f, p, row, n, true, (u64)p.top_k - 1, upto);
         all = upto;
     }
-    if (p.cut_p) to = border<TYPE, NT>(sh, p, row, n, sum, count, dsum, dcount, group, false, p.wanted(all) - 1, upto);
+    if (p.cut_p) to = border<TYPE, NT>(sh, f, p, row, n, false, p.wanted(all) - 1, upto);
     __syncthreads();
     each<TYPE, NT>(row, n, 0, groups, [&](int g, int e, const float (&x)[4]) {
         u64 s = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t k = key_of(x[i]);
-            if (k && place_of(k, e + i) <= to) s += p.kept(p.scaled(p.depth(k)));
-        }
+        for (int i = 0; i < 4; ++i)
+            if (p.bin(x[i]) < kBins && place_of(key_of(x[i]), e + i) <= to) s += p.kept(p.scaled(x[i]));
         s = wave_sum(s);
-        if (lane == 0) group[g] = s;
+        if (lane == 0) f.group[g] = s;
     });
     __syncthreads();
-    draw<TYPE, NT>(sh, a, r, p, 0, to, row, group);
+    draw<TYPE, NT>(sh, a, r, p, 0, to, row, f.group);
+}
+
+// From the list (and, without a short list, the cuts and the groups' sums) to
+// the token. f.listed and f.count are there; the workgroup has met since.
+template <int TYPE, int NT>
+__device__ __forceinline__ void finish(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, const Row& p, Cuts& c, const void* row) {
+    const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup;
+    int many = (int)f.listed;
+    if (many > kList) return long_way<TYPE, NT>(sh, f, a, r, p, row);
+    const Entry* list = f.list;
+    if (p.short_list) {                      // the cuts from the list's own weights
+        for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = 0;
+        for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = 0;
+        if (threadIdx.x == 0) f.listed2 = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < many; i += NT) atomicAdd(&f.sum[f.list[i].bin()], f.list[i].w());
+        __syncthreads();
+        c.find<NT>(sh, p, f.sum, f.count);
+        for (int i = threadIdx.x; i < many; i += NT) {
+            const Entry e = f.list[i];
+            if (e.bin() < c.sure)
+                atomicAdd(&f.group[(uint32_t)e.place / kGroup], p.kept(p.scaled(e.value())));
+            else if (c.listed(e.bin()))
+                f.list2[atomicAdd(&f.listed2, 1u)] = e;
+        }
+        __syncthreads();
+        many = (int)f.listed2;
+        list = f.list2;
+    }
+    const u64 to = many ? resolve<NT>(sh, p, c, list, many, f.group) : 0;
+    __syncthreads();
+    draw<TYPE, NT>(sh, a, r, p, c.sure, to, row, f.group);
 }
 
 __device__ __forceinline__ void take(const SampleArgs& a, int64_t r, uint32_t key, uint32_t index) {
@@ -563,49 +614,212 @@ __device__ __forceinline__ void take(const SampleArgs& a, int64_t r, uint32_t ke
 // --------------------------------------------------- a row to a workgroup
 
 template <int TYPE>
+__device__ __forceinline__ const char* row_of(const SampleArgs& a, int64_t r) {
+    return static_cast<const char*>(a.logits) + r * a.ld * (TYPE == kTypeF32 ? 4 : 2);
+}
+
+template <int TYPE>
 __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
     constexpr int NT = kRowThreads;
     __shared__ Shared sh;
-    __shared__ u64 sum[kBins], group[kGroups], dsum[256];
-    __shared__ uint32_t count[kBins], dcount[256], listed;
-    __shared__ Entry list[kList];
+    __shared__ Finish f;
     const int64_t r = blockIdx.x;
     const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup;
-    const char* row = static_cast<const char*>(a.logits) + r * a.ld * (TYPE == kTypeF32 ? 4 : 2);
-    if (threadIdx.x == 0) listed = 0;
-    for (int i = threadIdx.x; i < kBins; i += NT) sum[i] = 0, count[i] = 0;
-    uint32_t key, index;
-    largest<TYPE, NT>(sh, row, n, 0, groups, key, index);
+    const char* row = row_of<TYPE>(a, r);
+    if (threadIdx.x == 0) f.listed = 0;
+    for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = 0, f.count[i] = 0;
     Row p;
-    p.read(a, r, key);
+    p.read(a, r);
+    uint32_t key, index;
+    largest<TYPE, NT>(sh, row, n, 0, groups, p.greedy, key, index);
     if (key == 0 || p.greedy) return take(a, r, key, index);         // nothing to draw, or the largest
+    p.largest_is(key);
     Cuts c;
     c.none();
-    const bool cut = p.cut_k || p.cut_p;
-    if (cut) {
-        histogram<TYPE, NT>(p, row, n, 0, groups, sum, count);
+    if (p.cut_k || p.cut_p) {
+        histogram<TYPE, NT>(p, row, n, 0, groups, f.sum, f.count);
         __syncthreads();
-        c.find<NT>(sh, p, sum, count);
+        if (p.short_list)
+            c.find_short<NT>(sh, p, f.count);
+        else
+            c.find<NT>(sh, p, f.sum, f.count);
     }
-    sums_and_list<TYPE, NT>(p, c, row, n, 0, groups, group, list, &listed);
+    sums_and_list<TYPE, NT>(p, c, row, n, 0, groups, f.group, f.list, &f.listed);
     __syncthreads();
-    const int many = (int)listed;
-    if (many > kList) return long_way<TYPE, NT>(sh, a, r, p, row, sum, count, dsum, dcount, group);
-    const u64 to = many ? resolve<NT>(sh, p, c, list, many, group) : 0;
+    finish<TYPE, NT>(sh, f, a, r, p, c, row);
+}
+
+// ------------------------------------------------------ a row in slices
+
+// Scratch of a row. The first launch clears what the others add to.
+struct Held {
+    u64 sum[kBins];
+    uint32_t count[kBins];
+    Entry list[kList];
+    u64 group[kGroups];
+    uint32_t key[64], index[64], listed;
+};
+
+struct Slice {
+    int64_t r;
+    int s, from, to;
+    Held* held;
+    __device__ __forceinline__ Slice(const SampleArgs& a) {
+        const int groups = (int)((a.vocab + kGroup - 1) / kGroup), per = (groups + a.slices - 1) / a.slices;
+        r = blockIdx.x / (uint32_t)a.slices;
+        s = (int)(blockIdx.x - (uint32_t)r * (uint32_t)a.slices);
+        from = s * per < groups ? s * per : groups;
+        to = from + per < groups ? from + per : groups;
+        held = static_cast<Held*>(a.scratch) + r;
+    }
+};
+
+template <int TYPE>
+__global__ void __launch_bounds__(kSliceThreads) sample_max_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ Shared sh;
+    const Slice z(a);
+    const char* row = row_of<TYPE>(a, z.r);
+    Row p;
+    p.read(a, z.r);
+    if (!p.greedy && (p.cut_k || p.cut_p))
+        for (int i = z.s * NT + (int)threadIdx.x; i < kBins; i += a.slices * NT) z.held->sum[i] = 0, z.held->count[i] = 0;
+    if (z.s == 0 && threadIdx.x == 0) z.held->listed = 0;
+    uint32_t key, index;
+    largest<TYPE, NT>(sh, row, (int)a.vocab, z.from, z.to, p.greedy, key, index);
+    if (threadIdx.x == 0) z.held->key[z.s] = key, z.held->index[z.s] = index;
+}
+
+// The row's largest from those of its slices.
+__device__ __forceinline__ void largest_of(const SampleArgs& a, const Held* h, uint32_t& key, uint32_t& index) {
+    const int lane = threadIdx.x & 63;
+    key = lane < a.slices ? h->key[lane] : 0;
+    index = lane < a.slices ? h->index[lane] : ~0u;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+        const uint32_t k = __shfl_xor(key, i), w = __shfl_xor(index, i);
+        if (k > key || (k == key && w < index)) key = k, index = w;
+    }
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kSliceThreads) sample_histogram_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ u64 sum[kBins];
+    __shared__ uint32_t count[kBins];
+    const Slice z(a);
+    Row p;
+    p.read(a, z.r);
+    uint32_t key, index;
+    largest_of(a, z.held, key, index);
+    if (key == 0 || p.greedy || !(p.cut_k || p.cut_p)) return;
+    p.largest_is(key);
+    for (int i = threadIdx.x; i < kBins; i += NT) sum[i] = 0, count[i] = 0;
     __syncthreads();
-    draw<TYPE, NT>(sh, a, r, p, c.sure, to, row, group);
+    histogram<TYPE, NT>(p, row_of<TYPE>(a, z.r), (int)a.vocab, z.from, z.to, sum, count);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += NT) {
+        if (sum[i]) atomicAdd(&z.held->sum[i], sum[i]);
+        if (count[i]) atomicAdd(&z.held->count[i], count[i]);
+    }
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kSliceThreads) sample_list_kernel(SampleArgs a) {
+    constexpr int NT = kSliceThreads;
+    __shared__ Shared sh;
+    __shared__ u64 sum[kBins];
+    __shared__ uint32_t count[kBins];
+    const Slice z(a);
+    Row p;
+    p.read(a, z.r);
+    uint32_t key, index;
+    largest_of(a, z.held, key, index);
+    if (key == 0 || p.greedy) return;
+    p.largest_is(key);
+    Cuts c;
+    c.none();
+    if (p.cut_k || p.cut_p) {
+        for (int i = threadIdx.x; i < kBins; i += NT) sum[i] = z.held->sum[i], count[i] = z.held->count[i];
+        __syncthreads();
+        if (p.short_list)
+            c.find_short<NT>(sh, p, count);
+        else
+            c.find<NT>(sh, p, sum, count);
+    }
+    sums_and_list<TYPE, NT>(p, c, row_of<TYPE>(a, z.r), (int)a.vocab, z.from, z.to, z.held->group, z.held->list, &z.held->listed);
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(kRowThreads) sample_pick_kernel(SampleArgs a) {
+    constexpr int NT = kRowThreads;
+    __shared__ Shared sh;
+    __shared__ Finish f;
+    const int64_t r = blockIdx.x;
+    const Held* h = static_cast<const Held*>(a.scratch) + r;
+    Row p;
+    p.read(a, r);
+    uint32_t key, index;
+    largest_of(a, h, key, index);
+    if (key == 0 || p.greedy) return take(a, r, key, index);
+    p.largest_is(key);
+    const int groups = (int)((a.vocab + kGroup - 1) / kGroup);
+    const uint32_t listed = h->listed;
+    if (threadIdx.x == 0) f.listed = listed;
+    for (int i = threadIdx.x; i < (int)(listed < kList ? listed : kList); i += NT) f.list[i] = h->list[i];
+    if (p.cut_k || p.cut_p)
+        for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = h->sum[i], f.count[i] = h->count[i];
+    if (!p.short_list)
+        for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = h->group[i];
+    __syncthreads();
+    Cuts c;
+    c.none();
+    if (!p.short_list && (p.cut_k || p.cut_p)) c.find<NT>(sh, p, f.sum, f.count);
+    finish<TYPE, NT>(sh, f, a, r, p, c, row_of<TYPE>(a, r));
+}
+
+template <int TYPE>
+hipError_t launch_typed(const SampleArgs& a, hipStream_t stream) {
+    if (a.slices == 1) {
+        sample_row_kernel<TYPE><<<(unsigned)a.rows, kRowThreads, 0, stream>>>(a);
+        return hipGetLastError();
+    }
+    const unsigned grid = (unsigned)(a.rows * a.slices);
+    // what the numbers given for all rows rule out is not launched
+    const bool greedy = !a.temperatures && !(a.temperature > 0.f);
+    const bool cuts = a.top_ks || a.top_ps || a.top_p < 1.f || (a.top_k > 0 && a.top_k < a.vocab);
+    sample_max_kernel<TYPE><<<grid, kSliceThreads, 0, stream>>>(a);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (!greedy && cuts) {
+        sample_histogram_kernel<TYPE><<<grid, kSliceThreads, 0, stream>>>(a);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    if (!greedy) {
+        sample_list_kernel<TYPE><<<grid, kSliceThreads, 0, stream>>>(a);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    sample_pick_kernel<TYPE><<<(unsigned)a.rows, kRowThreads, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_sample(SampleArgs a, hipStream_t stream) {
+void plan_sample(SampleArgs* a) {
     int bits = 0;
-    while (((int64_t)1 << bits) < a.vocab) ++bits;
-    a.frac = 62 - bits < kFrac ? 62 - bits : kFrac;          // the sum of a row stays below 2^62
-    return with_type(a.type, [&](auto ty) {
-        sample_row_kernel<decltype(ty)::value><<<(unsigned)a.rows, kRowThreads, 0, stream>>>(a);
-        return hipGetLastError();
-    });
+    while (((int64_t)1 << bits) < a->vocab) ++bits;
+    a->frac = 62 - bits < kFrac ? 62 - bits : kFrac;         // the sum of a row stays below 2^62
+    const int64_t groups = (a->vocab + kGroup - 1) / kGroup;
+    int64_t s = a->rows >= 128 ? 1 : 768 / (a->rows ? a->rows : 1);
+    s = s < groups / 8 ? s : groups / 8;                     // two groups a wave at least
+    s = s < 64 ? s : 64;
+    a->slices = s > 1 ? (int)s : 1;
+}
+
+size_t sample_scratch(const SampleArgs& a) { return a.slices > 1 ? (size_t)a.rows * sizeof(Held) : 0; }
+
+hipError_t launch_sample(SampleArgs a, void* scratch, hipStream_t stream) {
+    a.scratch = scratch;
+    return with_type(a.type, [&](auto ty) { return launch_typed<decltype(ty)::value>(a, stream); });
 }
 
 }  // namespace frq
