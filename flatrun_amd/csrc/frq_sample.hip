@@ -34,7 +34,7 @@ constexpr int kFrac = 44;
 constexpr int kGroup = 256;                  // logits a wave takes at a time, four a lane
 constexpr int kGroups = 4096;                // of a row, at most
 constexpr int kList = 2048;                  // logits that are listed
-constexpr int kShort = 1024;                 // top_k up to which all that stay are listed
+constexpr int kShort = 1024;                 // top_k up to which all that stay are listed, and a bin more
 constexpr int kRowThreads = 1024, kSliceThreads = 256;
 constexpr float kInf = __builtin_inff();
 using u64 = unsigned long long;
@@ -66,21 +66,22 @@ __device__ __forceinline__ u64 wave_scan(u64 x, int lane) {          // up to an
     return x;
 }
 
-// Four consecutive logits; those from n on are -inf.
+// Four consecutive logits from e on.
 template <int TYPE>
-__device__ __forceinline__ void load4(const void* row, int e, int n, float (&x)[4]) {
-    if (e + 4 <= n) {
-        if constexpr (TYPE == kTypeF32) {
-            __builtin_memcpy(x, static_cast<const float*>(row) + e, 16);
-        } else {
-            uint16_t b[4];
-            __builtin_memcpy(b, static_cast<const uint16_t*>(row) + e, 8);
+__device__ __forceinline__ void load4(const void* row, int e, float (&x)[4]) {
+    if constexpr (TYPE == kTypeF32) {
+        __builtin_memcpy(x, static_cast<const float*>(row) + e, 16);
+    } else {
+        uint16_t b[4];
+        __builtin_memcpy(b, static_cast<const uint16_t*>(row) + e, 8);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                x[i] = TYPE == kTypeF16 ? f16_bits_to_f32(b[i]) : __builtin_bit_cast(float, (uint32_t)b[i] << 16);
-        }
-        return;
+        for (int i = 0; i < 4; ++i)
+            x[i] = TYPE == kTypeF16 ? f16_bits_to_f32(b[i]) : __builtin_bit_cast(float, (uint32_t)b[i] << 16);
     }
+}
+// The same where the row may end; those from n on are -inf.
+template <int TYPE>
+__device__ __forceinline__ void load_end(const void* row, int e, int n, float (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         x[i] = -kInf;
@@ -97,7 +98,7 @@ __device__ __forceinline__ void load4(const void* row, int e, int n, float (&x)[
 // A row's parameters, its largest logit, and weights under it.
 struct Row {
     double per, top, least;                  // log2(e) / T; the largest; the least weight that min_p leaves, times 2^frac
-    float top32, per32;
+    float top32, per32, finite;              // finite: the largest, 0 where that is inf
     int frac;
     float top_p;
     int64_t top_k;
@@ -119,7 +120,8 @@ struct Row {
     }
     __device__ __forceinline__ void largest_is(uint32_t key) {
         top32 = of_key(key);
-        top = (double)top32;
+        finite = top32 < kInf ? top32 : 0.f;
+        top = (double)finite;
     }
     // The bin of x, in fp32: all that is asked of it is that a smaller x has no
     // smaller bin. kBins: no weight, or no number.
@@ -129,9 +131,9 @@ struct Row {
     }
     // 2^(frac - t), t = log2(e) (max - x) / T, by whole steps of t and a
     // polynomial of degree 9 through Chebyshev's points of [-1/2, 1/2], within
-    // 4e-14 of itself.
+    // 4e-14 of itself, for an x that has a bin.
     __device__ __forceinline__ double scaled(float x) const {
-        const double t = __builtin_fmin(x == top32 ? 0.0 : (top - (double)x) * per, 60.0);
+        const double t = (top - (double)(x == top32 ? finite : x)) * per;
         const double whole = t + 6755399441055744.0, r = t - (whole - 6755399441055744.0);     // 1.5 2^52
         double y = -0x1.b63880a088780p-24;
         y = __builtin_fma(y, r, 0x1.63d136366f695p-20);
@@ -144,7 +146,8 @@ struct Row {
         y = __builtin_fma(y, r, -0x1.62e42fefa39efp-1);
         y = __builtin_fma(y, r, 1.0);
         const int n = frac - (int)(uint32_t)__builtin_bit_cast(u64, whole);
-        return __builtin_bit_cast(double, __builtin_bit_cast(u64, y) + ((u64)((uint32_t)n << 20) << 32));
+        const u64 bits = __builtin_bit_cast(u64, y);
+        return __builtin_bit_cast(double, (u64)(((uint32_t)n << 20) + (uint32_t)(bits >> 32)) << 32 | (uint32_t)bits);
     }
     // A scaled weight as a whole number, to nearest: below 2^52.
     static __device__ __forceinline__ u64 count(double y) {
@@ -271,23 +274,28 @@ struct Entry {
     __device__ __forceinline__ float value() const { return of_key(~(uint32_t)(place >> 32)); }
 };
 
-// Logits of the groups [from, to), wave by wave: f(index, four logits).
-template <int TYPE, int NT, typename F>
+// Logits of the groups [from, to), wave by wave: f(group, index, four logits).
+template <int TYPE, int NT, int kAhead = 4, typename F>
 __device__ __forceinline__ void each(const void* row, int n, int from, int to, F&& f) {
-    constexpr int kAhead = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int g = from + wave; g < to; g += kAhead * (NT / 64)) {
+    constexpr int kStride = NT / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int full = n / kGroup < to ? n / kGroup : to;              // groups up to here are whole
+    int g = from + wave;
+    for (; g + (kAhead - 1) * kStride < full; g += kAhead * kStride) {
         float x[kAhead][4];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int at = g + i * (NT / 64);
-            if (at < to) load4<TYPE>(row, at * kGroup + 4 * lane, n, x[i]);
-        }
+        for (int i = 0; i < kAhead; ++i) load4<TYPE>(row, (g + i * kStride) * kGroup + 4 * lane, x[i]);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int at = g + i * (NT / 64);
-            if (at < to) f(at, at * kGroup + 4 * lane, x[i]);
-        }
+        for (int i = 0; i < kAhead; ++i) f(g + i * kStride, (g + i * kStride) * kGroup + 4 * lane, x[i]);
+    }
+    for (; g < to; g += kStride) {
+        float x[4];
+        const int e = g * kGroup + 4 * lane;
+        if (g < full)
+            load4<TYPE>(row, e, x);
+        else
+            load_end<TYPE>(row, e, n, x);
+        f(g, e, x);
     }
 }
 
@@ -338,90 +346,157 @@ __device__ __forceinline__ void histogram(const Row& p, const void* row, int n, 
         });
     else
         each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+            u64 w[4];                        // without branches, so that the four go on side by side
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = Row::count(p.scaled(x[i]));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int b = p.bin(x[i]);
                 if (b >= kBins) continue;
-                atomicAdd(&sum[b], Row::count(p.scaled(x[i])));
+                atomicAdd(&sum[b], w[i]);
                 if (p.cut_k) atomicAdd(&count[b], 1u);
             }
         });
 }
 
-// Sums of what stays for certain, by group, and the list: entries that fit in
-// kList, all of them counted.
+// Sums of what stays for certain, by group (not with a short list, where all that
+// stays is listed), and the list: entries that fit in kList, all of them counted.
 template <int TYPE, int NT>
 __device__ __forceinline__ void sums_and_list(const Row& p, const Cuts& c, const void* row, int n, int from, int to, u64* group,
                                               Entry* list, uint32_t* listed) {
     const int lane = threadIdx.x & 63, last = c.last();
     each<TYPE, NT>(row, n, from, to, [&](int g, int e, const float (&x)[4]) {
-        u64 s = 0;
+        int b[4], least = kBins;
+        bool any = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int b = p.bin(x[i]);
-            if (b >= c.sure && (b > last || !c.listed(b))) continue;
-            const double y = p.scaled(x[i]);
-            if (b < c.sure) {
-                s += p.kept(y);
-            } else {
-                const uint32_t at = atomicAdd(listed, 1u);
-                if (at < kList) list[at] = Entry{place_of(key_of(x[i]), e + i), Row::count(y) | (u64)b << 48};
-            }
+            b[i] = p.bin(x[i]);
+            least = b[i] < least ? b[i] : least;
+            any |= b[i] >= c.sure && b[i] <= last;
         }
-        if (!p.short_list) {                 // else all that stays is listed
-            if (__builtin_amdgcn_ballot_w64(s != 0)) s = wave_sum(s);
+        if (!p.short_list) {
+            u64 s = 0;
+            if (__builtin_amdgcn_ballot_w64(least < c.sure)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double y = p.scaled(x[i]);
+                    s += b[i] < c.sure && y >= p.least ? Row::count(y) : 0;
+                }
+                s = wave_sum(s);
+            }
             if (lane == 0) group[g] = s;
+        }
+        if (__builtin_amdgcn_ballot_w64(any) == 0) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b[i] < c.sure || b[i] > last || !c.listed(b[i])) continue;
+            const uint32_t at = atomicAdd(listed, 1u);
+            if (at < kList) list[at] = Entry{place_of(key_of(x[i]), e + i), Row::count(p.scaled(x[i])) | (u64)b[i] << 48};
         }
     });
 }
 
-// What stays of the list: those up to `to` in its order. Their weights are added
-// to their groups.
+// LDS of a workgroup that finishes a row.
+struct Finish {
+    u64 sum[kBins], group[kGroups], dsum[256];
+    uint32_t count[kBins], dcount[256], listed;
+    Entry list[kList];
+    u64 sort[2][kList];
+};
+
+// What stays of the list: those up to a place in its order, which is returned.
+// Their weights are added to their groups. The list is put in order, by a bitonic
+// network on one number an entry (key, index and number in the list), 32 steps of
+// which leave the wave where there are 2048; then top_k counts and top_p sums.
 template <int NT>
-__device__ __forceinline__ u64 resolve(Shared& sh, const Row& p, const Cuts& c, const Entry* list, int many, u64* group) {
-    u64 kept_k = 0;
+__device__ __forceinline__ u64 resolve(Shared& sh, Finish& f, const Row& p, const Cuts& c, int many) {
     constexpr int kPer = kList / NT;
-    u64 before[kPer], rank[kPer];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = (int)threadIdx.x;
+    int size = 64;
+    while (size < many) size *= 2;
+    u64 v[kPer];
+#pragma unroll
     for (int x = 0; x < kPer; ++x) {
-        const int i = x * NT + (int)threadIdx.x;
-        before[x] = rank[x] = 0;
-        if (i >= many) continue;
-        const Entry mine = list[i];
-#pragma unroll 4
-        for (int o = 0; o < many; ++o) {
-            const Entry e = list[o];
-            if (e.place >= mine.place) continue;
-            const int b = e.bin();
-            if (b == c.k_bin) ++rank[x];
-            if (b >= c.p_from && b <= c.p_to) before[x] += e.w();
-        }
-        if (mine.bin() == c.k_bin && rank[x] < c.k_left) kept_k += mine.w();
+        const int i = x * NT + t;
+        const u64 place = i < many ? f.list[i].place : 0;
+        v[x] = i < many ? (place >> 32) << 32 | (u64)(uint32_t)place << 11 | (u64)i : ~(u64)0;
     }
+    static_assert(kList <= 1 << 11, "the number of an entry has 11 bits, its index 20");
+    int turn = 0;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j; j /= 2) {
+            if (j >= NT) {
+                if constexpr (kPer == 2) {
+                    const bool swap = v[0] > v[1];                   // k is the whole: rising
+                    const u64 a = swap ? v[1] : v[0], b = swap ? v[0] : v[1];
+                    v[0] = a, v[1] = b;
+                }
+                continue;
+            }
+            if (j >= 64) {
+#pragma unroll
+                for (int x = 0; x < kPer; ++x)
+                    if (x * NT < size) f.sort[turn][x * NT + t] = v[x];
+                __syncthreads();
+            }
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) {
+                if (x * NT >= size) continue;
+                const int i = x * NT + t;
+                const u64 o = j >= 64 ? f.sort[turn][i ^ j] : __shfl_xor(v[x], j);
+                const bool low = ((i & j) == 0) == ((i & k) == 0);   // keeps the smaller
+                v[x] = low == (o < v[x]) ? o : v[x];
+            }
+            if (j >= 64) turn ^= 1;
+        }
+    // entry i of the order: its weight, and the weights before it
+    Entry mine[kPer];
+    u64 upto[kPer], whole = 0, first = 0;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+        const int i = x * NT + t;
+        mine[x] = i < many ? f.list[v[x] & (kList - 1)] : Entry{~(u64)0, 0};
+        first += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < many && mine[x].bin() != c.k_bin));
+        upto[x] = wave_scan(mine[x].w(), lane);
+        __syncthreads();
+        if (lane == 63) sh.wave[wave] = upto[x];
+        __syncthreads();
+        u64 base = whole;
+        for (int w = 0; w < NT / 64; ++w) {
+            if (w < wave) base += sh.wave[w];
+            whole += sh.wave[w];
+        }
+        upto[x] += base;
+    }
+    first = group_sum<NT>(sh, lane == 0 ? first : 0);                // entries of the bins above top_k's
+    const u64 limit = p.short_list ? (u64)p.top_k : c.k_bin >= 0 ? first + c.k_left : ~(u64)0;
     u64 want = 0;
     if (p.cut_p) {
-        const u64 all = c.k_bin >= 0 ? c.k_before + group_sum<NT>(sh, kept_k) : c.all;
+        u64 kept_k = 0;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x)
+            if ((u64)(x * NT + t) < limit && (p.short_list || mine[x].bin() == c.k_bin)) kept_k += mine[x].w();
+        kept_k = group_sum<NT>(sh, kept_k);
+        const u64 all = p.short_list ? kept_k : c.k_bin >= 0 ? c.k_before + kept_k : c.all;
         want = all > 0 ? p.wanted(all) : 0;
     }
     u64 to = 0;
+#pragma unroll
     for (int x = 0; x < kPer; ++x) {
-        const int i = x * NT + (int)threadIdx.x;
-        if (i >= many) continue;
-        const Entry mine = list[i];
-        const int b = mine.bin();
-        const bool by_k = b != c.k_bin || rank[x] < c.k_left;
-        const bool by_p = !p.cut_p || (b >= c.p_from && b <= c.p_to && c.p_before + before[x] < want);
-        if (!by_k || !by_p) continue;
-        to = mine.place > to ? mine.place : to;
-        atomicAdd(&group[(uint32_t)mine.place / kGroup], p.kept(p.scaled(mine.value())));
+        const int i = x * NT + t, b = mine[x].bin();
+        if (i >= many || (u64)i >= limit) continue;
+        if (p.cut_p && (b < c.p_from || b > c.p_to || c.p_before + upto[x] - mine[x].w() >= want)) continue;
+        to = mine[x].place;                                          // they rise
+        const u64 w = p.kept(p.scaled(mine[x].value()));
+        if (w) atomicAdd(&f.group[(uint32_t)mine[x].place / kGroup], w);
     }
-    // the largest of the workgroup's
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) {
         const u64 o = __shfl_xor(to, i);
         to = o > to ? o : to;
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = to;
+    if (lane == 0) sh.wave[wave] = to;
     __syncthreads();
     for (int w = 0; w < NT / 64; ++w) to = sh.wave[w] > to ? sh.wave[w] : to;
     return to;
@@ -443,7 +518,7 @@ __device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r,
     if (threadIdx.x >= 64) return;
     const int e = (int)sh.found * kGroup + 4 * lane;
     float y[4];
-    load4<TYPE>(row, e, n, y);
+    load_end<TYPE>(row, e, n, y);
     u64 w[4], mine = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -466,18 +541,11 @@ __device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r,
     }
 }
 
-// LDS of a workgroup that finishes a row.
-struct Finish {
-    u64 sum[kBins], group[kGroups], dsum[256];
-    uint32_t count[kBins], dcount[256], listed, listed2;
-    Entry list[kList], list2[kList];
-};
-
 // A cut from the bits of x, for rows whose list is too long: eight bits at a time
 // within a bin, then the indices of equal ones. Returns the last place that stays,
 // and the weight up to it.
 template <int TYPE, int NT>
-__device__ __noinline__ u64 border(Shared& sh, Finish& f, const Row& p, const void* row, int n, bool by_count, u64 target, u64& upto) {
+__device__ __forceinline__ u64 border(Shared& sh, Finish& f, const Row& p, const void* row, int n, bool by_count, u64 target, u64& upto) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = (n + kGroup - 1) / kGroup;
     search<NT>(sh, kBins, target, [&](int i) { return by_count ? (u64)f.count[i] : f.sum[i]; });
     const int bin = (int)sh.found;
@@ -490,7 +558,7 @@ __device__ __noinline__ u64 border(Shared& sh, Finish& f, const Row& p, const vo
         __syncthreads();
         for (int i = threadIdx.x; i < 256; i += NT) f.dsum[i] = 0, f.dcount[i] = 0;
         __syncthreads();
-        each<TYPE, NT>(row, n, 0, groups, [&](int, int, const float (&x)[4]) {
+        each<TYPE, NT, 1>(row, n, 0, groups, [&](int, int, const float (&x)[4]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t k = key_of(x[i]);
@@ -512,7 +580,7 @@ __device__ __noinline__ u64 border(Shared& sh, Finish& f, const Row& p, const vo
     const u64 extra = (by_count ? target : target / w) + 1;
     upto += extra * w;
     __syncthreads();
-    each<TYPE, NT>(row, n, 0, groups, [&](int g, int, const float (&x)[4]) {
+    each<TYPE, NT, 1>(row, n, 0, groups, [&](int g, int, const float (&x)[4]) {
         u64 c = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) c += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_of(x[i]) == prefix));
@@ -524,7 +592,7 @@ __device__ __noinline__ u64 border(Shared& sh, Finish& f, const Row& p, const vo
         const u64 left = extra - 1 - sh.before;                      // equal ones of the group before the last
         const int e = (int)sh.found * kGroup + 4 * lane;
         float x[4];
-        load4<TYPE>(row, e, n, x);
+        load_end<TYPE>(row, e, n, x);
         u64 mine = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) mine += key_of(x[i]) == prefix;
@@ -543,7 +611,7 @@ __device__ __noinline__ u64 border(Shared& sh, Finish& f, const Row& p, const vo
 }
 
 template <int TYPE, int NT>
-__device__ __noinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, Row p, const void* row) {
+__device__ __forceinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, Row p, const void* row) {
     const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, lane = threadIdx.x & 63;
     p.short_list = false;                    // weights of all bins
     __syncthreads();
@@ -561,7 +629,7 @@ __device__ __noinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a
     }
     if (p.cut_p) to = border<TYPE, NT>(sh, f, p, row, n, false, p.wanted(all) - 1, upto);
     __syncthreads();
-    each<TYPE, NT>(row, n, 0, groups, [&](int g, int e, const float (&x)[4]) {
+    each<TYPE, NT, 1>(row, n, 0, groups, [&](int g, int e, const float (&x)[4]) {
         u64 s = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -574,33 +642,15 @@ __device__ __noinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a
 }
 
 // From the list (and, without a short list, the cuts and the groups' sums) to
-// the token. f.listed and f.count are there; the workgroup has met since.
+// the token. The workgroup has met since they were written.
 template <int TYPE, int NT>
-__device__ __forceinline__ void finish(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, const Row& p, Cuts& c, const void* row) {
-    const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup;
-    int many = (int)f.listed;
+__device__ __forceinline__ void finish(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, const Row& p, const Cuts& c, const void* row) {
+    const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, many = (int)f.listed;
     if (many > kList) return long_way<TYPE, NT>(sh, f, a, r, p, row);
-    const Entry* list = f.list;
-    if (p.short_list) {                      // the cuts from the list's own weights
-        for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = 0;
+    if (p.short_list) {                      // resolve meets before it adds
         for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = 0;
-        if (threadIdx.x == 0) f.listed2 = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < many; i += NT) atomicAdd(&f.sum[f.list[i].bin()], f.list[i].w());
-        __syncthreads();
-        c.find<NT>(sh, p, f.sum, f.count);
-        for (int i = threadIdx.x; i < many; i += NT) {
-            const Entry e = f.list[i];
-            if (e.bin() < c.sure)
-                atomicAdd(&f.group[(uint32_t)e.place / kGroup], p.kept(p.scaled(e.value())));
-            else if (c.listed(e.bin()))
-                f.list2[atomicAdd(&f.listed2, 1u)] = e;
-        }
-        __syncthreads();
-        many = (int)f.listed2;
-        list = f.list2;
     }
-    const u64 to = many ? resolve<NT>(sh, p, c, list, many, f.group) : 0;
+    const u64 to = many ? resolve<NT>(sh, f, p, c, many) : 0;
     __syncthreads();
     draw<TYPE, NT>(sh, a, r, p, c.sure, to, row, f.group);
 }
@@ -767,14 +817,18 @@ __global__ void __launch_bounds__(kRowThreads) sample_pick_kernel(SampleArgs a) 
     const uint32_t listed = h->listed;
     if (threadIdx.x == 0) f.listed = listed;
     for (int i = threadIdx.x; i < (int)(listed < kList ? listed : kList); i += NT) f.list[i] = h->list[i];
-    if (p.cut_k || p.cut_p)
-        for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = h->sum[i], f.count[i] = h->count[i];
-    if (!p.short_list)
-        for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = h->group[i];
-    __syncthreads();
     Cuts c;
     c.none();
-    if (!p.short_list && (p.cut_k || p.cut_p)) c.find<NT>(sh, p, f.sum, f.count);
+    if (p.short_list) {                      // the list holds all that may stay
+        c.sure = 0, c.p_from = 0, c.p_to = kBins - 1;
+        __syncthreads();
+    } else {
+        if (p.cut_k || p.cut_p)
+            for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = h->sum[i], f.count[i] = h->count[i];
+        for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = h->group[i];
+        __syncthreads();
+        if (p.cut_k || p.cut_p) c.find<NT>(sh, p, f.sum, f.count);
+    }
     finish<TYPE, NT>(sh, f, a, r, p, c, row_of<TYPE>(a, r));
 }
 
