@@ -20,7 +20,7 @@
 // flat row of 10^5 logits.
 //
 // Passes over a row: its largest; the histogram (not without top_k and top_p);
-// the sums of what stays by group of 256, and the list; the group that the draw
+// the sums of what stays by group of 1024, and the list; the group that the draw
 // falls into. One workgroup does them all where there are rows for the GPU, else
 // each pass is a launch of slices of all rows.
 #include "frq_kernels.h"
@@ -31,8 +31,8 @@ namespace {
 
 constexpr int kBins = 2048, kPerBit = 44;    // depths up to 46.5: 2^-46 is no weight any more
 constexpr int kFrac = 44;
-constexpr int kGroup = 256;                  // logits a wave takes at a time, four a lane
-constexpr int kGroups = 4096;                // of a row, at most
+constexpr int kGroup = 1024;                 // logits a wave takes at a time, four by four a lane
+constexpr int kGroups = 1024;                // of a row, at most
 constexpr int kList = 2048;                  // logits that are listed
 constexpr int kShort = 1024;                 // top_k up to which all that stay are listed, and a bin more
 constexpr int kRowThreads = 1024, kSliceThreads = 256;
@@ -66,20 +66,26 @@ __device__ __forceinline__ u64 wave_scan(u64 x, int lane) {          // up to an
     return x;
 }
 
-// Four consecutive logits from e on.
+// Four consecutive logits, as they are held.
 template <int TYPE>
-__device__ __forceinline__ void load4(const void* row, int e, float (&x)[4]) {
-    if constexpr (TYPE == kTypeF32) {
-        __builtin_memcpy(x, static_cast<const float*>(row) + e, 16);
-    } else {
-        uint16_t b[4];
-        __builtin_memcpy(b, static_cast<const uint16_t*>(row) + e, 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            x[i] = TYPE == kTypeF16 ? f16_bits_to_f32(b[i]) : __builtin_bit_cast(float, (uint32_t)b[i] << 16);
+struct Raw {
+    uint32_t w[TYPE == kTypeF32 ? 4 : 2];
+    __device__ __forceinline__ void load(const void* row, int e) {
+        __builtin_memcpy(w, static_cast<const char*>(row) + (int64_t)e * (TYPE == kTypeF32 ? 4 : 2), sizeof(w));
     }
-}
-// The same where the row may end; those from n on are -inf.
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (TYPE == kTypeF32)
+                x[i] = __builtin_bit_cast(float, w[i]);
+            else if constexpr (TYPE == kTypeF16)
+                x[i] = f16_bits_to_f32(w[i / 2] >> (16 * (i & 1)) & 0xFFFFu);
+            else
+                x[i] = __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        }
+    }
+};
+// Four consecutive logits where the row may end; those from n on are -inf.
 template <int TYPE>
 __device__ __forceinline__ void load_end(const void* row, int e, int n, float (&x)[4]) {
 #pragma unroll
@@ -100,6 +106,7 @@ struct Row {
     double per, top, least;                  // log2(e) / T; the largest; the least weight that min_p leaves, times 2^frac
     float top32, per32, finite;              // finite: the largest, 0 where that is inf
     int frac;
+    double c[9];                             // of the polynomial in scaled(), in scalar registers
     float top_p;
     int64_t top_k;
     bool greedy, cut_k, cut_p, short_list;
@@ -113,6 +120,14 @@ struct Row {
         per = 1.4426950408889634 / (double)__builtin_fminf(t, 3.4028235e38f);
         per32 = (float)(per * kPerBit);
         frac = a.frac;
+        const double k[9] = {-0x1.b63880a088780p-24, 0x1.63d136366f695p-20, -0x1.ffcb9515b5679p-17, 0x1.4308ac85aa8a7p-13,
+                             -0x1.5d87fe86fe7f7p-10, 0x1.3b2ab7181b755p-7, -0x1.c6b08d7047e52p-5, 0x1.ebfbdff823cedp-3,
+                             -0x1.62e42fefa39efp-1};
+#pragma unroll
+        for (int i = 0; i < 9; ++i) {
+            c[i] = k[i];
+            asm("" : "+s"(c[i]));            // else nine moves a weight
+        }
         least = least_p > 0.f ? (double)__builtin_fminf(least_p, 1.f) * (double)((u64)1 << frac) : 0.0;
         cut_k = top_k > 0 && top_k < a.vocab;
         cut_p = top_p < 1.f;
@@ -135,15 +150,9 @@ struct Row {
     __device__ __forceinline__ double scaled(float x) const {
         const double t = (top - (double)(x == top32 ? finite : x)) * per;
         const double whole = t + 6755399441055744.0, r = t - (whole - 6755399441055744.0);     // 1.5 2^52
-        double y = -0x1.b63880a088780p-24;
-        y = __builtin_fma(y, r, 0x1.63d136366f695p-20);
-        y = __builtin_fma(y, r, -0x1.ffcb9515b5679p-17);
-        y = __builtin_fma(y, r, 0x1.4308ac85aa8a7p-13);
-        y = __builtin_fma(y, r, -0x1.5d87fe86fe7f7p-10);
-        y = __builtin_fma(y, r, 0x1.3b2ab7181b755p-7);
-        y = __builtin_fma(y, r, -0x1.c6b08d7047e52p-5);
-        y = __builtin_fma(y, r, 0x1.ebfbdff823cedp-3);
-        y = __builtin_fma(y, r, -0x1.62e42fefa39efp-1);
+        double y = c[0];
+#pragma unroll
+        for (int i = 1; i < 9; ++i) y = __builtin_fma(y, r, c[i]);
         y = __builtin_fma(y, r, 1.0);
         const int n = frac - (int)(uint32_t)__builtin_bit_cast(u64, whole);
         const u64 bits = __builtin_bit_cast(u64, y);
@@ -274,28 +283,33 @@ struct Entry {
     __device__ __forceinline__ float value() const { return of_key(~(uint32_t)(place >> 32)); }
 };
 
-// Logits of the groups [from, to), wave by wave: f(group, index, four logits).
-template <int TYPE, int NT, int kAhead = 4, typename F>
+// Logits of the groups [from, to), wave by wave: f(group, index of the lane's
+// first, x), x[i][j] at 256 i + j from there. The next group is asked for before
+// one is worked on.
+template <int TYPE, int NT, typename F>
 __device__ __forceinline__ void each(const void* row, int n, int from, int to, F&& f) {
     constexpr int kStride = NT / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int full = n / kGroup < to ? n / kGroup : to;              // groups up to here are whole
     int g = from + wave;
-    for (; g + (kAhead - 1) * kStride < full; g += kAhead * kStride) {
-        float x[kAhead][4];
+    Raw<TYPE> raw[4];
+    if (g < full)
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) load4<TYPE>(row, (g + i * kStride) * kGroup + 4 * lane, x[i]);
+        for (int i = 0; i < 4; ++i) raw[i].load(row, g * kGroup + 256 * i + 4 * lane);
+    for (; g < full; g += kStride) {
+        float x[4][4];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) f(g + i * kStride, (g + i * kStride) * kGroup + 4 * lane, x[i]);
+        for (int i = 0; i < 4; ++i) raw[i].get(x[i]);
+        if (g + kStride < full)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i].load(row, (g + kStride) * kGroup + 256 * i + 4 * lane);
+        f(g, g * kGroup + 4 * lane, x);
     }
-    for (; g < to; g += kStride) {
-        float x[4];
-        const int e = g * kGroup + 4 * lane;
-        if (g < full)
-            load4<TYPE>(row, e, x);
-        else
-            load_end<TYPE>(row, e, n, x);
-        f(g, e, x);
+    if (g < to) {
+        float x[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_end<TYPE>(row, g * kGroup + 256 * i + 4 * lane, n, x[i]);
+        f(g, g * kGroup + 4 * lane, x);
     }
 }
 
@@ -308,16 +322,16 @@ __device__ __forceinline__ void largest(Shared& sh, const void* row, int n, int 
     float best = -kInf;
     int at = -1;
     if (where)
-        each<TYPE, NT>(row, n, from, to, [&](int, int e, const float (&x)[4]) {
+        each<TYPE, NT>(row, n, from, to, [&](int, int e, const float (&x)[4][4]) {
             // a lane meets its indices in rising order: the first of equals stays
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (x[i] > best) best = x[i], at = e + i;
+            for (int i = 0; i < 16; ++i)
+                if (x[i / 4][i % 4] > best) best = x[i / 4][i % 4], at = e + i / 4 * 256 + i % 4;
         });
     else
-        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4][4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) best = __builtin_fmaxf(best, x[i]);
+            for (int i = 0; i < 16; ++i) best = __builtin_fmaxf(best, x[i / 4][i % 4]);
         });
     key = key_of(best);
     index = (uint32_t)at;
@@ -333,28 +347,38 @@ __device__ __forceinline__ void largest(Shared& sh, const void* row, int n, int 
         if (sh.key[w] > key || (sh.key[w] == key && sh.index[w] < index)) key = sh.key[w], index = sh.index[w];
 }
 
+// Keeps a value's computation where it stands: what hides the 64-bit latency is
+// that many go on side by side, not that some are left out.
+__device__ __forceinline__ void here(u64& x) { asm volatile("" : "+v"(x)); }
+
 // The histogram of the groups, into LDS that is zero.
 template <int TYPE, int NT>
 __device__ __forceinline__ void histogram(const Row& p, const void* row, int n, int from, int to, u64* sum, uint32_t* count) {
     if (p.short_list)                        // counts alone
-        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
+        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4][4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int b = p.bin(x[i]);
+            for (int i = 0; i < 16; ++i) {
+                const int b = p.bin(x[i / 4][i % 4]);
                 if (b < kBins) atomicAdd(&count[b], 1u);
             }
         });
     else
-        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4]) {
-            u64 w[4];                        // without branches, so that the four go on side by side
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = Row::count(p.scaled(x[i]));
+        each<TYPE, NT>(row, n, from, to, [&](int, int, const float (&x)[4][4]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int b = p.bin(x[i]);
-                if (b >= kBins) continue;
-                atomicAdd(&sum[b], w[i]);
-                if (p.cut_k) atomicAdd(&count[b], 1u);
+                u64 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = Row::count(p.scaled(x[i][j]));
+                    here(w[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int b = p.bin(x[i][j]);
+                    if (b >= kBins) continue;
+                    atomicAdd(&sum[b], w[j]);
+                    if (p.cut_k) atomicAdd(&count[b], 1u);
+                }
             }
         });
 }
@@ -365,33 +389,41 @@ template <int TYPE, int NT>
 __device__ __forceinline__ void sums_and_list(const Row& p, const Cuts& c, const void* row, int n, int from, int to, u64* group,
                                               Entry* list, uint32_t* listed) {
     const int lane = threadIdx.x & 63, last = c.last();
-    each<TYPE, NT>(row, n, from, to, [&](int g, int e, const float (&x)[4]) {
-        int b[4], least = kBins;
-        bool any = false;
+    each<TYPE, NT>(row, n, from, to, [&](int g, int e, const float (&x)[4][4]) {
+        u64 s = 0;
+        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            b[i] = p.bin(x[i]);
-            least = b[i] < least ? b[i] : least;
-            any |= b[i] >= c.sure && b[i] <= last;
+            int b[4], least = kBins;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                b[j] = p.bin(x[i][j]);
+                least = b[j] < least ? b[j] : least;
+                any |= (uint32_t)(b[j] >= c.sure && b[j] <= last) << (4 * i + j);
+            }
+            if (p.short_list || __builtin_amdgcn_ballot_w64(least < c.sure) == 0) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double y = p.scaled(x[i][j]);
+                u64 w = Row::count(y);
+                here(w);
+                s += b[j] < c.sure && y >= p.least ? w : 0;
+            }
         }
         if (!p.short_list) {
-            u64 s = 0;
-            if (__builtin_amdgcn_ballot_w64(least < c.sure)) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const double y = p.scaled(x[i]);
-                    s += b[i] < c.sure && y >= p.least ? Row::count(y) : 0;
-                }
-                s = wave_sum(s);
-            }
+            if (__builtin_amdgcn_ballot_w64(s != 0)) s = wave_sum(s);
             if (lane == 0) group[g] = s;
         }
-        if (__builtin_amdgcn_ballot_w64(any) == 0) return;
+        while (any) {                        // few
+            const int i = __builtin_ctz(any);
+            any &= any - 1;
+            float y = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (b[i] < c.sure || b[i] > last || !c.listed(b[i])) continue;
+            for (int o = 0; o < 16; ++o) y = o == i ? x[o / 4][o % 4] : y;
+            const int b = p.bin(y);
+            if (!c.listed(b)) continue;
             const uint32_t at = atomicAdd(listed, 1u);
-            if (at < kList) list[at] = Entry{place_of(key_of(x[i]), e + i), Row::count(p.scaled(x[i])) | (u64)b[i] << 48};
+            if (at < kList) list[at] = Entry{place_of(key_of(y), e + i / 4 * 256 + i % 4), Row::count(p.scaled(y)) | (u64)b << 48};
         }
     });
 }
@@ -516,28 +548,35 @@ __device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r,
     target = target < all ? target : all - 1;
     search<NT>(sh, groups, target, [&](int i) { return group[i]; });
     if (threadIdx.x >= 64) return;
-    const int e = (int)sh.found * kGroup + 4 * lane;
-    float y[4];
-    load_end<TYPE>(row, e, n, y);
-    u64 w[4], mine = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int b = p.bin(y[i]);
-        w[i] = b < sure || (b < kBins && place_of(key_of(y[i]), e + i) <= to) ? p.kept(p.scaled(y[i])) : 0;
-        mine += w[i];
-    }
     u64 left = target - sh.before;
-    const u64 upto = wave_scan(mine, lane);
-    u64 base = upto - mine;
-    if (base <= left && left < upto) {
+    float y[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load_end<TYPE>(row, (int)sh.found * kGroup + 256 * q + 4 * lane, n, y[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int e = (int)sh.found * kGroup + 256 * q + 4 * lane;
+        u64 w[4], mine = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (base <= left && left < base + w[i]) {
-                a.tokens[r] = e + i;
-                if (a.probs) a.probs[r] = (float)((double)w[i] / (double)all);
-            }
-            base += w[i];
+            const int b = p.bin(y[q][i]);
+            w[i] = b < sure || (b < kBins && place_of(key_of(y[q][i]), e + i) <= to) ? p.kept(p.scaled(y[q][i])) : 0;
+            mine += w[i];
         }
+        const u64 upto = wave_scan(mine, lane);
+        u64 base = upto - mine;
+        if (base <= left && left < upto) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (base <= left && left < base + w[i]) {
+                    a.tokens[r] = e + i;
+                    if (a.probs) a.probs[r] = (float)((double)w[i] / (double)all);
+                }
+                base += w[i];
+            }
+        }
+        const u64 whole = __shfl(upto, 63);
+        if (left < whole) return;
+        left -= whole;
     }
 }
 
@@ -558,13 +597,14 @@ __device__ __forceinline__ u64 border(Shared& sh, Finish& f, const Row& p, const
         __syncthreads();
         for (int i = threadIdx.x; i < 256; i += NT) f.dsum[i] = 0, f.dcount[i] = 0;
         __syncthreads();
-        each<TYPE, NT, 1>(row, n, 0, groups, [&](int, int, const float (&x)[4]) {
+        each<TYPE, NT>(row, n, 0, groups, [&](int, int, const float (&x)[4][4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t k = key_of(x[i]);
-                if (p.bin(x[i]) != bin || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
+            for (int i = 0; i < 16; ++i) {
+                const float y = x[i / 4][i % 4];
+                const uint32_t k = key_of(y);
+                if (p.bin(y) != bin || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
                 const int digit = 255 - (int)(k >> shift & 255);
-                atomicAdd(&f.dsum[digit], Row::count(p.scaled(x[i])));
+                atomicAdd(&f.dsum[digit], Row::count(p.scaled(y)));
                 atomicAdd(&f.dcount[digit], 1u);
             }
         });
@@ -580,28 +620,33 @@ __device__ __forceinline__ u64 border(Shared& sh, Finish& f, const Row& p, const
     const u64 extra = (by_count ? target : target / w) + 1;
     upto += extra * w;
     __syncthreads();
-    each<TYPE, NT, 1>(row, n, 0, groups, [&](int g, int, const float (&x)[4]) {
+    each<TYPE, NT>(row, n, 0, groups, [&](int g, int, const float (&x)[4][4]) {
         u64 c = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_of(x[i]) == prefix));
+        for (int i = 0; i < 16; ++i) c += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key_of(x[i / 4][i % 4]) == prefix));
         if (lane == 0) f.group[g] = c;
     });
     __syncthreads();
     search<NT>(sh, groups, extra - 1, [&](int i) { return f.group[i]; });
     if (wave == 0) {
+        u64 base = 0;
         const u64 left = extra - 1 - sh.before;                      // equal ones of the group before the last
-        const int e = (int)sh.found * kGroup + 4 * lane;
-        float x[4];
-        load_end<TYPE>(row, e, n, x);
-        u64 mine = 0;
+        for (int q = 0; q < 4; ++q) {
+            const int e = (int)sh.found * kGroup + 256 * q + 4 * lane;
+            float x[4];
+            load_end<TYPE>(row, e, n, x);
+            u64 mine = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine += key_of(x[i]) == prefix;
-        u64 base = wave_scan(mine, lane) - mine;
+            for (int i = 0; i < 4; ++i) mine += key_of(x[i]) == prefix;
+            const u64 upto = wave_scan(mine, lane);
+            u64 at = base + upto - mine;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (key_of(x[i]) != prefix) continue;
-            if (base == left) sh.at = place_of(prefix, e + i);
-            ++base;
+            for (int i = 0; i < 4; ++i) {
+                if (key_of(x[i]) != prefix) continue;
+                if (at == left) sh.at = place_of(prefix, e + i);
+                ++at;
+            }
+            base += __shfl(upto, 63);
         }
     }
     __syncthreads();
@@ -629,11 +674,13 @@ __device__ __forceinline__ void long_way(Shared& sh, Finish& f, const SampleArgs
     }
     if (p.cut_p) to = border<TYPE, NT>(sh, f, p, row, n, false, p.wanted(all) - 1, upto);
     __syncthreads();
-    each<TYPE, NT, 1>(row, n, 0, groups, [&](int g, int e, const float (&x)[4]) {
+    each<TYPE, NT>(row, n, 0, groups, [&](int g, int e, const float (&x)[4][4]) {
         u64 s = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p.bin(x[i]) < kBins && place_of(key_of(x[i]), e + i) <= to) s += p.kept(p.scaled(x[i]));
+        for (int i = 0; i < 16; ++i) {
+            const float y = x[i / 4][i % 4];
+            if (p.bin(y) < kBins && place_of(key_of(y), e + i / 4 * 256 + i % 4) <= to) s += p.kept(p.scaled(y));
+        }
         s = wave_sum(s);
         if (lane == 0) f.group[g] = s;
     });
@@ -864,7 +911,7 @@ void plan_sample(SampleArgs* a) {
     a->frac = 62 - bits < kFrac ? 62 - bits : kFrac;         // the sum of a row stays below 2^62
     const int64_t groups = (a->vocab + kGroup - 1) / kGroup;
     int64_t s = a->rows >= 128 ? 1 : 768 / (a->rows ? a->rows : 1);
-    s = s < groups / 8 ? s : groups / 8;                     // two groups a wave at least
+    s = s < (groups + 3) / 4 ? s : (groups + 3) / 4;         // a group a wave
     s = s < 64 ? s : 64;
     a->slices = s > 1 ? (int)s : 1;
 }
