@@ -35,7 +35,7 @@ constexpr int kGroup = 1024;                 // logits a wave takes at a time, f
 constexpr int kGroups = 1024;                // of a row, at most
 constexpr int kList = 2048;                  // logits that are listed
 constexpr int kShort = 1024;                 // top_k up to which all that stay are listed, and a bin more
-constexpr int kRowThreads = 1024, kSliceThreads = 256;
+constexpr int kRowThreads = 1024, kSliceThreads = 256, kPickThreads = 512;
 constexpr float kInf = __builtin_inff();
 using u64 = unsigned long long;
 
@@ -187,6 +187,7 @@ __device__ __forceinline__ u64 group_sum(Shared& sh, u64 x) {
     if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = x;
     __syncthreads();
     x = 0;
+#pragma unroll
     for (int w = 0; w < NT / 64; ++w) x += sh.wave[w];
     return x;
 }
@@ -205,7 +206,8 @@ __device__ __forceinline__ void search(Shared& sh, int n, u64 target, F&& f) {
     if (lane == 63) sh.wave[wave] = upto;
     __syncthreads();
     u64 base = upto - mine;
-    for (int w = 0; w < wave; ++w) base += sh.wave[w];
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) base += w < wave ? sh.wave[w] : 0;
     if (base <= target && target < base + mine) {
         for (int i = 0; i < per && from + i < n; ++i) {
             const u64 x = f(from + i);
@@ -457,12 +459,17 @@ __device__ __forceinline__ u64 resolve(Shared& sh, Finish& f, const Row& p, cons
     int turn = 0;
     for (int k = 2; k <= size; k *= 2)
         for (int j = k / 2; j; j /= 2) {
-            if (j >= NT) {
-                if constexpr (kPer == 2) {
-                    const bool swap = v[0] > v[1];                   // k is the whole: rising
-                    const u64 a = swap ? v[1] : v[0], b = swap ? v[0] : v[1];
-                    v[0] = a, v[1] = b;
-                }
+            if (j >= NT) {                                           // both in one thread
+#pragma unroll
+                for (int d = 1; d < kPer; d *= 2)
+                    if (j == d * NT)
+#pragma unroll
+                        for (int x = 0; x < kPer; ++x) {
+                            if (x & d) continue;
+                            const bool rises = ((x * NT) & k) == 0, swap = (v[x] > v[x | d]) == rises;
+                            const u64 a = swap ? v[x | d] : v[x], b = swap ? v[x] : v[x | d];
+                            v[x] = a, v[x | d] = b;
+                        }
                 continue;
             }
             if (j >= 64) {
@@ -487,15 +494,19 @@ __device__ __forceinline__ u64 resolve(Shared& sh, Finish& f, const Row& p, cons
 #pragma unroll
     for (int x = 0; x < kPer; ++x) {
         const int i = x * NT + t;
-        mine[x] = i < many ? f.list[v[x] & (kList - 1)] : Entry{~(u64)0, 0};
+        mine[x] = Entry{~(u64)0, 0};
+        upto[x] = 0;
+        if (x * NT >= size) continue;
+        if (i < many) mine[x] = f.list[v[x] & (kList - 1)];
         first += (u64)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < many && mine[x].bin() != c.k_bin));
         upto[x] = wave_scan(mine[x].w(), lane);
         __syncthreads();
         if (lane == 63) sh.wave[wave] = upto[x];
         __syncthreads();
         u64 base = whole;
+#pragma unroll
         for (int w = 0; w < NT / 64; ++w) {
-            if (w < wave) base += sh.wave[w];
+            base += w < wave ? sh.wave[w] : 0;
             whole += sh.wave[w];
         }
         upto[x] += base;
@@ -537,13 +548,13 @@ __device__ __forceinline__ u64 resolve(Shared& sh, Finish& f, const Row& p, cons
 // The draw from the groups' sums: what stays are bins below `sure` and places up
 // to `to`. The whole workgroup calls.
 template <int TYPE, int NT>
-__device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r, const Row& p, int sure, u64 to, const void* row,
+__device__ __forceinline__ void draw(Shared& sh, const SampleArgs& a, int64_t r, float number, const Row& p, int sure, u64 to, const void* row,
                                      const u64* group) {
     const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, lane = threadIdx.x & 63;
     u64 all = 0;
     for (int i = threadIdx.x; i < groups; i += NT) all += group[i];
     all = group_sum<NT>(sh, all);
-    const double u = a.u[r], x = u > 0.0 ? u * (double)all : 0.0;
+    const double u = number, x = u > 0.0 ? u * (double)all : 0.0;
     u64 target = x < (double)all ? (u64)x : all - 1;
     target = target < all ? target : all - 1;
     search<NT>(sh, groups, target, [&](int i) { return group[i]; });
@@ -656,7 +667,7 @@ __device__ __forceinline__ u64 border(Shared& sh, Finish& f, const Row& p, const
 }
 
 template <int TYPE, int NT>
-__device__ __forceinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, Row p, const void* row) {
+__device__ __forceinline__ void long_way(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, float u, Row p, const void* row) {
     const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, lane = threadIdx.x & 63;
     p.short_list = false;                    // weights of all bins
     __syncthreads();
@@ -685,21 +696,21 @@ __device__ __forceinline__ void long_way(Shared& sh, Finish& f, const SampleArgs
         if (lane == 0) f.group[g] = s;
     });
     __syncthreads();
-    draw<TYPE, NT>(sh, a, r, p, 0, to, row, f.group);
+    draw<TYPE, NT>(sh, a, r, u, p, 0, to, row, f.group);
 }
 
 // From the list (and, without a short list, the cuts and the groups' sums) to
 // the token. The workgroup has met since they were written.
 template <int TYPE, int NT>
-__device__ __forceinline__ void finish(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, const Row& p, const Cuts& c, const void* row) {
+__device__ __forceinline__ void finish(Shared& sh, Finish& f, const SampleArgs& a, int64_t r, float u, const Row& p, const Cuts& c, const void* row) {
     const int n = (int)a.vocab, groups = (n + kGroup - 1) / kGroup, many = (int)f.listed;
-    if (many > kList) return long_way<TYPE, NT>(sh, f, a, r, p, row);
+    if (many > kList) return long_way<TYPE, NT>(sh, f, a, r, u, p, row);
     if (p.short_list) {                      // resolve meets before it adds
         for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = 0;
     }
     const u64 to = many ? resolve<NT>(sh, f, p, c, many) : 0;
     __syncthreads();
-    draw<TYPE, NT>(sh, a, r, p, c.sure, to, row, f.group);
+    draw<TYPE, NT>(sh, a, r, u, p, c.sure, to, row, f.group);
 }
 
 __device__ __forceinline__ void take(const SampleArgs& a, int64_t r, uint32_t key, uint32_t index) {
@@ -741,9 +752,10 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
         else
             c.find<NT>(sh, p, f.sum, f.count);
     }
+    const float u = a.u[r];
     sums_and_list<TYPE, NT>(p, c, row, n, 0, groups, f.group, f.list, &f.listed);
     __syncthreads();
-    finish<TYPE, NT>(sh, f, a, r, p, c, row);
+    finish<TYPE, NT>(sh, f, a, r, u, p, c, row);
 }
 
 // ------------------------------------------------------ a row in slices
@@ -848,35 +860,40 @@ __global__ void __launch_bounds__(kSliceThreads) sample_list_kernel(SampleArgs a
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kRowThreads) sample_pick_kernel(SampleArgs a) {
-    constexpr int NT = kRowThreads;
+__global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(SampleArgs a) {
+    constexpr int NT = kPickThreads;
     __shared__ Shared sh;
     __shared__ Finish f;
     const int64_t r = blockIdx.x;
     const Held* h = static_cast<const Held*>(a.scratch) + r;
+    const int groups = (int)((a.vocab + kGroup - 1) / kGroup);
+    // all that does not hang on what another read says is asked for at once
+    const float u = a.u[r];
+    const uint32_t listed = h->listed;
+    const Entry e0 = h->list[threadIdx.x];
+    const u64 g0 = h->group[threadIdx.x];
     Row p;
     p.read(a, r);
     uint32_t key, index;
     largest_of(a, h, key, index);
     if (key == 0 || p.greedy) return take(a, r, key, index);
     p.largest_is(key);
-    const int groups = (int)((a.vocab + kGroup - 1) / kGroup);
-    const uint32_t listed = h->listed;
     if (threadIdx.x == 0) f.listed = listed;
-    for (int i = threadIdx.x; i < (int)(listed < kList ? listed : kList); i += NT) f.list[i] = h->list[i];
+    f.list[threadIdx.x] = e0;
+    for (int i = NT + threadIdx.x; i < (int)(listed < kList ? listed : kList); i += NT) f.list[i] = h->list[i];
     Cuts c;
     c.none();
     if (p.short_list) {                      // the list holds all that may stay
         c.sure = 0, c.p_from = 0, c.p_to = kBins - 1;
-        __syncthreads();
     } else {
         if (p.cut_k || p.cut_p)
             for (int i = threadIdx.x; i < kBins; i += NT) f.sum[i] = h->sum[i], f.count[i] = h->count[i];
-        for (int i = threadIdx.x; i < groups; i += NT) f.group[i] = h->group[i];
-        __syncthreads();
-        if (p.cut_k || p.cut_p) c.find<NT>(sh, p, f.sum, f.count);
+        f.group[threadIdx.x] = g0;
+        for (int i = NT + threadIdx.x; i < groups; i += NT) f.group[i] = h->group[i];
     }
-    finish<TYPE, NT>(sh, f, a, r, p, c, row_of<TYPE>(a, r));
+    __syncthreads();
+    if (!p.short_list && (p.cut_k || p.cut_p)) c.find<NT>(sh, p, f.sum, f.count);
+    finish<TYPE, NT>(sh, f, a, r, u, p, c, row_of<TYPE>(a, r));
 }
 
 template <int TYPE>
@@ -899,7 +916,7 @@ hipError_t launch_typed(const SampleArgs& a, hipStream_t stream) {
         sample_list_kernel<TYPE><<<grid, kSliceThreads, 0, stream>>>(a);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
-    sample_pick_kernel<TYPE><<<(unsigned)a.rows, kRowThreads, 0, stream>>>(a);
+    sample_pick_kernel<TYPE><<<(unsigned)a.rows, kPickThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
