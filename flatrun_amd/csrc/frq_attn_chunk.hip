@@ -468,6 +468,355 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
     }
 }
 
+// ------------------------------------------------------ many rows to a tile
+//
+// W waves of 32 rows each share what is unpacked: 64 tokens at a time, every
+// wave its part (four words of codes a lane, of K or of V), into LDS, in the order
+// of the operands of v_mfma_f32_32x32x16_f16, while the 64 before are worked on.
+using float16v = float __attribute__((ext_vector_type(16)));
+constexpr int kKeys = 64;
+
+// Four words of a tile's K (k < NG / 2) or V codes and their scales, as a lane
+// holds them: of K the words (u, g) of token 16u + n, of V (g, u) of tokens 16u +
+// 4j .. 4j + 3. Word x: K u = (4k + x) / NG, g = (4k + x) % NG; V g = 2v + x / 2, u = x % 2.
+template <int NG>
+struct Unit {
+    uint32_t code[4], scale[8];
+    __device__ __forceinline__ void load(const uint8_t* t, int unit, int lane) {
+        const int n = lane & 15, j = lane >> 4;
+        const bool v = unit >= NG / 2;
+        const int k = v ? unit - NG / 2 : unit;
+        const uint4 x = *reinterpret_cast<const uint4*>(t + (v ? kv_vc_off(NG) : 0) + kv_word(4 * k, lane));
+        code[0] = x.x; code[1] = x.y; code[2] = x.z; code[3] = x.w;
+        if (v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)            // groups 2k and 2k + 1
+                    scale[2 * i + u] = *reinterpret_cast<const uint32_t*>(t + kv_vs_off(NG) + kv_scale(4 * j + i + 16 * u, 2 * k, NG));
+        } else {
+#pragma unroll
+            for (int x2 = 0; x2 < 2; ++x2) {           // words 2 x2 and 2 x2 + 1
+                const int w = 4 * k + 2 * x2;
+                scale[x2] = *reinterpret_cast<const uint32_t*>(t + kv_ks_off(NG) + kv_scale(n + 16 * (w / NG), w % NG, NG));
+            }
+        }
+    }
+    __device__ __forceinline__ bool large(bool v) const {            // beyond 8188, an inf or a NaN
+        us2 x = __builtin_bit_cast(us2, scale[0] & 0x7FFF7FFFu);
+        x = __builtin_elementwise_max(x, __builtin_bit_cast(us2, scale[1] & 0x7FFF7FFFu));
+        if (v)
+#pragma unroll
+            for (int i = 2; i < 8; ++i) x = __builtin_elementwise_max(x, __builtin_bit_cast(us2, scale[i] & 0x7FFF7FFFu));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(x, (us2){0x6FFF, 0x6FFF})) != 0;
+    }
+};
+
+template <int TYPE, int OUT, int NG, int W>
+__global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : NG == 2 ? 3 : 2) attn_chunk_rows_kernel(ChunkArgs a) {
+    using T = Val<TYPE>;
+    using O = Val<OUT>;
+    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 32 * W, NK = D / 16, ND = NG;
+    constexpr int kUnits = 2 * NG / W;                               // of a wave and 64 tokens
+    static_assert(kUnits * W == 2 * NG, "every wave has units");
+    constexpr int kBuf = kKeys * D;                                  // halves of K, then of V
+    __shared__ __attribute__((aligned(16))) _Float16 buf0[2 * kBuf], buf1[2 * kBuf];
+    __shared__ int flags[3], sh_bad;                                 // of a step: 1 a large scale, 2 blocks left out
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ln = lane & 31, h = lane >> 5;
+    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
+    uint32_t id = blockIdx.x;
+    const int split = (int)(id % (uint32_t)a.splits);
+    id /= (uint32_t)a.splits;
+    const int kvh = (int)(id % (uint32_t)a.kv_heads);
+    id /= (uint32_t)a.kv_heads;
+    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
+    Span sp;
+    if (!sp.read(a, seq)) return;
+    if (sp.bad) {
+        if (split) return;
+        for (int64_t i = block; i < sp.nq; i += a.blocks) {
+            typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)kvh * group * D;
+            for (int e = threadIdx.x; e < group * D; e += 64 * W) out[e] = O::one(__builtin_nanf(""));
+        }
+        return;
+    }
+    const int row0 = block * kRows, rows = sp.nq * group;
+    if (row0 >= rows) return;
+    const int end = sp.keys(row0 + kRows - 1, group);
+    const int tiles = (end + kKvTile - 1) / kKvTile;
+    const int first = split * (int)a.share;
+    const int last = tiles < first + (int)a.share ? tiles : first + (int)a.share;
+    if (first >= tiles && split) return;
+    const int whole = sp.keys(row0, group);                          // keys below this one every row of the workgroup sees
+    const int wrow = row0 + 32 * wave;                               // the wave's rows
+    const int seen = wrow < rows ? sp.keys(wrow + 31, group) : 0, own = wrow < rows ? sp.keys(wrow, group) : 0;
+
+    const const_ints table = constant(a.table) + (int64_t)seq * a.ld_table;
+    const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
+    const int64_t page_bytes = a.kv_heads * (int64_t)page_tiles * kTile;
+    const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
+    bool bad = false;
+    // past the last tile that one again: its tokens are masked
+    auto page_index = [&](int tile) { return (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36); };
+    auto look_up = [&](int tile) { return table[page_index(tile < last ? tile : last - 1)]; };
+    auto address = [&](int tile, int page) {
+        if ((uint32_t)page >= (uint64_t)a.pages) {
+            bad = true;
+            page = 0;
+        }
+        tile = tile < last ? tile : last - 1;
+        const uint32_t in = (uint32_t)tile - page_index(tile) * page_tiles;
+        return heads + page * page_bytes + (int64_t)in * kTile;
+    };
+    const int half = kUnits * wave / NG;                             // the wave's tile of a step's two
+    Unit<NG> raw[kUnits];
+    auto fetch = [&](const uint8_t* t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < kUnits; ++x) raw[x].load(t, (kUnits * wave + x) % NG, lane);
+    };
+    // the wave's units of the 64 tokens from tile0 on, unpacked into LDS
+    auto unpack = [&](int tile0, _Float16* buf, int* flag, bool small) __attribute__((always_inline)) {
+        const int n = lane & 15, j = lane >> 4;
+#pragma unroll
+        for (int x = 0; x < kUnits; ++x) {
+            const int unit = (kUnits * wave + x) % NG, tile = tile0 + half;
+            const bool v = unit >= NG / 2;
+            const int k = v ? unit - NG / 2 : unit;
+            Unit<NG>& r = raw[x];
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(r.large(v)) != 0, 0)) {
+                // as in the kernel above: what is behind the end, and in V what
+                // is no number where rows differ in what they see, becomes zero
+                const bool masked = tile0 * kKvTile + kKeys > whole;
+                bool any = false, big = false;
+                auto clean = [&](uint32_t& w, int token, int hi) {
+                    const uint32_t s = (hi ? w >> 16 : w) & 0x7FFFu;
+                    const bool past_end = token >= sp.len, no = s >= 0x7C00;
+                    big |= s > 0x6FFF && !past_end && !no;
+                    any |= v && no && masked && !past_end;
+                    if (past_end || (v && no && masked)) w &= hi ? 0xFFFFu : 0xFFFF0000u;
+                };
+                const int t0 = tile * kKvTile;
+                if (v) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + 4 * j + i / 2 + 16 * (i & 1), hi);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + n + 16 * ((4 * k + 2 * i + hi) / NG), hi);
+                }
+                const int f = (__builtin_amdgcn_ballot_w64(big) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(any) ? 2 : 0);
+                if (f && lane == 0) atomicOr(flag, f);
+            }
+            if (small) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r.scale[i] = bits_of(pair_of(r.scale[i]) * (half2v){0.125f16, 0.125f16});
+            }
+            if (v) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {                        // group g, tokens 16u + 4j + i
+                    const int g = 2 * k + w / 2, u = w & 1, hi = w / 2;
+                    const half2v d0 = halves(r.scale[u], r.scale[2 + u], hi), d1 = halves(r.scale[4 + u], r.scale[6 + u], hi);
+                    const uint32_t c = r.code[w];
+                    // operand of group g and tokens 32 half + 16u ..: lane 32 (j & 1) + channel, its four tokens j / 2
+                    half2v* to = reinterpret_cast<half2v*>(buf + kBuf + ((g * 4 + 2 * half + u) * 64 + 32 * (j & 1) + n) * 8 + 4 * (j >> 1));
+                    to[0] = low_pair(c) * d0;
+                    to[1] = low_pair(c >> 8) * d1;
+                    half2v* to2 = to + 16 * 4;                       // 16 channels on
+                    to2[0] = high_pair(c) * d0;
+                    to2[1] = high_pair(c >> 8) * d1;
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {                        // token 16u + n, channels 32g + 8j ..
+                    const int p = 4 * k + w, u = p / NG, g = p % NG;
+                    const half2v d = halves(r.scale[w / 2], r.scale[w / 2], w & 1);
+                    const uint32_t c = r.code[w];
+                    *reinterpret_cast<half8v*>(buf + ((4 * g + j) * kKeys + 32 * half + 16 * u + n) * 8) =
+                        join(low_pair(c) * d, high_pair(c) * d, low_pair(c >> 8) * d, high_pair(c >> 8) * d);
+                }
+            }
+        }
+    };
+    if (threadIdx.x == 0) flags[0] = flags[1] = flags[2] = sh_bad = 0;
+    int page = 0;                                                    // looked up a step before its tile is asked for
+    if (first < last) {
+        fetch(address(first + half, look_up(first + half)));
+        page = look_up(first + 2 + half);
+    }
+
+    // the lane's row
+    int row = wrow + ln;
+    row = row < rows ? row : rows - 1;
+    const int qi = row / group, head = kvh * group + row - qi * group, lim = sp.past + qi;
+    half8v qf[NK];
+    float rs;
+    {
+        const typename T::Elem* q = static_cast<const typename T::Elem*>(a.q) + (sp.q0 + qi) * a.ld_q + (int64_t)head * D;
+        float x[NK][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) T::load8(q + 16 * s + 8 * h, x[s]);
+#pragma unroll
+        for (int s = 0; s < NK; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t b = __builtin_bit_cast(uint32_t, x[s][e]) & 0x7FFFFFFFu;
+                top = top > b ? top : b;
+            }
+        const uint32_t other = __shfl_xor(top, 32);
+        top = top > other ? top : other;
+        const int up = top ? 140 - (int)(top >> 23) : 0;
+#pragma unroll
+        for (int s = 0; s < NK; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qf[s][e] = (_Float16)__builtin_ldexpf(x[s][e], up);
+        rs = top >= 0x7F800000u ? __builtin_nanf("") : __builtin_ldexpf(a.scale * kLog2e, -up);
+    }
+    float16v o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -kInf, nref = 0.f, l = 0.f;
+
+    __syncthreads();
+    if (first < last) {
+        unpack(first, buf0, &flags[0], false);
+        fetch(address(first + 2 + half, page));
+        page = look_up(first + 4 + half);
+    }
+    int at = 0;                                                      // of this step's flags
+    auto step = [&](int tile, _Float16* cur, _Float16* next) __attribute__((always_inline)) {
+        __syncthreads();                                             // this buffer is there, and everyone is done with the other
+        float up = 1.f, down = 1.f, under = kUnder;
+        const int f = flags[at], next_at = at == 2 ? 0 : at + 1;
+        if (threadIdx.x == 0) flags[next_at == 2 ? 0 : next_at + 1] = 0;    // the last step's: everyone has read them
+        if (__builtin_expect(f & 1, 0)) {                            // once more, at an eighth
+            fetch(address(tile + half, look_up(tile + half)));
+            unpack(tile, cur, &flags[at], true);
+            fetch(address(tile + 2 + half, look_up(tile + 2 + half)));
+            __syncthreads();
+            up = 8.f;
+            down = 0.125f;
+            under = kUnder + 3.f;
+        }
+        if (tile + 2 < last) {
+            unpack(tile + 2, next, &flags[next_at], false);
+            fetch(address(tile + 4 + half, page));
+            page = look_up(tile + 6 + half);
+        }
+        at = next_at;
+        const int kt = tile * kKvTile;
+        if (kt >= seen) return;                                      // nothing here for the wave
+        float16v st[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < NK; ++s)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const half8v kf = *reinterpret_cast<const half8v*>(cur + ((2 * s + h) * kKeys + 32 * t + ln) * 8);
+                st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[t], 0, 0, 0);
+            }
+        const float by = rs * up;
+        if (__builtin_expect(kt + kKeys > own || kt + kKeys > last * kKvTile, 0)) {
+            // of the split's own tiles, what the row sees
+            const int e = last * kKvTile - 1, left = (lim < e ? lim : e) - kt - 4 * h;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * t + 8 * (i >> 2) + (i & 3) > left) st[t][i] = -kInf;
+        }
+        float top = st[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, st[t][i]);
+        top *= by;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + kLag) != 0, 0)) {
+            const float all = __builtin_fmaxf(top, __shfl_xor(top, 32)), mn = all > m + kLag ? all : m;
+            const float keep = mn == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            nref = mn == -kInf ? 0.f : -mn;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= keep;
+        }
+        half8v pf[4];
+        float sum = 0.f;
+        const float ref = nref + under;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            half2v p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + 2 * e], by, ref));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + 2 * e + 1], by, ref));
+                p[e] = half2v{(_Float16)p0, (_Float16)p1};
+                sum = __builtin_amdgcn_fdot2(p[e], (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
+            }
+            pf[s] = join(p[0], p[1], p[2], p[3]);
+        }
+        l = __builtin_fmaf(sum, down, l);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const half8v vf = *reinterpret_cast<const half8v*>(cur + kBuf + ((d * 4 + s) * 64 + lane) * 8);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[s], o[d], 0, 0, 0);
+            }
+        if (__builtin_expect(f & 2, 0)) {
+            for (int t = 0; t < kKeys && kt + t < sp.len && tile + t / kKvTile < last; ++t) {
+                const uint8_t* there = address(tile + t / kKvTile, look_up(tile + t / kKvTile));
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint16_t b = *reinterpret_cast<const uint16_t*>(there + kv_vs_off(NG) + kv_scale(t % kKvTile, g, NG));
+                    if ((b & 0x7C00) == 0x7C00 && kt + t <= lim) o[g] += __builtin_nanf("");
+                }
+            }
+        }
+    };
+    for (int tile = first; tile < last; tile += 4) {
+        step(tile, buf0, buf1);
+        if (tile + 2 < last) step(tile + 2, buf1, buf0);
+    }
+    if (bad) sh_bad = 1;
+    __syncthreads();
+    if (sh_bad) l = __builtin_nanf("");
+    l += __shfl_xor(l, 32);
+    if (wrow + ln >= rows) return;
+    if (a.splits > 1) {
+        float* part = a.part + (((int64_t)(seq * a.kv_heads + kvh) * a.blocks + block) * a.splits + split) * kRows * (D + 4) +
+                      (32 * wave + ln) * (D + 4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4v*>(part + 32 * d + 2 * i + 4 * h) = float4v{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (h == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+        return;
+    }
+    const float inv = 1.0f / l;
+    typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + qi) * a.ld_out + (int64_t)head * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {                            // columns 32 d + 2 i + 4 h and the next three
+            typename O::Elem y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = O::one(lim < 0 ? 0.f : l == 0.f ? __builtin_nanf("") : o[d][i + e] * inv);
+            __builtin_memcpy(__builtin_assume_aligned(out + 32 * d + 2 * i + 4 * h, 4 * sizeof(y[0])), y, sizeof(y));
+        }
+}
+
 // A row's parts of all splits, joined in their order, four columns a thread. A
 // workgroup has D / 4 threads for each of its rows (few splits), or eight (of
 // 128) such sets on the splits of one row, which meet in LDS.
@@ -539,14 +888,19 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(ChunkArgs a, int k
 
 template <int TYPE, int OUT, int NG, int R>
 hipError_t launch_one(const ChunkArgs& a, hipStream_t stream) {
+    constexpr int kW = NG == 4 ? 8 : 4, kRows = R ? 16 * R : 32 * kW;    // R 0: many rows to a tile
     const int64_t units = a.seqs * a.kv_heads * a.blocks;
-    attn_chunk_kernel<TYPE, OUT, NG, R><<<(unsigned)(units * a.splits), 64 * kWaves, 0, stream>>>(a);
+    const unsigned grid = (unsigned)(units * a.splits);
+    if constexpr (R == 0)
+        attn_chunk_rows_kernel<TYPE, OUT, NG, kW><<<grid, 64 * kW, 0, stream>>>(a);
+    else
+        attn_chunk_kernel<TYPE, OUT, NG, R><<<grid, 64 * kWaves, 0, stream>>>(a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
     constexpr int kSets = 256 / (8 * NG);
     if (a.splits > 8)
-        attn_chunk_join_kernel<OUT, NG, true><<<(unsigned)(units * 16 * R), 256, 0, stream>>>(a, 16 * R);
+        attn_chunk_join_kernel<OUT, NG, true><<<(unsigned)(units * kRows), 256, 0, stream>>>(a, kRows);
     else
-        attn_chunk_join_kernel<OUT, NG, false><<<(unsigned)(units * ((16 * R + kSets - 1) / kSets)), 256, 0, stream>>>(a, 16 * R);
+        attn_chunk_join_kernel<OUT, NG, false><<<(unsigned)(units * ((kRows + kSets - 1) / kSets)), 256, 0, stream>>>(a, kRows);
     return hipGetLastError();
 }
 
@@ -555,6 +909,7 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
     const auto run = [&](auto ng) {
         constexpr int kN = decltype(ng)::value;
         switch (a.tiles) {
+            case 0: return launch_one<TYPE, OUT, kN, 0>(a, stream);
             case 1: return launch_one<TYPE, OUT, kN, 1>(a, stream);
             case 2: return launch_one<TYPE, OUT, kN, 2>(a, stream);
             default:
@@ -572,18 +927,23 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
 
 }  // namespace
 
+// Rows of a workgroup.
+static int64_t block_rows(const ChunkArgs& a) { return a.tiles ? 16 * a.tiles : a.head_dim == 128 ? 256 : 128; }
+
 bool plan_attn_chunk(ChunkArgs* a) {
     const int64_t rows = a->max_q * (a->q_heads / a->kv_heads), keys = (a->max_len + kKvTile - 1) / kKvTile;
-    a->tiles = rows <= 16 ? 1 : rows <= 32 || a->head_dim == 256 ? 2 : rows <= 48 ? 3 : 4;
-    a->blocks = (rows + 16 * a->tiles - 1) / (16 * a->tiles);
+    a->tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && a->head_dim != 256 ? 3 : rows <= 128 && a->head_dim != 256 ? 4 : 0;
+    const int64_t per = block_rows(*a);
+    a->blocks = (rows + per - 1) / per;
     const int64_t units = a->seqs * a->kv_heads * a->blocks;
-    if (units >= (int64_t)1 << 23) return false;                     // a launch has fewer than 2^32 threads
+    if (units >= (int64_t)1 << 22) return false;                     // a launch has fewer than 2^32 threads
     int64_t splits = units >= 512 ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
     const int64_t most = (keys + 4 * kWaves - 1) / (4 * kWaves);     // four tiles a wave at least
     splits = splits < most ? splits : most;
     splits = splits > 0 ? splits : 1;
     a->share = (keys + splits - 1) / splits;
     a->share = a->share > 0 ? a->share : 1;
+    if (a->tiles == 0) a->share += a->share & 1;                     // 64 tokens a step
     a->splits = (keys + a->share - 1) / a->share;
     a->splits = a->splits > 0 ? a->splits : 1;
     a->per_page = ((uint64_t)1 << 36) / ((uint64_t)a->page_tokens / kKvTile) + 1;
@@ -592,7 +952,7 @@ bool plan_attn_chunk(ChunkArgs* a) {
 
 size_t attn_chunk_scratch(const ChunkArgs& a) {
     if (a.splits == 1) return 0;
-    return sizeof(float) * (size_t)(a.seqs * a.kv_heads * a.blocks * a.splits * 16 * a.tiles) * (size_t)(a.head_dim + 4);
+    return sizeof(float) * (size_t)(a.seqs * a.kv_heads * a.blocks * a.splits * block_rows(a)) * (size_t)(a.head_dim + 4);
 }
 
 hipError_t launch_attn_chunk(ChunkArgs a, float* scratch, hipStream_t stream) {

@@ -147,11 +147,11 @@ def test_a_dominant_token_among_many_small_ones(frq):
 
 def test_scores_that_grow_along_the_keys(frq):
     """The reference moves in every tile, by little and by much."""
-    for step in (0.5, 30.0):
+    for step, new in ((0.5, 6), (30.0, 6), (0.5, 200), (30.0, 200)):
         m = 700
         k = torch.zeros((m, 1, 64))
         k[:, 0, 0] = torch.arange(m) // 32 * step
-        s = Setup([6], [m], 2, 1, 64, k=k, seed=3)
+        s = Setup([new], [m], 2, 1, 64, k=k, seed=3)
         s.q[:] = 0
         s.q[:, 0, 0], s.q[:, 1, 0] = 8.0, -8.0
         s.check(s.run(out_dtype="f32"), out_dtype="f32")
@@ -159,10 +159,11 @@ def test_scores_that_grow_along_the_keys(frq):
 
 @pytest.mark.parametrize("size", [1e-6, 1e-3, 1.0, 3e4, 3e5])
 @pytest.mark.parametrize("what", ["k", "v"])
-def test_small_and_large_values(frq, what, size):
+@pytest.mark.parametrize("new,d", [(9, 64), (90, 64), (90, 128), (20, 256)])
+def test_small_and_large_values(frq, what, size, new, d):
     g = torch.Generator().manual_seed(5)
-    x = size * torch.randn((400, 2, 64), generator=g).clamp(-1.7, 1.7)
-    s = Setup([9], [400], 4, 2, 64, seed=4, stale=True, **{what: x})
+    x = size * torch.randn((400, 2, d), generator=g).clamp(-1.7, 1.7)
+    s = Setup([new], [400], 4, 2, d, seed=4, stale=True, **{what: x})
     if what == "k":
         s.q = (s.q.float() / max(size, 1e-3)).to(torch.bfloat16)
     s.check(s.run(out_dtype="f32"), out_dtype="f32")
@@ -175,11 +176,13 @@ def test_small_and_large_queries(frq, size):
     s.check(s.run(out_dtype="f32", scale=0.125 / size), out_dtype="f32", scale=0.125 / size)
 
 
-def test_large_values_beside_ordinary_ones(frq):
+@pytest.mark.parametrize("new", [20, 150])
+@pytest.mark.parametrize("at", [40, 120, 299])
+def test_large_values_beside_ordinary_ones(frq, new, at):
     """A tile with values past fp16: the channels of the others to 2^-21 beside."""
-    s = Setup([20], [100], 2, 1, 128, seed=8)
-    s.v[40, 0, :32] = 4e5
-    s = Setup([20], [100], 2, 1, 128, seed=8, v=s.v)
+    v = Setup([new], [300], 2, 1, 128, seed=8).v
+    v[at, 0, :32] = 4e5
+    s = Setup([new], [300], 2, 1, 128, seed=8, v=v, stale=True)
     s.check(s.run(out_dtype="f32"), out_dtype="f32")
 
 
@@ -205,32 +208,35 @@ def test_no_number_reaches_a_query_that_does_not_see_it(frq, d, hq, new, m, at):
             assert np.array_equal(got[~sees], clean[~sees])
 
 
-def test_no_number_in_a_query_stays_in_its_row(frq):
-    s = Setup([9], [50], 4, 2, 64, seed=2)
+@pytest.mark.parametrize("new", [9, 99])
+def test_no_number_in_a_query_stays_in_its_row(frq, new):
+    s = Setup([new], [150], 4, 2, 64, seed=2)
     want = s.run(out_dtype="f32")
     s.q[3, 1, 5], s.q[7, 2, 0] = NAN, float("inf")
     got = s.run(out_dtype="f32")
-    hit = np.zeros((9, 4), bool)
+    hit = np.zeros((new, 4), bool)
     hit[3, 1] = hit[7, 2] = True
     assert np.isnan(got[hit]).all() and np.array_equal(got[~hit], want[~hit])
 
 
-def test_what_the_device_arrays_must_not_say(frq):
+@pytest.mark.parametrize("more", [0, 200])
+def test_what_the_device_arrays_must_not_say(frq, more):
     """Lengths and pages that are not the call's give NaN, offsets outside nothing; the others stay right."""
-    s = Setup([4, 6, 5], [40, 300, 64], 4, 2, 64, seed=11)
+    n = [4, 6 + more, 5]
+    s = Setup(n, [40, 300, 64], 4, 2, 64, seed=11)
     want = s.run(out_dtype="f32")
-    a, b, c = slice(0, 4), slice(4, 10), slice(10, 15)
-    for kw, hit in ((dict(lens=[40, 301, 64]), b), (dict(max_q=5), b), (dict(lens=[40, 1 << 30, 64]), b),
+    a, b, c = slice(0, 4), slice(4, 10 + more), slice(10 + more, 15 + more)
+    for kw, hit in ((dict(lens=[40, 301, 64]), b), (dict(max_q=5 + more), b), (dict(lens=[40, 1 << 30, 64]), b),
                     (dict(table=np.where(np.arange(3)[:, None] == 2, s.pages, s.table)), c),
                     (dict(table=np.where(np.arange(3)[:, None] == 0, -1, s.table)), a)):
         got = s.run(out_dtype="f32", **kw)
-        miss = np.ones(15, bool)
+        miss = np.ones(15 + more, bool)
         miss[hit] = False
         assert np.isnan(got[hit]).all() and np.array_equal(got[miss], want[miss]), kw
     assert np.all(s.run(out_dtype="f32", lens=[-5, 300, 64])[a] == 0)
-    got = s.run(out_dtype="f32", cu=[0, 4, 10, 99])
-    assert np.all(got[c] == 5) and np.array_equal(got[:10], want[:10])
-    got = s.run(out_dtype="f32", cu=[-3, 4, 10, 15])
+    got = s.run(out_dtype="f32", cu=[0, 4, 10 + more, 999])
+    assert np.all(got[c] == 5) and np.array_equal(got[:10 + more], want[:10 + more])
+    got = s.run(out_dtype="f32", cu=[-3, 4, 10 + more, 15 + more])
     assert np.all(got[a] == 5) and np.array_equal(got[4:], want[4:])
 
 
