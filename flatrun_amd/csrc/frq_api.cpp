@@ -1362,7 +1362,7 @@ int frq_dev_attn_chunk(int type, const void* q, int64_t ld_q, const void* cache,
     if (max_q * (q_heads / kv_heads) >= ((int64_t)1 << 31) - 256)
         return fail(FRQ_ERR_UNSUPPORTED, "attn_chunk: more rows of a key head than 2^31");
     frq::ChunkArgs a{type,   out_type, q,     ld_q,    cache, pages,  page_tokens, kv_heads, head_dim, table, ld_table, lens, cu_q, seqs,
-                     tokens_q, max_q,  max_len, out, ld_out, q_heads, scale,       0,        0,        0,     0,        0,    nullptr};
+                     tokens_q, max_q,  max_len, out, ld_out, q_heads, scale};
     if (!frq::plan_attn_chunk(&a)) return fail(FRQ_ERR_UNSUPPORTED, "attn_chunk: more blocks than a launch takes");
     hipStream_t s = static_cast<hipStream_t>(stream);
     float* part;

@@ -31,6 +31,8 @@ constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnder = 5.f, kLag = 7.f;      // of the weights' powers of two: see the head of the file
 constexpr float kInf = __builtin_inff();
+constexpr int kHeldBlocks = 1000000;                 // blocks of rows from which on keys are unpacked once
+constexpr size_t kHeldMost = (size_t)1 << 30;  // bytes of them
 
 // Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
 // 0x6400 | n is 1024 + n; under the mask 0xF0 it is 1024 + 16 n.
@@ -512,16 +514,134 @@ struct Unit {
     }
 };
 
-template <int TYPE, int OUT, int NG, int W>
-__global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : NG == 2 ? 3 : 2) attn_chunk_rows_kernel(ChunkArgs a) {
+// A unit's values to where the products read them: K and V of 64 tokens, `half`
+// the unit's tile of the two.
+template <int NG>
+__device__ __forceinline__ void put_unit(const Unit<NG>& r, int unit, int half, int lane, _Float16* kb, _Float16* vb) {
+    const int n = lane & 15, j = lane >> 4;
+    if (unit >= NG / 2) {
+        const int k = unit - NG / 2;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {                                // group g, tokens 16u + 4j + i
+            const int g = 2 * k + w / 2, u = w & 1, hi = w / 2;
+            const half2v d0 = halves(r.scale[u], r.scale[2 + u], hi), d1 = halves(r.scale[4 + u], r.scale[6 + u], hi);
+            const uint32_t c = r.code[w];
+            // operand of group g and tokens 32 half + 16u ..: lane 32 (j & 1) + channel, its four tokens j / 2
+            half2v* to = reinterpret_cast<half2v*>(vb + ((g * 4 + 2 * half + u) * 64 + 32 * (j & 1) + n) * 8 + 4 * (j >> 1));
+            const uint2 low = make_uint2(bits_of(low_pair(c) * d0), bits_of(low_pair(c >> 8) * d1));
+            const uint2 high = make_uint2(bits_of(high_pair(c) * d0), bits_of(high_pair(c >> 8) * d1));
+            *reinterpret_cast<uint2*>(to) = low;
+            *reinterpret_cast<uint2*>(to + 16 * 4) = high;           // 16 channels on
+        }
+    } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {                                // token 16u + n, channels 32g + 8j ..
+            const int p = 4 * unit + w, u = p / NG, g = p % NG;
+            const half2v d = halves(r.scale[w / 2], r.scale[w / 2], w & 1);
+            const uint32_t c = r.code[w];
+            *reinterpret_cast<half8v*>(kb + ((4 * g + j) * kKeys + 32 * half + 16 * u + n) * 8) =
+                join(low_pair(c) * d, high_pair(c) * d, low_pair(c >> 8) * d, high_pair(c >> 8) * d);
+        }
+    }
+}
+// What is not ordinary in a unit of tokens t0 ..: behind the sequence's end zeros,
+// and in V, if asked for, in place of what is no number. 1: a large scale is left, 2:
+// no number in V.
+template <int NG>
+__device__ __forceinline__ int clean_unit(Unit<NG>& r, int unit, int t0, int len, bool zero, int lane) {
+    const int n = lane & 15, j = lane >> 4;
+    const bool v = unit >= NG / 2;
+    bool any = false, big = false;
+    auto clean = [&](uint32_t& w, int token, int hi) {
+        const uint32_t s = (hi ? w >> 16 : w) & 0x7FFFu;
+        const bool past_end = token >= len, no = s >= 0x7C00;
+        big |= s > 0x6FFF && !past_end && !no;
+        any |= v && no && !past_end;
+        if (past_end || (v && no && zero)) w &= hi ? 0xFFFFu : 0xFFFF0000u;
+    };
+    if (v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + 4 * j + i / 2 + 16 * (i & 1), hi);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + n + 16 * ((4 * unit + 2 * i + hi) / NG), hi);
+    }
+    return (__builtin_amdgcn_ballot_w64(big) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(any) ? 2 : 0);
+}
+template <int NG>
+__device__ __forceinline__ void eighth(Unit<NG>& r) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.scale[i] = bits_of(pair_of(r.scale[i]) * (half2v){0.125f16, 0.125f16});
+}
+
+// Every key and value of the call unpacked once, 64 tokens of a key head to a
+// workgroup, in the order in which LDS holds them: for chunks of so many rows
+// that unpacking them for each 256 or 128 would be most of the work. A word beside
+// them says what is not ordinary: 1 V at an eighth, 2 no number in V, 4 K at an
+// eighth, 8 a page outside the cache.
+constexpr int unpack_waves(int ng) { return ng == 2 ? 4 : 8; }
+template <int NG>
+__global__ void __launch_bounds__(64 * unpack_waves(NG)) attn_chunk_unpack_kernel(ChunkArgs a) {
+    constexpr int W = unpack_waves(NG), kUnits = 2 * NG / W, kBuf = kKeys * 32 * NG;
+    __shared__ int sh_flags;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t id = blockIdx.x / (uint32_t)a.steps;
+    const int step = (int)(blockIdx.x - id * (uint32_t)a.steps);
+    const int seq = (int)(id / (uint32_t)a.kv_heads), kvh = (int)(id % (uint32_t)a.kv_heads);
+    Span sp;
+    if (!sp.read(a, seq) || sp.bad || step * kKeys >= sp.len) return;
+    const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
+    const int half = kUnits * wave / NG, tiles = (sp.len + kKvTile - 1) / kKvTile, want = 2 * step + half;
+    const int tile = want < tiles ? want : tiles - 1;
+    const uint32_t in = (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36);
+    int page = constant(a.table)[(int64_t)seq * a.ld_table + in];
+    int f = 0;
+    if ((uint32_t)page >= (uint64_t)a.pages) {
+        f = 8;
+        page = 0;
+    }
+    const uint8_t* t = static_cast<const uint8_t*>(a.cache) +
+                       ((page * a.kv_heads + kvh) * (int64_t)page_tiles + ((uint32_t)tile - in * page_tiles)) * kv_tile_bytes(NG);
+    Unit<NG> raw[kUnits];
+#pragma unroll
+    for (int x = 0; x < kUnits; ++x) raw[x].load(t, (kUnits * wave + x) % NG, lane);
+    if (threadIdx.x == 0) sh_flags = 0;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kUnits; ++x) {
+        const int unit = (kUnits * wave + x) % NG;
+        const bool v = unit >= NG / 2;
+        if (__builtin_amdgcn_ballot_w64(raw[x].large(v)) == 0) continue;
+        const int c = clean_unit<NG>(raw[x], unit, want * kKvTile, sp.len, false, lane);
+        f |= v ? c : (c & 1) << 2;
+    }
+    if (f && lane == 0) atomicOr(&sh_flags, f);
+    __syncthreads();
+    f = sh_flags;
+    _Float16* to = static_cast<_Float16*>(a.held) + (int64_t)blockIdx.x * (2 * kBuf);
+#pragma unroll
+    for (int x = 0; x < kUnits; ++x) {
+        const int unit = (kUnits * wave + x) % NG;
+        if (f & (unit >= NG / 2 ? 1 : 4)) eighth<NG>(raw[x]);
+        put_unit<NG>(raw[x], unit, half, lane, to, to + kBuf);
+    }
+    if (threadIdx.x == 0) a.held_flags[blockIdx.x] = f;
+}
+
+template <int TYPE, int OUT, int NG, int W, bool HELD>
+__global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kernel(ChunkArgs a) {
     using T = Val<TYPE>;
     using O = Val<OUT>;
     constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 32 * W, NK = D / 16, ND = NG;
     constexpr int kUnits = 2 * NG / W;                               // of a wave and 64 tokens
     static_assert(kUnits * W == 2 * NG, "every wave has units");
-    constexpr int kBuf = kKeys * D;                                  // halves of K, then of V
-    __shared__ __attribute__((aligned(16))) _Float16 buf0[2 * kBuf], buf1[2 * kBuf];
-    __shared__ int flags[3], sh_bad;                                 // of a step: 1 a large scale, 2 blocks left out
+    constexpr int kBuf = kKeys * D;
+    __shared__ __attribute__((aligned(16))) _Float16 kb0[kBuf], kb1[kBuf], vb0[kBuf], vb1[kBuf];
+    __shared__ int flags[2][3], sh_bad;                              // of a step's K and V: 1 a large scale, 2 blocks left out
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 31, h = lane >> 5;
@@ -576,77 +696,63 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : NG == 2 ? 3 : 2) attn_ch
 #pragma unroll
         for (int x = 0; x < kUnits; ++x) raw[x].load(t, (kUnits * wave + x) % NG, lane);
     };
-    // the wave's units of the 64 tokens from tile0 on, unpacked into LDS
-    auto unpack = [&](int tile0, _Float16* buf, int* flag, bool small) __attribute__((always_inline)) {
-        const int n = lane & 15, j = lane >> 4;
+    // The wave's units, all of K or all of V (but for 256-wide heads, whose waves
+    // have both), of the 64 tokens from tile0 on, unpacked into LDS.
+    auto unpack = [&](int x, int tile0, _Float16* buf, int* flag, bool small) __attribute__((always_inline)) {
+        const int unit = (kUnits * wave + x) % NG;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(raw[x].large(unit >= NG / 2)) != 0, 0)) {
+            // a zero weight does not take a NaN out of a product: where rows
+            // differ in what they see, it leaves V and is added below
+            const int f = clean_unit<NG>(raw[x], unit, (tile0 + half) * kKvTile, sp.len, tile0 * kKvTile + kKeys > whole, lane);
+            if (f && lane == 0) atomicOr(flag, f);
+        }
+        if (small) eighth<NG>(raw[x]);
+        put_unit<NG>(raw[x], unit, half, lane, buf, buf);
+    };
+    auto is_v = [&](int x) { return (kUnits * wave + x) % NG >= NG / 2; };
+    // K of step k into kb, V of step v into vb, and the wave's next ones asked for:
+    // pages are looked up a step before their tile is
+    int pages[2] = {0, 0};
+    constexpr bool kBoth = kUnits == NG;                             // a wave has units of K and of V
+    auto fetch_units = [&](bool v, int tile, int page) __attribute__((always_inline)) {
+        const uint8_t* t = address(tile + half, page);
 #pragma unroll
-        for (int x = 0; x < kUnits; ++x) {
-            const int unit = (kUnits * wave + x) % NG, tile = tile0 + half;
-            const bool v = unit >= NG / 2;
-            const int k = v ? unit - NG / 2 : unit;
-            Unit<NG>& r = raw[x];
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(r.large(v)) != 0, 0)) {
-                // as in the kernel above: what is behind the end, and in V what
-                // is no number where rows differ in what they see, becomes zero
-                const bool masked = tile0 * kKvTile + kKeys > whole;
-                bool any = false, big = false;
-                auto clean = [&](uint32_t& w, int token, int hi) {
-                    const uint32_t s = (hi ? w >> 16 : w) & 0x7FFFu;
-                    const bool past_end = token >= sp.len, no = s >= 0x7C00;
-                    big |= s > 0x6FFF && !past_end && !no;
-                    any |= v && no && masked && !past_end;
-                    if (past_end || (v && no && masked)) w &= hi ? 0xFFFFu : 0xFFFF0000u;
-                };
-                const int t0 = tile * kKvTile;
-                if (v) {
+        for (int x = 0; x < kUnits; ++x)
+            if (is_v(x) == v) raw[x].load(t, (kUnits * wave + x) % NG, lane);
+    };
+    auto unpack_units = [&](bool v, int tile, _Float16* buf, int* flag, bool small) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+        for (int x = 0; x < kUnits; ++x)
+            if (is_v(x) == v) unpack(x, tile, buf, flag, small);
+    };
+    if (threadIdx.x < 6) flags[threadIdx.x / 3][threadIdx.x % 3] = 0;
+    if (threadIdx.x == 6) sh_bad = 0;
+    const bool has_k = !HELD && (kBoth || !is_v(0)), has_v = !HELD && (kBoth || is_v(0));
+    if (!HELD && first < last) {
+        const int now = look_up(first + half);
+        if (has_k) fetch_units(false, first, now);
+        if (has_v) fetch_units(true, first, now);
+        pages[0] = pages[1] = look_up(first + 2 + half);
+    }
+    // HELD: the unpacked steps of the sequence and key head, and their words
+    const int64_t blocks64 = ((int64_t)seq * a.kv_heads + kvh) * a.steps;
+    const _Float16* held = static_cast<const _Float16*>(a.held) + blocks64 * (2 * kBuf);
+    const const_ints words = constant(a.held_flags) + blocks64;
+    // Asynchronous copy of a step's K (or V), as it lies, 16 bytes a lane and turn.
+    auto copy = [&](int tile, bool v, _Float16* to) __attribute__((always_inline)) {
+        constexpr int kTurns = kBuf / 8 / (64 * W);
+        const __amdgpu_buffer_rsrc_t r = buffer_rsrc(held + (int64_t)(tile / 2) * (2 * kBuf) + (v ? kBuf : 0), kBuf * 2);
 #pragma unroll
-                        for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + 4 * j + i / 2 + 16 * (i & 1), hi);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + n + 16 * ((4 * k + 2 * i + hi) / NG), hi);
-                }
-                const int f = (__builtin_amdgcn_ballot_w64(big) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(any) ? 2 : 0);
-                if (f && lane == 0) atomicOr(flag, f);
-            }
-            if (small) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) r.scale[i] = bits_of(pair_of(r.scale[i]) * (half2v){0.125f16, 0.125f16});
-            }
-            if (v) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {                        // group g, tokens 16u + 4j + i
-                    const int g = 2 * k + w / 2, u = w & 1, hi = w / 2;
-                    const half2v d0 = halves(r.scale[u], r.scale[2 + u], hi), d1 = halves(r.scale[4 + u], r.scale[6 + u], hi);
-                    const uint32_t c = r.code[w];
-                    // operand of group g and tokens 32 half + 16u ..: lane 32 (j & 1) + channel, its four tokens j / 2
-                    half2v* to = reinterpret_cast<half2v*>(buf + kBuf + ((g * 4 + 2 * half + u) * 64 + 32 * (j & 1) + n) * 8 + 4 * (j >> 1));
-                    to[0] = low_pair(c) * d0;
-                    to[1] = low_pair(c >> 8) * d1;
-                    half2v* to2 = to + 16 * 4;                       // 16 channels on
-                    to2[0] = high_pair(c) * d0;
-                    to2[1] = high_pair(c >> 8) * d1;
-                }
-            } else {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {                        // token 16u + n, channels 32g + 8j ..
-                    const int p = 4 * k + w, u = p / NG, g = p % NG;
-                    const half2v d = halves(r.scale[w / 2], r.scale[w / 2], w & 1);
-                    const uint32_t c = r.code[w];
-                    *reinterpret_cast<half8v*>(buf + ((4 * g + j) * kKeys + 32 * half + 16 * u + n) * 8) =
-                        join(low_pair(c) * d, high_pair(c) * d, low_pair(c >> 8) * d, high_pair(c >> 8) * d);
-                }
-            }
+        for (int i = 0; i < kTurns; ++i) {
+            const int at16 = (i * W + wave) * 64;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + at16 * 8), 16,
+                                                     (at16 + lane) * 16, 0, 0, 0);
         }
     };
-    if (threadIdx.x == 0) flags[0] = flags[1] = flags[2] = sh_bad = 0;
-    int page = 0;                                                    // looked up a step before its tile is asked for
-    if (first < last) {
-        fetch(address(first + half, look_up(first + half)));
-        page = look_up(first + 2 + half);
+    if (HELD && first < last) {
+        copy(first, false, kb0);
+        copy(first, true, vb0);
+        if (first + 2 < last) copy(first + 2, false, kb1);
     }
 
     // the lane's row
@@ -684,46 +790,130 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : NG == 2 ? 3 : 2) attn_ch
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -kInf, nref = 0.f, l = 0.f;
 
-    __syncthreads();
-    if (first < last) {
-        unpack(first, buf0, &flags[0], false);
-        fetch(address(first + 2 + half, page));
-        page = look_up(first + 4 + half);
-    }
-    int at = 0;                                                      // of this step's flags
-    auto step = [&](int tile, _Float16* cur, _Float16* next) __attribute__((always_inline)) {
-        __syncthreads();                                             // this buffer is there, and everyone is done with the other
-        float up = 1.f, down = 1.f, under = kUnder;
-        const int f = flags[at], next_at = at == 2 ? 0 : at + 1;
-        if (threadIdx.x == 0) flags[next_at == 2 ? 0 : next_at + 1] = 0;    // the last step's: everyone has read them
-        if (__builtin_expect(f & 1, 0)) {                            // once more, at an eighth
-            fetch(address(tile + half, look_up(tile + half)));
-            unpack(tile, cur, &flags[at], true);
-            fetch(address(tile + 2 + half, look_up(tile + 2 + half)));
-            __syncthreads();
-            up = 8.f;
-            down = 0.125f;
-            under = kUnder + 3.f;
-        }
-        if (tile + 2 < last) {
-            unpack(tile + 2, next, &flags[next_at], false);
-            fetch(address(tile + 4 + half, page));
-            page = look_up(tile + 6 + half);
-        }
-        at = next_at;
-        const int kt = tile * kKvTile;
-        if (kt >= seen) return;                                      // nothing here for the wave
-        float16v st[2];
+    auto scores = [&](const _Float16* kb, float16v (&st)[2]) __attribute__((always_inline)) {   // of the first step
 #pragma unroll
         for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.f;
 #pragma unroll
         for (int s = 0; s < NK; ++s)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const half8v kf = *reinterpret_cast<const half8v*>(cur + ((2 * s + h) * kKeys + 32 * t + ln) * 8);
+                const half8v kf = *reinterpret_cast<const half8v*>(kb + ((2 * s + h) * kKeys + 32 * t + ln) * 8);
                 st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[t], 0, 0, 0);
             }
+    };
+    int at = 0;                                                      // this step's flags
+    // once more, at an eighth, where a scale is large
+    auto again = [&](bool v, int tile, _Float16* buf, int* flag) __attribute__((always_inline)) {
+        const int after = tile + 2;
+        if (v ? has_v : has_k) {
+            fetch_units(v, tile, look_up(tile + half));
+            unpack_units(v, tile, buf, flag, true);
+            fetch_units(v, after, look_up(after + half));
+        }
+        __syncthreads();
+    };
+    // the waves meet, and what any of them has copied is there
+    auto meet = [&]() __attribute__((always_inline)) {
+        if constexpr (HELD) {
+            __builtin_amdgcn_s_waitcnt(0x0070);                      // vmcnt(0), lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+        } else {
+            __syncthreads();
+        }
+    };
+    float16v sa[2], sb[2];
+    float up = 1.f;                                                  // of the scores at hand
+    int fv_now = 0;                                                  // HELD: this step's word
+    meet();
+    if (HELD && first < last) {
+        fv_now = words[first / 2];
+        up = fv_now & 4 ? 8.f : 1.f;
+        scores(kb0, sa);
+    }
+    if (!HELD && first < last) {
+        if (has_k) {
+            unpack_units(false, first, kb0, &flags[0][0], false);
+            fetch_units(false, first + 2, pages[0]);
+            pages[0] = look_up(first + 4 + half);
+        }
+        if (has_v) {
+            unpack_units(true, first, vb0, &flags[1][0], false);
+            fetch_units(true, first + 2, pages[1]);
+            pages[1] = look_up(first + 4 + half);
+        }
+        __syncthreads();
+        if (__builtin_expect(flags[0][0] & 1, 0)) {
+            again(false, first, kb0, &flags[0][0]);
+            up = 8.f;
+        }
+        scores(kb0, sa);
+        if (has_k && first + 2 < last) {
+            unpack_units(false, first + 2, kb1, &flags[0][1], false);
+            fetch_units(false, first + 4, pages[0]);
+            pages[0] = look_up(first + 6 + half);
+        }
+    }
+    // Softmax and P V of a step, whose scores st holds, and the scores of the next:
+    // K is a step ahead of V, so that those products go on beside the exponentials.
+    auto step = [&](int tile, float16v (&st)[2], float16v (&sn)[2], _Float16* k_next, _Float16* k_after, _Float16* v_now,
+                    _Float16* v_next) __attribute__((always_inline)) {
+        meet();                                                      // K of the next step and V of this one are there
+        const bool more = tile + 2 < last;
+        int fv;
+        float down = 1.f, under = kUnder, up_next = 1.f;
+        if constexpr (HELD) {
+            fv = fv_now;
+            if (tile + 4 < last) copy(tile + 4, false, k_after);
+            if (more) {
+                copy(tile + 2, true, v_next);
+                fv_now = words[tile / 2 + 1];
+                up_next = fv_now & 4 ? 8.f : 1.f;
+            }
+            bad |= (fv & 8) != 0;
+            if (__builtin_expect((fv & 2) && tile * kKvTile + kKeys > whole, 0)) {
+                // a zero weight does not take a NaN out of a product: it leaves V
+                // and is added below for the rows that see it
+                for (int i = threadIdx.x; i < kBuf / 2; i += 64 * W) {
+                    uint32_t& w = reinterpret_cast<uint32_t*>(v_now)[i];
+                    const uint32_t x = w;
+                    w = x & ~(((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u));
+                }
+                __syncthreads();
+            }
+            if (fv & 1) {
+                down = 0.125f;
+                under = kUnder + 3.f;
+            }
+        } else {
+            const int n1 = at == 2 ? 0 : at + 1, n2 = n1 == 2 ? 0 : n1 + 1;
+            const int fk = flags[0][n1];
+            fv = flags[1][at];
+            if (threadIdx.x == 0) flags[0][at] = flags[1][n2] = 0;   // read for the last time before this barrier
+            if (__builtin_expect(fv & 1, 0)) {
+                again(true, tile, v_now, &flags[1][at]);
+                down = 0.125f;
+                under = kUnder + 3.f;
+            }
+            if (__builtin_expect(more && (fk & 1), 0)) {
+                again(false, tile + 2, k_next, &flags[0][n1]);
+                up_next = 8.f;
+            }
+            if (has_k && tile + 4 < last) {
+                unpack_units(false, tile + 4, k_after, &flags[0][n2], false);
+                fetch_units(false, tile + 6, pages[0]);
+                pages[0] = look_up(tile + 8 + half);
+            }
+            if (has_v && more) {
+                unpack_units(true, tile + 2, v_next, &flags[1][n1], false);
+                fetch_units(true, tile + 4, pages[1]);
+                pages[1] = look_up(tile + 6 + half);
+            }
+            at = n1;
+        }
         const float by = rs * up;
+        up = up_next;
+        const int kt = tile * kKvTile;
+        if (kt >= seen) return;                                      // nothing here for the wave, nor further on
         if (__builtin_expect(kt + kKeys > own || kt + kKeys > last * kKvTile, 0)) {
             // of the split's own tiles, what the row sees
             const int e = last * kKvTile - 1, left = (lim < e ? lim : e) - kt - 4 * h;
@@ -750,30 +940,48 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : NG == 2 ? 3 : 2) attn_ch
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= keep;
         }
-        half8v pf[4];
-        float sum = 0.f;
+        // The next step's scores (of whatever LDS holds, where there is none)
+        // beside this one's exponentials, operands four products ahead.
+        auto k_of = [&](int x) { return *reinterpret_cast<const half8v*>(k_next + ((2 * (x >> 1) + h) * kKeys + 32 * (x & 1) + ln) * 8); };
+        auto v_of = [&](int x) { return *reinterpret_cast<const half8v*>(v_now + ((x % ND * 4 + x / ND) * 64 + lane) * 8); };
+        constexpr int kPer = 16 / NK;                                // of the 32 scores to a product
+        half8v ahead[4];
+        uint32_t pw[16];
+        float sum = 0.f, odd = 0.f;
         const float ref = nref + under;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            half2v p[4];
+        for (int x = 0; x < 4; ++x) ahead[x] = k_of(x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + 2 * e], by, ref));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + 2 * e + 1], by, ref));
-                p[e] = half2v{(_Float16)p0, (_Float16)p1};
-                sum = __builtin_amdgcn_fdot2(p[e], (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
+        for (int i = 0; i < 16; ++i) sn[0][i] = sn[1][i] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 2 * NK; ++x) {
+            sn[x & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[x & 3], qf[x >> 1], sn[x & 1], 0, 0, 0);
+            ahead[x & 3] = x + 4 < 2 * NK ? k_of(x + 4) : v_of(x + 4 - 2 * NK);
+#pragma unroll
+            for (int y = 0; y < kPer; ++y) {
+                const int i = x * kPer + y;
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i >> 4][i & 15], by, ref));
+                if (i & 1) {
+                    const half2v w = {(_Float16)odd, (_Float16)p};
+                    pw[i / 2] = bits_of(w);
+                    sum = __builtin_amdgcn_fdot2(w, (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
+                } else {
+                    odd = p;
+                }
             }
-            pf[s] = join(p[0], p[1], p[2], p[3]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         l = __builtin_fmaf(sum, down, l);
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const half8v vf = *reinterpret_cast<const half8v*>(cur + kBuf + ((d * 4 + s) * 64 + lane) * 8);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[s], o[d], 0, 0, 0);
-            }
-        if (__builtin_expect(f & 2, 0)) {
+        for (int x = 0; x < 4 * ND; ++x) {
+            const int s = x / ND, d = x % ND;
+            const half8v pf = join(pair_of(pw[4 * s]), pair_of(pw[4 * s + 1]), pair_of(pw[4 * s + 2]), pair_of(pw[4 * s + 3]));
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[x & 3], pf, o[d], 0, 0, 0);
+            if (x + 4 < 4 * ND) ahead[x & 3] = v_of(x + 4);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_expect(fv & 2, 0)) {
             for (int t = 0; t < kKeys && kt + t < sp.len && tile + t / kKvTile < last; ++t) {
                 const uint8_t* there = address(tile + t / kKvTile, look_up(tile + t / kKvTile));
 #pragma unroll
@@ -785,8 +993,8 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : NG == 2 ? 3 : 2) attn_ch
         }
     };
     for (int tile = first; tile < last; tile += 4) {
-        step(tile, buf0, buf1);
-        if (tile + 2 < last) step(tile + 2, buf1, buf0);
+        step(tile, sa, sb, kb1, kb0, vb0, vb1);
+        if (tile + 2 < last) step(tile + 2, sb, sa, kb0, kb1, vb1, vb0);
     }
     if (bad) sh_bad = 1;
     __syncthreads();
@@ -886,15 +1094,22 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(ChunkArgs a, int k
     __builtin_memcpy(__builtin_assume_aligned(out + 4 * col, 4 * sizeof(y[0])), y, sizeof(y));
 }
 
+// R: column tiles of a workgroup, 0 for many rows to a tile, -1 for those of
+// unpacked keys.
 template <int TYPE, int OUT, int NG, int R>
 hipError_t launch_one(const ChunkArgs& a, hipStream_t stream) {
-    constexpr int kW = NG == 4 ? 8 : 4, kRows = R ? 16 * R : 32 * kW;    // R 0: many rows to a tile
+    constexpr int kW = NG == 4 ? 8 : 4, kRows = R > 0 ? 16 * R : 32 * kW;
     const int64_t units = a.seqs * a.kv_heads * a.blocks;
     const unsigned grid = (unsigned)(units * a.splits);
-    if constexpr (R == 0)
-        attn_chunk_rows_kernel<TYPE, OUT, NG, kW><<<grid, 64 * kW, 0, stream>>>(a);
-    else
+    if constexpr (R > 0) {
         attn_chunk_kernel<TYPE, OUT, NG, R><<<grid, 64 * kWaves, 0, stream>>>(a);
+    } else if constexpr (R == 0) {
+        attn_chunk_rows_kernel<TYPE, OUT, NG, kW, false><<<grid, 64 * kW, 0, stream>>>(a);
+    } else {
+        attn_chunk_unpack_kernel<NG><<<(unsigned)(a.seqs * a.kv_heads * a.steps), 64 * unpack_waves(NG), 0, stream>>>(a);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        attn_chunk_rows_kernel<TYPE, OUT, NG, kW, true><<<grid, 64 * kW, 0, stream>>>(a);
+    }
     if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
     constexpr int kSets = 256 / (8 * NG);
     if (a.splits > 8)
@@ -909,6 +1124,7 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
     const auto run = [&](auto ng) {
         constexpr int kN = decltype(ng)::value;
         switch (a.tiles) {
+            case -1: return launch_one<TYPE, OUT, kN, -1>(a, stream);
             case 0: return launch_one<TYPE, OUT, kN, 0>(a, stream);
             case 1: return launch_one<TYPE, OUT, kN, 1>(a, stream);
             case 2: return launch_one<TYPE, OUT, kN, 2>(a, stream);
@@ -928,22 +1144,35 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
 }  // namespace
 
 // Rows of a workgroup.
-static int64_t block_rows(const ChunkArgs& a) { return a.tiles ? 16 * a.tiles : a.head_dim == 128 ? 256 : 128; }
+static int64_t block_rows(const ChunkArgs& a) { return a.tiles > 0 ? 16 * a.tiles : a.head_dim == 128 ? 256 : 128; }
+
+static size_t part_bytes(const ChunkArgs& a) {
+    if (a.splits == 1) return 0;
+    return sizeof(float) * (size_t)(a.seqs * a.kv_heads * a.blocks * a.splits * block_rows(a)) * (size_t)(a.head_dim + 4);
+}
+static size_t held_bytes(const ChunkArgs& a) {
+    return a.tiles < 0 ? (size_t)(a.seqs * a.kv_heads * a.steps) * (size_t)(256 * a.head_dim) : 0;
+}
 
 bool plan_attn_chunk(ChunkArgs* a) {
     const int64_t rows = a->max_q * (a->q_heads / a->kv_heads), keys = (a->max_len + kKvTile - 1) / kKvTile;
     a->tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && a->head_dim != 256 ? 3 : rows <= 128 && a->head_dim != 256 ? 4 : 0;
     const int64_t per = block_rows(*a);
     a->blocks = (rows + per - 1) / per;
+    a->steps = (keys + 1) / 2;
+    if (a->tiles == 0 && a->blocks >= kHeldBlocks) {
+        a->tiles = -1;
+        if (a->seqs * a->kv_heads * a->steps >= (int64_t)1 << 22 || held_bytes(*a) > kHeldMost) a->tiles = 0;
+    }
     const int64_t units = a->seqs * a->kv_heads * a->blocks;
     if (units >= (int64_t)1 << 22) return false;                     // a launch has fewer than 2^32 threads
-    int64_t splits = units >= 512 ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
+    int64_t splits = units >= (a->tiles <= 0 ? 256 : 512) ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
     const int64_t most = (keys + 4 * kWaves - 1) / (4 * kWaves);     // four tiles a wave at least
     splits = splits < most ? splits : most;
     splits = splits > 0 ? splits : 1;
     a->share = (keys + splits - 1) / splits;
     a->share = a->share > 0 ? a->share : 1;
-    if (a->tiles == 0) a->share += a->share & 1;                     // 64 tokens a step
+    if (a->tiles <= 0) a->share += a->share & 1;                     // 64 tokens a step
     a->splits = (keys + a->share - 1) / a->share;
     a->splits = a->splits > 0 ? a->splits : 1;
     a->per_page = ((uint64_t)1 << 36) / ((uint64_t)a->page_tokens / kKvTile) + 1;
@@ -951,12 +1180,13 @@ bool plan_attn_chunk(ChunkArgs* a) {
 }
 
 size_t attn_chunk_scratch(const ChunkArgs& a) {
-    if (a.splits == 1) return 0;
-    return sizeof(float) * (size_t)(a.seqs * a.kv_heads * a.blocks * a.splits * block_rows(a)) * (size_t)(a.head_dim + 4);
+    return (part_bytes(a) + 255) / 256 * 256 + held_bytes(a) + (a.tiles < 0 ? sizeof(int32_t) * (size_t)(a.seqs * a.kv_heads * a.steps) : 0);
 }
 
 hipError_t launch_attn_chunk(ChunkArgs a, float* scratch, hipStream_t stream) {
     a.part = scratch;
+    a.held = reinterpret_cast<char*>(scratch) + (part_bytes(a) + 255) / 256 * 256;
+    a.held_flags = reinterpret_cast<int32_t*>(static_cast<char*>(a.held) + held_bytes(a));
     if (a.type == kTypeBF16)
         return a.out_type == kTypeF32 ? launch_typed<kTypeBF16, kTypeF32>(a, stream)
                                       : launch_typed<kTypeBF16, kTypeBF16>(a, stream);

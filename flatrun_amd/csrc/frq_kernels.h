@@ -346,12 +346,15 @@ struct ChunkArgs {
     void* out;
     int64_t ld_out, q_heads;
     float scale;
-    // plan_attn_chunk: column tiles of 16 rows of a workgroup, workgroups of the
-    // longest chunk and a key head, the parts its keys are split into, and the
-    // tiles of a part
-    int64_t tiles, blocks, splits, share;
+    // plan_attn_chunk: column tiles of 16 rows of a workgroup (0: many rows to a
+    // workgroup, -1: and the keys unpacked before), workgroups of the longest chunk
+    // and a key head, the parts its keys are split into, the tiles of a part, and
+    // the steps of 64 tokens of the longest sequence
+    int64_t tiles, blocks, splits, share, steps;
     uint64_t per_page;           // 2^36 / tiles of a page, rounded up
     float* part;
+    void* held;                  // unpacked keys and values, and a word for each step
+    int32_t* held_flags;
 };
 bool plan_attn_chunk(ChunkArgs* a);       // false: more than a launch takes
 size_t attn_chunk_scratch(const ChunkArgs& a);
