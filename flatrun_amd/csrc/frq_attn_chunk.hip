@@ -31,7 +31,7 @@ constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnder = 5.f, kLag = 7.f;      // of the weights' powers of two: see the head of the file
 constexpr float kInf = __builtin_inff();
-constexpr int kHeldBlocks = 1000000;                 // blocks of rows from which on keys are unpacked once
+constexpr int kHeldRows = 256;                 // rows of a key head from which on keys are unpacked once
 constexpr size_t kHeldMost = (size_t)1 << 30;  // bytes of them
 
 // Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
     id /= (uint32_t)a.splits;
     const int kvh = (int)(id % (uint32_t)a.kv_heads);
     id /= (uint32_t)a.kv_heads;
-    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
+    const int seq = (int)(a.together ? id % (uint32_t)a.seqs : id / (uint32_t)a.blocks);
+    const int block = (int)(a.blocks - 1 - (a.together ? id / (uint32_t)a.seqs : id % (uint32_t)a.blocks));    // the longest rows first
     Span sp;
     if (!sp.read(a, seq)) return;
     if (sp.bad) {
@@ -470,11 +471,12 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
     }
 }
 
-// ------------------------------------------------------ many rows to a tile
+// --------------------------------------------------------------- many rows
 //
-// W waves of 32 rows each share what is unpacked: 64 tokens at a time, every
-// wave its part (four words of codes a lane, of K or of V), into LDS, in the order
-// of the operands of v_mfma_f32_32x32x16_f16, while the 64 before are worked on.
+// Where hundreds of rows read the same keys, unpacking them for every 64 would be
+// half of the work: one kernel unpacks every key and value of the call once, into
+// scratch, and a second one has W waves of 32 rows each share what it copies from
+// there, 64 tokens at a time, to LDS, on v_mfma_f32_32x32x16_f16.
 using float16v = float __attribute__((ext_vector_type(16)));
 constexpr int kKeys = 64;
 
@@ -544,11 +546,10 @@ __device__ __forceinline__ void put_unit(const Unit<NG>& r, int unit, int half, 
         }
     }
 }
-// What is not ordinary in a unit of tokens t0 ..: behind the sequence's end zeros,
-// and in V, if asked for, in place of what is no number. 1: a large scale is left, 2:
-// no number in V.
+// What is not ordinary in a unit of tokens t0 ..: zeros behind the sequence's end,
+// and 1 for a large scale, 2 for no number in V.
 template <int NG>
-__device__ __forceinline__ int clean_unit(Unit<NG>& r, int unit, int t0, int len, bool zero, int lane) {
+__device__ __forceinline__ int clean_unit(Unit<NG>& r, int unit, int t0, int len, int lane) {
     const int n = lane & 15, j = lane >> 4;
     const bool v = unit >= NG / 2;
     bool any = false, big = false;
@@ -557,7 +558,7 @@ __device__ __forceinline__ int clean_unit(Unit<NG>& r, int unit, int t0, int len
         const bool past_end = token >= len, no = s >= 0x7C00;
         big |= s > 0x6FFF && !past_end && !no;
         any |= v && no && !past_end;
-        if (past_end || (v && no && zero)) w &= hi ? 0xFFFFu : 0xFFFF0000u;
+        if (past_end) w &= hi ? 0xFFFFu : 0xFFFF0000u;
     };
     if (v) {
 #pragma unroll
@@ -578,10 +579,8 @@ __device__ __forceinline__ void eighth(Unit<NG>& r) {
     for (int i = 0; i < 8; ++i) r.scale[i] = bits_of(pair_of(r.scale[i]) * (half2v){0.125f16, 0.125f16});
 }
 
-// Every key and value of the call unpacked once, 64 tokens of a key head to a
-// workgroup, in the order in which LDS holds them: for chunks of so many rows
-// that unpacking them for each 256 or 128 would be most of the work. A word beside
-// them says what is not ordinary: 1 V at an eighth, 2 no number in V, 4 K at an
+// Every key and value of the call, 64 tokens of a key head to a workgroup, in the
+// order in which LDS will hold them. A word beside them says what is not ordinary: 1 V at an eighth, 2 no number in V, 4 K at an
 // eighth, 8 a page outside the cache.
 constexpr int unpack_waves(int ng) { return ng == 2 ? 4 : 8; }
 template <int NG>
@@ -616,7 +615,7 @@ __global__ void __launch_bounds__(64 * unpack_waves(NG)) attn_chunk_unpack_kerne
         const int unit = (kUnits * wave + x) % NG;
         const bool v = unit >= NG / 2;
         if (__builtin_amdgcn_ballot_w64(raw[x].large(v)) == 0) continue;
-        const int c = clean_unit<NG>(raw[x], unit, want * kKvTile, sp.len, false, lane);
+        const int c = clean_unit<NG>(raw[x], unit, want * kKvTile, sp.len, lane);
         f |= v ? c : (c & 1) << 2;
     }
     if (f && lane == 0) atomicOr(&sh_flags, f);
@@ -632,16 +631,14 @@ __global__ void __launch_bounds__(64 * unpack_waves(NG)) attn_chunk_unpack_kerne
     if (threadIdx.x == 0) a.held_flags[blockIdx.x] = f;
 }
 
-template <int TYPE, int OUT, int NG, int W, bool HELD>
+template <int TYPE, int OUT, int NG, int W>
 __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kernel(ChunkArgs a) {
     using T = Val<TYPE>;
     using O = Val<OUT>;
-    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 32 * W, NK = D / 16, ND = NG;
-    constexpr int kUnits = 2 * NG / W;                               // of a wave and 64 tokens
-    static_assert(kUnits * W == 2 * NG, "every wave has units");
-    constexpr int kBuf = kKeys * D;
+    constexpr int D = 32 * NG, kRows = 32 * W, NK = D / 16, ND = NG, kBuf = kKeys * D;
+    // a K and a V tile twice, used in turn: objects of their own, so that the
+    // compiler sees that a read of one need not wait for the copies into the other
     __shared__ __attribute__((aligned(16))) _Float16 kb0[kBuf], kb1[kBuf], vb0[kBuf], vb1[kBuf];
-    __shared__ int flags[2][3], sh_bad;                              // of a step's K and V: 1 a large scale, 2 blocks left out
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ln = lane & 31, h = lane >> 5;
@@ -651,7 +648,8 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kerne
     id /= (uint32_t)a.splits;
     const int kvh = (int)(id % (uint32_t)a.kv_heads);
     id /= (uint32_t)a.kv_heads;
-    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
+    const int seq = (int)(a.together ? id % (uint32_t)a.seqs : id / (uint32_t)a.blocks);
+    const int block = (int)(a.blocks - 1 - (a.together ? id / (uint32_t)a.seqs : id % (uint32_t)a.blocks));    // the longest rows first
     Span sp;
     if (!sp.read(a, seq)) return;
     if (sp.bad) {
@@ -666,90 +664,28 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kerne
     if (row0 >= rows) return;
     const int end = sp.keys(row0 + kRows - 1, group);
     const int tiles = (end + kKvTile - 1) / kKvTile;
-    const int first = split * (int)a.share;
+    const int first = split * (int)a.share;                          // even
     const int last = tiles < first + (int)a.share ? tiles : first + (int)a.share;
     if (first >= tiles && split) return;
     const int whole = sp.keys(row0, group);                          // keys below this one every row of the workgroup sees
     const int wrow = row0 + 32 * wave;                               // the wave's rows
     const int seen = wrow < rows ? sp.keys(wrow + 31, group) : 0, own = wrow < rows ? sp.keys(wrow, group) : 0;
 
-    const const_ints table = constant(a.table) + (int64_t)seq * a.ld_table;
-    const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
-    const int64_t page_bytes = a.kv_heads * (int64_t)page_tiles * kTile;
-    const uint8_t* heads = static_cast<const uint8_t*>(a.cache) + (int64_t)kvh * page_tiles * kTile;
-    bool bad = false;
-    // past the last tile that one again: its tokens are masked
-    auto page_index = [&](int tile) { return (uint32_t)(((uint64_t)(uint32_t)tile * a.per_page) >> 36); };
-    auto look_up = [&](int tile) { return table[page_index(tile < last ? tile : last - 1)]; };
-    auto address = [&](int tile, int page) {
-        if ((uint32_t)page >= (uint64_t)a.pages) {
-            bad = true;
-            page = 0;
-        }
-        tile = tile < last ? tile : last - 1;
-        const uint32_t in = (uint32_t)tile - page_index(tile) * page_tiles;
-        return heads + page * page_bytes + (int64_t)in * kTile;
-    };
-    const int half = kUnits * wave / NG;                             // the wave's tile of a step's two
-    Unit<NG> raw[kUnits];
-    auto fetch = [&](const uint8_t* t) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < kUnits; ++x) raw[x].load(t, (kUnits * wave + x) % NG, lane);
-    };
-    // The wave's units, all of K or all of V (but for 256-wide heads, whose waves
-    // have both), of the 64 tokens from tile0 on, unpacked into LDS.
-    auto unpack = [&](int x, int tile0, _Float16* buf, int* flag, bool small) __attribute__((always_inline)) {
-        const int unit = (kUnits * wave + x) % NG;
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(raw[x].large(unit >= NG / 2)) != 0, 0)) {
-            // a zero weight does not take a NaN out of a product: where rows
-            // differ in what they see, it leaves V and is added below
-            const int f = clean_unit<NG>(raw[x], unit, (tile0 + half) * kKvTile, sp.len, tile0 * kKvTile + kKeys > whole, lane);
-            if (f && lane == 0) atomicOr(flag, f);
-        }
-        if (small) eighth<NG>(raw[x]);
-        put_unit<NG>(raw[x], unit, half, lane, buf, buf);
-    };
-    auto is_v = [&](int x) { return (kUnits * wave + x) % NG >= NG / 2; };
-    // K of step k into kb, V of step v into vb, and the wave's next ones asked for:
-    // pages are looked up a step before their tile is
-    int pages[2] = {0, 0};
-    constexpr bool kBoth = kUnits == NG;                             // a wave has units of K and of V
-    auto fetch_units = [&](bool v, int tile, int page) __attribute__((always_inline)) {
-        const uint8_t* t = address(tile + half, page);
-#pragma unroll
-        for (int x = 0; x < kUnits; ++x)
-            if (is_v(x) == v) raw[x].load(t, (kUnits * wave + x) % NG, lane);
-    };
-    auto unpack_units = [&](bool v, int tile, _Float16* buf, int* flag, bool small) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < kUnits; ++x)
-            if (is_v(x) == v) unpack(x, tile, buf, flag, small);
-    };
-    if (threadIdx.x < 6) flags[threadIdx.x / 3][threadIdx.x % 3] = 0;
-    if (threadIdx.x == 6) sh_bad = 0;
-    const bool has_k = !HELD && (kBoth || !is_v(0)), has_v = !HELD && (kBoth || is_v(0));
-    if (!HELD && first < last) {
-        const int now = look_up(first + half);
-        if (has_k) fetch_units(false, first, now);
-        if (has_v) fetch_units(true, first, now);
-        pages[0] = pages[1] = look_up(first + 2 + half);
-    }
-    // HELD: the unpacked steps of the sequence and key head, and their words
-    const int64_t blocks64 = ((int64_t)seq * a.kv_heads + kvh) * a.steps;
-    const _Float16* held = static_cast<const _Float16*>(a.held) + blocks64 * (2 * kBuf);
-    const const_ints words = constant(a.held_flags) + blocks64;
+    // the unpacked steps of the sequence and key head, and their words
+    const int64_t steps0 = ((int64_t)seq * a.kv_heads + kvh) * a.steps;
+    const _Float16* held = static_cast<const _Float16*>(a.held) + steps0 * (2 * kBuf);
+    const const_ints words = constant(a.held_flags) + steps0;
     // Asynchronous copy of a step's K (or V), as it lies, 16 bytes a lane and turn.
     auto copy = [&](int tile, bool v, _Float16* to) __attribute__((always_inline)) {
         constexpr int kTurns = kBuf / 8 / (64 * W);
         const __amdgpu_buffer_rsrc_t r = buffer_rsrc(held + (int64_t)(tile / 2) * (2 * kBuf) + (v ? kBuf : 0), kBuf * 2);
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
-            const int at16 = (i * W + wave) * 64;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + at16 * 8), 16,
-                                                     (at16 + lane) * 16, 0, 0, 0);
+            const int at = (i * W + wave) * 64;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + at * 8), 16, (at + lane) * 16, 0, 0, 0);
         }
     };
-    if (HELD && first < last) {
+    if (first < last) {
         copy(first, false, kb0);
         copy(first, true, vb0);
         if (first + 2 < last) copy(first + 2, false, kb1);
@@ -790,126 +726,54 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kerne
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -kInf, nref = 0.f, l = 0.f;
 
-    auto scores = [&](const _Float16* kb, float16v (&st)[2]) __attribute__((always_inline)) {   // of the first step
+    // the waves meet, and what any of them has copied is there
+    auto meet = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0x0070);                          // vmcnt(0), lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+    };
+    bool bad = false;
+    float16v sa[2], sb[2];
+    float up = 1.f;                                                  // of the scores at hand
+    int word = 0;                                                    // of the next step
+    meet();
+    if (first < last) {
+        word = words[first / 2];
+        up = word & 4 ? 8.f : 1.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st[0][i] = st[1][i] = 0.f;
+        for (int i = 0; i < 16; ++i) sa[0][i] = sa[1][i] = 0.f;
 #pragma unroll
         for (int s = 0; s < NK; ++s)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const half8v kf = *reinterpret_cast<const half8v*>(kb + ((2 * s + h) * kKeys + 32 * t + ln) * 8);
-                st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[t], 0, 0, 0);
+                const half8v kf = *reinterpret_cast<const half8v*>(kb0 + ((2 * s + h) * kKeys + 32 * t + ln) * 8);
+                sa[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], sa[t], 0, 0, 0);
             }
-    };
-    int at = 0;                                                      // this step's flags
-    // once more, at an eighth, where a scale is large
-    auto again = [&](bool v, int tile, _Float16* buf, int* flag) __attribute__((always_inline)) {
-        const int after = tile + 2;
-        if (v ? has_v : has_k) {
-            fetch_units(v, tile, look_up(tile + half));
-            unpack_units(v, tile, buf, flag, true);
-            fetch_units(v, after, look_up(after + half));
-        }
-        __syncthreads();
-    };
-    // the waves meet, and what any of them has copied is there
-    auto meet = [&]() __attribute__((always_inline)) {
-        if constexpr (HELD) {
-            __builtin_amdgcn_s_waitcnt(0x0070);                      // vmcnt(0), lgkmcnt(0)
-            __builtin_amdgcn_s_barrier();
-        } else {
-            __syncthreads();
-        }
-    };
-    float16v sa[2], sb[2];
-    float up = 1.f;                                                  // of the scores at hand
-    int fv_now = 0;                                                  // HELD: this step's word
-    meet();
-    if (HELD && first < last) {
-        fv_now = words[first / 2];
-        up = fv_now & 4 ? 8.f : 1.f;
-        scores(kb0, sa);
-    }
-    if (!HELD && first < last) {
-        if (has_k) {
-            unpack_units(false, first, kb0, &flags[0][0], false);
-            fetch_units(false, first + 2, pages[0]);
-            pages[0] = look_up(first + 4 + half);
-        }
-        if (has_v) {
-            unpack_units(true, first, vb0, &flags[1][0], false);
-            fetch_units(true, first + 2, pages[1]);
-            pages[1] = look_up(first + 4 + half);
-        }
-        __syncthreads();
-        if (__builtin_expect(flags[0][0] & 1, 0)) {
-            again(false, first, kb0, &flags[0][0]);
-            up = 8.f;
-        }
-        scores(kb0, sa);
-        if (has_k && first + 2 < last) {
-            unpack_units(false, first + 2, kb1, &flags[0][1], false);
-            fetch_units(false, first + 4, pages[0]);
-            pages[0] = look_up(first + 6 + half);
-        }
     }
     // Softmax and P V of a step, whose scores st holds, and the scores of the next:
     // K is a step ahead of V, so that those products go on beside the exponentials.
     auto step = [&](int tile, float16v (&st)[2], float16v (&sn)[2], _Float16* k_next, _Float16* k_after, _Float16* v_now,
                     _Float16* v_next) __attribute__((always_inline)) {
         meet();                                                      // K of the next step and V of this one are there
-        const bool more = tile + 2 < last;
-        int fv;
-        float down = 1.f, under = kUnder, up_next = 1.f;
-        if constexpr (HELD) {
-            fv = fv_now;
-            if (tile + 4 < last) copy(tile + 4, false, k_after);
-            if (more) {
-                copy(tile + 2, true, v_next);
-                fv_now = words[tile / 2 + 1];
-                up_next = fv_now & 4 ? 8.f : 1.f;
-            }
-            bad |= (fv & 8) != 0;
-            if (__builtin_expect((fv & 2) && tile * kKvTile + kKeys > whole, 0)) {
-                // a zero weight does not take a NaN out of a product: it leaves V
-                // and is added below for the rows that see it
-                for (int i = threadIdx.x; i < kBuf / 2; i += 64 * W) {
-                    uint32_t& w = reinterpret_cast<uint32_t*>(v_now)[i];
-                    const uint32_t x = w;
-                    w = x & ~(((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u));
-                }
-                __syncthreads();
-            }
-            if (fv & 1) {
-                down = 0.125f;
-                under = kUnder + 3.f;
-            }
-        } else {
-            const int n1 = at == 2 ? 0 : at + 1, n2 = n1 == 2 ? 0 : n1 + 1;
-            const int fk = flags[0][n1];
-            fv = flags[1][at];
-            if (threadIdx.x == 0) flags[0][at] = flags[1][n2] = 0;   // read for the last time before this barrier
-            if (__builtin_expect(fv & 1, 0)) {
-                again(true, tile, v_now, &flags[1][at]);
-                down = 0.125f;
-                under = kUnder + 3.f;
-            }
-            if (__builtin_expect(more && (fk & 1), 0)) {
-                again(false, tile + 2, k_next, &flags[0][n1]);
-                up_next = 8.f;
-            }
-            if (has_k && tile + 4 < last) {
-                unpack_units(false, tile + 4, k_after, &flags[0][n2], false);
-                fetch_units(false, tile + 6, pages[0]);
-                pages[0] = look_up(tile + 8 + half);
-            }
-            if (has_v && more) {
-                unpack_units(true, tile + 2, v_next, &flags[1][n1], false);
-                fetch_units(true, tile + 4, pages[1]);
-                pages[1] = look_up(tile + 6 + half);
-            }
-            at = n1;
+        const int f = word;
+        float up_next = 1.f;
+        if (tile + 4 < last) copy(tile + 4, false, k_after);
+        if (tile + 2 < last) {
+            copy(tile + 2, true, v_next);
+            word = words[tile / 2 + 1];
+            up_next = word & 4 ? 8.f : 1.f;
         }
+        bad |= (f & 8) != 0;
+        if (__builtin_expect((f & 2) && tile * kKvTile + kKeys > whole, 0)) {
+            // a zero weight does not take a NaN out of a product: it leaves V
+            // and is added below for the rows that see it
+            for (int i = threadIdx.x; i < kBuf / 2; i += 64 * W) {
+                uint32_t& w = reinterpret_cast<uint32_t*>(v_now)[i];
+                const uint32_t x = w;
+                w = x & ~(((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u));
+            }
+            __syncthreads();
+        }
+        const float down = f & 1 ? 0.125f : 1.f, under = f & 1 ? kUnder + 3.f : kUnder;
         const float by = rs * up;
         up = up_next;
         const int kt = tile * kKvTile;
@@ -981,9 +845,15 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kerne
             if (x + 4 < 4 * ND) ahead[x & 3] = v_of(x + 4);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (__builtin_expect(fv & 2, 0)) {
-            for (int t = 0; t < kKeys && kt + t < sp.len && tile + t / kKvTile < last; ++t) {
-                const uint8_t* there = address(tile + t / kKvTile, look_up(tile + t / kKvTile));
+        if (__builtin_expect(f & 2, 0)) {
+            const const_ints table = constant(a.table) + (int64_t)seq * a.ld_table;
+            const uint32_t page_tiles = (uint32_t)a.page_tokens / kKvTile;
+            for (int t = 0; t < kKeys && kt + t < sp.len; ++t) {
+                const uint32_t at = (uint32_t)(kt + t) / kKvTile, in = (uint32_t)(((uint64_t)at * a.per_page) >> 36);
+                const int page = table[in];
+                if ((uint32_t)page >= (uint64_t)a.pages) break;
+                const uint8_t* there = static_cast<const uint8_t*>(a.cache) +
+                                       ((page * a.kv_heads + kvh) * (int64_t)page_tiles + (at - in * page_tiles)) * kv_tile_bytes(NG);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const uint16_t b = *reinterpret_cast<const uint16_t*>(there + kv_vs_off(NG) + kv_scale(t % kKvTile, g, NG));
@@ -996,9 +866,7 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kerne
         step(tile, sa, sb, kb1, kb0, vb0, vb1);
         if (tile + 2 < last) step(tile + 2, sb, sa, kb0, kb1, vb1, vb0);
     }
-    if (bad) sh_bad = 1;
-    __syncthreads();
-    if (sh_bad) l = __builtin_nanf("");
+    if (bad) l = __builtin_nanf("");
     l += __shfl_xor(l, 32);
     if (wrow + ln >= rows) return;
     if (a.splits > 1) {
@@ -1094,21 +962,19 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(ChunkArgs a, int k
     __builtin_memcpy(__builtin_assume_aligned(out + 4 * col, 4 * sizeof(y[0])), y, sizeof(y));
 }
 
-// R: column tiles of a workgroup, 0 for many rows to a tile, -1 for those of
-// unpacked keys.
+// R: column tiles of a workgroup, or minus the waves of 32 rows of one that works
+// on unpacked keys.
 template <int TYPE, int OUT, int NG, int R>
 hipError_t launch_one(const ChunkArgs& a, hipStream_t stream) {
-    constexpr int kW = NG == 4 ? 8 : 4, kRows = R > 0 ? 16 * R : 32 * kW;
+    constexpr int kRows = R > 0 ? 16 * R : -32 * R;
     const int64_t units = a.seqs * a.kv_heads * a.blocks;
     const unsigned grid = (unsigned)(units * a.splits);
     if constexpr (R > 0) {
         attn_chunk_kernel<TYPE, OUT, NG, R><<<grid, 64 * kWaves, 0, stream>>>(a);
-    } else if constexpr (R == 0) {
-        attn_chunk_rows_kernel<TYPE, OUT, NG, kW, false><<<grid, 64 * kW, 0, stream>>>(a);
     } else {
         attn_chunk_unpack_kernel<NG><<<(unsigned)(a.seqs * a.kv_heads * a.steps), 64 * unpack_waves(NG), 0, stream>>>(a);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        attn_chunk_rows_kernel<TYPE, OUT, NG, kW, true><<<grid, 64 * kW, 0, stream>>>(a);
+        attn_chunk_rows_kernel<TYPE, OUT, NG, -R><<<grid, -64 * R, 0, stream>>>(a);
     }
     if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
     constexpr int kSets = 256 / (8 * NG);
@@ -1124,8 +990,10 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
     const auto run = [&](auto ng) {
         constexpr int kN = decltype(ng)::value;
         switch (a.tiles) {
-            case -1: return launch_one<TYPE, OUT, kN, -1>(a, stream);
-            case 0: return launch_one<TYPE, OUT, kN, 0>(a, stream);
+            case -8:
+                if constexpr (kN == 4) return launch_one<TYPE, OUT, kN, -8>(a, stream);
+                return hipErrorInvalidValue;
+            case -4: return launch_one<TYPE, OUT, kN, -4>(a, stream);
             case 1: return launch_one<TYPE, OUT, kN, 1>(a, stream);
             case 2: return launch_one<TYPE, OUT, kN, 2>(a, stream);
             default:
@@ -1144,7 +1012,7 @@ hipError_t launch_typed(const ChunkArgs& a, hipStream_t stream) {
 }  // namespace
 
 // Rows of a workgroup.
-static int64_t block_rows(const ChunkArgs& a) { return a.tiles > 0 ? 16 * a.tiles : a.head_dim == 128 ? 256 : 128; }
+static int64_t block_rows(const ChunkArgs& a) { return a.tiles > 0 ? 16 * a.tiles : -32 * a.tiles; }
 
 static size_t part_bytes(const ChunkArgs& a) {
     if (a.splits == 1) return 0;
@@ -1154,27 +1022,51 @@ static size_t held_bytes(const ChunkArgs& a) {
     return a.tiles < 0 ? (size_t)(a.seqs * a.kv_heads * a.steps) * (size_t)(256 * a.head_dim) : 0;
 }
 
+// How the rows are cut (a.tiles) and the keys split, by the steps of 64 tokens that
+// the slowest CU comes to, where every workgroup has as many keys as the longest
+// sequence, and some for its start and end and for the joining.
+static int64_t cut(ChunkArgs* a, int64_t rows, int64_t slots, int64_t most) {
+    a->blocks = (rows + block_rows(*a) - 1) / block_rows(*a);
+    const int64_t units = a->seqs * a->kv_heads * a->blocks;
+    int64_t best = 0;
+    for (int64_t s = 1; s <= most && (s == 1 || units * s <= 4 * slots); ++s) {
+        const int64_t each = (a->steps + s - 1) / s, cost = (units * s + slots - 1) / slots * (each + 4) + (s > 1 ? 6 + s : 0);
+        if (best && cost >= best) continue;
+        best = cost;
+        a->splits = s;
+    }
+    return best;
+}
+
 bool plan_attn_chunk(ChunkArgs* a) {
     const int64_t rows = a->max_q * (a->q_heads / a->kv_heads), keys = (a->max_len + kKvTile - 1) / kKvTile;
-    a->tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && a->head_dim != 256 ? 3 : rows <= 128 && a->head_dim != 256 ? 4 : 0;
-    const int64_t per = block_rows(*a);
-    a->blocks = (rows + per - 1) / per;
+    const bool wide = a->head_dim == 256;
     a->steps = (keys + 1) / 2;
-    if (a->tiles == 0 && a->blocks >= kHeldBlocks) {
-        a->tiles = -1;
-        if (a->seqs * a->kv_heads * a->steps >= (int64_t)1 << 22 || held_bytes(*a) > kHeldMost) a->tiles = 0;
+    a->tiles = -4;
+    if (rows >= kHeldRows && a->seqs * a->kv_heads * a->steps < (int64_t)1 << 22 && held_bytes(*a) <= kHeldMost) {
+        const int64_t cost4 = cut(a, rows, wide ? 256 : 512, 16);
+        if (a->head_dim == 128) {
+            // eight waves to a copy of the keys where that leaves no CU empty: a
+            // step of two workgroups of four takes about a tenth longer
+            const int64_t splits4 = a->splits, blocks4 = a->blocks;
+            a->tiles = -8;
+            if (cut(a, rows, 256, 16) * 10 > cost4 * 11) a->tiles = -4, a->splits = splits4, a->blocks = blocks4;
+        }
+        a->share = 2 * ((a->steps + a->splits - 1) / a->splits);
+    } else {
+        a->tiles = rows <= 16 ? 1 : rows <= 32 || wide ? 2 : rows <= 48 ? 3 : 4;
+        a->blocks = (rows + block_rows(*a) - 1) / block_rows(*a);
+        const int64_t units = a->seqs * a->kv_heads * a->blocks;
+        int64_t splits = units >= 512 ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
+        const int64_t most = (keys + 4 * kWaves - 1) / (4 * kWaves);  // four tiles a wave at least
+        splits = splits < most ? splits : most;
+        a->share = splits > 1 ? (keys + splits - 1) / splits : keys;
     }
+    a->share = a->share > 0 ? a->share : 1;
+    a->splits = keys > a->share ? (keys + a->share - 1) / a->share : 1;
     const int64_t units = a->seqs * a->kv_heads * a->blocks;
     if (units >= (int64_t)1 << 22) return false;                     // a launch has fewer than 2^32 threads
-    int64_t splits = units >= (a->tiles <= 0 ? 256 : 512) ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
-    const int64_t most = (keys + 4 * kWaves - 1) / (4 * kWaves);     // four tiles a wave at least
-    splits = splits < most ? splits : most;
-    splits = splits > 0 ? splits : 1;
-    a->share = (keys + splits - 1) / splits;
-    a->share = a->share > 0 ? a->share : 1;
-    if (a->tiles <= 0) a->share += a->share & 1;                     // 64 tokens a step
-    a->splits = (keys + a->share - 1) / a->share;
-    a->splits = a->splits > 0 ? a->splits : 1;
+    a->together = units * a->splits <= 1024;
     a->per_page = ((uint64_t)1 << 36) / ((uint64_t)a->page_tokens / kKvTile) + 1;
     return true;
 }

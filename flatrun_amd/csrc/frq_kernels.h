@@ -346,11 +346,12 @@ struct ChunkArgs {
     void* out;
     int64_t ld_out, q_heads;
     float scale;
-    // plan_attn_chunk: column tiles of 16 rows of a workgroup (0: many rows to a
-    // workgroup, -1: and the keys unpacked before), workgroups of the longest chunk
+    // plan_attn_chunk: column tiles of 16 rows of a workgroup (where keys are
+    // unpacked before, minus its waves of 32 rows), workgroups of the longest chunk
     // and a key head, the parts its keys are split into, the tiles of a part, and
     // the steps of 64 tokens of the longest sequence
     int64_t tiles, blocks, splits, share, steps;
+    int together;                // sequences take turns in the order of the grid
     uint64_t per_page;           // 2^36 / tiles of a page, rounded up
     float* part;
     void* held;                  // unpacked keys and values, and a word for each step
