@@ -54,6 +54,15 @@ __device__ __forceinline__ half2v halves(uint32_t a, uint32_t b, int h) {
     return pair_of(__builtin_amdgcn_perm(b, a, h ? 0x07060302u : 0x05040100u));
 }
 
+// A scale, half hi of w, of a token that is behind the end (it becomes zero) or
+// not: 1 beyond 8188, 2 no number.
+__device__ __forceinline__ int clean_half(uint32_t& w, int hi, bool past_end) {
+    const uint32_t s = (hi ? w >> 16 : w) & 0x7FFFu;
+    if (past_end) w &= hi ? 0xFFFFu : 0xFFFF0000u;
+    return past_end || s <= 0x6FFF ? 0 : s < 0x7C00 ? 1 : 2;
+}
+__device__ __forceinline__ uint32_t eighth(uint32_t w) { return bits_of(pair_of(w) * (half2v){0.125f16, 0.125f16}); }
+
 // A lane's share of a tile's K or V scales, to look for what is not ordinary.
 template <int NG>
 struct Flat {
@@ -106,6 +115,29 @@ struct Span {
     }
 };
 
+// Block `t` of all sequences' blocks of kRows rows, those of the longest sequence
+// first, so that the last workgroups to start are short ones (8 chunks of 201 to
+// 512 after 300 to 4096: 172 us without). Up to 64 sequences, a lane each. false:
+// there is none.
+__device__ __forceinline__ bool longest_first(const ChunkArgs& a, int t, int group, int kRows, int lane, int& seq, int& block) {
+    int blocks = 0, len = -1;
+    if (lane < a.seqs) {
+        const int64_t n = (int64_t)a.cu_q[lane + 1] - a.cu_q[lane];
+        len = a.lens[lane];
+        blocks = n <= 0 ? 0 : n > a.max_q ? (int)a.blocks : (int)((n * group + kRows - 1) / kRows);
+    }
+    int start = 0;
+    for (int i = 0; i < a.seqs; ++i) {
+        const int l = __builtin_amdgcn_readlane(len, i), b = __builtin_amdgcn_readlane(blocks, i);
+        start += l > len || (l == len && i < lane) ? b : 0;
+    }
+    const uint64_t here = __builtin_amdgcn_ballot_w64(start <= t && t < start + blocks);
+    if (here == 0) return false;
+    seq = (int)__builtin_ctzll(here);
+    block = __builtin_amdgcn_readlane(blocks, seq) - 1 - (t - __builtin_amdgcn_readlane(start, seq));
+    return true;
+}
+
 template <int TYPE, int OUT, int NG, int R>
 __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kernel(ChunkArgs a) {
     using T = Val<TYPE>;
@@ -124,8 +156,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
     id /= (uint32_t)a.splits;
     const int kvh = (int)(id % (uint32_t)a.kv_heads);
     id /= (uint32_t)a.kv_heads;
-    const int seq = (int)(a.together ? id % (uint32_t)a.seqs : id / (uint32_t)a.blocks);
-    const int block = (int)(a.blocks - 1 - (a.together ? id / (uint32_t)a.seqs : id % (uint32_t)a.blocks));    // the longest rows first
+    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
     Span sp;
     if (!sp.read(a, seq)) return;
     if (sp.bad) {
@@ -258,42 +289,20 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
         page = look_up(tile + 2 * kWaves);
         const int kt = tile * kKvTile;
         const bool masked = kt + kKvTile > whole;
-        float up = 1.f, down = 1.f, under = kUnder;
-        uint64_t gone = 0;                                           // blocks taken out of the product
-        // a scale beyond 8188, or no number?
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(fk.large() || fv.large()) != 0, 0)) {
-            // Behind the sequence's end nothing is known, and a zero weight does
-            // not take a NaN out of a product: where rows differ in what they
-            // see, a block of V that is no number leaves the product, to be
-            // added below for the rows that see it.
-            bool any = false, big = false;
-            auto clean = [&](uint32_t& w, bool v, int token, int h) {
-                const uint32_t half = h ? 0xFFFF0000u : 0xFFFFu, s = (h ? w >> 16 : w) & 0x7FFFu;
-                const bool past_end = token >= sp.len, no = s >= 0x7C00;
-                big |= s > 0x6FFF && !past_end && !no;
-                any |= v && no && masked && !past_end;
-                if (past_end || (v && no && masked)) w &= ~half;
-            };
+        float up = 1.f;
+        // A scale beyond 8188, an inf or a NaN? What is behind the sequence's end
+        // is nobody's and becomes zero.
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(fk.large()) != 0, 0)) {
+            bool big = false;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const int p = (u * NG + g) / 2, h = (u * NG + g) & 1;
-                    clean(ks[p], false, kt + 16 * u + n, h);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) clean(vs[i][p], true, kt + 16 * u + 4 * j + i, h);
-                }
-            gone = __builtin_amdgcn_ballot_w64(any);
+            for (int x = 0; x < 2 * NG; ++x) {
+                const int token = kt + 16 * (x / NG) + n;
+                big |= clean_half(ks[x / 2], x & 1, token >= sp.len) == 1;
+            }
             if (__builtin_amdgcn_ballot_w64(big)) {
                 up = 8.f;
-                down = 0.125f;
-                under = kUnder + 3.f;
 #pragma unroll
-                for (int p = 0; p < NG; ++p) {
-                    ks[p] = bits_of(pair_of(ks[p]) * (half2v){0.125f16, 0.125f16});
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) vs[i][p] = bits_of(pair_of(vs[i][p]) * (half2v){0.125f16, 0.125f16});
-                }
+                for (int p = 0; p < NG; ++p) ks[p] = eighth(ks[p]);
             }
         }
         // scores of tokens 16u + 4j .. 4j + 3: K of 16 tokens and 32 channels at a time
@@ -350,7 +359,7 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
             }
             half2v p[4];
             float sum = 0.f;
-            const float ref = nref[c] + under;
+            const float ref = nref[c] + kUnder;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -360,10 +369,38 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
                     p[2 * u + i / 2] = half2v{(_Float16)p0, (_Float16)p1};
                     sum = __builtin_amdgcn_fdot2(p[2 * u + i / 2], (half2v){(_Float16)1.f, (_Float16)1.f}, sum, false);
                 }
-            l[c] = __builtin_fmaf(sum, down, l[c]);
+            l[c] += sum;
             pf[c] = join(p[0], p[1], p[2], p[3]);
         }
         // V of 16 channels at a time
+        int odd = 0;                                                 // 1 a large scale, 2 blocks taken out of the product
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(fv.large()) != 0, 0)) {
+            // A zero weight does not take a NaN out of a product: where rows
+            // differ in what they see, a block that is no number leaves it, to be
+            // added below for the rows that see it.
+            bool any = false, big = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < 2 * NG; ++x) {
+                    const int token = kt + 16 * (x / NG) + 4 * j + i;
+                    const int f = clean_half(vs[i][x / 2], x & 1, token >= sp.len);
+                    big |= f == 1;
+                    any |= f == 2 && masked;
+                    if (f == 2 && masked) vs[i][x / 2] &= x & 1 ? 0xFFFFu : 0xFFFF0000u;
+                }
+            odd = (__builtin_amdgcn_ballot_w64(big) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(any) ? 2 : 0);
+        }
+        if (__builtin_expect(odd & 1, 0)) {                          // values past fp16: all at an eighth for this tile
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int p = 0; p < NG; ++p) vs[i][p] = eighth(vs[i][p]);
+#pragma unroll
+            for (int c = 0; c < R; ++c)
+#pragma unroll
+                for (int d = 0; d < 2 * NG; ++d) o[c][d] *= 0.125f;
+        }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const uint32_t w0 = vc[2 * g], w1 = vc[2 * g + 1];
@@ -384,8 +421,14 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (__builtin_expect(odd & 1, 0)) {
+#pragma unroll
+            for (int c = 0; c < R; ++c)
+#pragma unroll
+                for (int d = 0; d < 2 * NG; ++d) o[c][d] *= 8.f;
+        }
         fetch_v(next);
-        if (__builtin_expect(gone != 0, 0)) {
+        if (__builtin_expect(odd & 2, 0)) {
             for (int t = 0; t < kKvTile && kt + t < sp.len; ++t)
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
@@ -551,32 +594,19 @@ __device__ __forceinline__ void put_unit(const Unit<NG>& r, int unit, int half, 
 template <int NG>
 __device__ __forceinline__ int clean_unit(Unit<NG>& r, int unit, int t0, int len, int lane) {
     const int n = lane & 15, j = lane >> 4;
-    const bool v = unit >= NG / 2;
     bool any = false, big = false;
-    auto clean = [&](uint32_t& w, int token, int hi) {
-        const uint32_t s = (hi ? w >> 16 : w) & 0x7FFFu;
-        const bool past_end = token >= len, no = s >= 0x7C00;
-        big |= s > 0x6FFF && !past_end && !no;
-        any |= v && no && !past_end;
-        if (past_end) w &= hi ? 0xFFFFu : 0xFFFF0000u;
-    };
-    if (v) {
+    if (unit >= NG / 2) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + 4 * j + i / 2 + 16 * (i & 1), hi);
+        for (int x = 0; x < 16; ++x) {
+            const int f = clean_half(r.scale[x / 2], x & 1, t0 + 4 * j + x / 4 + 16 * (x / 2 & 1) >= len);
+            big |= f == 1;
+            any |= f == 2;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int hi = 0; hi < 2; ++hi) clean(r.scale[i], t0 + n + 16 * ((4 * unit + 2 * i + hi) / NG), hi);
+        for (int x = 0; x < 4; ++x) big |= clean_half(r.scale[x / 2], x & 1, t0 + n + 16 * ((4 * unit + x) / NG) >= len) == 1;
     }
     return (__builtin_amdgcn_ballot_w64(big) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(any) ? 2 : 0);
-}
-template <int NG>
-__device__ __forceinline__ void eighth(Unit<NG>& r) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.scale[i] = bits_of(pair_of(r.scale[i]) * (half2v){0.125f16, 0.125f16});
 }
 
 // Every key and value of the call, 64 tokens of a key head to a workgroup, in the
@@ -625,7 +655,9 @@ __global__ void __launch_bounds__(64 * unpack_waves(NG)) attn_chunk_unpack_kerne
 #pragma unroll
     for (int x = 0; x < kUnits; ++x) {
         const int unit = (kUnits * wave + x) % NG;
-        if (f & (unit >= NG / 2 ? 1 : 4)) eighth<NG>(raw[x]);
+        if (f & (unit >= NG / 2 ? 1 : 4))
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[x].scale[i] = eighth(raw[x].scale[i]);
         put_unit<NG>(raw[x], unit, half, lane, to, to + kBuf);
     }
     if (threadIdx.x == 0) a.held_flags[blockIdx.x] = f;
@@ -648,8 +680,8 @@ __global__ void __launch_bounds__(64 * W, NG == 8 ? 1 : 2) attn_chunk_rows_kerne
     id /= (uint32_t)a.splits;
     const int kvh = (int)(id % (uint32_t)a.kv_heads);
     id /= (uint32_t)a.kv_heads;
-    const int seq = (int)(a.together ? id % (uint32_t)a.seqs : id / (uint32_t)a.blocks);
-    const int block = (int)(a.blocks - 1 - (a.together ? id / (uint32_t)a.seqs : id % (uint32_t)a.blocks));    // the longest rows first
+    int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);    // the longest rows first
+    if (a.sorted && !longest_first(a, (int)id, group, kRows, lane, seq, block)) return;
     Span sp;
     if (!sp.read(a, seq)) return;
     if (sp.bad) {
@@ -1022,15 +1054,22 @@ static size_t held_bytes(const ChunkArgs& a) {
     return a.tiles < 0 ? (size_t)(a.seqs * a.kv_heads * a.steps) * (size_t)(256 * a.head_dim) : 0;
 }
 
-// How the rows are cut (a.tiles) and the keys split, by the steps of 64 tokens that
-// the slowest CU comes to, where every workgroup has as many keys as the longest
-// sequence, and some for its start and end and for the joining.
+// How the rows are cut (a.tiles) and the keys split, by the steps of 64 tokens (some
+// 2 us) that the slowest CU comes to, where every workgroup has as many keys as the
+// longest sequence, four more for its start and end, and the parts, written and
+// read at 4 TB/s.
+// Two workgroups of four waves on a CU take a fourteenth longer than one of eight,
+// one alone two thirds of that.
 static int64_t cut(ChunkArgs* a, int64_t rows, int64_t slots, int64_t most) {
     a->blocks = (rows + block_rows(*a) - 1) / block_rows(*a);
     const int64_t units = a->seqs * a->kv_heads * a->blocks;
+    const int64_t part = a->seqs * a->max_q * a->q_heads * (a->head_dim + 4);     // floats
     int64_t best = 0;
     for (int64_t s = 1; s <= most && (s == 1 || units * s <= 4 * slots); ++s) {
-        const int64_t each = (a->steps + s - 1) / s, cost = (units * s + slots - 1) / slots * (each + 4) + (s > 1 ? 6 + s : 0);
+        const int64_t each = (a->steps + s - 1) / s, over = units * s % slots;
+        const int64_t rounds = slots == 256 ? (units * s + 255) / 256 * 14
+                                            : units * s / slots * 15 + (over == 0 ? 0 : over <= 256 ? 10 : 15);
+        const int64_t cost = rounds * (each + 4) + (s > 1 ? 14 * (3 + s * part / 1000000) : 0);
         if (best && cost >= best) continue;
         best = cost;
         a->splits = s;
@@ -1046,11 +1085,10 @@ bool plan_attn_chunk(ChunkArgs* a) {
     if (rows >= kHeldRows && a->seqs * a->kv_heads * a->steps < (int64_t)1 << 22 && held_bytes(*a) <= kHeldMost) {
         const int64_t cost4 = cut(a, rows, wide ? 256 : 512, 16);
         if (a->head_dim == 128) {
-            // eight waves to a copy of the keys where that leaves no CU empty: a
-            // step of two workgroups of four takes about a tenth longer
+            // eight waves to a copy of the keys where that leaves no CU empty
             const int64_t splits4 = a->splits, blocks4 = a->blocks;
             a->tiles = -8;
-            if (cut(a, rows, 256, 16) * 10 > cost4 * 11) a->tiles = -4, a->splits = splits4, a->blocks = blocks4;
+            if (cut(a, rows, 256, 16) > cost4) a->tiles = -4, a->splits = splits4, a->blocks = blocks4;
         }
         a->share = 2 * ((a->steps + a->splits - 1) / a->splits);
     } else {
@@ -1066,7 +1104,7 @@ bool plan_attn_chunk(ChunkArgs* a) {
     a->splits = keys > a->share ? (keys + a->share - 1) / a->share : 1;
     const int64_t units = a->seqs * a->kv_heads * a->blocks;
     if (units >= (int64_t)1 << 22) return false;                     // a launch has fewer than 2^32 threads
-    a->together = units * a->splits <= 1024;
+    a->sorted = a->seqs > 1 && a->seqs <= 64;
     a->per_page = ((uint64_t)1 << 36) / ((uint64_t)a->page_tokens / kKvTile) + 1;
     return true;
 }

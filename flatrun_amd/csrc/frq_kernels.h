@@ -351,7 +351,7 @@ struct ChunkArgs {
     // and a key head, the parts its keys are split into, the tiles of a part, and
     // the steps of 64 tokens of the longest sequence
     int64_t tiles, blocks, splits, share, steps;
-    int together;                // sequences take turns in the order of the grid
+    int sorted;                  // the longest sequences first
     uint64_t per_page;           // 2^36 / tiles of a page, rounded up
     float* part;
     void* held;                  // unpacked keys and values, and a word for each step
