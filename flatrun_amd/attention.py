@@ -5,13 +5,14 @@ The reference runs it in NumPy on the host, K and V kept as growing fp32
 buffers (model/qwen2.py:1520-1624, runtime/kv_cache.py:35-113). Here:
 
     qkv ─▶ qk_norm_rope ─▶ q, k, v ─▶ KVCache4.write ─▶ attn_decode   (one token a sequence)
+                                │                  └──▶ attn_chunk   (a prompt's later chunk, several new tokens)
                                 └──────────────────────▶ attn_prefill (prompts)
 
 :class:`KVCache4` holds K and V in 4 bits in pages, :func:`rope_table` makes
 the rotary table (64-bit, once per model), :class:`BlockAttention` is the
 step with its buffers. The kernels are ``device.qk_norm_rope``,
-``device.kv4_write`` / ``kv4_read``, ``device.attn_decode`` and
-``device.attn_prefill``.
+``device.kv4_write`` / ``kv4_read``, ``device.attn_decode``,
+``device.attn_chunk`` and ``device.attn_prefill``.
 """
 
 from __future__ import annotations
@@ -156,7 +157,9 @@ class BlockAttention:
     * prompts: the heads as bf16, into the cache, and attn_prefill on them;
       where a prompt of the step has tokens in the cache already (it comes in
       chunks), all keys of the step's prompts, new ones too, are what the cache
-      reads back.
+      reads back -- or, with ``direct=True`` on the first layer, attn_chunk
+      attends to the cache as it lies: no copy of the context, keys and values
+      rounded to fp16 rather than bf16 on their way into the products.
 
     A step may hold both; what a single token gets does not depend on its
     neighbours (but for the last bits of sums). Single tokens that stand side
@@ -172,14 +175,16 @@ class BlockAttention:
 
     def __init__(self, cache: KVCache4, q_heads: int, table, n_pos: int, max_rows: int = 0, max_seqs: int = 0,
                  max_context: int = 0, rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None,
-                 eps: float = 1e-6, stream=None, first: BlockAttention | None = None):
+                 eps: float = 1e-6, stream=None, first: BlockAttention | None = None, direct: bool = False):
         if q_heads % cache.kv_heads:
             raise ValueError("q_heads must be a multiple of the cache's kv_heads")
         self.cache, self.q_heads, self.table, self.n_pos = cache, int(q_heads), table, int(n_pos)
         self.rot, self.interleaved, self.eps = rot, interleaved, eps
         self.q_norm, self.k_norm, self.stream = q_norm, k_norm, stream
-        self._first = first
+        self._first, self.direct = first, bool(direct)
         if first is not None:
+            if direct:
+                raise ValueError("direct is the first layer's to say")
             self._share(first, max_rows, max_seqs, max_context)
             return
         if min(int(max_rows), int(max_seqs), int(max_context)) < 1:
@@ -243,7 +248,8 @@ class BlockAttention:
         # keys, its own: attn_decode overwrites what comes of it
         keys = np.where(single, 0, lens) if context else np.array(counts)
         cu_q = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
-        cu_k = np.concatenate([[0], np.cumsum(keys)]).astype(np.int32)
+        direct = context and self.direct     # lengths then, in the place of offsets
+        cu_k = np.concatenate([keys, [0]] if direct else [[0], np.cumsum(keys)]).astype(np.int32)
         ints = np.concatenate([np.concatenate(positions).astype(np.int32), lens, cu_q, cu_k, table.reshape(-1)])
         lib, check = _lib.lib(), _lib.check
         if self.stream is None:              # earlier steps still read these buffers
@@ -258,14 +264,14 @@ class BlockAttention:
         b, at = len(seqs), self._ints.ptr
         p = {"rows": rows, "batch": b, "positions": at, "lens": at + 4 * rows, "cu_q": at + 4 * (rows + b),
              "cu_k": at + 4 * (rows + 2 * b + 1), "table": at + 4 * (rows + 3 * b + 2), "max_q": max(counts),
-             "max_k": int(keys.max()), "tokens_k": int(keys.sum()), "prompts": not all(single), "context": context,
+             "max_k": int(keys.max()), "tokens_k": int(keys.sum()), "prompts": not all(single), "context": context, "direct": direct,
              "max_len": max_len or max([int(n) for n, one in zip(lens, single) if one], default=0), "tokens": []}
         for i in range(b):                   # runs of single tokens: (sequence, row, count)
             if single[i] and i and single[i - 1]:
                 p["tokens"][-1][2] += 1
             elif single[i]:
                 p["tokens"].append([i, int(cu_q[i]), 1])
-        if context:
+        if context and not direct:
             self._plan_context(p, table, keys)
         for s, n in zip(seqs, counts):
             s.length += n
@@ -306,6 +312,10 @@ class BlockAttention:
     def _prompts(self, p: dict, qkv) -> None:
         c, rows, s = self.cache, p["rows"], self.stream
         self._heads(p, qkv, 0, rows, "bf16")
+        if p["direct"]:
+            device.attn_chunk(self.q, c, p["table"], p["cu_k"], p["cu_q"], self.out, p["batch"], rows, self.q_heads,
+                              max_q=p["max_q"], max_len=p["max_k"], out_dtype="f32", ld_table=self.max_pages, stream=s)
+            return
         k, v, cu_k = self.k, self.v, p["cu_q"]
         if p["context"]:
             k, v, cu_k = p["ctx_k"], p["ctx_v"], p["cu_k"]

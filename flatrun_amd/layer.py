@@ -19,7 +19,8 @@ otherwise, same bits); all on one stream.
 Attention, norms and residuals are not quantized matvecs; the caller supplies
 them as functions on device buffers (or does them itself between :meth:`qkv`,
 :meth:`o` and :meth:`mlp`). :class:`flatrun_amd.attention.BlockAttention` is
-such a function for the attention, rotary positions and 4-bit cache included.
+such a function for the attention, rotary positions and 4-bit cache included,
+:class:`Residual` has the one for the residual and norm.
 
 o_proj is a projection like the others here. In the reference its native
 branch never runs: o's weight comes from ``_fetch_linear_with_quant`` ->
@@ -150,3 +151,46 @@ class DecoderProjections:
 
     def __exit__(self, *exc) -> None:
         self.close()
+
+
+class Residual:
+    """The residual rows of a model and the norms along them, fp32 on the device:
+    what stands between two blocks and between a block's attention and its MLP
+    (model/qwen2.py:1388-1773, NumPy).
+
+        xn = r.start(x, norms[0], rows)                  # x: embeddings, the residual from here on
+        for i, (block, step) in enumerate(layers):
+            out = block.forward(xn, rows, attention=step, post_attention=lambda o, n: r.add(o, mlp_norms[i], n))
+            xn = r.add(out, norms[i + 1], rows)          # the last: the norm before the vocabulary
+
+    Weights are device buffers of ``hidden`` floats. ``xn`` is one buffer, written
+    anew by every call; all calls are enqueued on the stream."""
+
+    def __init__(self, hidden: int, max_rows: int = 1, eps: float = 1e-6, stream=None):
+        if int(hidden) < 1 or int(max_rows) < 1:
+            raise ValueError("hidden and max_rows must be at least 1")
+        self.hidden, self.max_rows, self.eps, self.stream = int(hidden), int(max_rows), float(eps), stream
+        self.xn = device.DeviceBuffer(4 * self.hidden * self.max_rows)
+        self.rows = None
+
+    def _norm(self, x, weight, rows: int, **kw):
+        if not 1 <= int(rows) <= self.max_rows:
+            raise ValueError(f"rows must be in 1..{self.max_rows}, got {rows}")
+        device.add_rms_norm(x, self.xn, rows, self.hidden, weight=weight, eps=self.eps, stream=self.stream, **kw)
+        return self.xn
+
+    def start(self, x, weight, rows: int = 1):
+        """The norm of x, whose rows are the residual that later calls add to."""
+        xn = self._norm(x, weight, rows)
+        self.rows = x
+        return xn
+
+    def add(self, delta, weight, rows: int = 1):
+        """residual += delta, and its norm."""
+        if self.rows is None:
+            raise ValueError("start() first")
+        return self._norm(delta, weight, rows, residual=self.rows, sum_out=self.rows)
+
+    def close(self) -> None:
+        self.xn.free()
+        self.rows = None
