@@ -43,6 +43,27 @@ __device__ __forceinline__ int q8_code(float y, float d) {
     return (int)__builtin_fminf(__builtin_fmaxf(q, -127.f), 127.f);
 }
 
+// Eight codes. y times 1 / d is within 2^-22 of the quotient: where that may
+// decide the rounding, at 5e-5 from a half and nearer, the quotient itself is
+// taken (one wave in ten). 2^23 + 2^22 rounds to integers and leaves them in the low byte.
+__device__ __forceinline__ void q8_codes(const float (&y)[8], float d, uint32_t& lo, uint32_t& hi) {
+    const float magic = 12582912.f, one_over = d == 0.f ? 0.f : 1.0f / d;
+    uint32_t c[8];
+    float off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = __builtin_amdgcn_fmed3f(y[i] * one_over, -127.f, 127.f), m = q + magic;
+        c[i] = __builtin_bit_cast(uint32_t, m);
+        off = __builtin_fmaxf(off, __builtin_fabsf(q - (m - magic)));
+    }
+    if (off > 0.49995f || !(d < __builtin_inff())) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = (uint32_t)q8_code(y[i], d);
+    }
+    lo = (c[0] & 255) | (c[1] & 255) << 8 | (c[2] & 255) << 16 | c[3] << 24;
+    hi = (c[4] & 255) | (c[5] & 255) << 8 | (c[6] & 255) << 16 | c[7] << 24;
+}
+
 template <int TYPE>
 __device__ __forceinline__ float round_to(float x) {
     if constexpr (TYPE == kTypeBF16) return __builtin_bit_cast(float, (uint32_t)f32_to_bf16_bits(x) << 16);
@@ -58,6 +79,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
     __shared__ double part[16];
     const int64_t row = blockIdx.x;
     const int hidden = (int)a.hidden, step = (int)blockDim.x * 8;
+    const bool pairs = OUT == kQ8 && a.hidden % 64 == 0 && a.ld_out % 64 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0;
     float h[CH][8];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -80,6 +102,12 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
             if (a.sum) TR::store8(static_cast<typename TR::Elem*>(a.sum) + row * a.ld_sum + e, h[c]);
         }
     }
+    float w[CH][8];                      // on their way while the sum is made
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int e = c * step + (int)threadIdx.x * 8;
+        if (a.weight && e < hidden) Val<kTypeF32>::load8(a.weight + e, w[c]);
+    }
     double ss = 0.0;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -91,31 +119,33 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
     for (int c = 0; c < CH; ++c) {
         const int e = c * step + (int)threadIdx.x * 8;
         if (e >= hidden) break;                          // whole blocks of 32: four lanes go together
-        float w[8], y[8];
-        if (a.weight) Val<kTypeF32>::load8(a.weight + e, w);
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (float)((double)h[c][i] * f * (a.weight ? (double)w[i] : 1.0));
+        for (int i = 0; i < 8; ++i) y[i] = (float)((double)h[c][i] * f * (a.weight ? (double)w[c][i] : 1.0));
         if constexpr (OUT == kQ8) {
-            float top = 0.f;
-            bool odd = false;
+            uint32_t most = 0;           // |y| as integers: in order, NaN above infinity
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                top = __builtin_fmaxf(top, __builtin_fabsf(y[i]));
-                odd |= !(__builtin_fabsf(y[i]) < __builtin_inff());
+                const uint32_t m = __builtin_bit_cast(uint32_t, y[i]) & 0x7FFFFFFFu;
+                most = m > most ? m : most;
             }
-            if (odd) top = __builtin_inff();
-            top = __builtin_fmaxf(top, __shfl_xor(top, 1));
-            top = __builtin_fmaxf(top, __shfl_xor(top, 2));
-            const uint16_t bits = top < __builtin_inff() ? q8_scale(top) : 0x7E00;
-            const float d = f16_bits_to_f32(bits);
-            uint32_t lo = 0, hi = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                lo |= (uint32_t)(q8_code(y[i], d) & 255) << (8 * i);
-                hi |= (uint32_t)(q8_code(y[4 + i], d) & 255) << (8 * i);
-            }
+            most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+            most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+            const uint16_t bits = most < 0x7F800000u ? q8_scale(__builtin_bit_cast(float, most)) : 0x7E00;
+            uint32_t lo, hi;
+            q8_codes(y, f16_bits_to_f32(bits), lo, hi);
             uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.out) + (row * a.ld_out + e) / 32 * kQ8Bytes);
             const int j = threadIdx.x & 3;
+            if (pairs) {
+                // two blocks are 17 words: the second's codes lie on words, the first's two bytes behind
+                const bool second = threadIdx.x & 4;
+                const uint32_t before = (uint32_t)__shfl_up((int)hi, 1);
+                uint32_t* words = reinterpret_cast<uint32_t*>(to + second) + 2 * j;
+                if (second && j == 0) words[-1] = before >> 16 | (uint32_t)bits << 16;
+                words[0] = second ? lo : (j ? before >> 16 : bits) | lo << 16;
+                words[1] = second ? hi : lo >> 16 | hi << 16;
+                continue;
+            }
             if (j == 0) to[0] = bits;
             to[1 + 4 * j] = (uint16_t)lo;
             to[2 + 4 * j] = (uint16_t)(lo >> 16);
