@@ -433,7 +433,7 @@ __device__ __forceinline__ void sums_and_list(const Row& p, const Cuts& c, const
 // LDS of a workgroup that finishes a row.
 struct Finish {
     u64 sum[kBins], group[kGroups], dsum[256];
-    uint32_t count[kBins], dcount[256], listed;
+    uint32_t count[kBins], dcount[512], listed;
     Entry list[kList];
     u64 sort[2][kList];
 };
@@ -456,8 +456,23 @@ __device__ __forceinline__ u64 resolve(Shared& sh, Finish& f, const Row& p, cons
         v[x] = i < many ? (place >> 32) << 32 | (u64)(uint32_t)place << 11 | (u64)i : ~(u64)0;
     }
     static_assert(kList <= 1 << 11, "the number of an entry has 11 bits, its index 20");
+    if (size <= NT / 2) {                    // few: every entry counts those before it, NT / size threads an entry
+        const int i = t & (size - 1), part = t / size, len = (many * size + NT - 1) / NT;
+        uint32_t* before = f.dcount;
+        if (t < size) before[t] = 0, f.sort[0][t] = v[0];
+        __syncthreads();
+        const u64 own = f.sort[0][i];
+        uint32_t c = 0;
+        const int to = (part + 1) * len < many ? (part + 1) * len : many;
+        for (int j = part * len; j < to; ++j) c += f.sort[0][j] < own;
+        if (i < many) atomicAdd(&before[i], c);
+        __syncthreads();
+        if (t < many) f.sort[1][before[t]] = v[0];
+        __syncthreads();
+        if (t < many) v[0] = f.sort[1][t];
+    }
     int turn = 0;
-    for (int k = 2; k <= size; k *= 2)
+    for (int k = 2; size > NT / 2 && k <= size; k *= 2)
         for (int j = k / 2; j; j /= 2) {
             if (j >= NT) {                                           // both in one thread
 #pragma unroll
