@@ -138,37 +138,27 @@ __device__ __forceinline__ bool longest_first(const ChunkArgs& a, int t, int gro
     return true;
 }
 
-template <int TYPE, int OUT, int NG, int R>
-__global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kernel(ChunkArgs a) {
+// LDS of a workgroup of R column tiles.
+template <int NG, int R>
+struct FewShared {
+    __attribute__((aligned(16))) float o[2][R * 2 * NG][64][4];      // [R NG][64] queries until the sums' turn comes
+    float m[kWaves][16 * R], l[kWaves][16 * R];
+};
+
+// A workgroup's part of a row block: the column tiles that have rows, R of MAX
+// (32 sequences of 2 to 9 tokens, 4 heads to a key head, after 100 to 8000: 67 us,
+// 85 with all three tiles for every one).
+template <int TYPE, int OUT, int NG, int R, int MAX>
+__device__ __forceinline__ void few_rows(const ChunkArgs& a, FewShared<NG, MAX>& sh, const Span& sp, int seq, int kvh, int block, int split,
+                                         int group) {
     using T = Val<TYPE>;
     using O = Val<OUT>;
-    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 16 * R;
+    constexpr int D = 32 * NG, kTile = kv_tile_bytes(NG), kRows = 16 * MAX;
     constexpr bool kHeld = NG * R <= 8;            // queries in registers, or in LDS
-    __shared__ __attribute__((aligned(16))) float sh_o[2][R * 2 * NG][64][4];
-    __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
-    half8v (*sh_q)[64] = reinterpret_cast<half8v(*)[64]>(&sh_o[0][0][0][0]);    // [R NG][64], until the sums' turn comes
-
+    half8v (*sh_q)[64] = reinterpret_cast<half8v(*)[64]>(&sh.o[0][0][0][0]);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, j = lane >> 4;
-    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
-    uint32_t id = blockIdx.x;
-    const int split = (int)(id % (uint32_t)a.splits);
-    id /= (uint32_t)a.splits;
-    const int kvh = (int)(id % (uint32_t)a.kv_heads);
-    id /= (uint32_t)a.kv_heads;
-    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
-    Span sp;
-    if (!sp.read(a, seq)) return;
-    if (sp.bad) {
-        if (split) return;
-        for (int64_t i = block; i < sp.nq; i += a.blocks) {
-            typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)kvh * group * D;
-            for (int e = threadIdx.x; e < group * D; e += 64 * kWaves) out[e] = O::one(__builtin_nanf(""));
-        }
-        return;
-    }
     const int row0 = block * kRows, rows = sp.nq * group;
-    if (row0 >= rows) return;
     const int end = sp.keys(row0 + kRows - 1, group);                // keys that the workgroup's rows see
     const int tiles = (end + kKvTile - 1) / kKvTile;
     const int first = split * (int)a.share;
@@ -453,22 +443,22 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
         l[c] += __shfl_xor(l[c], 16);
         l[c] += __shfl_xor(l[c], 32);
         if (j == 0) {
-            sh_m[wave][16 * c + n] = m[c];
-            sh_l[wave][16 * c + n] = l[c];
+            sh.m[wave][16 * c + n] = m[c];
+            sh.l[wave][16 * c + n] = l[c];
         }
     }
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < R; ++c) {
-        float mm = sh_m[0][16 * c + n];
+        float mm = sh.m[0][16 * c + n];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh_m[w][16 * c + n]);
+        for (int w = 1; w < kWaves; ++w) mm = __builtin_fmaxf(mm, sh.m[w][16 * c + n]);
         const float base = mm == -kInf ? 0.f : mm, f = __builtin_amdgcn_exp2f(m[c] - base);
 #pragma unroll
         for (int d = 0; d < 2 * NG; ++d) o[c][d] *= f;
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += sh_l[w][16 * c + n] * __builtin_amdgcn_exp2f(sh_m[w][16 * c + n] - base);
+        for (int w = 0; w < kWaves; ++w) sum += sh.l[w][16 * c + n] * __builtin_amdgcn_exp2f(sh.m[w][16 * c + n] - base);
         l[c] = sum;
         m[c] = mm;
     }
@@ -478,13 +468,13 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
 #pragma unroll
             for (int c = 0; c < R; ++c)
 #pragma unroll
-                for (int d = 0; d < 2 * NG; ++d) *reinterpret_cast<float4v*>(sh_o[wave - half][c * 2 * NG + d][lane]) = o[c][d];
+                for (int d = 0; d < 2 * NG; ++d) *reinterpret_cast<float4v*>(sh.o[wave - half][c * 2 * NG + d][lane]) = o[c][d];
         __syncthreads();
         if (wave < half)
 #pragma unroll
             for (int c = 0; c < R; ++c)
 #pragma unroll
-                for (int d = 0; d < 2 * NG; ++d) o[c][d] += *reinterpret_cast<const float4v*>(sh_o[wave][c * 2 * NG + d][lane]);
+                for (int d = 0; d < 2 * NG; ++d) o[c][d] += *reinterpret_cast<const float4v*>(sh.o[wave][c * 2 * NG + d][lane]);
         __syncthreads();
     }
     if (wave) return;
@@ -512,6 +502,38 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
             __builtin_memcpy(__builtin_assume_aligned(out + 16 * d + 4 * j, 4 * sizeof(y[0])), y, sizeof(y));
         }
     }
+}
+
+template <int TYPE, int OUT, int NG, int R>
+__global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kernel(ChunkArgs a) {
+    using O = Val<OUT>;
+    constexpr int D = 32 * NG, kRows = 16 * R;
+    __shared__ FewShared<NG, R> sh;
+    const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
+    uint32_t id = blockIdx.x;
+    const int split = (int)(id % (uint32_t)a.splits);
+    id /= (uint32_t)a.splits;
+    const int kvh = (int)(id % (uint32_t)a.kv_heads);
+    id /= (uint32_t)a.kv_heads;
+    const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
+    Span sp;
+    if (!sp.read(a, seq)) return;
+    if (sp.bad) {
+        if (split) return;
+        for (int64_t i = block; i < sp.nq; i += a.blocks) {
+            typename O::Elem* out = static_cast<typename O::Elem*>(a.out) + (sp.q0 + i) * a.ld_out + (int64_t)kvh * group * D;
+            for (int e = threadIdx.x; e < group * D; e += 64 * kWaves) out[e] = O::one(__builtin_nanf(""));
+        }
+        return;
+    }
+    const int rest = sp.nq * group - block * kRows;
+    if (rest <= 0) return;
+    if (rest <= 16)
+        few_rows<TYPE, OUT, NG, 1, R>(a, sh, sp, seq, kvh, block, split, group);
+    else if (R > 2 && rest <= 32)
+        few_rows<TYPE, OUT, NG, (R > 2 ? 2 : R), R>(a, sh, sp, seq, kvh, block, split, group);
+    else
+        few_rows<TYPE, OUT, NG, R, R>(a, sh, sp, seq, kvh, block, split, group);
 }
 
 // --------------------------------------------------------------- many rows
