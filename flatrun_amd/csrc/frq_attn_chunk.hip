@@ -511,8 +511,11 @@ __global__ void __launch_bounds__(64 * kWaves, NG == 8 ? 1 : 2) attn_chunk_kerne
     __shared__ FewShared<NG, R> sh;
     const int group = (int)((uint32_t)a.q_heads / (uint32_t)a.kv_heads);
     uint32_t id = blockIdx.x;
-    const int split = (int)(id % (uint32_t)a.splits);
+    // Workgroup i goes to XCD i % 8: the parts go round from row to row, else an XCD
+    // would have all the last ones, which short sequences do not have.
+    int split = (int)(id % (uint32_t)a.splits);
     id /= (uint32_t)a.splits;
+    split = (int)(((uint32_t)split + id) % (uint32_t)a.splits);
     const int kvh = (int)(id % (uint32_t)a.kv_heads);
     id /= (uint32_t)a.kv_heads;
     const int seq = (int)(id / (uint32_t)a.blocks), block = (int)(a.blocks - 1 - id % (uint32_t)a.blocks);
