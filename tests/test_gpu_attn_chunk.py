@@ -303,3 +303,79 @@ def test_one_token_agrees_with_decode(frq):
     device.attn_decode(s.q.float().cuda(), s.cache, dev(s.table), dev(np.array(s.lens, np.int32)), out, 6, 8, 700)
     torch.cuda.synchronize()
     assert np.abs(got - f64(out)).max() <= 4e-3
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("new", [[2, 5, 8, 10, 13, 16, 0, 1], [1, 4, 12, 7], [30, 1, 17, 31, 9], [3, 8]])
+def test_sequences_that_differ_in_rows(frq, hq, hkv, d, new):
+    """Column tiles without rows are left out, a sequence at a time: each as it is alone."""
+    lens = [n + 150 * i for i, n in enumerate(new)]
+    s = Setup(new, lens, hq, hkv, d, page=32, seed=len(new), stale=True)
+    s.check(s.run(out_dtype="f32"), out_dtype="f32")
+
+
+@pytest.mark.parametrize("new,hq", [(3, 4), (37, 8)])
+def test_more_sequences_than_lanes(frq, new, hq):
+    """Past 64 the blocks go by number, not by length."""
+    n = [new - i % 3 for i in range(70)]
+    lens = [0 if i == 5 else m + (i * 37) % 211 for i, m in enumerate(n)]
+    s = Setup(n, lens, hq, 1, 64, page=32, seed=new, stale=True)
+    got = s.run(tail=1)
+    s.check(got)
+    at = sum(n[:5])
+    assert np.all(got[at:at + n[5]] == 0)
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 3e4, 3e5])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_and_large_values_of_many_rows(frq, what, size, d):
+    x = size * torch.randn((300, 1, d), generator=torch.Generator().manual_seed(6)).clamp(-1.7, 1.7)
+    s = Setup([150], [300], 2, 1, d, seed=5, stale=True, **{what: x})
+    if what == "k":
+        s.q = (s.q.float() / max(size, 1e-3)).to(torch.bfloat16)
+    s.check(s.run(out_dtype="f32"), out_dtype="f32")
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e4, 1e30])
+def test_small_and_large_queries_of_many_rows(frq, size):
+    s = Setup([140], [200], 4, 2, 64, seed=6)
+    s.q = (s.q.float() * size).to(torch.bfloat16)
+    s.check(s.run(out_dtype="f32", scale=0.125 / size), out_dtype="f32", scale=0.125 / size)
+
+
+def test_many_rows_in_replays(frq):
+    """Two captured calls share the stream's scratch, the unpacked keys among it: the eager bits every time."""
+    st = device.Stream()
+    two = [Setup([90, 40], [900, 2000], 8, 2, 128, seed=17), Setup([70], [1500], 8, 2, 64, seed=18)]
+    want = [s.run() for s in two]
+    held, graphs = [], []
+
+    def call(s, o):
+        device.attn_chunk(o[0], s.cache, o[1], o[2], o[3], o[4], len(s.new), sum(s.new), 8, max(s.new), max(s.lens), stream=st)
+
+    for s in two:
+        held.append((s.q.cuda(), dev(s.table), dev(np.array(s.lens, np.int32)), dev(s.cu),
+                     torch.zeros((sum(s.new), 8, s.d), dtype=torch.bfloat16, device="cuda")))
+    torch.cuda.synchronize()
+    for s, o in zip(two, held):
+        call(s, o)
+    st.synchronize()
+    for s, o in zip(two, held):
+        with device.Graph.capture(st) as g:
+            call(s, o)
+        graphs.append(g)
+    for _ in range(3):
+        for o in held:
+            o[4].zero_()
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.launch(st)
+        st.synchronize()
+        assert all(np.array_equal(f64(o[4]), w) for o, w in zip(held, want))
+        call(two[0], held[0])
+        st.synchronize()
+        assert np.array_equal(f64(held[0][4]), want[0])
+    for g in graphs:
+        g.destroy()
+    st.destroy()
