@@ -35,17 +35,24 @@ __device__ __forceinline__ double group_sum(double x, double* part) {
     return x;
 }
 
-// fp16(top / 127), held to 65504, and the code of y: correctly rounded quotients.
+// fp16(top / 127), held to 65504, and the code of y: the exact quotient rounded
+// once. Near a half the remainder decides: a quotient rounded to fp32 first would
+// now and then be the half itself.
 __device__ __forceinline__ uint16_t q8_scale(float top) { return f32_to_f16_bits(__builtin_fminf(top / 127.0f, 65504.f)); }
 __device__ __forceinline__ int q8_code(float y, float d) {
     if (d == 0.f) return 0;
-    const float q = __builtin_rintf(y / d);
-    return (int)__builtin_fminf(__builtin_fmaxf(q, -127.f), 127.f);
+    const float q = __builtin_fminf(__builtin_fmaxf(y / d, -127.f), 127.f);
+    float k = __builtin_rintf(q);
+    if (__builtin_fabsf(q - k) > 0.499f) {
+        const float half = k + (q > k ? 0.5f : -0.5f), left = __builtin_fmaf(-half, d, y);
+        k = left > 0.f ? half + 0.5f : left < 0.f ? half - 0.5f : __builtin_rintf(half);
+    }
+    return (int)k;
 }
 
 // Eight codes. y times 1 / d is within 2^-22 of the quotient: where that may
-// decide the rounding, at 5e-5 from a half and nearer, the quotient itself is
-// taken (one wave in ten). 2^23 + 2^22 rounds to integers and leaves them in the low byte.
+// decide the rounding, at 5e-5 from a half and nearer, the remainder does (one
+// wave in ten). 2^23 + 2^22 rounds to integers and leaves them in the low byte.
 __device__ __forceinline__ void q8_codes(const float (&y)[8], float d, uint32_t& lo, uint32_t& hi) {
     const float magic = 12582912.f, one_over = d == 0.f ? 0.f : 1.0f / d;
     uint32_t c[8];

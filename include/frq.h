@@ -512,8 +512,8 @@ int frq_dev_attn_chunk(int type, const void* q, int64_t ld_q, const void* cache,
  * are the same. The norm is computed in 64 bits and rounded once. out_type
  * FRQ_Q8_0: rows of Q8_0 blocks as frq_dev_dequant and frq_dev_gemv read them
  * (hidden and ld_out, in elements, multiples of 32): of the fp32 values, 32 at a
- * time, d = fp16(max|y| / 127) held to 65504, codes round_even(y / d) held to
- * +-127; a block with an inf or a NaN has d = NaN. */
+ * time, d = fp16(max|y| / 127) held to 65504, codes the exact y / d rounded once
+ * to even, held to +-127; a block with an inf or a NaN has d = NaN. */
 int frq_dev_add_rms_norm(int x_type, const void* x, int64_t ld_x, int res_type, const void* residual, int64_t ld_res,
                          void* sum, int64_t ld_sum, const float* weight, float eps, int out_type, void* out,
                          int64_t ld_out, int64_t rows, int64_t hidden, void* stream);

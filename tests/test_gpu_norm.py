@@ -186,3 +186,25 @@ def test_graph_replay(frq):
         check(o, oracle(want, None, 1e-6), "f32")
     g.destroy()
     s.destroy()
+
+
+@pytest.mark.parametrize("hidden", [4096, 20032])
+def test_codes_next_to_a_half(frq, hidden):
+    """y one last place beside d (k + 1/2): the quotient rounded to fp32 may be the half itself, the code is the
+    exact quotient's. A row of ones under weights w has y = w / sqrt(1 + eps), here w itself (eps 0)."""
+    rng = np.random.default_rng(hidden)
+    w = np.zeros((hidden // 32, 32), np.float32)
+    d = np.exp2(rng.uniform(-14, 3, hidden // 32)).astype(np.float16).astype(np.float32)
+    half = rng.integers(0, 126, w.shape) + 0.5
+    step = rng.choice([-1, 0, 1], w.shape)
+    w[:] = (half * d[:, None]).astype(np.float32)
+    w = np.where(step < 0, np.nextafter(w, np.float32(-1)), np.where(step > 0, np.nextafter(w, np.float32(1e9)), w)).astype(np.float32)
+    w[:, 7] = 127 * d                                    # the largest: the scale is d again
+    w *= rng.choice(np.array([-1, 1], np.float32), w.shape)
+    out = empty(1, hidden, "q8_0")
+    device.add_rms_norm(torch.ones((1, hidden), device="cuda"), out, 1, hidden, weight=torch.as_tensor(w.reshape(-1)).cuda(), eps=0.0,
+                        out_dtype="q8_0")
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(-1, 34)
+    assert np.array_equal(got[:, :2].copy().view(np.float16)[:, 0].astype(np.float32), d)
+    assert np.array_equal(got[:, 2:].view(np.int8), np.rint(w.astype(np.float64) / d.astype(np.float64)[:, None]))
