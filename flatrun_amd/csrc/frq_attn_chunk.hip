@@ -16,6 +16,17 @@
 // 2^5, at most 2^12 (2^-12 of themselves, or 2^-30 of the row's largest), summed
 // as they are rounded; scores, maxima and sums are fp32. A tile with a scale
 // beyond 8188, whose values pass fp16, is worked on at an eighth of its values.
+//
+// What bounds it: few rows, the loads of the cache beside the unpacking, some 260
+// vector instructions a tile of 32 tokens and 128 channels whatever the rows, and 45
+// a column tile for its softmax. 17 tokens after 131000, 16 heads of 128 over 8: 51
+// us and 5 for the joining, 3.0 TB/s, vector instructions 58 % of the time, matrix cores
+// 24 %. 32 sequences of 2 to 9 tokens after 100 to 8000: 66 and 6 us, 2.2 TB/s; the
+// short ones leave a wave of two on a SIMD. 5 tokens after 1500, 14 heads over 2 of
+// 64: 8.5 and 5.4. Many rows, the matrix cores at the clock that the power leaves:
+// 2048 tokens after 32768, 32 heads over 8: 34 us to unpack and 1050 to 1085 for the
+// products (1.13 TF of them), matrix cores 58 % busy, vector 36, LDS 29. 8 chunks of
+// 201 to 512 after 300 to 4096, 28 heads over 4: 13.5 and 105 to 118.
 #include "frq_kernels.h"
 #include "frq_kv4.h"
 
@@ -31,7 +42,11 @@ constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUnder = 5.f, kLag = 7.f;      // of the weights' powers of two: see the head of the file
 constexpr float kInf = __builtin_inff();
-constexpr int kHeldRows = 256;                 // rows of a key head from which on keys are unpacked once
+// Rows of a key head from which on keys are unpacked once, for a kernel whose waves
+// share copies of them. After 32768 tokens, 32 heads of 128 over 8, both: 128 rows 81
+// us that way and 71 without, 512 rows 117 and 147, 2048 rows 300 and 376; 128 rows
+// of 256-wide heads 55 and 40.
+constexpr int kHeldRows = 256;
 constexpr size_t kHeldMost = (size_t)1 << 30;  // bytes of them
 
 // Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
@@ -1110,16 +1125,19 @@ bool plan_attn_chunk(ChunkArgs* a) {
     if (rows >= kHeldRows && a->seqs * a->kv_heads * a->steps < (int64_t)1 << 22 && held_bytes(*a) <= kHeldMost) {
         const int64_t cost4 = cut(a, rows, wide ? 256 : 512, 16);
         if (a->head_dim == 128) {
-            // eight waves to a copy of the keys where that leaves no CU empty
+            // eight waves to a copy of the keys where that leaves no CU empty: 2048 tokens
+            // after 32768 1059 us, with four 1163; 8 of 350 after 2200 161 and 140
             const int64_t splits4 = a->splits, blocks4 = a->blocks;
             a->tiles = -8;
             if (cut(a, rows, 256, 16) > cost4) a->tiles = -4, a->splits = splits4, a->blocks = blocks4;
         }
         a->share = 2 * ((a->steps + a->splits - 1) / a->splits);
     } else {
-        a->tiles = rows <= 16 ? 1 : rows <= 32 || wide ? 2 : rows <= 48 ? 3 : 4;
+        a->tiles = rows <= 16 ? 1 : rows <= 32 || wide ? 2 : rows <= 48 ? 3 : 4;     // 256-wide: two fill the registers
         a->blocks = (rows + block_rows(*a) - 1) / block_rows(*a);
         const int64_t units = a->seqs * a->kv_heads * a->blocks;
+        // two workgroups a CU; twice as many where sequences may end early (1536: 32
+        // ragged sequences 62 us, not 71, 32 equal ones of 4000 42, not 37)
         int64_t splits = units >= 512 ? 1 : ((units >= a->kv_heads * 2 ? 1024 : 512) + units - 1) / units;
         // two tiles a wave at least: 5 tokens after 4000, 32 heads over 8: 12.7 us in a
         // graph, 16.1 with four; of 8 sequences after 100 to 4000: 21.1, 24.8 with one

@@ -23,6 +23,14 @@
 // the sums of what stays by group of 1024, and the list; the group that the draw
 // falls into. One workgroup does them all where there are rows for the GPU, else
 // each pass is a launch of slices of all rows.
+//
+// What bounds it: one row, the launches and the chain of each (152064 fp32 logits,
+// top_k 50 and top_p: 3.8, 5.0, 7.3 and 9.1 us); 64 rows of 131072 from the whole,
+// the 64-bit weights (16 us of vector instructions, 67 % of the time) between a pass
+// at 5.3 TB/s for the largest (6.3) and the draw (8.5). 256 rows of 152064, each with
+// parameters of its own: 138 us for up to three passes; the slowest rows, with a
+// top_p of their own, weigh every logit twice, and vector instructions fill 39 %
+// (in slices, with the shares evened out, 146 to 184).
 #include "frq_kernels.h"
 #include "frq_vals.h"
 
@@ -942,6 +950,7 @@ void plan_sample(SampleArgs* a) {
     while (((int64_t)1 << bits) < a->vocab) ++bits;
     a->frac = 62 - bits < kFrac ? 62 - bits : kFrac;         // the sum of a row stays below 2^62
     const int64_t groups = (a->vocab + kGroup - 1) / kGroup;
+    // three workgroups a CU; whole rows from 128 on (256 rows: 138 us, 146 at best in slices)
     int64_t s = a->rows >= 128 ? 1 : 768 / (a->rows ? a->rows : 1);
     s = s < (groups + 3) / 4 ? s : (groups + 3) / 4;         // a group a wave
     s = s < 64 ? s : 64;

@@ -488,12 +488,14 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
  * largest; in a tile of 32 tokens with a value beyond 65504, k and v to 2^-21.
  * No NaN in the cache reaches a query that does not see its token. lens[s] >
  * max_len, more queries than max_q or a page outside the cache: NaN; offsets
- * outside q: the sequence is not computed. Few rows: the keys are split over
- * workgroups, whose results (at most 1024 + as many as there are key heads and
- * sequences, of 64 rows) use the stream's scratch and are joined in a fixed
- * order. The division follows from the shapes: the same call gives the same
- * bits. max_len up to 2^29; seqs, key heads and blocks of 16 to 64 rows together
- * below 2^23. */
+ * outside q: the sequence is not computed. The stream's scratch holds the
+ * results of workgroups that share a row's keys (joined in a fixed order; at most
+ * 140 MB) and, where a key head has 256 rows or more (max_q * q_heads /
+ * kv_heads), the unpacked keys and values of all sequences at max_len each
+ * (4 head_dim bytes a token and key head; beyond 1 GiB they are unpacked by
+ * every workgroup instead). The division follows from the shapes: the same call
+ * gives the same bits. max_len up to 2^29; seqs, key heads and blocks of rows (16
+ * to 256) together below 2^22. */
 int frq_dev_attn_chunk(int type, const void* q, int64_t ld_q, const void* cache, size_t cache_bytes, int64_t pages,
                        int64_t page_tokens, int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t ld_table,
                        const int32_t* lens, const int32_t* cu_q, int64_t seqs, int64_t tokens_q, int64_t max_q,
@@ -532,8 +534,8 @@ int frq_dev_add_rms_norm(int x_type, const void* x, int64_t ld_x, int res_type, 
  * nothing. -inf and NaN logits are never drawn; a row of nothing else gives token
  * -1 and probability 0; where logits are inf, only those are drawn. Weights are
  * computed in 64 bits and held to 2^-45 of the largest (2^-43 at 2^20 logits),
- * sums are exact: tokens do not depend on how the work is divided. Some kilobytes
- * of the stream's scratch a row. */
+ * sums are exact: tokens do not depend on how the work is divided. Up to 127
+ * rows use 66 KB of the stream's scratch each. */
 int frq_dev_sample(int type, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* u,
                    float temperature, const float* temperatures, int64_t top_k, const int32_t* top_ks, float top_p,
                    const float* top_ps, float min_p, const float* min_ps, int32_t* tokens, float* probs, void* stream);
