@@ -47,7 +47,10 @@ constexpr float kInf = __builtin_inff();
 // us that way and 71 without, 512 rows 117 and 147, 2048 rows 300 and 376; 128 rows
 // of 256-wide heads 55 and 40.
 constexpr int kHeldRows = 256;
-constexpr size_t kHeldMost = (size_t)1 << 30;  // bytes of them
+// Bytes of them: with the parts (at most 140 MB) and the words below the 1 GiB up to
+// which a stream's scratch doubles, so that contexts that grow do not leave a buffer
+// behind at every step.
+constexpr size_t kHeldMost = (size_t)864 << 20;
 
 // Eight codes of a word as fp16 integers c - 8, pairs (nibble r, nibble r + 4).
 // 0x6400 | n is 1024 + n; under the mask 0xF0 it is 1024 + 16 n.

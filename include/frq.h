@@ -492,7 +492,7 @@ int frq_dev_attn_prefill(int type, const void* q, int64_t ld_q, int64_t hs_q, co
  * results of workgroups that share a row's keys (joined in a fixed order; at most
  * 140 MB) and, where a key head has 256 rows or more (max_q * q_heads /
  * kv_heads), the unpacked keys and values of all sequences at max_len each
- * (4 head_dim bytes a token and key head; beyond 1 GiB they are unpacked by
+ * (4 head_dim bytes a token and key head; beyond 864 MiB they are unpacked by
  * every workgroup instead). The division follows from the shapes: the same call
  * gives the same bits. max_len up to 2^29; seqs, key heads and blocks of rows (16
  * to 256) together below 2^22. */
