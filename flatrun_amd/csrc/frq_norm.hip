@@ -15,9 +15,11 @@
 // a code of the 8-bit form. Memory bounds the kernel either way.
 //
 // A workgroup holds a row in registers, eight elements at a time a thread (sixteen
-// of 16-bit rows in half the threads: the same 25.5 us). Rows
-// of other sizes and alignments (and those past 16384 elements) take a second
-// kernel, which reads them twice, an element a thread.
+// of 16-bit rows in half the threads: the same 25.5 us); rows of up to 256 share
+// one (100000 of 96, fp32: 24.8 us, 34.9 with a wave each). Rows of other sizes and
+// alignments take a second kernel, an element a thread at a time, held in registers
+// too up to 16384 (8192 of 4097, fp32 to bf16: 130 us, 180 read twice; 20000 of 1001:
+// 53 and 85, where aligned rows of 1000 take 50).
 #include "frq_kernels.h"
 #include "frq_vals.h"
 
@@ -84,31 +86,34 @@ __device__ __forceinline__ float round_to(float x) {
     return x;
 }
 
-// Eight elements a thread, CH times.
-template <int X, int R, int OUT, int CH>
-__global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
+// Eight elements a thread, CH times; a row to a workgroup or, where `lanes` of a
+// wave hold it (SMALL), several.
+template <int X, int R, int OUT, int CH, bool SMALL>
+__global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a, int lanes) {
     using TX = Val<X>;
     using TR = Val<R>;
     __shared__ double part[16];
-    const int64_t row = blockIdx.x;
+    const int tid = SMALL ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x;
+    const int64_t row = SMALL ? (int64_t)blockIdx.x * (256 / lanes) + (int)threadIdx.x / lanes : blockIdx.x;
+    if (SMALL && row >= a.rows) return;                  // all of a row's lanes, which meet nobody else
     const int hidden = (int)a.hidden, step = (int)blockDim.x * 8;
     const bool pairs = OUT == kQ8 && a.hidden % 64 == 0 && a.ld_out % 64 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0;
     float h[CH][8];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e = c * step + (int)threadIdx.x * 8;
+        const int e = c * step + tid * 8;
         if (e < hidden) TX::load8(static_cast<const typename TX::Elem*>(a.x) + row * a.ld_x + e, h[c]);
     }
     if (a.residual) {
         float r[CH][8];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int e = c * step + (int)threadIdx.x * 8;
+            const int e = c * step + tid * 8;
             if (e < hidden) TR::load8(static_cast<const typename TR::Elem*>(a.residual) + row * a.ld_res + e, r[c]);
         }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int e = c * step + (int)threadIdx.x * 8;
+            const int e = c * step + tid * 8;
             if (e >= hidden) break;
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[c][i] = round_to<R>(h[c][i] + r[c][i]);
@@ -118,19 +123,23 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
     float w[CH][8];                      // on their way while the sum is made
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e = c * step + (int)threadIdx.x * 8;
+        const int e = c * step + tid * 8;
         if (a.weight && e < hidden) Val<kTypeF32>::load8(a.weight + e, w[c]);
     }
     double ss = 0.0;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-        if (c * step + (int)threadIdx.x * 8 < hidden)
+        if (c * step + tid * 8 < hidden)
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)h[c][i], (double)h[c][i], ss);
-    const double f = 1.0 / __builtin_sqrt(group_sum(ss, part) / (double)hidden + (double)a.eps);
+    if constexpr (SMALL)
+        for (int i = 1; i < lanes; i <<= 1) ss += __shfl_xor(ss, i);
+    else
+        ss = group_sum(ss, part);
+    const double f = 1.0 / __builtin_sqrt(ss / (double)hidden + (double)a.eps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e = c * step + (int)threadIdx.x * 8;
+        const int e = c * step + tid * 8;
         if (e >= hidden) break;                          // whole blocks of 32: four lanes go together
         float y[8];
 #pragma unroll
@@ -148,10 +157,10 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(NormArgs a) {
             uint32_t lo, hi;
             q8_codes(y, f16_bits_to_f32(bits), lo, hi);
             uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(a.out) + (row * a.ld_out + e) / 32 * kQ8Bytes);
-            const int j = threadIdx.x & 3;
+            const int j = tid & 3;
             if (pairs) {
                 // two blocks are 17 words: the second's codes lie on words, the first's two bytes behind
-                const bool second = threadIdx.x & 4;
+                const bool second = tid & 4;
                 const uint32_t before = (uint32_t)__shfl_up((int)hi, 1);
                 uint32_t* words = reinterpret_cast<uint32_t*>(to + second) + 2 * j;
                 if (second && j == 0) words[-1] = before >> 16 | (uint32_t)bits << 16;
@@ -183,31 +192,44 @@ __device__ __forceinline__ void store_one(int type, void* p, int64_t i, float x)
         static_cast<uint16_t*>(p)[i] = type == kTypeF16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
 }
 
-// Any size and alignment: a row twice, an element a thread; 32 lanes share a block.
-__global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
-    __shared__ double part[4];
+// CH elements of a row, `step` apart; those from n on are 0.
+template <int CH>
+__device__ __forceinline__ void load_some(int type, const void* p, int64_t base, int e, int step, int n, float (&x)[CH]) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) x[c] = 0.f;
+    if (type == kTypeF32) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (e + c * step < n) x[c] = static_cast<const float*>(p)[base + e + c * step];
+    } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (e + c * step < n) x[c] = __builtin_bit_cast(float, (uint32_t) static_cast<const uint16_t*>(p)[base + e + c * step]);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, x[c]);
+            x[c] = type == kTypeF16 ? f16_bits_to_f32(b) : __builtin_bit_cast(float, b << 16);
+        }
+    }
+}
+
+// Rows of any size and alignment, an element a thread at a time: CH times, held in
+// registers, or (CH 0) as often as it takes, a row twice. 32 lanes share a block.
+template <int CH>
+__global__ void __launch_bounds__(1024) norm_any_kernel(NormArgs a) {
+    __shared__ double part[16];
     const int64_t row = blockIdx.x;
-    auto sum_at = [&](int64_t e) {
-        const float x = load_one(a.x_type, a.x, row * a.ld_x + e);
-        if (!a.residual) return x;
-        const float h = x + load_one(a.res_type, a.residual, row * a.ld_res + e);
+    const int nt = (int)blockDim.x;
+    auto rounded = [&](float h) {
         return a.res_type == kTypeF32 ? h : a.res_type == kTypeF16 ? round_to<kTypeF16>(h) : round_to<kTypeBF16>(h);
     };
-    double ss = 0.0;
-    for (int64_t e = threadIdx.x; e < a.hidden; e += 256) {
-        const float h = sum_at(e);
-        if (a.sum) store_one(a.res_type, a.sum, row * a.ld_sum + e, h);
-        ss = __builtin_fma((double)h, (double)h, ss);
-    }
-    const double f = 1.0 / __builtin_sqrt(group_sum(ss, part) / (double)a.hidden + (double)a.eps);
-    for (int64_t e = threadIdx.x; e < a.hidden; e += 256) {
-        // the sum may stand where x or the residual stood
-        const float h = a.sum ? load_one(a.res_type, a.sum, row * a.ld_sum + e) : sum_at(e);
+    auto sum_at = [&](int64_t e) {
+        const float x = load_one(a.x_type, a.x, row * a.ld_x + e);
+        return a.residual ? rounded(x + load_one(a.res_type, a.residual, row * a.ld_res + e)) : x;
+    };
+    auto put = [&](int64_t e, float h, double f) {
         const float y = (float)((double)h * f * (a.weight ? (double)a.weight[e] : 1.0));
-        if (a.out_type != kQ8) {
-            store_one(a.out_type, a.out, row * a.ld_out + e, y);
-            continue;
-        }
+        if (a.out_type != kQ8) return store_one(a.out_type, a.out, row * a.ld_out + e, y);
         float top = __builtin_fabsf(y) < __builtin_inff() ? __builtin_fabsf(y) : __builtin_inff();
 #pragma unroll
         for (int i = 1; i < 32; i <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, i));
@@ -215,15 +237,48 @@ __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs a) {
         uint8_t* to = static_cast<uint8_t*>(a.out) + (row * a.ld_out + e) / 32 * kQ8Bytes;
         if ((e & 31) == 0) *reinterpret_cast<uint16_t*>(to) = bits;
         to[2 + (e & 31)] = (uint8_t)q8_code(y, f16_bits_to_f32(bits));
+    };
+    double ss = 0.0;
+    if constexpr (CH > 0) {
+        const int n = (int)a.hidden, e0 = (int)threadIdx.x;
+        float h[CH];
+        load_some<CH>(a.x_type, a.x, row * a.ld_x, e0, nt, n, h);
+        if (a.residual) {
+            float r[CH];
+            load_some<CH>(a.res_type, a.residual, row * a.ld_res, e0, nt, n, r);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) h[c] = rounded(h[c] + r[c]);
+            if (a.sum)
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+                    if (e0 + c * nt < n) store_one(a.res_type, a.sum, row * a.ld_sum + e0 + c * nt, h[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) ss = __builtin_fma((double)h[c], (double)h[c], ss);
+        const double f = 1.0 / __builtin_sqrt(group_sum(ss, part) / (double)n + (double)a.eps);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (e0 + c * nt < n) put(e0 + c * nt, h[c], f);
+        return;
     }
+    for (int64_t e = threadIdx.x; e < a.hidden; e += nt) {
+        const float h = sum_at(e);
+        if (a.sum) store_one(a.res_type, a.sum, row * a.ld_sum + e, h);
+        ss = __builtin_fma((double)h, (double)h, ss);
+    }
+    const double f = 1.0 / __builtin_sqrt(group_sum(ss, part) / (double)a.hidden + (double)a.eps);
+    // the sum may stand where x or the residual stood
+    for (int64_t e = threadIdx.x; e < a.hidden; e += nt) put(e, a.sum ? load_one(a.res_type, a.sum, row * a.ld_sum + e) : sum_at(e), f);
 }
 
 template <int X, int R, int OUT>
 hipError_t launch_typed(const NormArgs& a, unsigned threads, hipStream_t stream) {
-    if (a.hidden <= (int64_t)threads * 8)
-        norm_rows_kernel<X, R, OUT, 1><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+    if (threads < 64)
+        norm_rows_kernel<X, R, OUT, 1, true><<<(unsigned)((a.rows * threads + 255) / 256), 256, 0, stream>>>(a, (int)threads);
+    else if (a.hidden <= (int64_t)threads * 8)
+        norm_rows_kernel<X, R, OUT, 1, false><<<(unsigned)a.rows, threads, 0, stream>>>(a, 0);
     else
-        norm_rows_kernel<X, R, OUT, 2><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+        norm_rows_kernel<X, R, OUT, 2, false><<<(unsigned)a.rows, threads, 0, stream>>>(a, 0);
     return hipGetLastError();
 }
 
@@ -237,10 +292,17 @@ hipError_t launch_part(const NormArgs& a, hipStream_t stream) {
                       (!a.sum || aligned(a.sum, a.ld_sum, a.res_type)) && (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0 &&
                       (a.out_type == kQ8 || aligned(a.out, a.ld_out, a.out_type));
     if (!wide) {
-        norm_any_kernel<<<(unsigned)a.rows, 256, 0, stream>>>(a);
+        unsigned threads = 64;
+        while (threads < 1024 && (int64_t)threads * 8 < a.hidden) threads *= 2;
+        if (a.hidden <= (int64_t)threads * 8)
+            norm_any_kernel<8><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+        else if (a.hidden <= (int64_t)threads * 16)
+            norm_any_kernel<16><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+        else
+            norm_any_kernel<0><<<(unsigned)a.rows, threads, 0, stream>>>(a);
         return hipGetLastError();
     }
-    unsigned threads = 64;
+    unsigned threads = 8;
     while (threads < 1024 && (int64_t)threads * 8 < a.hidden) threads *= 2;
     return with_type(a.x_type, [&](auto x) {
         return with_type(a.residual ? a.res_type : kTypeF32, [&](auto r) {

@@ -208,3 +208,23 @@ def test_codes_next_to_a_half(frq, hidden):
     got = out.cpu().numpy().reshape(-1, 34)
     assert np.array_equal(got[:, :2].copy().view(np.float16)[:, 0].astype(np.float32), d)
     assert np.array_equal(got[:, 2:].view(np.int8), np.rint(w.astype(np.float64) / d.astype(np.float64)[:, None]))
+
+
+@pytest.mark.parametrize("hidden", [8, 32, 64, 72, 128, 192, 256, 264, 97, 511, 8191, 8193, 16383])
+@pytest.mark.parametrize("rows", [1, 31, 33, 259])
+def test_rows_that_share_a_workgroup_or_hold_one_element_a_lane(frq, hidden, rows):
+    for src, res, out in (("f32", "f32", "f32"), ("bf16", "f32", "bf16"), ("f16", "f16", "f16")) + (
+            (("bf16", "bf16", "q8_0"),) if hidden % 32 == 0 else ()):
+        x, r = make(rows, hidden, src, seed=hidden), make(rows, hidden, res, seed=rows)
+        w = np.random.default_rng(hidden).standard_normal(hidden).astype(np.float32)
+        h = (x.float() + r.float()).to(TORCH[res])
+        total, o = torch.full_like(h, 9).cuda(), empty(rows + 1, hidden, out)
+        device.add_rms_norm(x.cuda(), o, rows, hidden, weight=dev(w), residual=r.cuda(), sum_out=total, x_dtype=src, res_dtype=res,
+                            out_dtype=out)
+        torch.cuda.synchronize()
+        assert torch.equal(total.cpu(), h) and torch.all(o[rows] == 7)
+        want = oracle(h, w, 1e-6)
+        if out == "q8_0":
+            assert np.array_equal(o[:rows].cpu().numpy().reshape(-1, 34), blocks(want))
+        else:
+            check(o[:rows], want, out)
