@@ -228,3 +228,30 @@ def test_rows_that_share_a_workgroup_or_hold_one_element_a_lane(frq, hidden, row
             assert np.array_equal(o[:rows].cpu().numpy().reshape(-1, 34), blocks(want))
         else:
             check(o[:rows], want, out)
+
+
+@pytest.mark.parametrize("hidden", [8, 7])
+def test_more_rows_than_a_launch_takes(frq, hidden):
+    rows = (1 << 21) + 5
+    x = torch.arange(rows, device="cuda", dtype=torch.float32)[:, None] % 1000 + torch.arange(1, hidden + 1, device="cuda")
+    out = torch.full((rows + 1, hidden), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    device.add_rms_norm(x, out, rows, hidden)
+    torch.cuda.synchronize()
+    y = x.double()
+    want = y / torch.sqrt((y * y).mean(-1, keepdim=True) + float(np.float32(1e-6)))
+    assert torch.all((out[:rows].double() - want).abs() <= (2.0 ** -24 + 2.0 ** -30) * want.abs()) and torch.all(out[rows] == 7)
+
+
+@pytest.mark.parametrize("hidden", [64, 67])
+def test_rows_past_32_bits(frq, hidden):
+    ld = (1 << 30) + 8
+    x = torch.zeros((3, ld), dtype=torch.bfloat16, device="cuda")
+    x[:, :hidden] = make(3, hidden, "bf16", seed=1).cuda()
+    out = torch.empty((3, hidden), device="cuda")
+    torch.cuda.synchronize()
+    device.add_rms_norm(x, out, 3, hidden, x_dtype="bf16", ld_x=ld, residual=x, sum_out=x, res_dtype="bf16", ld_res=ld, ld_sum=ld)
+    torch.cuda.synchronize()
+    h = 2 * make(3, hidden, "bf16", seed=1).float()
+    assert torch.equal(x[:, :hidden].float().cpu(), h) and torch.all(x[:, hidden:hidden + 64] == 0)
+    check(out, oracle(h, None, float(np.float32(1e-6))), "f32")

@@ -221,3 +221,25 @@ def test_graph_replay_and_two_streams(frq):
         check(xs[3 - i].numpy(), us[3 - i], got, *spelled(rows, dict(top_p=0.9)))
     g.destroy()
     s.destroy()
+
+
+def test_rows_past_32_bits(frq):
+    vocab, ld = 5001, (1 << 30) + 4
+    x = logits(3, vocab, 9, "bf16")
+    wide = torch.zeros((3, ld), dtype=torch.bfloat16, device="cuda")
+    wide[:, :vocab] = x.cuda()
+    torch.cuda.synchronize()
+    u = uniform(3, 9)
+    for par in (dict(top_k=50, top_p=0.9), dict(temperature=0.0), dict(min_p=0.01)):
+        check(x.float().numpy(), u, run(wide, u, "bf16", ld=ld, vocab=vocab, **par), *spelled(3, par))
+
+
+def test_a_call_of_rows_and_the_rows_alone(frq):
+    """Whole rows and slices of rows see the same weights and sums: the same tokens and probabilities."""
+    rows, vocab = 140, 20011
+    x, u = logits(rows, vocab, 10).cuda(), uniform(rows, 10)
+    for par in (dict(), dict(top_k=300, top_p=0.95), dict(top_p=0.9, temperature=0.6, min_p=0.001), dict(top_k=3000)):
+        tok, prob = run(x, u, **par)
+        for i in (0, 77, 139):
+            one = run(x[i:i + 1], u[i:i + 1], **par)
+            assert one[0][0] == tok[i] and one[1][0] == prob[i], (i, par)
